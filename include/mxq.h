@@ -675,6 +675,72 @@ int mx_swiglu_q8(mx_stream_t s, const uint16_t* gate, const uint16_t* up, uint16
 int mx_swiglu_oai_q8(mx_stream_t s, const uint16_t* gate, const uint16_t* up, uint16_t* y, void* q8_out, uint64_t n, float alpha,
                      float limit);
 
+/* ---------------------------------------------------------------- rotary positions, the key-value cache and the attention of one token
+ * What a decode or prefill step does between the q/k/v projections and the output projection.  Rows are fp16.  Strides count elements from a
+ * token's row to the next token's (heads lie side by side in a row, D values each), so the parts of a fused projection are taken as they lie.
+ *
+ * Rotation: pair i < n_rot / 2 of a head is turned by positions[t] * freqs[i] radians (freqs: device, 64 bits, so that far positions keep
+ * their angle) and multiplied by mscale: y0 = x0 c - x1 s, y1 = x0 s + x1 c in fp32, one rounding to fp16.  interleaved = 0 pairs
+ * elements i and i + n_rot / 2, 1 pairs 2i and 2i + 1; elements from n_rot on are copied.  n_rot % 16 == 0, 16 <= n_rot <= D.
+ *
+ * Cache: pages of `page_size` tokens (a multiple of 16; one page for each sequence makes it a plain cache), each [Hkv][page_size][D], of fp16
+ * (D % 16 == 0) or of Q8_0 planes, int8 values and an fp16 scale for each 32 of a head (D % 32 == 0; scales [Hkv][page_size][D / 32]); D <= 256.
+ * A token's slot is page * page_size + offset.  Q8_0 is the weight format's arithmetic: d = fp16(amax / 127), q = round-half-away(x * (127 / amax));
+ * it quantises the fp16 values that the fp16 cache would hold.  A block that holds a NaN or an infinity reads back as NaN; one whose amax is
+ * above 65471 has a scale whose 127-fold passes fp16 and reads back with infinities.  n_pages * page_size < 2^31; offsets into a plane take 64 bits.
+ *
+ * All row pointers and planes of values 16-byte aligned, scale planes 2-byte, strides multiples of 8.
+ *
+ * mx_rope_freqs (host): freqs[i] = base^(-2i / n_rot) / factors[i] (factors: n_rot / 2 floats or NULL), slowed down by `scale` (1 / the
+ * factor by which the context grows; 1: as trained).  ext_factor 0: every pair alike (linear).  ext_factor > 0 (YaRN): with dim(r) = n_rot ln(n_ctx_orig / (2 pi r)) / (2 ln base),
+ * pairs up to floor(dim(beta_fast)) keep ext_factor of their own frequency, those from ceil(dim(beta_slow)) on are slowed down, those between are mixed
+ * linearly, and mscale = attn_factor * (1 + 0.1 ln(1 / scale)); otherwise mscale = attn_factor.
+ * mx_rope: x and y are [T] rows of n_heads heads; y may be x (same stride).
+ * mx_rope_kv_write_*: q -> q_out rotated; k rotated and v as it is into the cache at slots[t]; q rows may be rotated in place.  A slot outside [0, n_pages * page_size)
+ * (a padded token) writes nothing to the cache.  The slots of one call must be distinct.
+ * mx_kv_write_*: the same without rotation and queries.
+ * mx_kv_read_*: tokens 0 .. rows[b + 1] - rows[b] - 1 of every sequence b, by the pages of page_table[b][max_pages], to rows rows[b] ... of k_out and v_out
+ * ([total_rows][Hkv][D] fp16; rows: B + 1 non-decreasing int32 on the device, of at most total_rows).  Rows from rows[B] on are left as they were.
+ * Tokens whose page is outside [0, n_pages) or past the table read as zeros.  */
+int mx_rope_freqs(uint32_t n_rot, double base, double scale, double ext_factor, double attn_factor, double beta_fast, double beta_slow,
+                  uint32_t n_ctx_orig, const float* factors, double* freqs, float* mscale);
+int mx_rope(mx_stream_t s, const uint16_t* x, uint64_t x_stride, uint16_t* y, uint64_t y_stride, const int32_t* positions, const double* freqs, uint32_t T,
+            uint32_t n_heads, uint32_t D, uint32_t n_rot, int interleaved, float mscale);
+int mx_rope_kv_write_f16(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride,
+                         uint16_t* q_out, uint64_t q_out_stride, uint16_t* k_cache, uint16_t* v_cache, const int32_t* positions, const int32_t* slots,
+                         const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved, float mscale,
+                         uint32_t n_pages, uint32_t page_size);
+int mx_rope_kv_write_q8_0(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride,
+                          uint16_t* q_out, uint64_t q_out_stride, int8_t* k_qs, uint16_t* k_d, int8_t* v_qs, uint16_t* v_d, const int32_t* positions,
+                          const int32_t* slots, const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved,
+                          float mscale, uint32_t n_pages, uint32_t page_size);
+int mx_kv_write_f16(mx_stream_t s, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride, uint16_t* k_cache, uint16_t* v_cache,
+                    const int32_t* slots, uint32_t T, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size);
+int mx_kv_write_q8_0(mx_stream_t s, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride, int8_t* k_qs, uint16_t* k_d, int8_t* v_qs,
+                     uint16_t* v_d, const int32_t* slots, uint32_t T, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size);
+int mx_kv_read_f16(mx_stream_t s, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* page_table, uint32_t max_pages, const int32_t* rows,
+                   uint16_t* k_out, uint16_t* v_out, uint32_t total_rows, uint32_t B, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size);
+int mx_kv_read_q8_0(mx_stream_t s, const int8_t* k_qs, const uint16_t* k_d, const int8_t* v_qs, const uint16_t* v_d, const int32_t* page_table,
+                    uint32_t max_pages, const int32_t* rows, uint16_t* k_out, uint16_t* v_out, uint32_t total_rows, uint32_t B, uint32_t Hkv, uint32_t D,
+                    uint32_t n_pages, uint32_t page_size);
+/* mx_attn_decode_*: one query token for each of B sequences: out[b][h] = sum_t p_t v_t / (sum_t p_t + exp(sink_h - m)), p_t = exp(scale q . k_t - m), over the tokens
+ * t of [max(0, len - window), len) (window 0: all), len = seq_lens[b] cut to what page_table[b][max_pages] holds; query head h reads
+ * key-value head h / (Hq / Hkv) (Hq % Hkv == 0).  sinks: Hq floats or NULL.  Scores, softmax and sums are fp32.  A sequence without tokens (len <= 0) gives zeros; tokens
+ * whose page is outside [0, n_pages) count as masked; what the cache holds behind a sequence's end is never used, whatever it is.
+ * out: [B][Hq][D] fp16; out_q8 (may be NULL, Hq * D % 32 == 0): the block_q8_1x stream of the rounded out, as the output
+ * projection's int-dot product takes it, bit-identical to mx_quantize_q8_1(out).
+ * max_len: no sequence is expected to be longer; it decides how the lengths are split over workgroups (longer ones are right, and slower).  ws: 16-byte aligned,
+ * mx_attn_decode_ws_bytes of the same arguments (0 bytes: NULL will do); its contents on entry do not matter.  */
+int mx_attn_decode_ws_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t max_len, uint32_t window, uint64_t* bytes);
+int mx_attn_decode_f16(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* page_table,
+                       uint32_t max_pages, const int32_t* seq_lens, const float* sinks, uint16_t* out, void* out_q8, uint32_t B, uint32_t Hq,
+                       uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size, uint32_t max_len, uint32_t window, float scale, void* ws,
+                       uint64_t ws_bytes);
+int mx_attn_decode_q8_0(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const int8_t* k_qs, const uint16_t* k_d, const int8_t* v_qs,
+                        const uint16_t* v_d, const int32_t* page_table, uint32_t max_pages, const int32_t* seq_lens, const float* sinks, uint16_t* out,
+                        void* out_q8, uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size, uint32_t max_len,
+                        uint32_t window, float scale, void* ws, uint64_t ws_bytes);
+
 /* build_moe_packing  src/model/qwen3moe_pack.cpp:5-31 (host pointers): stable counting sort by expert.  */
 int mx_build_moe_packing(const int32_t* topk_ids, const float* topk_w, uint32_t T, uint32_t K, uint32_t E,
                          uint32_t* expert_offsets, int32_t* sorted_idx, float* weights_packed, int32_t* tk_to_packed);

@@ -9,7 +9,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 HEADER = os.path.join(_HERE, "..", "include", "mxq.h")
 LIB_PATH = os.path.join(_HERE, "libmxq.so")
 
-_CTYPES = {"uint32_t": C.c_uint32, "uint64_t": C.c_uint64, "int": C.c_int, "float": C.c_float,
+_CTYPES = {"uint32_t": C.c_uint32, "uint64_t": C.c_uint64, "int": C.c_int, "float": C.c_float, "double": C.c_double,
            "mx_stream_t": C.c_void_p, "size_t": C.c_size_t, "int32_t": C.c_int32}
 
 

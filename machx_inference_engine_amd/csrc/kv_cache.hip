@@ -1,0 +1,319 @@
+// kv_cache.hip — rotary positions and the paged key-value cache: rotation of query and key rows, writing (with Q8_0 quantisation) and reading back.
+#include <math.h>
+
+#include "mxq_device.h"
+#include "mxq_host.h"
+
+namespace mxq {
+
+constexpr int kRowThreads = 256;
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float float8 __attribute__((ext_vector_type(8)));
+
+// cos and sin of `turns` revolutions.  The angle is cut to a quarter turn in 64 bits (a position of 2^20 has 2^-12 radians left in 32), what is
+// left is rounded once, and the two Taylor polynomials below are good to 2^-26 on [-pi/4, pi/4].
+__device__ __forceinline__ float2 cos_sin_turns(double turns) {
+    const double quarters = turns * 4.0, k = rint(quarters);
+    const float a = (float)((quarters - k) * 1.5707963267948966), a2 = a * a;
+    float s = fmaf(a2, 2.7557319e-6f, -1.9841270e-4f);
+    s = fmaf(a2, s, 8.3333333e-3f);
+    s = fmaf(a2, s, -1.6666667e-1f);
+    s = fmaf(a * a2, s, a);
+    float c = fmaf(a2, -2.7557319e-7f, 2.4801587e-5f);
+    c = fmaf(a2, c, -1.3888889e-3f);
+    c = fmaf(a2, c, 4.1666667e-2f);
+    c = fmaf(a2, c, -0.5f);
+    c = fmaf(a2, c, 1.0f);
+    const int q = (int)(k - 4.0 * floor(k * 0.25));
+    const float cc = (q & 1) ? s : c, ss = (q & 1) ? c : s;
+    return make_float2((q == 1 || q == 2) ? -cc : cc, (q & 2) ? -ss : ss);
+}
+
+struct RowsArgs {
+    const half_t *q, *k, *v;
+    uint64_t q_stride, k_stride, v_stride, q_out_stride;
+    half_t* q_out;
+    void *k_cache, *v_cache;       // fp16, or int8
+    half_t *k_d, *v_d;             // Q8_0 scales
+    const int32_t *positions, *slots;
+    const double* freqs;
+    uint32_t Hq, Hkv, chunks, n_rot, heads_per_wg, groups, page_size, n_slots;  // chunks = D / 8, groups: workgroups of a token
+    float mscale;
+};
+
+__device__ __forceinline__ uint32_t max_bits4(uint32_t v) {  // over four adjacent lanes
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));
+}
+
+// One workgroup takes heads_per_wg heads (query, key, value heads in this order) of one token, one thread 8 consecutive elements of a head.  A thread
+// loads its own 8 and, in the half layout, the 8 that they are paired with before the barrier behind which the sines are ready, and stores after it:
+// rows may be rotated in place.
+template <bool ROPE, bool Q8, bool INTER>
+__global__ __launch_bounds__(kRowThreads) void rows_kernel(RowsArgs a) {
+    __shared__ float2 cs[128];
+    const uint32_t tid = threadIdx.x, t = blockIdx.x / a.groups, D = a.chunks * 8;
+    const uint32_t hw = tid / a.chunks, c = tid - hw * a.chunks, h = (blockIdx.x - t * a.groups) * a.heads_per_wg + hw;
+    const bool live = hw < a.heads_per_wg && h < a.Hq + 2 * a.Hkv;
+    const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hkv;
+    const uint32_t hk = is_q ? h : is_v ? h - a.Hq - a.Hkv : h - a.Hq;
+    half8 own = {}, other = {};
+    const bool turned = ROPE && !is_v && c * 8 < a.n_rot;
+    const uint32_t half_chunks = a.n_rot / 16;
+    const bool first = c < half_chunks;
+    if (live) {
+        const half_t* row = (is_q ? a.q + t * a.q_stride : is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride) + (size_t)hk * D;
+        own = *reinterpret_cast<const half8*>(row + c * 8);
+        if (!INTER && turned) other = *reinterpret_cast<const half8*>(row + (first ? c + half_chunks : c - half_chunks) * 8);
+    }
+    if (ROPE) {
+        if (tid < a.n_rot / 2) {
+            const float2 v = cos_sin_turns((double)a.positions[t] * (a.freqs[tid] * 0.15915494309189535));
+            cs[tid] = make_float2(v.x * a.mscale, v.y * a.mscale);
+        }
+        __syncthreads();
+    }
+    if (!live) return;   // whole groups of four lanes: chunks % 4 == 0 wherever they exchange values
+    half8 y = own;
+    if (turned) {
+        if (INTER) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 w = cs[c * 4 + i];
+                const float x0 = (float)own[2 * i], x1 = (float)own[2 * i + 1];
+                y[2 * i] = f32_to_f16_rne(fmaf(x0, w.x, -(x1 * w.y)));
+                y[2 * i + 1] = f32_to_f16_rne(fmaf(x0, w.y, x1 * w.x));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float2 w = cs[(first ? c : c - half_chunks) * 8 + i];
+                const float x = (float)own[i], o = (float)other[i];
+                y[i] = f32_to_f16_rne(first ? fmaf(x, w.x, -(o * w.y)) : fmaf(o, w.y, x * w.x));
+            }
+        }
+    }
+    if (is_q) {
+        *reinterpret_cast<half8*>(a.q_out + t * a.q_out_stride + (size_t)h * D + c * 8) = y;
+        return;
+    }
+    const uint32_t slot = (uint32_t)a.slots[t];
+    if (slot >= a.n_slots) return;
+    const uint32_t page = slot / a.page_size, at = slot - page * a.page_size;
+    const size_t crow = ((size_t)page * a.Hkv + hk) * a.page_size + at;
+    void* cache = is_v ? a.v_cache : a.k_cache;
+    if (!Q8) {
+        *reinterpret_cast<half8*>(static_cast<half_t*>(cache) + crow * D + c * 8) = y;
+    } else {
+        // the largest magnitude by its bits: a NaN's are above all others, so that it reaches the scale
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, f2u(fabsf((float)y[i])));
+        const float amax = u2f(max_bits4(top)), inv = amax > 0.f ? 127.0f / amax : 0.f;
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i / 4] |= (uint32_t)(round_away_i((float)y[i] * inv) & 0xFF) << (8 * (i % 4));
+        *reinterpret_cast<uint2*>(static_cast<int8_t*>(cache) + crow * D + c * 8) = make_uint2(w[0], w[1]);
+        if ((c & 3) == 0) (is_v ? a.v_d : a.k_d)[crow * (D / 32) + c / 4] = f32_to_f16_rne(amax / 127.0f);
+    }
+}
+
+template <bool ROPE, bool Q8>
+static int launch_rows(mx_stream_t s, RowsArgs a, uint32_t T, int interleaved) {
+    a.heads_per_wg = kRowThreads / a.chunks;
+    a.groups = (a.Hq + 2 * a.Hkv + a.heads_per_wg - 1) / a.heads_per_wg;
+    MX_REQUIRE_SHAPE((uint64_t)a.groups * T < (1ull << 31));
+    const dim3 grid(a.groups * T);
+    if (ROPE && interleaved) hipLaunchKernelGGL((rows_kernel<ROPE, Q8, ROPE>), grid, dim3(kRowThreads), 0, as_stream(s), a);
+    else hipLaunchKernelGGL((rows_kernel<ROPE, Q8, false>), grid, dim3(kRowThreads), 0, as_stream(s), a);
+    return launch_status();
+}
+
+// Reading back: a workgroup takes 16 tokens of one sequence (they lie in one page) and all heads, a thread 8 elements at a time.
+// Tile numbers are dealt by floor(rows[b] / 16) + b, which leaves room for every sequence's ceil(length / 16).
+template <bool Q8>
+__global__ __launch_bounds__(256) void kv_read_kernel(const void* k_cache, const half_t* k_d, const void* v_cache, const half_t* v_d, const int32_t* page_table,
+                                                      uint32_t max_pages, const int32_t* rows, half_t* k_out, half_t* v_out, uint32_t total, uint32_t B,
+                                                      uint32_t Hkv, uint32_t chunks, uint32_t n_pages, uint32_t page_size) {
+    const uint32_t lane = threadIdx.x & 63u, tile = blockIdx.x;
+    uint32_t lo = 0, n = B;
+    while (n > 1) {   // the last b whose first tile is not behind this one: 64 candidates at a time
+        const uint32_t step = (n + 63) / 64, i = lane * step;
+        const bool behind = i < n && (uint32_t)rows[lo + i] / 16 + lo + i <= tile;
+        const uint32_t cnt = max(1u, (uint32_t)__popcll(__ballot(behind)));
+        lo += (cnt - 1) * step;
+        n = min(step, n - (cnt - 1) * step);
+    }
+    const uint32_t b = lo, row0 = (uint32_t)rows[b], end = min((uint32_t)rows[b + 1], total), first = row0 / 16 + b;
+    if (tile < first || row0 >= end) return;
+    const uint32_t t0 = (tile - first) * 16;
+    if (t0 >= end - row0) return;
+    const uint32_t count = min(16u, end - row0 - t0), col = t0 / page_size, D = chunks * 8;
+    const uint32_t page = col < max_pages ? (uint32_t)page_table[(size_t)b * max_pages + col] : 0xFFFFFFFFu;
+    const bool good = page < n_pages;
+    const uint32_t per_head = 16 * chunks, items = 2 * Hkv * per_head;
+    for (uint32_t i = threadIdx.x; i < items; i += 256) {
+        const uint32_t hh = i / per_head, r = i - hh * per_head, tok = r / chunks, c = r - tok * chunks;
+        if (tok >= count) continue;
+        const bool is_v = hh >= Hkv;
+        const uint32_t h = is_v ? hh - Hkv : hh;
+        half8 y = {};
+        if (good) {
+            const size_t crow = ((size_t)page * Hkv + h) * page_size + (t0 - col * page_size) + tok;
+            const void* cache = is_v ? v_cache : k_cache;
+            if (!Q8) {
+                y = *reinterpret_cast<const half8*>(static_cast<const half_t*>(cache) + crow * D + c * 8);
+            } else {
+                const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(cache) + crow * D + c * 8);
+                const float d = (float)(is_v ? v_d : k_d)[crow * (D / 32) + c / 4];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = f32_to_f16_rne((float)(int8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3))) * d);
+            }
+        }
+        *reinterpret_cast<half8*>((is_v ? v_out : k_out) + ((size_t)(row0 + t0 + tok) * Hkv + h) * D + c * 8) = y;
+    }
+}
+
+// ---------------------------------------------------------------- argument checks (before any HIP call)
+static int check_cache(bool q8, const void* k, const void* k_d, const void* v, const void* v_d, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size) {
+    MX_REQUIRE_PTR(k); MX_REQUIRE_PTR(v);
+    if (q8) { MX_REQUIRE_PTR(k_d); MX_REQUIRE_PTR(v_d); }
+    MX_REQUIRE_SHAPE(Hkv > 0 && Hkv <= 65535 && D > 0 && D <= 256 && D % (q8 ? 32 : 16) == 0);
+    MX_REQUIRE_SHAPE(n_pages > 0 && page_size > 0 && page_size % 16 == 0 && (uint64_t)n_pages * page_size < (1ull << 31));
+    MX_REQUIRE_ALIGN(k, 16); MX_REQUIRE_ALIGN(v, 16);
+    if (q8) { MX_REQUIRE_ALIGN(k_d, 2); MX_REQUIRE_ALIGN(v_d, 2); }
+    return MX_OK;
+}
+static int check_rows(const void* p, uint64_t stride, uint64_t width) {
+    MX_REQUIRE_PTR(p);
+    MX_REQUIRE_SHAPE(stride % 8 == 0 && stride >= width);
+    MX_REQUIRE_ALIGN(p, 16);
+    return MX_OK;
+}
+static int check_rotation(const void* positions, const void* freqs, uint32_t D, uint32_t n_rot) {
+    MX_REQUIRE_PTR(positions); MX_REQUIRE_PTR(freqs);
+    MX_REQUIRE_SHAPE(n_rot >= 16 && n_rot <= D && n_rot % 16 == 0);
+    MX_REQUIRE_ALIGN(positions, 4); MX_REQUIRE_ALIGN(freqs, 8);
+    return MX_OK;
+}
+
+static int rope_kv_write(mx_stream_t s, bool q8, const uint16_t* q, uint64_t q_stride, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride,
+                         uint16_t* q_out, uint64_t q_out_stride, void* k_cache, uint16_t* k_d, void* v_cache, uint16_t* v_d, const int32_t* positions,
+                         const int32_t* slots, const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved,
+                         float mscale, uint32_t n_pages, uint32_t page_size) {
+    if (int rc = check_cache(q8, k_cache, k_d, v_cache, v_d, Hkv, D, n_pages, page_size)) return rc;
+    if (int rc = check_rows(k, k_stride, (uint64_t)Hkv * D)) return rc;
+    if (int rc = check_rows(v, v_stride, (uint64_t)Hkv * D)) return rc;
+    MX_REQUIRE_PTR(slots);
+    MX_REQUIRE_ALIGN(slots, 4);
+    MX_REQUIRE_SHAPE(T > 0 && Hq <= 65535);
+    if (freqs) {
+        MX_REQUIRE_SHAPE(Hq > 0);
+        if (int rc = check_rows(q, q_stride, (uint64_t)Hq * D)) return rc;
+        if (int rc = check_rows(q_out, q_out_stride, (uint64_t)Hq * D)) return rc;
+        if (int rc = check_rotation(positions, freqs, D, n_rot)) return rc;
+    }
+    RowsArgs a = {};
+    a.q = reinterpret_cast<const half_t*>(q); a.k = reinterpret_cast<const half_t*>(k); a.v = reinterpret_cast<const half_t*>(v);
+    a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride; a.q_out_stride = q_out_stride;
+    a.q_out = reinterpret_cast<half_t*>(q_out);
+    a.k_cache = k_cache; a.v_cache = v_cache;
+    a.k_d = reinterpret_cast<half_t*>(k_d); a.v_d = reinterpret_cast<half_t*>(v_d);
+    a.positions = positions; a.slots = slots; a.freqs = freqs;
+    a.Hq = Hq; a.Hkv = Hkv; a.chunks = D / 8; a.n_rot = n_rot; a.page_size = page_size; a.n_slots = n_pages * page_size;
+    a.mscale = mscale;
+    if (freqs) return q8 ? launch_rows<true, true>(s, a, T, interleaved) : launch_rows<true, false>(s, a, T, interleaved);
+    return q8 ? launch_rows<false, true>(s, a, T, 0) : launch_rows<false, false>(s, a, T, 0);
+}
+
+static int kv_read(mx_stream_t s, bool q8, const void* k, const uint16_t* k_d, const void* v, const uint16_t* v_d, const int32_t* page_table, uint32_t max_pages,
+                   const int32_t* rows, uint16_t* k_out, uint16_t* v_out, uint32_t total_rows, uint32_t B, uint32_t Hkv, uint32_t D, uint32_t n_pages,
+                   uint32_t page_size) {
+    if (int rc = check_cache(q8, k, k_d, v, v_d, Hkv, D, n_pages, page_size)) return rc;
+    MX_REQUIRE_PTR(page_table); MX_REQUIRE_PTR(rows); MX_REQUIRE_PTR(k_out); MX_REQUIRE_PTR(v_out);
+    MX_REQUIRE_SHAPE(B > 0 && B <= (1u << 24) && max_pages > 0 && total_rows > 0 && total_rows < (1u << 31));
+    MX_REQUIRE_ALIGN(page_table, 4); MX_REQUIRE_ALIGN(rows, 4); MX_REQUIRE_ALIGN(k_out, 16); MX_REQUIRE_ALIGN(v_out, 16);
+    const dim3 grid(total_rows / 16 + B);
+    auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, as_stream(s), k, reinterpret_cast<const half_t*>(k_d), v, reinterpret_cast<const half_t*>(v_d), page_table,
+                           max_pages, rows, reinterpret_cast<half_t*>(k_out), reinterpret_cast<half_t*>(v_out), total_rows, B, Hkv, D / 8, n_pages, page_size);
+        return launch_status();
+    };
+    return q8 ? launch(kv_read_kernel<true>) : launch(kv_read_kernel<false>);
+}
+
+}  // namespace mxq
+
+using namespace mxq;
+
+extern "C" {
+
+int mx_rope_freqs(uint32_t n_rot, double base, double scale, double ext_factor, double attn_factor, double beta_fast, double beta_slow, uint32_t n_ctx_orig,
+                  const float* factors, double* freqs, float* mscale) {
+    MX_REQUIRE_PTR(freqs); MX_REQUIRE_PTR(mscale);
+    const bool yarn = ext_factor != 0.0;
+    MX_REQUIRE_SHAPE(n_rot >= 16 && n_rot <= 256 && n_rot % 16 == 0 && base > 1.0 && scale > 0.0 && ext_factor >= 0.0 && ext_factor <= 1.0);
+    MX_REQUIRE_SHAPE(!yarn || (n_ctx_orig > 0 && beta_fast > 0.0 && beta_slow > 0.0 && beta_fast >= beta_slow));
+    const double pi = 3.14159265358979323846, n = n_rot;
+    auto dim = [&](double turns) { return n * log(n_ctx_orig / (turns * 2.0 * pi)) / (2.0 * log(base)); };
+    const double low = yarn ? fmax(0.0, floor(dim(beta_fast))) : 0.0, high = yarn ? fmin(n - 1.0, ceil(dim(beta_slow))) : 0.0;
+    for (uint32_t i = 0; i < n_rot / 2; ++i) {
+        const double f = pow(base, -2.0 * i / n) / (factors ? (double)factors[i] : 1.0);
+        const double keep = yarn ? ext_factor * (1.0 - fmin(1.0, fmax(0.0, (i - low) / fmax(0.001, high - low)))) : 0.0;
+        freqs[i] = f * scale * (1.0 - keep) + f * keep;
+    }
+    *mscale = (float)(attn_factor * (yarn ? 1.0 + 0.1 * log(1.0 / scale) : 1.0));
+    return MX_OK;
+}
+
+int mx_rope(mx_stream_t s, const uint16_t* x, uint64_t x_stride, uint16_t* y, uint64_t y_stride, const int32_t* positions, const double* freqs, uint32_t T,
+            uint32_t n_heads, uint32_t D, uint32_t n_rot, int interleaved, float mscale) {
+    MX_REQUIRE_SHAPE(T > 0 && n_heads > 0 && n_heads <= 65535 && D > 0 && D <= 256 && D % 16 == 0);
+    if (int rc = check_rows(x, x_stride, (uint64_t)n_heads * D)) return rc;
+    if (int rc = check_rows(y, y_stride, (uint64_t)n_heads * D)) return rc;
+    if (int rc = check_rotation(positions, freqs, D, n_rot)) return rc;
+    RowsArgs a = {};
+    a.q = reinterpret_cast<const half_t*>(x); a.q_out = reinterpret_cast<half_t*>(y);
+    a.q_stride = x_stride; a.q_out_stride = y_stride;
+    a.positions = positions; a.freqs = freqs;
+    a.Hq = n_heads; a.chunks = D / 8; a.n_rot = n_rot; a.mscale = mscale;
+    return launch_rows<true, false>(s, a, T, interleaved);
+}
+
+int mx_rope_kv_write_f16(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride,
+                         uint16_t* q_out, uint64_t q_out_stride, uint16_t* k_cache, uint16_t* v_cache, const int32_t* positions, const int32_t* slots,
+                         const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved, float mscale,
+                         uint32_t n_pages, uint32_t page_size) {
+    MX_REQUIRE_PTR(freqs);
+    return rope_kv_write(s, false, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, k_cache, nullptr, v_cache, nullptr, positions, slots, freqs, T, Hq,
+                         Hkv, D, n_rot, interleaved, mscale, n_pages, page_size);
+}
+int mx_rope_kv_write_q8_0(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride,
+                          uint16_t* q_out, uint64_t q_out_stride, int8_t* k_qs, uint16_t* k_d, int8_t* v_qs, uint16_t* v_d, const int32_t* positions,
+                          const int32_t* slots, const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved,
+                          float mscale, uint32_t n_pages, uint32_t page_size) {
+    MX_REQUIRE_PTR(freqs);
+    return rope_kv_write(s, true, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, k_qs, k_d, v_qs, v_d, positions, slots, freqs, T, Hq, Hkv, D, n_rot,
+                         interleaved, mscale, n_pages, page_size);
+}
+int mx_kv_write_f16(mx_stream_t s, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride, uint16_t* k_cache, uint16_t* v_cache,
+                    const int32_t* slots, uint32_t T, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size) {
+    return rope_kv_write(s, false, nullptr, 0, k, k_stride, v, v_stride, nullptr, 0, k_cache, nullptr, v_cache, nullptr, nullptr, slots, nullptr, T, 0, Hkv, D, 0, 0,
+                         1.f, n_pages, page_size);
+}
+int mx_kv_write_q8_0(mx_stream_t s, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride, int8_t* k_qs, uint16_t* k_d, int8_t* v_qs,
+                     uint16_t* v_d, const int32_t* slots, uint32_t T, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size) {
+    return rope_kv_write(s, true, nullptr, 0, k, k_stride, v, v_stride, nullptr, 0, k_qs, k_d, v_qs, v_d, nullptr, slots, nullptr, T, 0, Hkv, D, 0, 0, 1.f, n_pages,
+                         page_size);
+}
+int mx_kv_read_f16(mx_stream_t s, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* page_table, uint32_t max_pages, const int32_t* rows,
+                   uint16_t* k_out, uint16_t* v_out, uint32_t total_rows, uint32_t B, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size) {
+    return kv_read(s, false, k_cache, nullptr, v_cache, nullptr, page_table, max_pages, rows, k_out, v_out, total_rows, B, Hkv, D, n_pages, page_size);
+}
+int mx_kv_read_q8_0(mx_stream_t s, const int8_t* k_qs, const uint16_t* k_d, const int8_t* v_qs, const uint16_t* v_d, const int32_t* page_table,
+                    uint32_t max_pages, const int32_t* rows, uint16_t* k_out, uint16_t* v_out, uint32_t total_rows, uint32_t B, uint32_t Hkv, uint32_t D,
+                    uint32_t n_pages, uint32_t page_size) {
+    return kv_read(s, true, k_qs, k_d, v_qs, v_d, page_table, max_pages, rows, k_out, v_out, total_rows, B, Hkv, D, n_pages, page_size);
+}
+
+}  // extern "C"

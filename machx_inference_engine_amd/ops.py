@@ -787,6 +787,142 @@ def gated_rms_norm_q8(x, z, weight, eps):
     return y, q8
 
 
+# ---------------------------------------------------------------- rotary positions, the key-value cache, the attention of one token
+def _want(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _dev(t, dtype, what):
+    """Address of a contiguous tensor of this type on the current device."""
+    if t is None or t.dtype != dtype or not t.is_contiguous() or not t.is_cuda or t.get_device() != torch.cuda.current_device():
+        raise ValueError("%s must be a contiguous %s tensor on the current device" % (what, dtype))
+    return t.data_ptr()
+
+
+def _rows(t, what):
+    """(address, elements from a row to the next) of fp16 rows [T, heads, D] whose heads lie side by side."""
+    if t.dtype != torch.float16 or t.dim() != 3 or not t.is_cuda or t.get_device() != torch.cuda.current_device():
+        raise ValueError("%s must be a fp16 tensor [T, heads, D] on the current device" % what)
+    T, H, D = t.shape
+    st = t.stride()
+    if (st[2] != 1 and D > 1) or (st[1] != D and H > 1):
+        raise ValueError("%s: the heads of a row must lie side by side" % what)
+    return t.data_ptr(), st[0] if T > 1 else max(st[0], H * D + -(H * D) % 8)
+
+
+def _cache(cache):
+    """(format, plane addresses, pages, heads, page size, D) of a cache: (k, v) fp16 or (k_qs, k_d, v_qs, v_d) Q8_0 planes."""
+    n = len(cache)
+    _want(n in (2, 4), "a cache is (k, v) or (k_qs, k_d, v_qs, v_d)")
+    shape = cache[0].shape
+    _want(len(shape) == 4, "cache planes are [pages, heads, page size, D]")
+    if n == 2:
+        _want(cache[1].shape == shape, "the planes of a cache have one shape")
+        return "f16", (_dev(cache[0], torch.float16, "k"), _dev(cache[1], torch.float16, "v")), shape
+    scales = shape[:3] + (shape[3] // 32,)
+    _want(cache[2].shape == shape and cache[1].shape == scales and cache[3].shape == scales, "the planes of a cache have one shape, its scales one for each 32")
+    return "q8_0", (_dev(cache[0], torch.int8, "k_qs"), _dev(cache[1], torch.float16, "k_d"), _dev(cache[2], torch.int8, "v_qs"), _dev(cache[3], torch.float16, "v_d")), shape
+
+
+def kv_cache(fmt, n_pages, n_kv_heads, page_size, head_dim, device="cuda"):
+    """The planes of an empty paged cache: fmt "f16" -> (k, v) fp16 [n_pages, n_kv_heads, page_size, head_dim]; "q8_0" -> (k_qs, k_d, v_qs, v_d),
+    int8 of that shape with fp16 scales [..., head_dim / 32].  A token's slot is page * page_size + offset."""
+    shape = (n_pages, n_kv_heads, page_size, head_dim)
+    if fmt == "f16":
+        return tuple(torch.zeros(shape, dtype=torch.float16, device=device) for _ in range(2))
+    _want(fmt == "q8_0" and head_dim % 32 == 0, "a cache is f16, or q8_0 with heads of whole blocks of 32")
+    plane = lambda: (torch.zeros(shape, dtype=torch.int8, device=device), torch.zeros(shape[:3] + (head_dim // 32,), dtype=torch.float16, device=device))  # noqa: E731
+    return plane() + plane()
+
+
+def rope_freqs(n_rot, base=10000.0, scale=1.0, ext_factor=0.0, attn_factor=1.0, beta_fast=32.0, beta_slow=1.0, n_ctx_orig=0, factors=None):
+    """-> (float64 [n_rot / 2] on the host: radians a position, mscale).  scale: 1 / the factor by which the context grows; ext_factor > 0: YaRN;
+    factors: a divisor for every pair."""
+    freqs, mscale = np.empty(n_rot // 2, np.float64), np.empty(1, np.float32)
+    f = None if factors is None else np.ascontiguousarray(factors, np.float32)
+    _want(f is None or f.shape == freqs.shape, "factors: one for every pair")
+    _host("mx_rope_freqs", n_rot, float(base), float(scale), float(ext_factor), float(attn_factor), float(beta_fast), float(beta_slow), n_ctx_orig,
+          None if f is None else f.ctypes.data, freqs.ctypes.data, mscale.ctypes.data)
+    return torch.from_numpy(freqs), float(mscale[0])
+
+
+def rope(x, positions, freqs, interleaved=False, mscale=1.0, y=None):
+    """x fp16 [T, heads, D] (any row stride), positions int32 [T], freqs float64 [n_rot / 2] -> y, the rotated rows (y=x: in place)."""
+    T, H, D = x.shape
+    if y is None:
+        y = torch.empty((T, H, D), dtype=torch.float16, device=x.device)
+    _want(y.shape == x.shape and positions.shape == (T,), "y has x's shape, positions one entry for each row")
+    _call("mx_rope", *_rows(x, "x"), *_rows(y, "y"), _dev(positions, torch.int32, "positions"), _dev(freqs, torch.float64, "freqs"), T, H, D,
+          2 * freqs.numel(), int(interleaved), mscale)
+    return y
+
+
+def rope_kv_write(q, k, v, positions, slots, cache, freqs, interleaved=False, mscale=1.0, q_out=None):
+    """Rotates q [T, Hq, D] -> q_out (returned) and k [T, Hkv, D]; writes k and v to the cache's slots (int32 [T]; outside the cache: skipped)."""
+    fmt, planes, (n_pages, Hkv, page_size, D) = _cache(cache)
+    T, Hq = q.shape[0], q.shape[1]
+    if q_out is None:
+        q_out = torch.empty((T, Hq, D), dtype=torch.float16, device=q.device)
+    _want(q.shape == (T, Hq, D) and k.shape == (T, Hkv, D) and v.shape == k.shape and q_out.shape == q.shape, "q, k, v and the cache do not fit together")
+    _want(positions.shape == (T,) and slots.shape == (T,), "positions and slots have one entry for each row")
+    _call("mx_rope_kv_write_" + fmt, *_rows(q, "q"), *_rows(k, "k"), *_rows(v, "v"), *_rows(q_out, "q_out"), *planes, _dev(positions, torch.int32, "positions"),
+          _dev(slots, torch.int32, "slots"), _dev(freqs, torch.float64, "freqs"), T, Hq, Hkv, D, 2 * freqs.numel(), int(interleaved), mscale, n_pages, page_size)
+    return q_out
+
+
+def kv_write(k, v, slots, cache):
+    """k, v fp16 [T, Hkv, D] as they are into the cache's slots (int32 [T]; outside the cache: skipped)."""
+    fmt, planes, (n_pages, Hkv, page_size, D) = _cache(cache)
+    T = k.shape[0]
+    _want(k.shape == (T, Hkv, D) and v.shape == k.shape and slots.shape == (T,), "k, v, slots and the cache do not fit together")
+    _call("mx_kv_write_" + fmt, *_rows(k, "k"), *_rows(v, "v"), *planes, _dev(slots, torch.int32, "slots"), T, Hkv, D, n_pages, page_size)
+
+
+def kv_read(cache, page_table, rows, total_rows, out=None):
+    """The first rows[b + 1] - rows[b] tokens of every sequence b (rows int32 [B + 1], page_table int32 [B, max_pages]) -> k, v fp16 [total_rows, Hkv, D]."""
+    fmt, planes, (n_pages, Hkv, page_size, D) = _cache(cache)
+    B, max_pages = page_table.shape
+    _want(rows.shape == (B + 1,), "rows has one entry more than there are sequences")
+    k, v = out if out is not None else (torch.empty((total_rows, Hkv, D), dtype=torch.float16, device=rows.device) for _ in range(2))
+    _want(k.shape == (total_rows, Hkv, D) and v.shape == k.shape, "outputs are [total_rows, heads, D]")
+    _call("mx_kv_read_" + fmt, *planes, _dev(page_table, torch.int32, "page_table"), max_pages, _dev(rows, torch.int32, "rows"), _dev(k, torch.float16, "k_out"),
+          _dev(v, torch.float16, "v_out"), total_rows, B, Hkv, D, n_pages, page_size)
+    return k, v
+
+
+def attn_decode_ws_bytes(B, Hq, Hkv, D, max_len, window=0):
+    n = ctypes.c_uint64()
+    rc = lib.mx_attn_decode_ws_bytes(B, Hq, Hkv, D, max_len, window, ctypes.addressof(n))
+    if rc != 0:
+        raise MxError("mx_attn_decode_ws_bytes", rc)
+    return n.value
+
+
+def attn_decode(q, cache, page_table, seq_lens, scale=None, window=0, sinks=None, max_len=None, out=None, out_q8=None, ws=None):
+    """One query q [B, Hq, D] for each sequence over its seq_lens[b] (int32) tokens in the pages page_table[b] (int32 [B, max_pages]) -> fp16 [B, Hq, D].
+    scale: D ** -0.5 unless given; window: the last tokens only; sinks: fp32 [Hq]; max_len: the longest sequence, where the host knows it; out_q8: uint8
+    buffer for the block_q8_1x stream of the output rows; ws: a workspace of attn_decode_ws_bytes."""
+    fmt, planes, (n_pages, Hkv, page_size, D) = _cache(cache)
+    B, Hq = q.shape[0], q.shape[1]
+    max_pages = page_table.shape[1]
+    _want(q.shape == (B, Hq, D) and page_table.shape[0] == B and seq_lens.shape == (B,) and (sinks is None or sinks.shape == (Hq,)),
+          "q, page_table, seq_lens, sinks and the cache do not fit together")
+    if max_len is None:
+        max_len = max_pages * page_size
+    if out is None:
+        out = torch.empty((B, Hq, D), dtype=torch.float16, device=q.device)
+    _want(out.shape == q.shape and (out_q8 is None or out_q8.numel() * out_q8.element_size() == B * Hq * D // 32 * Q81X_BYTES), "out or out_q8 has another size")
+    if ws is None:
+        need = attn_decode_ws_bytes(B, Hq, Hkv, D, max_len, window)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _call("mx_attn_decode_" + fmt, *_rows(q, "q"), *planes, _dev(page_table, torch.int32, "page_table"), max_pages, _dev(seq_lens, torch.int32, "seq_lens"),
+          None if sinks is None else _dev(sinks, torch.float32, "sinks"), _dev(out, torch.float16, "out"), None if out_q8 is None else _dev(out_q8, torch.uint8, "out_q8"),
+          B, Hq, Hkv, D, n_pages, page_size, max_len, window, D ** -0.5 if scale is None else scale, None if ws is None else _dev(ws, ws.dtype, "ws"),
+          0 if ws is None else ws.numel() * ws.element_size())
+    return out
+
+
 # ---------------------------------------------------------------- prefill GEMM (MFMA)
 def gemm_q4_K(A, W, M, K, N, y=None):
     return _gemm("q4_K", A, (_u8(W),), M, K, N, y)
