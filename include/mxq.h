@@ -689,7 +689,7 @@ int mx_swiglu_oai_q8(mx_stream_t s, const uint16_t* gate, const uint16_t* up, ui
  * it quantises the fp16 values that the fp16 cache would hold.  A block that holds a NaN or an infinity reads back as NaN; one whose amax is
  * above 65471 has a scale whose 127-fold passes fp16 and reads back with infinities.  n_pages * page_size < 2^31; offsets into a plane take 64 bits.
  *
- * All row pointers and planes of values 16-byte aligned, scale planes 2-byte, strides multiples of 8.
+ * All row pointers and planes 16-byte aligned, strides multiples of 8.
  *
  * mx_rope_freqs (host): freqs[i] = base^(-2i / n_rot) / factors[i] (factors: n_rot / 2 floats or NULL), slowed down by `scale` (1 / the
  * factor by which the context grows; 1: as trained).  ext_factor 0: every pair alike (linear).  ext_factor > 0 (YaRN): with dim(r) = n_rot ln(n_ctx_orig / (2 pi r)) / (2 ln base),

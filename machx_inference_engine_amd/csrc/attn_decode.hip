@@ -5,6 +5,10 @@
 namespace mxq {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint32_t kTile = 32;   // tokens of a tile
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 struct AttnArgs {
     const half_t* q;
@@ -15,70 +19,416 @@ struct AttnArgs {
     const float* sinks;
     half_t* out;
     uint8_t* out_q8;
-    uint32_t Hq, Hkv, D, max_pages, n_pages, page_size, window;
-    float scale;
+    float *part_o, *part_ml;        // split lengths: [B][Hq][splits][D] sums and [B][Hq][splits] (maximum, sum of weights)
+    uint32_t Hq, Hkv, D, max_pages, n_pages, page_size, page_shift, window, splits, chunk_tiles;   // page_shift: log2 of a page size that is a power of two, else 32
+    float scale;                    // times log2(e)
 };
 
-// One workgroup of four waves for each (sequence, query head); wave w takes the tokens w, w + 4, ...; the lanes of a wave share the elements of a row.
-template <bool Q8>
-__global__ __launch_bounds__(256) void attn_decode_kernel(AttnArgs a) {
-    __shared__ float ms[4], ls[4], os[4][256];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, h = blockIdx.x, b = blockIdx.y, hk = h / (a.Hq / a.Hkv);
-    const uint64_t capacity = (uint64_t)a.max_pages * a.page_size;
+// The tokens of sequence b: [start, end), in tiles of 32 that begin at multiples of 32, dealt in chunks of `chunk` tiles to the workgroups of the sequence.
+struct Span {
+    uint32_t start, end, tile0, tiles, chunk;
+};
+__device__ __forceinline__ Span span_of(const AttnArgs& a, uint32_t b) {
     const int32_t raw = a.lens[b];
-    const uint32_t len = raw <= 0 ? 0u : (uint32_t)min((uint64_t)raw, capacity), start = a.window && len > a.window ? len - a.window : 0u;
-    float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
+    const uint64_t capacity = (uint64_t)a.max_pages * a.page_size;
+    Span s;
+    s.end = raw <= 0 ? 0u : (uint32_t)min((uint64_t)raw, capacity);
+    s.start = a.window && s.end > a.window ? s.end - a.window : 0u;
+    s.tile0 = s.start / kTile;
+    s.tiles = s.end ? (s.end - 1) / kTile + 1 - s.tile0 : 0u;
+    s.chunk = max(a.chunk_tiles, (s.tiles + a.splits - 1) / a.splits);   // a sequence longer than was expected still fits the splits
+    return s;
+}
+
+// Final rows: four consecutive elements of a thread's, all of 8 threads in one block of 32 (D % 32 == 0 where a stream is wanted).
+__device__ __forceinline__ void store_rows(const AttnArgs& a, size_t at, const float (&o)[4], bool live) {
+    half_t h[4];
+    float v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t d = lane + 64 * i;
-        q[i] = d < a.D ? (float)a.q[b * a.q_stride + (size_t)h * a.D + d] * (a.scale * kLog2e) : 0.f;
+        h[i] = f32_to_f16_rne(o[i]);
+        v[i] = (float)h[i];
     }
-    for (uint32_t t = start + wave; t < len; t += 4) {
-        const uint32_t col = t / a.page_size, page = (uint32_t)a.table[(size_t)b * a.max_pages + col];
-        if (page >= a.n_pages) continue;
-        const size_t row = ((size_t)page * a.Hkv + hk) * a.page_size + (t - col * a.page_size);
-        float x = 0.f, v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t d = lane + 64 * i;
-            v[i] = 0.f;
-            if (d >= a.D) continue;
-            float k;
-            if (Q8) {
-                k = (float)static_cast<const int8_t*>(a.k)[row * a.D + d] * (float)a.k_d[row * (a.D / 32) + d / 32];
-                v[i] = (float)static_cast<const int8_t*>(a.v)[row * a.D + d] * (float)a.v_d[row * (a.D / 32) + d / 32];
-            } else {
-                k = (float)static_cast<const half_t*>(a.k)[row * a.D + d];
-                v[i] = (float)static_cast<const half_t*>(a.v)[row * a.D + d];
-            }
-            x += q[i] * k;
+    if (live) *reinterpret_cast<uint2*>(a.out + at) = *reinterpret_cast<const uint2*>(h);
+    if (a.out_q8) emit_q8_1x(v, threadIdx.x & 7u, live, a.out_q8 + at / 32 * kQ81xBytes);
+}
+
+// Largest / sum over the four 16-lane rows of a wave, in every lane: permlane swaps bring the other rows' values.
+__device__ __forceinline__ float rows_max(float v) {
+    auto r = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
+    v = fmaxf(u2f(r[0]), u2f(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(f2u(v), f2u(v), false, false);
+    return fmaxf(u2f(r[0]), u2f(r[1]));
+}
+__device__ __forceinline__ float rows_sum(float v) {
+    auto r = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
+    v = u2f(r[0]) + u2f(r[1]);
+    r = __builtin_amdgcn_permlane16_swap(f2u(v), f2u(v), false, false);
+    return u2f(r[0]) + u2f(r[1]);
+}
+
+__device__ __forceinline__ uint32_t pick(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
+// Two unsigned bytes u (bytes `sel` of w) as the fp16 pair u - 128: 0x6400 + u is 1024 + u.
+__device__ __forceinline__ half2_t bytes_f16(uint32_t w, uint32_t sel) {
+    const half2_t bias = {(half_t)-1152.f, (half_t)-1152.f};
+    return __builtin_bit_cast(half2_t, pick(w, 0x64646464u, sel)) + bias;
+}
+
+// One workgroup takes one key-value head of one sequence, up to 16 of the query heads that share it, and one chunk of the tokens; its waves take the
+// chunk's tiles of 32 tokens in turn, each with a running maximum and sum of its own.
+//
+// Scores: S^T[token][head] = K Q^T, mfma 16x16x32 with K's rows as they lie (a lane loads 8 elements of one token).  Row r of the two 16-row products of
+// a tile is token 8 (r / 4) + r % 4 (+ 4), so that a lane, which gets 4 rows of a product, ends up with the 8 consecutive tokens 8g .. 8g + 7 of one head (g = lane / 16):
+// exactly the operand layout of the second product, O^T[d][head] += V^T P^T, whose other operand is 8 tokens of one d a lane.  A
+// lane loads elements E c .. E c + E - 1 (c = lane % 16, E = DP / 16) of its 8 tokens, whole rows by 16 lanes, and turns them in registers by byte permutes;
+// nothing goes through LDS before the end.  The weights are two fp16 parts, the second what the first's rounding left (2^-21 of it), so only the result's rounding to
+// fp16 is felt.  Q8_0: keys are exact as fp16 integers and their scales are folded into the fp32 products of each block; values are rounded to fp16 as they are dequantised.
+template <bool Q8, int DP, int NBLK, bool FULL>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_decode_kernel(AttnArgs a) {
+    constexpr int E = DP / 16, NB = DP / 32;
+    constexpr int KW = Q8 ? 2 : 4, VW = Q8 ? E / 4 : E / 2;   // dwords of a lane's key chunk and of its part of one value row
+    constexpr int OS = DP + 4;                                  // LDS row stride of the waves' sums
+    extern __shared__ float lds[];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, r = lane & 15u, g = lane >> 4;
+    const uint32_t G = a.Hq / a.Hkv, tiles_of_heads = (G + 15) / 16;
+    const uint32_t hk = blockIdx.y / tiles_of_heads, head0 = (blockIdx.y - hk * tiles_of_heads) * 16, heads = min(16u, G - head0), b = blockIdx.z;
+    const uint32_t D = FULL ? (Q8 ? NBLK * 32 : DP) : Q8 ? NBLK * 32 : a.D;
+    const Span sp = span_of(a, b);
+    const uint32_t first = blockIdx.x * sp.chunk, last = min(first + sp.chunk, sp.tiles);
+    const size_t out0 = ((size_t)b * a.Hq + hk * G + head0) * D;
+    if (first >= last) {
+        if (blockIdx.x == 0) {   // no tokens at all: zeros, whatever the sinks (several splits: the joining kernel sees to it)
+            if (a.splits == 1)
+                for (uint32_t i = threadIdx.x * 4; i < (heads * D + 1023) / 1024 * 1024; i += blockDim.x * 4) {
+                    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+                    store_rows(a, out0 + i, zero, i < heads * D);
+                }
         }
-        x = __shfl(group_sum<64>(x), 63);
-        const float top = fmaxf(m, x), ref = top == -INFINITY ? 0.f : top, keep = exp2f(m - ref), p = exp2f(x - ref);
-        m = top;
-        l = l * keep + p;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = o[i] * keep + p * v[i];
+        return;
     }
-    if (lane == 0) {
-        ms[wave] = m;
-        ls[wave] = l;
-    }
+
+    half8 qf[NB];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) os[wave][lane + 64 * i] = o[i];
+    for (int n = 0; n < NB; ++n) {
+        qf[n] = half8{};
+        const uint32_t d = n * 32 + g * 8;
+        if (r < heads && d < D) qf[n] = *reinterpret_cast<const half8*>(a.q + b * a.q_stride + (size_t)(hk * G + head0 + r) * D + d);
+    }
+
+    typedef const __attribute__((address_space(4))) int32_t* table_t;
+    const table_t table = (table_t)(uintptr_t)(a.table + (size_t)b * a.max_pages);
+    struct Ref {             // where the two halves of a tile lie: rows of the planes, and whether their pages are the cache's
+        size_t row[2];
+        uint32_t token;
+        bool ok[2];
+    };
+    auto page_of = [&](uint32_t t) { return a.page_shift < 32 ? t >> a.page_shift : t / a.page_size; };
+    auto locate = [&](uint32_t tile) {
+        Ref f;
+        f.token = (sp.tile0 + tile) * kTile;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t t = f.token + 16 * h, col = page_of(t), off = t - col * a.page_size;
+            const uint32_t page = (uint32_t)table[min(col, a.max_pages - 1)];
+            f.ok[h] = page < a.n_pages;
+            f.row[h] = ((size_t)(f.ok[h] ? page : 0u) * a.Hkv + hk) * a.page_size + off;
+        }
+        return f;
+    };
+
+    uint32_t kr[2][NB][KW], vr[8][VW];
+    uint32_t ks[Q8 ? 4 * NBLK : 1], vs[Q8 ? 4 * NBLK : 1];   // scales of the lane's 8 tokens, [token][block]
+    const uint32_t k_in = (8 * ((r >> 2) & 1u) + (r & 3u)) * D + g * 8, v_in = 8 * (g & 1u) * D + r * E;
+    auto load_k = [&](const Ref& f) {
+        const size_t at = (r >> 3 ? f.row[1] : f.row[0]) * D + k_in;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                const size_t i = at + (uint32_t)(t * 4 * D + n * 32);
+                if (Q8) {
+                    if (n < NBLK) *reinterpret_cast<uint2*>(kr[t][n]) = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.k) + i);
+                } else if (FULL || n * 32 + g * 8 < D) {
+                    *reinterpret_cast<uint4*>(kr[t][n]) = *reinterpret_cast<const uint4*>(static_cast<const half_t*>(a.k) + i);
+                }
+            }
+        if (Q8) {
+            const uint4* p = reinterpret_cast<const uint4*>(a.k_d + ((g >> 1 ? f.row[1] : f.row[0]) + 8 * (g & 1u)) * NBLK);
+#pragma unroll
+            for (int n = 0; n < NBLK; ++n) *reinterpret_cast<uint4*>(ks + 4 * n) = p[n];
+        }
+    };
+    auto load_v = [&](const Ref& f) {
+        const size_t row = g >> 1 ? f.row[1] : f.row[0], at = row * D + v_in;
+        if (FULL || r * E < D) {
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const char* p = static_cast<const char*>(a.v) + (at + t * D) * (Q8 ? 1 : 2);
+                if (VW == 1) vr[t][0] = *reinterpret_cast<const uint32_t*>(p);
+                else if (VW == 2) *reinterpret_cast<uint2*>(vr[t]) = *reinterpret_cast<const uint2*>(p);
+                else
+#pragma unroll
+                    for (int w = 0; w < VW / 4; ++w) *reinterpret_cast<uint4*>(vr[t] + 4 * w) = reinterpret_cast<const uint4*>(p)[w];
+            }
+        }
+        if (Q8) {
+            const uint4* p = reinterpret_cast<const uint4*>(a.v_d + (row + 8 * (g & 1u)) * NBLK);
+#pragma unroll
+            for (int n = 0; n < NBLK; ++n) *reinterpret_cast<uint4*>(vs + 4 * n) = p[n];
+        }
+    };
+    if (!FULL) {   // lanes behind the head's end load nothing
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int w = 0; w < KW; ++w) kr[t][n][w] = 0;
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vr[t][w] = 0;
+    }
+
+    float m = -INFINITY, l = 0.f;
+    floatx4 o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+    uint32_t tile = first + wave;
+    if (tile < last) {
+        Ref cur = locate(tile), next = cur;
+        load_k(cur);
+        load_v(cur);
+        if (tile + waves < last) next = locate(tile + waves);
+#pragma unroll 1
+        for (; tile < last; tile += waves) {
+            const bool more = tile + waves < last;
+            // ---- scores
+            float x[8];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                floatx4 s = {0.f, 0.f, 0.f, 0.f};
+                float folded[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int n = 0; n < (Q8 ? NBLK : NB); ++n) {
+                    if (Q8) {
+                        half8 kf;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const half2_t h = bytes_f16(kr[t][n][w / 2] ^ 0x80808080u, w & 1 ? 0x00070006u : 0x00050004u);
+                            kf[2 * w] = h[0];
+                            kf[2 * w + 1] = h[1];
+                        }
+                        const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
+                        const floatx4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[n], zero, 0, 0, 0);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int i = (4 * t + j) * NBLK + n;
+                            folded[j] = fmaf(p[j], h2f((i & 1 ? ks[i / 2] >> 16 : ks[i / 2]) & 0xFFFFu), folded[j]);
+                        }
+                    } else {
+                        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, *reinterpret_cast<const uint4*>(kr[t][n])), qf[n], s, 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[4 * t + j] = (Q8 ? folded[j] : s[j]) * a.scale;
+            }
+            const bool full = cur.token >= sp.start && cur.token + kTile <= sp.end && cur.ok[0] && cur.ok[1];
+            if (!full) {   // masked tokens: no weight, and values of zero, since what lies there may be no number
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t t = cur.token + 8 * g + i;
+                    const bool ok = t >= sp.start && t < sp.end && (g >> 1 ? cur.ok[1] : cur.ok[0]);
+                    if (!ok) x[i] = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) vr[i][w] = ok ? vr[i][w] : 0u;
+                    if (Q8)
+#pragma unroll
+                        for (int n = 0; n < NBLK; ++n) {
+                            const int at = i * NBLK + n;
+                            if (!ok) vs[at / 2] &= at & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                        }
+                }
+            }
+            if (more) load_k(next);
+            // ---- running maximum and sum
+            float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+            top = fmaxf(m, rows_max(top));
+            const float ref = top == -INFINITY ? 0.f : top;
+            if (__any(top > m)) {
+                const float keep = __builtin_amdgcn_exp2f(m - ref);
+                l *= keep;
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[e][j] *= keep;
+                m = top;
+            }
+            half8 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float p = __builtin_amdgcn_exp2f(x[i] - ref);
+                l += p;
+                hi[i] = (half_t)p;
+                lo[i] = (half_t)(p - (float)hi[i]);
+            }
+            // ---- values
+            half2_t sc[Q8 ? 4 : 1];
+            if (Q8) {   // the scales of the lane's block, by pairs of tokens
+                const uint32_t mine = r * E / 32;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t v = 0;
+#pragma unroll
+                    for (int n = 0; n < NBLK; ++n) {
+                        const int i0 = 2 * w * NBLK + n, i1 = i0 + NBLK;
+                        const uint32_t pair = pick(vs[i1 / 2], vs[i0 / 2], (i1 & 1 ? 0x07060000u : 0x05040000u) | (i0 & 1 ? 0x0302u : 0x0100u));
+                        v = n == 0 || mine == (uint32_t)n ? pair : v;
+                    }
+                    sc[w] = __builtin_bit_cast(half2_t, v);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                half8 f0, f1;   // elements e and e + 1 of 8 tokens
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    half2_t h0, h1;
+                    if (Q8) {
+                        const uint32_t both = pick(vr[2 * w + 1][e / 4] , vr[2 * w][e / 4], e & 2 ? 0x07030602u : 0x05010400u) ^ 0x80808080u;
+                        h0 = bytes_f16(both, 0x00050004u) * sc[w];
+                        h1 = bytes_f16(both, 0x00070006u) * sc[w];
+                    } else {
+                        h0 = __builtin_bit_cast(half2_t, pick(vr[2 * w + 1][e / 2], vr[2 * w][e / 2], 0x05040100u));
+                        h1 = __builtin_bit_cast(half2_t, pick(vr[2 * w + 1][e / 2], vr[2 * w][e / 2], 0x07060302u));
+                    }
+                    f0[2 * w] = h0[0]; f0[2 * w + 1] = h0[1];
+                    f1[2 * w] = h1[0]; f1[2 * w + 1] = h1[1];
+                }
+                o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f0, hi, o[e], 0, 0, 0);
+                o[e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f1, hi, o[e + 1], 0, 0, 0);
+                o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f0, lo, o[e], 0, 0, 0);
+                o[e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f1, lo, o[e + 1], 0, 0, 0);
+            }
+            if (more) {
+                load_v(next);
+                cur = next;
+                if (tile + 2 * waves < last) next = locate(tile + 2 * waves);
+            }
+        }
+    }
+
+    // ---- the waves' sums: lane (r, g) holds elements 4 E g .. 4 E g + 4 E - 1 of head r
+    l = rows_sum(l);
+    float* ml = lds;                         // [waves][16] (maximum, sum)
+    float* os = lds + waves * 32;            // [waves][heads][OS]
+    if (g == 0) {
+        ml[(wave * 16 + r) * 2] = m;
+        ml[(wave * 16 + r) * 2 + 1] = l;
+    }
+    if (r < heads) {
+        float* row = os + (wave * heads + r) * OS + 4 * E * g;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < E; e += 4) *reinterpret_cast<floatx4*>(row + E * j + e) = floatx4{o[e][j], o[e + 1][j], o[e + 2][j], o[e + 3][j]};
+    }
     __syncthreads();
-    const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
-    float top = sink;
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, ms[w]);
-    if (top == -INFINITY) top = 0.f;
-    float total = exp2f(sink - top), sum = 0.f;
-    const uint32_t d = threadIdx.x;
-    for (int w = 0; w < 4; ++w) {
-        const float f = exp2f(ms[w] - top);
-        total += f * ls[w];
-        sum += f * os[w][d];
+    for (uint32_t i = threadIdx.x * 4; i < (heads * D + 1023) / 1024 * 1024; i += blockDim.x * 4) {
+        const bool live = i < heads * D;
+        const uint32_t h = live ? i / D : 0, d = live ? i - h * D : 0;
+        const uint32_t hq = hk * G + head0 + h;
+        const float sink = a.splits == 1 && a.sinks ? a.sinks[hq] * kLog2e : -INFINITY;
+        float top = sink, total = 0.f;
+        for (uint32_t w = 0; w < waves; ++w) top = fmaxf(top, ml[(w * 16 + h) * 2]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+        for (uint32_t w = 0; w < waves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(ml[(w * 16 + h) * 2] - ref);
+            total += f * ml[(w * 16 + h) * 2 + 1];
+            sum += f * *reinterpret_cast<const floatx4*>(os + (w * heads + h) * OS + d);
+        }
+        if (a.splits == 1) {
+            const float all = total + __builtin_amdgcn_exp2f(sink - ref), inv = 1.0f / all;
+            const bool none = total == 0.f;
+            const float y[4] = {none ? 0.f : sum[0] * inv, none ? 0.f : sum[1] * inv, none ? 0.f : sum[2] * inv, none ? 0.f : sum[3] * inv};
+            store_rows(a, out0 + i, y, live);
+        } else if (live) {
+            const size_t at = ((size_t)b * a.Hq + hq) * a.splits + blockIdx.x;
+            *reinterpret_cast<floatx4*>(a.part_o + at * D + d) = sum;
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(top, total);
+        }
     }
-    if (d < a.D) a.out[((size_t)b * a.Hq + h) * a.D + d] = f32_to_f16_rne(total == 0.f ? 0.f : sum / total);
+}
+
+// Joins the splits: four elements of one head a thread.
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, uint32_t n4) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    const bool live = i < n4;
+    const uint32_t per = a.D / 4, row = (live ? i : 0) / per, d = ((live ? i : 0) - row * per) * 4, b = row / a.Hq, h = row - b * a.Hq;
+    const Span sp = span_of(a, b);
+    const uint32_t used = live ? (sp.tiles + sp.chunk - 1) / sp.chunk : 0;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)row * a.splits;
+    const float* po = a.part_o + (size_t)row * a.splits * a.D + d;
+    const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
+    float top = sink, total = 0.f;
+    for (uint32_t s = 0; s < used; ++s) top = fmaxf(top, ml[s].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t s = 0; s < used; ++s) {
+        const float2 v = ml[s];
+        const float f = __builtin_amdgcn_exp2f(v.x - ref);
+        total += f * v.y;
+        sum += f * *reinterpret_cast<const floatx4*>(po + (size_t)s * a.D);
+    }
+    const float inv = 1.0f / (total + __builtin_amdgcn_exp2f(sink - ref));
+    const bool none = total == 0.f;
+    const float y[4] = {none ? 0.f : sum[0] * inv, none ? 0.f : sum[1] * inv, none ? 0.f : sum[2] * inv, none ? 0.f : sum[3] * inv};
+    store_rows(a, (size_t)(live ? i : 0) * 4, y, live);
+}
+
+// How the lengths are split: workgroups of four waves, each at least two tiles long, until they fill the CUs three deep.
+struct Plan {
+    uint32_t splits, chunk_tiles;
+};
+static Plan plan_of(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t max_len, uint32_t window) {
+    const uint32_t span = window && window < max_len ? window : max_len;
+    const uint32_t tiles = span / kTile + (window && window < max_len ? 2 : 1);
+    const uint64_t base = (uint64_t)B * Hkv * ((Hq / Hkv + 15) / 16);
+    const uint64_t want = (768 + base - 1) / base;
+    uint32_t chunk = (uint32_t)((tiles + want - 1) / want);
+    if (chunk < 8) chunk = 8;
+    const uint32_t splits = (tiles + chunk - 1) / chunk;
+    return {splits, chunk};
+}
+
+template <bool Q8, int DP, int NBLK, bool FULL>
+static int launch_form(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads) {
+    static LdsLimit limit;
+    const uint32_t waves = 4, lds = (waves * 32 + waves * heads * (DP + 4)) * 4;
+    if (lds > kLdsDefaultLimit)
+        if (int rc = raise_lds_limit(reinterpret_cast<const void*>(attn_decode_kernel<Q8, DP, NBLK, FULL>), limit, (4 * 32 + 4 * 16 * (DP + 4)) * 4)) return rc;
+    hipLaunchKernelGGL((attn_decode_kernel<Q8, DP, NBLK, FULL>), grid, dim3(waves * 64), lds, as_stream(s), a);
+    return launch_status();
+}
+static int launch_attn(mx_stream_t s, const AttnArgs& a, bool q8, dim3 grid, uint32_t heads) {
+    if (q8) switch (a.D / 32) {
+        case 1: return launch_form<true, 64, 1, false>(s, a, grid, heads);
+        case 2: return launch_form<true, 64, 2, true>(s, a, grid, heads);
+        case 3: return launch_form<true, 128, 3, false>(s, a, grid, heads);
+        case 4: return launch_form<true, 128, 4, true>(s, a, grid, heads);
+        case 5: return launch_form<true, 256, 5, false>(s, a, grid, heads);
+        case 6: return launch_form<true, 256, 6, false>(s, a, grid, heads);
+        case 7: return launch_form<true, 256, 7, false>(s, a, grid, heads);
+        default: return launch_form<true, 256, 8, true>(s, a, grid, heads);
+    }
+    if (a.D == 64) return launch_form<false, 64, 2, true>(s, a, grid, heads);
+    if (a.D < 64) return launch_form<false, 64, 2, false>(s, a, grid, heads);
+    if (a.D == 128) return launch_form<false, 128, 4, true>(s, a, grid, heads);
+    if (a.D < 128) return launch_form<false, 128, 4, false>(s, a, grid, heads);
+    if (a.D == 256) return launch_form<false, 256, 8, true>(s, a, grid, heads);
+    return launch_form<false, 256, 8, false>(s, a, grid, heads);
 }
 
 static int attn_decode(mx_stream_t s, bool q8, const uint16_t* q, uint64_t q_stride, const void* k, const uint16_t* k_d, const void* v, const uint16_t* v_d,
@@ -93,14 +443,35 @@ static int attn_decode(mx_stream_t s, bool q8, const uint16_t* q, uint64_t q_str
     MX_REQUIRE_SHAPE(!out_q8 || (uint64_t)Hq * D % 32 == 0);
     MX_REQUIRE_ALIGN(q, 16); MX_REQUIRE_ALIGN(k, 16); MX_REQUIRE_ALIGN(v, 16); MX_REQUIRE_ALIGN(out, 16); MX_REQUIRE_ALIGN(out_q8, 8);
     MX_REQUIRE_ALIGN(page_table, 4); MX_REQUIRE_ALIGN(seq_lens, 4); MX_REQUIRE_ALIGN(sinks, 4);
-    if (q8) { MX_REQUIRE_ALIGN(k_d, 2); MX_REQUIRE_ALIGN(v_d, 2); }
-    AttnArgs a = {reinterpret_cast<const half_t*>(q), q_stride, k, v, reinterpret_cast<const half_t*>(k_d), reinterpret_cast<const half_t*>(v_d), page_table,
-                  seq_lens, sinks, reinterpret_cast<half_t*>(out), static_cast<uint8_t*>(out_q8), Hq, Hkv, D, max_pages, n_pages, page_size, window, scale};
-    (void)max_len; (void)ws; (void)ws_bytes;
-    if (q8) hipLaunchKernelGGL((attn_decode_kernel<true>), dim3(Hq, B), dim3(256), 0, as_stream(s), a);
-    else hipLaunchKernelGGL((attn_decode_kernel<false>), dim3(Hq, B), dim3(256), 0, as_stream(s), a);
-    if (int rc = launch_status()) return rc;
-    return out_q8 ? mx_quantize_q8_1(s, out, out_q8, (uint64_t)B * Hq * D) : MX_OK;
+    if (q8) { MX_REQUIRE_ALIGN(k_d, 16); MX_REQUIRE_ALIGN(v_d, 16); }
+    const Plan p = plan_of(B, Hq, Hkv, max_len, window);
+    const uint64_t parts = p.splits > 1 ? (uint64_t)B * Hq * p.splits : 0, need = parts * (D + 2) * 4;
+    if (need) {
+        MX_REQUIRE_PTR(ws);
+        MX_REQUIRE_ALIGN(ws, 16);
+        if (ws_bytes < need) return MX_ERR_WORKSPACE;
+    }
+    AttnArgs a = {};
+    a.q = reinterpret_cast<const half_t*>(q); a.q_stride = q_stride;
+    a.k = k; a.v = v; a.k_d = reinterpret_cast<const half_t*>(k_d); a.v_d = reinterpret_cast<const half_t*>(v_d);
+    a.table = page_table; a.lens = seq_lens; a.sinks = sinks;
+    a.out = reinterpret_cast<half_t*>(out);
+    a.out_q8 = D % 32 == 0 ? static_cast<uint8_t*>(out_q8) : nullptr;   // heads of half a block: the quantizer, after the rows
+    a.part_o = static_cast<float*>(ws); a.part_ml = static_cast<float*>(ws) + parts * D;
+    a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.max_pages = max_pages; a.n_pages = n_pages; a.page_size = page_size;
+    a.page_shift = (page_size & (page_size - 1)) == 0 ? (uint32_t)__builtin_ctz(page_size) : 32u;
+    a.window = window; a.splits = p.splits; a.chunk_tiles = p.chunk_tiles;
+    a.scale = scale * kLog2e;
+    const uint32_t G = Hq / Hkv, heads = G < 16 ? G : 16;
+    const uint64_t groups = (uint64_t)Hkv * ((G + 15) / 16);
+    MX_REQUIRE_SHAPE(groups <= 65535 && (uint64_t)B * Hq * D < (1ull << 33));
+    if (int rc = launch_attn(s, a, q8, dim3(p.splits, (uint32_t)groups, B), heads)) return rc;
+    if (p.splits > 1) {
+        const uint32_t n4 = (uint32_t)((uint64_t)B * Hq * D / 4);
+        hipLaunchKernelGGL(attn_join_kernel, dim3((n4 + 255) / 256), dim3(256), 0, as_stream(s), a, n4);
+        if (int rc = launch_status()) return rc;
+    }
+    return out_q8 && !a.out_q8 ? mx_quantize_q8_1(s, out, out_q8, (uint64_t)B * Hq * D) : MX_OK;
 }
 
 }  // namespace mxq
@@ -112,8 +483,8 @@ extern "C" {
 int mx_attn_decode_ws_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t max_len, uint32_t window, uint64_t* bytes) {
     MX_REQUIRE_PTR(bytes);
     MX_REQUIRE_SHAPE(B > 0 && B <= 65535 && Hkv > 0 && Hq > 0 && Hq <= 65535 && Hq % Hkv == 0 && D > 0 && D <= 256 && D % 16 == 0);
-    (void)max_len; (void)window;
-    *bytes = 0;
+    const Plan p = plan_of(B, Hq, Hkv, max_len, window);
+    *bytes = p.splits > 1 ? (uint64_t)B * Hq * p.splits * (D + 2) * 4 : 0;
     return MX_OK;
 }
 

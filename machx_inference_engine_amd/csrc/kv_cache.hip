@@ -181,7 +181,7 @@ static int check_cache(bool q8, const void* k, const void* k_d, const void* v, c
     MX_REQUIRE_SHAPE(Hkv > 0 && Hkv <= 65535 && D > 0 && D <= 256 && D % (q8 ? 32 : 16) == 0);
     MX_REQUIRE_SHAPE(n_pages > 0 && page_size > 0 && page_size % 16 == 0 && (uint64_t)n_pages * page_size < (1ull << 31));
     MX_REQUIRE_ALIGN(k, 16); MX_REQUIRE_ALIGN(v, 16);
-    if (q8) { MX_REQUIRE_ALIGN(k_d, 2); MX_REQUIRE_ALIGN(v_d, 2); }
+    if (q8) { MX_REQUIRE_ALIGN(k_d, 16); MX_REQUIRE_ALIGN(v_d, 16); }
     return MX_OK;
 }
 static int check_rows(const void* p, uint64_t stride, uint64_t width) {
