@@ -53,6 +53,17 @@ __device__ __forceinline__ void store_rows(const AttnArgs& a, size_t at, const f
     if (a.out_q8) emit_q8_1x(v, threadIdx.x & 7u, live, a.out_q8 + at / 32 * kQ81xBytes);
 }
 
+// The cache is read once: its lines need not stay.
+#ifndef NT
+#define NT 1
+#endif
+template <class T>
+__device__ __forceinline__ T load_once(const void* p) {
+    typedef uint32_t vec __attribute__((ext_vector_type(sizeof(T) / 4)));
+    if (NT) return __builtin_bit_cast(T, __builtin_nontemporal_load(reinterpret_cast<const vec*>(p)));
+    return __builtin_bit_cast(T, *reinterpret_cast<const vec*>(p));
+}
+
 // Largest / sum over the four 16-lane rows of a wave, in every lane: permlane swaps bring the other rows' values.
 __device__ __forceinline__ float rows_max(float v) {
     auto r = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
@@ -65,6 +76,13 @@ __device__ __forceinline__ float rows_sum(float v) {
     v = u2f(r[0]) + u2f(r[1]);
     r = __builtin_amdgcn_permlane16_swap(f2u(v), f2u(v), false, false);
     return u2f(r[0]) + u2f(r[1]);
+}
+
+// What a wave's lanes wrote to LDS is there for its other lanes: one wave's LDS accesses keep their order, so only the compiler is told.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 __device__ __forceinline__ uint32_t pick(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
@@ -84,9 +102,10 @@ __device__ __forceinline__ half2_t bytes_f16(uint32_t w, uint32_t sel) {
 // nothing goes through LDS before the end.  The weights are two fp16 parts, the second what the first's rounding left (2^-21 of it), so only the result's rounding to
 // fp16 is felt.  Q8_0: keys are exact as fp16 integers and their scales are folded into the fp32 products of each block; values are rounded to fp16 as they are dequantised.
 template <bool Q8, int DP, int NBLK, bool FULL>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_decode_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void attn_decode_kernel(AttnArgs a) {
     constexpr int E = DP / 16, NB = DP / 32;
-    constexpr int KW = Q8 ? 2 : 4, VW = Q8 ? E / 4 : E / 2;   // dwords of a lane's key chunk and of its part of one value row
+    constexpr int VW = Q8 ? E / 4 : E / 2;                     // dwords of a lane's part of one value row
+    constexpr int CPR = DP / (Q8 ? 16 : 8), RPI = 64 / CPR, KI = kTile / RPI;   // 16-byte pieces of a key row, rows of a load, loads of a tile
     constexpr int OS = DP + 4;                                  // LDS row stride of the waves' sums
     extern __shared__ float lds[];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, r = lane & 15u, g = lane >> 4;
@@ -117,73 +136,96 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_decode_kernel(Att
 
     typedef const __attribute__((address_space(4))) int32_t* table_t;
     const table_t table = (table_t)(uintptr_t)(a.table + (size_t)b * a.max_pages);
-    struct Ref {             // where the two halves of a tile lie: rows of the planes, and whether their pages are the cache's
-        size_t row[2];
-        uint32_t token;
-        bool ok[2];
+    struct Ref {             // a tile's first token and, for its two halves, page and place in the page
+        uint32_t token, page[2], off[2];
     };
     auto page_of = [&](uint32_t t) { return a.page_shift < 32 ? t >> a.page_shift : t / a.page_size; };
     auto locate = [&](uint32_t tile) {
         Ref f;
         f.token = (sp.tile0 + tile) * kTile;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t t = f.token + 16 * h, col = page_of(t), off = t - col * a.page_size;
-            const uint32_t page = (uint32_t)table[min(col, a.max_pages - 1)];
-            f.ok[h] = page < a.n_pages;
-            f.row[h] = ((size_t)(f.ok[h] ? page : 0u) * a.Hkv + hk) * a.page_size + off;
-        }
+        const uint32_t c0 = page_of(f.token), o0 = f.token - c0 * a.page_size;
+        const bool next = o0 + 16 >= a.page_size;
+        const uint32_t c1 = next ? c0 + 1 : c0;
+        f.off[0] = o0;
+        f.off[1] = next ? 0 : o0 + 16;
+        f.page[0] = (uint32_t)table[c0];                          // c0 < max_pages: the tile's first token is in front of the sequence's end
+        f.page[1] = (uint32_t)table[min(c1, a.max_pages - 1)];
         return f;
     };
+    auto row_of = [&](const Ref& f, int h) { return ((size_t)(f.page[h] < a.n_pages ? f.page[h] : 0u) * a.Hkv + hk) * a.page_size + f.off[h]; };
 
-    uint32_t kr[2][NB][KW], vr[8][VW];
-    uint32_t ks[Q8 ? 4 * NBLK : 1], vs[Q8 ? 4 * NBLK : 1];   // scales of the lane's 8 tokens, [token][block]
-    const uint32_t k_in = (8 * ((r >> 2) & 1u) + (r & 3u)) * D + g * 8, v_in = 8 * (g & 1u) * D + r * E;
+    uint32_t kr[KI][4], vr[8][VW];
+    constexpr int SL = (16 * NBLK + 63) / 64;                 // dwords of a tile's scales in a lane
+    uint32_t ks[SL], vs[SL];
+    // keys: whole rows by CPR lanes each, into the wave's LDS tile, where a row's pieces lie permuted (piece p at p ^ f, f = row % 4 + 4 (row / 8 % 2), which
+    // is lane % 8 of its reader), so that the 16 lanes that read the same piece of 16 rows meet different banks
+    constexpr uint32_t ROW = CPR * 16;
+    constexpr uint32_t SCALES = Q8 ? kTile * NBLK * 2 : 0, WAVE = kTile * ROW + 2 * SCALES;   // LDS of a wave: keys, their scales [token][block], the values' [block][token]
+    char* const keys = reinterpret_cast<char*>(lds) + wave * WAVE;
+    half_t* const k_scales = reinterpret_cast<half_t*>(keys + kTile * ROW);
+    half_t* const v_scales = reinterpret_cast<half_t*>(keys + kTile * ROW + SCALES);
+    const uint32_t lr = lane / CPR, lp = lane % CPR, v_in = 8 * (g & 1u) * D + r * E;
     auto load_k = [&](const Ref& f) {
-        const size_t at = (r >> 3 ? f.row[1] : f.row[0]) * D + k_in;
+        const size_t row0 = row_of(f, 0), row1 = row_of(f, 1);
+        if (FULL || lp * 16 < D * (Q8 ? 1 : 2)) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                const size_t i = at + (uint32_t)(t * 4 * D + n * 32);
-                if (Q8) {
-                    if (n < NBLK) *reinterpret_cast<uint2*>(kr[t][n]) = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.k) + i);
-                } else if (FULL || n * 32 + g * 8 < D) {
-                    *reinterpret_cast<uint4*>(kr[t][n]) = *reinterpret_cast<const uint4*>(static_cast<const half_t*>(a.k) + i);
-                }
+            for (int i = 0; i < KI; ++i) {
+                const char* base = static_cast<const char*>(a.k) + (i * RPI >= 16 ? row1 : row0) * D * (Q8 ? 1 : 2);
+                *reinterpret_cast<uint4*>(kr[i]) = load_once<uint4>(base + ((i * RPI & 15) + lr) * D * (Q8 ? 1 : 2) + lp * 16);
             }
-        if (Q8) {
-            const uint4* p = reinterpret_cast<const uint4*>(a.k_d + ((g >> 1 ? f.row[1] : f.row[0]) + 8 * (g & 1u)) * NBLK);
-#pragma unroll
-            for (int n = 0; n < NBLK; ++n) *reinterpret_cast<uint4*>(ks + 4 * n) = p[n];
         }
     };
+    auto load_scales = [&](const Ref& f) {
+        const size_t row0 = row_of(f, 0), row1 = row_of(f, 1);
+#pragma unroll
+        for (int i = 0; i < SL; ++i) {
+            const uint32_t w = i * 64 + lane;          // 8 * NBLK dwords of each half
+            if (SL * 64 == 16 * NBLK || w < 16 * NBLK) {
+                const size_t at = w < 8 * NBLK ? row0 * NBLK + 2 * w : row1 * NBLK + 2 * (w - 8 * NBLK);
+                ks[i] = *reinterpret_cast<const uint32_t*>(a.k_d + at);
+                vs[i] = *reinterpret_cast<const uint32_t*>(a.v_d + at);
+            }
+        }
+    };
+    auto stage_scales = [&]() {
+#pragma unroll
+        for (int i = 0; i < SL; ++i) {
+            const uint32_t w = i * 64 + lane;
+            if (SL * 64 == 16 * NBLK || w < 16 * NBLK) {
+                reinterpret_cast<uint32_t*>(k_scales)[w] = ks[i];
+                const uint32_t t0 = 2 * w / NBLK, n0 = 2 * w % NBLK, t1 = (2 * w + 1) / NBLK, n1 = (2 * w + 1) % NBLK;
+                reinterpret_cast<uint16_t*>(v_scales)[n0 * kTile + t0] = (uint16_t)vs[i];
+                reinterpret_cast<uint16_t*>(v_scales)[n1 * kTile + t1] = (uint16_t)(vs[i] >> 16);
+            }
+        }
+    };
+    auto stage_k = [&]() {
+#pragma unroll
+        for (int i = 0; i < KI; ++i) {
+            const uint32_t row = i * RPI + lr, f = ((row & 3u) | (row >> 1 & 4u)) & (CPR - 1);
+            *reinterpret_cast<uint4*>(keys + row * ROW + (lp ^ f) * 16) = *reinterpret_cast<const uint4*>(kr[i]);
+        }
+    };
+    const char* const key_row = keys + (8 * (r >> 2) + (r & 3u)) * ROW;
     auto load_v = [&](const Ref& f) {
-        const size_t row = g >> 1 ? f.row[1] : f.row[0], at = row * D + v_in;
+        const size_t row0 = row_of(f, 0), row1 = row_of(f, 1), row = g >> 1 ? row1 : row0, at = row * D + v_in;
         if (FULL || r * E < D) {
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
                 const char* p = static_cast<const char*>(a.v) + (at + t * D) * (Q8 ? 1 : 2);
-                if (VW == 1) vr[t][0] = *reinterpret_cast<const uint32_t*>(p);
-                else if (VW == 2) *reinterpret_cast<uint2*>(vr[t]) = *reinterpret_cast<const uint2*>(p);
+                if (VW == 1) vr[t][0] = load_once<uint32_t>(p);
+                else if (VW == 2) *reinterpret_cast<uint2*>(vr[t]) = load_once<uint2>(p);
                 else
 #pragma unroll
-                    for (int w = 0; w < VW / 4; ++w) *reinterpret_cast<uint4*>(vr[t] + 4 * w) = reinterpret_cast<const uint4*>(p)[w];
+                    for (int w = 0; w < VW / 4; ++w) *reinterpret_cast<uint4*>(vr[t] + 4 * w) = load_once<uint4>(p + 16 * w);
             }
-        }
-        if (Q8) {
-            const uint4* p = reinterpret_cast<const uint4*>(a.v_d + (row + 8 * (g & 1u)) * NBLK);
-#pragma unroll
-            for (int n = 0; n < NBLK; ++n) *reinterpret_cast<uint4*>(vs + 4 * n) = p[n];
         }
     };
     if (!FULL) {   // lanes behind the head's end load nothing
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int i = 0; i < KI; ++i)
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
-#pragma unroll
-                for (int w = 0; w < KW; ++w) kr[t][n][w] = 0;
+            for (int w = 0; w < 4; ++w) kr[i][w] = 0;
 #pragma unroll
         for (int t = 0; t < 8; ++t)
 #pragma unroll
@@ -199,24 +241,38 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_decode_kernel(Att
     if (tile < last) {
         Ref cur = locate(tile), next = cur;
         load_k(cur);
+        if (Q8) load_scales(cur);
         load_v(cur);
         if (tile + waves < last) next = locate(tile + waves);
 #pragma unroll 1
         for (; tile < last; tile += waves) {
             const bool more = tile + waves < last;
             // ---- scores
+            wave_sync();                     // the tile before has been read
+            stage_k();
+            if (Q8) stage_scales();
+            wave_sync();
+            if (more) {
+                load_k(next);
+                if (Q8) load_scales(next);
+            }
             float x[8];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 floatx4 s = {0.f, 0.f, 0.f, 0.f};
                 float folded[4] = {0.f, 0.f, 0.f, 0.f};
+                uint32_t kd[2 * NBLK];      // scales of the lane's 4 tokens
+#pragma unroll
+                for (int n = 0; Q8 && n < NBLK; ++n) *reinterpret_cast<uint2*>(kd + 2 * n) = reinterpret_cast<const uint2*>(k_scales + (8 * g + 4 * t) * NBLK)[n];
 #pragma unroll
                 for (int n = 0; n < (Q8 ? NBLK : NB); ++n) {
+                    const uint32_t f = (r & 7u) & (CPR - 1);
                     if (Q8) {
+                        const uint2 kw = *reinterpret_cast<const uint2*>(key_row + t * 4 * ROW + ((2 * n + (g >> 1)) ^ f) * 16 + 8 * (g & 1u));
                         half8 kf;
 #pragma unroll
                         for (int w = 0; w < 4; ++w) {
-                            const half2_t h = bytes_f16(kr[t][n][w / 2] ^ 0x80808080u, w & 1 ? 0x00070006u : 0x00050004u);
+                            const half2_t h = bytes_f16((w < 2 ? kw.x : kw.y) ^ 0x80808080u, w & 1 ? 0x00070006u : 0x00050004u);
                             kf[2 * w] = h[0];
                             kf[2 * w + 1] = h[1];
                         }
@@ -224,34 +280,30 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_decode_kernel(Att
                         const floatx4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[n], zero, 0, 0, 0);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const int i = (4 * t + j) * NBLK + n;
-                            folded[j] = fmaf(p[j], h2f((i & 1 ? ks[i / 2] >> 16 : ks[i / 2]) & 0xFFFFu), folded[j]);
+                            const int i = j * NBLK + n;
+                            folded[j] = fmaf(p[j], h2f((i & 1 ? kd[i / 2] >> 16 : kd[i / 2]) & 0xFFFFu), folded[j]);
                         }
                     } else {
-                        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, *reinterpret_cast<const uint4*>(kr[t][n])), qf[n], s, 0, 0, 0);
+                        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const half8*>(key_row + t * 4 * ROW + ((4 * n + g) ^ f) * 16), qf[n], s, 0, 0, 0);
                     }
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[4 * t + j] = (Q8 ? folded[j] : s[j]) * a.scale;
             }
-            const bool full = cur.token >= sp.start && cur.token + kTile <= sp.end && cur.ok[0] && cur.ok[1];
+            const bool ok0 = cur.page[0] < a.n_pages, ok1 = cur.page[1] < a.n_pages, full = cur.token >= sp.start && cur.token + kTile <= sp.end && ok0 && ok1;
+            half8 sc = {};       // scales of the lane's 8 values' block
+            if (Q8) sc = *reinterpret_cast<const half8*>(v_scales + min(r * E / 32, NBLK - 1u) * kTile + 8 * g);
             if (!full) {   // masked tokens: no weight, and values of zero, since what lies there may be no number
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const uint32_t t = cur.token + 8 * g + i;
-                    const bool ok = t >= sp.start && t < sp.end && (g >> 1 ? cur.ok[1] : cur.ok[0]);
-                    if (!ok) x[i] = -INFINITY;
+                    const bool ok = t >= sp.start && t < sp.end && (g >> 1 ? ok1 : ok0);
+                    x[i] = ok ? x[i] : -INFINITY;
+                    sc[i] = ok ? sc[i] : (half_t)0.f;
 #pragma unroll
                     for (int w = 0; w < VW; ++w) vr[i][w] = ok ? vr[i][w] : 0u;
-                    if (Q8)
-#pragma unroll
-                        for (int n = 0; n < NBLK; ++n) {
-                            const int at = i * NBLK + n;
-                            if (!ok) vs[at / 2] &= at & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-                        }
                 }
             }
-            if (more) load_k(next);
             // ---- running maximum and sum
             float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
             top = fmaxf(m, rows_max(top));
@@ -274,21 +326,6 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_decode_kernel(Att
                 lo[i] = (half_t)(p - (float)hi[i]);
             }
             // ---- values
-            half2_t sc[Q8 ? 4 : 1];
-            if (Q8) {   // the scales of the lane's block, by pairs of tokens
-                const uint32_t mine = r * E / 32;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    uint32_t v = 0;
-#pragma unroll
-                    for (int n = 0; n < NBLK; ++n) {
-                        const int i0 = 2 * w * NBLK + n, i1 = i0 + NBLK;
-                        const uint32_t pair = pick(vs[i1 / 2], vs[i0 / 2], (i1 & 1 ? 0x07060000u : 0x05040000u) | (i0 & 1 ? 0x0302u : 0x0100u));
-                        v = n == 0 || mine == (uint32_t)n ? pair : v;
-                    }
-                    sc[w] = __builtin_bit_cast(half2_t, v);
-                }
-            }
 #pragma unroll
             for (int e = 0; e < E; e += 2) {
                 half8 f0, f1;   // elements e and e + 1 of 8 tokens
@@ -297,8 +334,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_decode_kernel(Att
                     half2_t h0, h1;
                     if (Q8) {
                         const uint32_t both = pick(vr[2 * w + 1][e / 4] , vr[2 * w][e / 4], e & 2 ? 0x07030602u : 0x05010400u) ^ 0x80808080u;
-                        h0 = bytes_f16(both, 0x00050004u) * sc[w];
-                        h1 = bytes_f16(both, 0x00070006u) * sc[w];
+                        h0 = bytes_f16(both, 0x00050004u) * half2_t{sc[2 * w], sc[2 * w + 1]};
+                        h1 = bytes_f16(both, 0x00070006u) * half2_t{sc[2 * w], sc[2 * w + 1]};
                     } else {
                         h0 = __builtin_bit_cast(half2_t, pick(vr[2 * w + 1][e / 2], vr[2 * w][e / 2], 0x05040100u));
                         h1 = __builtin_bit_cast(half2_t, pick(vr[2 * w + 1][e / 2], vr[2 * w][e / 2], 0x07060302u));
@@ -321,6 +358,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_decode_kernel(Att
 
     // ---- the waves' sums: lane (r, g) holds elements 4 E g .. 4 E g + 4 E - 1 of head r
     l = rows_sum(l);
+    __syncthreads();                         // the key tiles' place is taken
     float* ml = lds;                         // [waves][16] (maximum, sum)
     float* os = lds + waves * 32;            // [waves][heads][OS]
     if (g == 0) {
@@ -362,30 +400,47 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_decode_kernel(Att
     }
 }
 
-// Joins the splits: four elements of one head a thread.
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, uint32_t n4) {
-    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-    const bool live = i < n4;
-    const uint32_t per = a.D / 4, row = (live ? i : 0) / per, d = ((live ? i : 0) - row * per) * 4, b = row / a.Hq, h = row - b * a.Hq;
+// Joins the splits of one head of one sequence: D / 4 threads by `groups` parts of the splits, each thread four elements.
+constexpr uint32_t kMostSplits = 768;
+__global__ __launch_bounds__(512) void attn_join_kernel(AttnArgs a, uint32_t groups) {
+    __shared__ float weight[kMostSplits];
+    extern __shared__ float sums[];          // [groups][D]
+    const uint32_t row = blockIdx.x, b = row / a.Hq, h = row - b * a.Hq, tid = threadIdx.x, lane = tid & 63u;
     const Span sp = span_of(a, b);
-    const uint32_t used = live ? (sp.tiles + sp.chunk - 1) / sp.chunk : 0;
+    const uint32_t used = (sp.tiles + sp.chunk - 1) / sp.chunk;
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)row * a.splits;
-    const float* po = a.part_o + (size_t)row * a.splits * a.D + d;
     const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
-    float top = sink, total = 0.f;
-    for (uint32_t s = 0; s < used; ++s) top = fmaxf(top, ml[s].x);
+    // every wave finds the maximum and the sum for itself
+    float top = sink;
+    for (uint32_t s = lane; s < used; s += 64) top = fmaxf(top, ml[s].x);
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
     const float ref = top == -INFINITY ? 0.f : top;
-    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t s = 0; s < used; ++s) {
+    float total = 0.f;
+    for (uint32_t s = lane; s < used; s += 64) {
         const float2 v = ml[s];
         const float f = __builtin_amdgcn_exp2f(v.x - ref);
         total += f * v.y;
-        sum += f * *reinterpret_cast<const floatx4*>(po + (size_t)s * a.D);
+        if (tid < 64) weight[s] = f;
     }
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x);
+    __syncthreads();
+    const uint32_t per = a.D / 4, part = tid / per, d = (tid - part * per) * 4;
+    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (part < groups) {
+        const float* po = a.part_o + (size_t)row * a.splits * a.D + d;
+#pragma unroll 4
+        for (uint32_t s = part; s < used; s += groups) sum += weight[s] * *reinterpret_cast<const floatx4*>(po + (size_t)s * a.D);
+        if (groups > 1) *reinterpret_cast<floatx4*>(sums + part * a.D + d) = sum;
+    }
+    if (groups > 1) __syncthreads();
+    if (part != 0) return;
+    for (uint32_t p = 1; p < groups; ++p) sum += *reinterpret_cast<const floatx4*>(sums + p * a.D + d);
     const float inv = 1.0f / (total + __builtin_amdgcn_exp2f(sink - ref));
     const bool none = total == 0.f;
     const float y[4] = {none ? 0.f : sum[0] * inv, none ? 0.f : sum[1] * inv, none ? 0.f : sum[2] * inv, none ? 0.f : sum[3] * inv};
-    store_rows(a, (size_t)(live ? i : 0) * 4, y, live);
+    store_rows(a, (size_t)row * a.D + d, y, true);
 }
 
 // How the lengths are split: workgroups of four waves, each at least two tiles long, until they fill the CUs three deep.
@@ -406,7 +461,7 @@ static Plan plan_of(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t max_len, uin
 template <bool Q8, int DP, int NBLK, bool FULL>
 static int launch_form(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads) {
     static LdsLimit limit;
-    const uint32_t waves = 4, lds = (waves * 32 + waves * heads * (DP + 4)) * 4;
+    const uint32_t waves = 4, keys = waves * kTile * (Q8 ? DP + 4 * NBLK : 2 * DP), sums = (waves * 32 + waves * heads * (DP + 4)) * 4, lds = keys > sums ? keys : sums;
     if (lds > kLdsDefaultLimit)
         if (int rc = raise_lds_limit(reinterpret_cast<const void*>(attn_decode_kernel<Q8, DP, NBLK, FULL>), limit, (4 * 32 + 4 * 16 * (DP + 4)) * 4)) return rc;
     hipLaunchKernelGGL((attn_decode_kernel<Q8, DP, NBLK, FULL>), grid, dim3(waves * 64), lds, as_stream(s), a);
@@ -464,11 +519,13 @@ static int attn_decode(mx_stream_t s, bool q8, const uint16_t* q, uint64_t q_str
     a.scale = scale * kLog2e;
     const uint32_t G = Hq / Hkv, heads = G < 16 ? G : 16;
     const uint64_t groups = (uint64_t)Hkv * ((G + 15) / 16);
-    MX_REQUIRE_SHAPE(groups <= 65535 && (uint64_t)B * Hq * D < (1ull << 33));
+    MX_REQUIRE_SHAPE(groups <= 65535 && (uint64_t)B * Hq < (1ull << 31));
     if (int rc = launch_attn(s, a, q8, dim3(p.splits, (uint32_t)groups, B), heads)) return rc;
     if (p.splits > 1) {
-        const uint32_t n4 = (uint32_t)((uint64_t)B * Hq * D / 4);
-        hipLaunchKernelGGL(attn_join_kernel, dim3((n4 + 255) / 256), dim3(256), 0, as_stream(s), a, n4);
+        uint32_t groups = (p.splits + 3) / 4;
+        if (groups > 512 / (D / 4)) groups = 512 / (D / 4);
+        const uint32_t threads = (groups * (D / 4) + 63) / 64 * 64;
+        hipLaunchKernelGGL(attn_join_kernel, dim3(B * Hq), dim3(threads), groups * D * 4, as_stream(s), a, groups);
         if (int rc = launch_status()) return rc;
     }
     return out_q8 && !a.out_q8 ? mx_quantize_q8_1(s, out, out_q8, (uint64_t)B * Hq * D) : MX_OK;
