@@ -5,7 +5,7 @@
 namespace mxq {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kTile = 32;   // tokens of a tile
+constexpr uint32_t kTile = 32, kWaves = 4, kLeastShare = kWaves;   // tokens of a tile, waves of a workgroup, tiles of a share at least
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -19,24 +19,79 @@ struct AttnArgs {
     const float* sinks;
     half_t* out;
     uint8_t* out_q8;
-    float *part_o, *part_ml;        // split lengths: [B][Hq][splits][D] sums and [B][Hq][splits] (maximum, sum of weights)
-    uint32_t Hq, Hkv, D, max_pages, n_pages, page_size, page_shift, window, splits, chunk_tiles;   // page_shift: log2 of a page size that is a power of two, else 32
+    float *part_o, *part_ml;        // parts of sequences: [part][Hq][D] sums and [part][Hq] (maximum, sum of weights)
+    uint32_t* parts;                // [B] (first part, how many)
+    uint32_t B, Hq, Hkv, D, max_pages, n_pages, page_size, page_shift, window, shares;   // page_shift: log2 of a page size that is a power of two, else 32
     float scale;                    // times log2(e)
 };
 
-// The tokens of sequence b: [start, end), in tiles of 32 that begin at multiples of 32, dealt in chunks of `chunk` tiles to the workgroups of the sequence.
+// The tokens of a sequence: [start, end), in tiles of 32 that begin at multiples of 32.
 struct Span {
-    uint32_t start, end, tile0, tiles, chunk;
+    uint32_t start, end, tile0, tiles;
 };
-__device__ __forceinline__ Span span_of(const AttnArgs& a, uint32_t b) {
-    const int32_t raw = a.lens[b];
+__device__ __forceinline__ Span span_of(const AttnArgs& a, int32_t len) {
     const uint64_t capacity = (uint64_t)a.max_pages * a.page_size;
     Span s;
-    s.end = raw <= 0 ? 0u : (uint32_t)min((uint64_t)raw, capacity);
+    s.end = len <= 0 ? 0u : (uint32_t)min((uint64_t)len, capacity);
     s.start = a.window && s.end > a.window ? s.end - a.window : 0u;
     s.tile0 = s.start / kTile;
     s.tiles = s.end ? (s.end - 1) / kTile + 1 - s.tile0 : 0u;
-    s.chunk = max(a.chunk_tiles, (s.tiles + a.splits - 1) / a.splits);   // a sequence longer than was expected still fits the splits
+    return s;
+}
+
+// Sum over the lanes up to this one.
+__device__ __forceinline__ uint32_t lanes_upto(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, true);    // row_shr:1, 2, 4, 8 within 16 lanes
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);   // the last lane of rows 0 and 2 to rows 1 and 3
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);   // lane 31 to rows 2 and 3
+    return v;
+}
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+
+// Equal shares: the tiles of all sequences in a row, cut into `shares` ranges of `per` tiles (at least kLeastShare).  A workgroup's range may end one sequence
+// and begin another; its part of sequence b has the number share + b, which no other part has, and the parts of one sequence are consecutive.
+struct Share {
+    uint32_t per, left;      // tiles of a share; of this one
+    uint32_t b, from;        // the sequence that it begins in, and at which of its tiles
+    int32_t len;             // that sequence's entry
+};
+__device__ __forceinline__ Share share_of(const AttnArgs& a, uint32_t share, uint32_t lane) {
+    uint32_t total = 0, upto = 0, own = 0;
+    int32_t len = 0;
+    for (uint32_t i0 = 0; i0 < a.B; i0 += 64) {
+        len = i0 + lane < a.B ? a.lens[i0 + lane] : 0;
+        own = span_of(a, len).tiles;
+        if (own == 0 && i0 + lane < a.B && share == 0 && blockIdx.y == 0)
+            *reinterpret_cast<uint2*>(a.parts + 2 * (i0 + lane)) = make_uint2(0, 0);   // no part: zeros, whatever the sinks
+        upto = lanes_upto(own);
+        total += lane_value(upto, 63);
+    }
+    Share s;
+    s.per = max(kLeastShare, (total + a.shares - 1) / a.shares);
+    const uint64_t at = (uint64_t)share * s.per;
+    s.left = at < total ? min(s.per, total - (uint32_t)at) : 0u;
+    s.b = s.from = 0;
+    s.len = 0;
+    uint32_t before = 0;
+    for (uint32_t i0 = 0; s.left && i0 < a.B; i0 += 64) {
+        if (a.B > 64) {      // up to 64 sequences: as they were
+            len = i0 + lane < a.B ? a.lens[i0 + lane] : 0;
+            own = span_of(a, len).tiles;
+            upto = lanes_upto(own);
+        }
+        const uint64_t hit = __ballot(before + upto > (uint32_t)at);
+        if (hit) {
+            const int first = __ffsll((unsigned long long)hit) - 1;
+            s.b = i0 + first;
+            s.from = (uint32_t)at - before - lane_value(upto - own, first);
+            s.len = (int32_t)lane_value((uint32_t)len, first);
+            break;
+        }
+        before += lane_value(upto, 63);
+    }
     return s;
 }
 
@@ -54,14 +109,10 @@ __device__ __forceinline__ void store_rows(const AttnArgs& a, size_t at, const f
 }
 
 // The cache is read once: its lines need not stay.
-#ifndef NT
-#define NT 1
-#endif
 template <class T>
 __device__ __forceinline__ T load_once(const void* p) {
     typedef uint32_t vec __attribute__((ext_vector_type(sizeof(T) / 4)));
-    if (NT) return __builtin_bit_cast(T, __builtin_nontemporal_load(reinterpret_cast<const vec*>(p)));
-    return __builtin_bit_cast(T, *reinterpret_cast<const vec*>(p));
+    return __builtin_bit_cast(T, __builtin_nontemporal_load(reinterpret_cast<const vec*>(p)));
 }
 
 // Largest / sum over the four 16-lane rows of a wave, in every lane: permlane swaps bring the other rows' values.
@@ -102,36 +153,53 @@ __device__ __forceinline__ half2_t bytes_f16(uint32_t w, uint32_t sel) {
 // nothing goes through LDS before the end.  The weights are two fp16 parts, the second what the first's rounding left (2^-21 of it), so only the result's rounding to
 // fp16 is felt.  Q8_0: keys are exact as fp16 integers and their scales are folded into the fp32 products of each block; values are rounded to fp16 as they are dequantised.
 template <bool Q8, int DP, int NBLK, bool FULL>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void attn_decode_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 ? 3 : 2) void attn_decode_kernel(AttnArgs a) {
     constexpr int E = DP / 16, NB = DP / 32;
-    constexpr int VW = Q8 ? E / 4 : E / 2;                     // dwords of a lane's part of one value row
+    constexpr int VW = Q8 ? E / 4 : E / 2;                     // dwords of a lane's part of one value row, in VP pieces (wide fp16 heads: 8 of each half)
+    constexpr int VP = !Q8 && E == 16 ? 2 : 1;
     constexpr int CPR = DP / (Q8 ? 16 : 8), RPI = 64 / CPR, KI = kTile / RPI;   // 16-byte pieces of a key row, rows of a load, loads of a tile
     constexpr int OS = DP + 4;                                  // LDS row stride of the waves' sums
+    constexpr uint32_t ROW = CPR * 16;
+    constexpr uint32_t SCALES = Q8 ? kTile * NBLK * 2 : 0, WAVE = kTile * ROW + 2 * SCALES;   // LDS of a wave: keys, their scales [token][block], the values' [block][token]
     extern __shared__ float lds[];
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, r = lane & 15u, g = lane >> 4;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15u, g = lane >> 4;
     const uint32_t G = a.Hq / a.Hkv, tiles_of_heads = (G + 15) / 16;
-    const uint32_t hk = blockIdx.y / tiles_of_heads, head0 = (blockIdx.y - hk * tiles_of_heads) * 16, heads = min(16u, G - head0), b = blockIdx.z;
+    const uint32_t hk = blockIdx.y / tiles_of_heads, head0 = (blockIdx.y - hk * tiles_of_heads) * 16, heads = min(16u, G - head0);
     const uint32_t D = FULL ? (Q8 ? NBLK * 32 : DP) : Q8 ? NBLK * 32 : a.D;
-    const Span sp = span_of(a, b);
-    const uint32_t first = blockIdx.x * sp.chunk, last = min(first + sp.chunk, sp.tiles);
+    const bool shared = a.shares != 0;
+    const uint32_t share = blockIdx.x;
+    Share sh = {1, 1, blockIdx.x, 0, 0};
+    if (shared) sh = share_of(a, share, lane);
+    else sh.len = a.lens[sh.b];
+    uint32_t b = sh.b, first = sh.from, left = sh.left;
+    int32_t len = __builtin_amdgcn_readfirstlane(sh.len);
+    for (; left; len = __builtin_amdgcn_readfirstlane(left ? a.lens[b + 1] : 0), ++b) {
+    const Span sp = span_of(a, len);
+    const uint32_t last = shared ? min(sp.tiles, first + left) : sp.tiles;
+    const bool whole = first == 0 && last == sp.tiles;     // the result itself, not a part of it
     const size_t out0 = ((size_t)b * a.Hq + hk * G + head0) * D;
-    if (first >= last) {
-        if (blockIdx.x == 0) {   // no tokens at all: zeros, whatever the sinks (several splits: the joining kernel sees to it)
-            if (a.splits == 1)
-                for (uint32_t i = threadIdx.x * 4; i < (heads * D + 1023) / 1024 * 1024; i += blockDim.x * 4) {
-                    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-                    store_rows(a, out0 + i, zero, i < heads * D);
-                }
+    if (shared) {
+        if (sp.tiles == 0) continue;
+        if (first == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+            // the first tile is tile per - left of the share; the last share may be shorter, but what begins in it ends in it
+            *reinterpret_cast<uint2*>(a.parts + 2 * b) = make_uint2(share + b, (sh.per - left + sp.tiles - 1) / sh.per + 1);
         }
-        return;
+        left -= last - first;
+    } else {
+        left = 0;
     }
 
-    half8 qf[NB];
+    // queries: in registers, or (wide heads, whose other operands fill them) in LDS behind the waves' tiles, the same for every wave
+    constexpr bool QL = DP > 128;
+    half8 qf[QL ? 1 : NB];
+    half8* const ql = reinterpret_cast<half8*>(reinterpret_cast<char*>(lds) + kWaves * WAVE) + lane;
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-        qf[n] = half8{};
+        half8 q = {};
         const uint32_t d = n * 32 + g * 8;
-        if (r < heads && d < D) qf[n] = *reinterpret_cast<const half8*>(a.q + b * a.q_stride + (size_t)(hk * G + head0 + r) * D + d);
+        if (r < heads && d < D) q = *reinterpret_cast<const half8*>(a.q + b * a.q_stride + (size_t)(hk * G + head0 + r) * D + d);
+        if (QL) ql[n * 64] = q;        // every wave writes the same values
+        else qf[QL ? 0 : n] = q;
     }
 
     typedef const __attribute__((address_space(4))) int32_t* table_t;
@@ -159,12 +227,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void attn_decode_kernel(Att
     uint32_t ks[SL], vs[SL];
     // keys: whole rows by CPR lanes each, into the wave's LDS tile, where a row's pieces lie permuted (piece p at p ^ f, f = row % 4 + 4 (row / 8 % 2), which
     // is lane % 8 of its reader), so that the 16 lanes that read the same piece of 16 rows meet different banks
-    constexpr uint32_t ROW = CPR * 16;
-    constexpr uint32_t SCALES = Q8 ? kTile * NBLK * 2 : 0, WAVE = kTile * ROW + 2 * SCALES;   // LDS of a wave: keys, their scales [token][block], the values' [block][token]
     char* const keys = reinterpret_cast<char*>(lds) + wave * WAVE;
     half_t* const k_scales = reinterpret_cast<half_t*>(keys + kTile * ROW);
     half_t* const v_scales = reinterpret_cast<half_t*>(keys + kTile * ROW + SCALES);
-    const uint32_t lr = lane / CPR, lp = lane % CPR, v_in = 8 * (g & 1u) * D + r * E;
+    const uint32_t lr = lane / CPR, lp = lane % CPR, v_in = 8 * (g & 1u) * D + r * (E / VP);
     auto load_k = [&](const Ref& f) {
         const size_t row0 = row_of(f, 0), row1 = row_of(f, 1);
         if (FULL || lp * 16 < D * (Q8 ? 1 : 2)) {
@@ -208,18 +274,17 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void attn_decode_kernel(Att
     };
     const char* const key_row = keys + (8 * (r >> 2) + (r & 3u)) * ROW;
     auto load_v = [&](const Ref& f) {
-        const size_t row0 = row_of(f, 0), row1 = row_of(f, 1), row = g >> 1 ? row1 : row0, at = row * D + v_in;
-        if (FULL || r * E < D) {
+        const size_t row0 = row_of(f, 0), row1 = row_of(f, 1), at = (g >> 1 ? row1 : row0) * D + v_in;
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const char* p = static_cast<const char*>(a.v) + (at + t * D) * (Q8 ? 1 : 2);
+        for (int t = 0; t < 8; ++t)
+#pragma unroll
+            for (int w = 0; w < VP; ++w) {
+                if (!FULL && w * 128 + r * (E / VP) >= D) continue;
+                const char* p = static_cast<const char*>(a.v) + (at + t * D + w * 128) * (Q8 ? 1 : 2);
                 if (VW == 1) vr[t][0] = load_once<uint32_t>(p);
                 else if (VW == 2) *reinterpret_cast<uint2*>(vr[t]) = load_once<uint2>(p);
-                else
-#pragma unroll
-                    for (int w = 0; w < VW / 4; ++w) *reinterpret_cast<uint4*>(vr[t] + 4 * w) = load_once<uint4>(p + 16 * w);
+                else *reinterpret_cast<uint4*>(vr[t] + 4 * w) = load_once<uint4>(p);
             }
-        }
     };
     if (!FULL) {   // lanes behind the head's end load nothing
 #pragma unroll
@@ -243,10 +308,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void attn_decode_kernel(Att
         load_k(cur);
         if (Q8) load_scales(cur);
         load_v(cur);
-        if (tile + waves < last) next = locate(tile + waves);
+        if (tile + kWaves < last) next = locate(tile + kWaves);
 #pragma unroll 1
-        for (; tile < last; tile += waves) {
-            const bool more = tile + waves < last;
+        for (; tile < last; tile += kWaves) {
+            const bool more = tile + kWaves < last;
             // ---- scores
             wave_sync();                     // the tile before has been read
             stage_k();
@@ -257,16 +322,18 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void attn_decode_kernel(Att
                 if (Q8) load_scales(next);
             }
             float x[8];
+            floatx4 score[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            uint32_t kd[2][2 * NBLK];       // scales of the lane's 4 tokens of either product
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                floatx4 s = {0.f, 0.f, 0.f, 0.f};
-                float folded[4] = {0.f, 0.f, 0.f, 0.f};
-                uint32_t kd[2 * NBLK];      // scales of the lane's 4 tokens
+            for (int t = 0; Q8 && t < 2; ++t)
 #pragma unroll
-                for (int n = 0; Q8 && n < NBLK; ++n) *reinterpret_cast<uint2*>(kd + 2 * n) = reinterpret_cast<const uint2*>(k_scales + (8 * g + 4 * t) * NBLK)[n];
+                for (int n = 0; n < NBLK; ++n) *reinterpret_cast<uint2*>(kd[t] + 2 * n) = reinterpret_cast<const uint2*>(k_scales + (8 * g + 4 * t) * NBLK)[n];
 #pragma unroll
-                for (int n = 0; n < (Q8 ? NBLK : NB); ++n) {
-                    const uint32_t f = (r & 7u) & (CPR - 1);
+            for (int n = 0; n < (Q8 ? NBLK : NB); ++n) {
+                const uint32_t f = (r & 7u) & (CPR - 1);
+                const half8 q = QL ? ql[n * 64] : qf[QL ? 0 : n];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
                     if (Q8) {
                         const uint2 kw = *reinterpret_cast<const uint2*>(key_row + t * 4 * ROW + ((2 * n + (g >> 1)) ^ f) * 16 + 8 * (g & 1u));
                         half8 kf;
@@ -277,19 +344,19 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void attn_decode_kernel(Att
                             kf[2 * w + 1] = h[1];
                         }
                         const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
-                        const floatx4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[n], zero, 0, 0, 0);
+                        const floatx4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q, zero, 0, 0, 0);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const int i = j * NBLK + n;
-                            folded[j] = fmaf(p[j], h2f((i & 1 ? kd[i / 2] >> 16 : kd[i / 2]) & 0xFFFFu), folded[j]);
+                            score[t][j] = fmaf(p[j], h2f((i & 1 ? kd[t][i / 2] >> 16 : kd[t][i / 2]) & 0xFFFFu), score[t][j]);
                         }
                     } else {
-                        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const half8*>(key_row + t * 4 * ROW + ((4 * n + g) ^ f) * 16), qf[n], s, 0, 0, 0);
+                        score[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const half8*>(key_row + t * 4 * ROW + ((4 * n + g) ^ f) * 16), q, score[t], 0, 0, 0);
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[4 * t + j] = (Q8 ? folded[j] : s[j]) * a.scale;
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = score[i / 4][i % 4] * a.scale;
             const bool ok0 = cur.page[0] < a.n_pages, ok1 = cur.page[1] < a.n_pages, full = cur.token >= sp.start && cur.token + kTile <= sp.end && ok0 && ok1;
             half8 sc = {};       // scales of the lane's 8 values' block
             if (Q8) sc = *reinterpret_cast<const half8*>(v_scales + min(r * E / 32, NBLK - 1u) * kTile + 8 * g);
@@ -351,7 +418,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void attn_decode_kernel(Att
             if (more) {
                 load_v(next);
                 cur = next;
-                if (tile + 2 * waves < last) next = locate(tile + 2 * waves);
+                if (tile + 2 * kWaves < last) next = locate(tile + 2 * kWaves);
             }
         }
     }
@@ -360,78 +427,91 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 3) void attn_decode_kernel(Att
     l = rows_sum(l);
     __syncthreads();                         // the key tiles' place is taken
     float* ml = lds;                         // [waves][16] (maximum, sum)
-    float* os = lds + waves * 32;            // [waves][heads][OS]
+    float* os = lds + kWaves * 32;            // [waves][heads][OS]
     if (g == 0) {
         ml[(wave * 16 + r) * 2] = m;
         ml[(wave * 16 + r) * 2 + 1] = l;
     }
     if (r < heads) {
-        float* row = os + (wave * heads + r) * OS + 4 * E * g;
+        float* row = os + (wave * heads + r) * OS + 4 * (E / VP) * g;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int e = 0; e < E; e += 4) *reinterpret_cast<floatx4*>(row + E * j + e) = floatx4{o[e][j], o[e + 1][j], o[e + 2][j], o[e + 3][j]};
+            for (int e = 0; e < E; e += 4)
+                *reinterpret_cast<floatx4*>(row + (E / VP) * j + e / (E / VP) * 128 + e % (E / VP)) = floatx4{o[e][j], o[e + 1][j], o[e + 2][j], o[e + 3][j]};
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x * 4; i < (heads * D + 1023) / 1024 * 1024; i += blockDim.x * 4) {
+    for (uint32_t i = threadIdx.x * 4; i < (heads * D + kWaves * 256 - 1) / (kWaves * 256) * (kWaves * 256); i += kWaves * 256) {
         const bool live = i < heads * D;
         const uint32_t h = live ? i / D : 0, d = live ? i - h * D : 0;
         const uint32_t hq = hk * G + head0 + h;
-        const float sink = a.splits == 1 && a.sinks ? a.sinks[hq] * kLog2e : -INFINITY;
+        const float sink = whole && a.sinks ? a.sinks[hq] * kLog2e : -INFINITY;
         float top = sink, total = 0.f;
-        for (uint32_t w = 0; w < waves; ++w) top = fmaxf(top, ml[(w * 16 + h) * 2]);
+        for (uint32_t w = 0; w < kWaves; ++w) top = fmaxf(top, ml[(w * 16 + h) * 2]);
         const float ref = top == -INFINITY ? 0.f : top;
         floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-        for (uint32_t w = 0; w < waves; ++w) {
+        for (uint32_t w = 0; w < kWaves; ++w) {
             const float f = __builtin_amdgcn_exp2f(ml[(w * 16 + h) * 2] - ref);
             total += f * ml[(w * 16 + h) * 2 + 1];
             sum += f * *reinterpret_cast<const floatx4*>(os + (w * heads + h) * OS + d);
         }
-        if (a.splits == 1) {
+        if (whole) {
             const float all = total + __builtin_amdgcn_exp2f(sink - ref), inv = 1.0f / all;
             const bool none = total == 0.f;
             const float y[4] = {none ? 0.f : sum[0] * inv, none ? 0.f : sum[1] * inv, none ? 0.f : sum[2] * inv, none ? 0.f : sum[3] * inv};
             store_rows(a, out0 + i, y, live);
         } else if (live) {
-            const size_t at = ((size_t)b * a.Hq + hq) * a.splits + blockIdx.x;
+            const size_t at = (size_t)(share + b) * a.Hq + hq;
             *reinterpret_cast<floatx4*>(a.part_o + at * D + d) = sum;
             if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(top, total);
         }
     }
+    first = 0;
+    if (left) __syncthreads();               // the sums have been read
+    }
 }
 
-// Joins the splits of one head of one sequence: D / 4 threads by `groups` parts of the splits, each thread four elements.
-constexpr uint32_t kMostSplits = 768;
+// Joins the parts of one head of one sequence: D / 4 threads for each of `groups` groups of parts, each thread four elements.
 __global__ __launch_bounds__(512) void attn_join_kernel(AttnArgs a, uint32_t groups) {
-    __shared__ float weight[kMostSplits];
     extern __shared__ float sums[];          // [groups][D]
     const uint32_t row = blockIdx.x, b = row / a.Hq, h = row - b * a.Hq, tid = threadIdx.x, lane = tid & 63u;
-    const Span sp = span_of(a, b);
-    const uint32_t used = (sp.tiles + sp.chunk - 1) / sp.chunk;
-    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)row * a.splits;
+    const uint32_t per = a.D / 4, part = tid / per, d = (tid - part * per) * 4;
+    const uint2 parts = *reinterpret_cast<const uint2*>(a.parts + 2 * b);
+    const uint32_t first = parts.x, n = parts.y;
+    if (n == 1) return;                      // the result is there
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)first * a.Hq + h;
+    const float* po = a.part_o + ((size_t)first * a.Hq + h) * a.D + d;
     const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
+    // the first sums are requested before their weights are known
+    constexpr uint32_t kAhead = 4;
+    floatx4 ahead[kAhead];
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i) {
+        const uint32_t s = part + i * groups;
+        ahead[i] = part < groups && s < n ? *reinterpret_cast<const floatx4*>(po + (size_t)s * a.Hq * a.D) : floatx4{0.f, 0.f, 0.f, 0.f};
+    }
     // every wave finds the maximum and the sum for itself
     float top = sink;
-    for (uint32_t s = lane; s < used; s += 64) top = fmaxf(top, ml[s].x);
+    for (uint32_t s = lane; s < n; s += 64) top = fmaxf(top, ml[(size_t)s * a.Hq].x);
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
     const float ref = top == -INFINITY ? 0.f : top;
     float total = 0.f;
-    for (uint32_t s = lane; s < used; s += 64) {
-        const float2 v = ml[s];
-        const float f = __builtin_amdgcn_exp2f(v.x - ref);
-        total += f * v.y;
-        if (tid < 64) weight[s] = f;
+    for (uint32_t s = lane; s < n; s += 64) {
+        const float2 v = ml[(size_t)s * a.Hq];
+        total += __builtin_amdgcn_exp2f(v.x - ref) * v.y;
     }
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x);
-    __syncthreads();
-    const uint32_t per = a.D / 4, part = tid / per, d = (tid - part * per) * 4;
     floatx4 sum = {0.f, 0.f, 0.f, 0.f};
     if (part < groups) {
-        const float* po = a.part_o + (size_t)row * a.splits * a.D + d;
-#pragma unroll 4
-        for (uint32_t s = part; s < used; s += groups) sum += weight[s] * *reinterpret_cast<const floatx4*>(po + (size_t)s * a.D);
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            const uint32_t s = part + i * groups;
+            if (s < n) sum += __builtin_amdgcn_exp2f(ml[(size_t)s * a.Hq].x - ref) * ahead[i];
+        }
+        for (uint32_t s = part + kAhead * groups; s < n; s += groups)
+            sum += __builtin_amdgcn_exp2f(ml[(size_t)s * a.Hq].x - ref) * *reinterpret_cast<const floatx4*>(po + (size_t)s * a.Hq * a.D);
         if (groups > 1) *reinterpret_cast<floatx4*>(sums + part * a.D + d) = sum;
     }
     if (groups > 1) __syncthreads();
@@ -443,28 +523,36 @@ __global__ __launch_bounds__(512) void attn_join_kernel(AttnArgs a, uint32_t gro
     store_rows(a, (size_t)row * a.D + d, y, true);
 }
 
-// How the lengths are split: workgroups of four waves, each at least two tiles long, until they fill the CUs three deep.
+// Short sequences take a workgroup each.  Otherwise the tiles are shared equally by as many workgroups as stream the cache fastest, two for each CU (one where heads are
+// wide): 64 x 8192 fp16 tokens of 8 heads of 128, us by workgroups: 256 318, 512 321, 768 330, 2048 332; Q8_0 205, 176, 183 (768), ...; one Q8_0 sequence of 131071
+// 59, 54, 57, 66.  A share is two tiles a wave at least, but one where that leaves most CUs idle (one Q8_0 sequence of 2000: 11.1 -> 9.8 us; of 8000: 11.9, 12.8).
 struct Plan {
-    uint32_t splits, chunk_tiles;
+    uint32_t shares;         // 0: a workgroup for each sequence and group of heads
+    uint64_t ws_bytes;
 };
-static Plan plan_of(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t max_len, uint32_t window) {
+constexpr uint32_t kDirectTiles = 4 * kWaves;
+static Plan plan_of(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t max_len, uint32_t window) {
     const uint32_t span = window && window < max_len ? window : max_len;
-    const uint32_t tiles = span / kTile + (window && window < max_len ? 2 : 1);
-    const uint64_t base = (uint64_t)B * Hkv * ((Hq / Hkv + 15) / 16);
-    const uint64_t want = (768 + base - 1) / base;
-    uint32_t chunk = (uint32_t)((tiles + want - 1) / want);
-    if (chunk < 8) chunk = 8;
-    const uint32_t splits = (tiles + chunk - 1) / chunk;
-    return {splits, chunk};
+    const uint64_t tiles = span / kTile + (window && window < max_len ? 2 : 1), all = B * tiles;
+    const uint64_t groups = (uint64_t)Hkv * ((Hq / Hkv + 15) / 16);
+    if (tiles <= kDirectTiles) return {0, 0};
+    auto up = [](uint64_t x, uint64_t y) { return (x + y - 1) / y; };
+    uint64_t most = up(all, kLeastShare);
+    if (most * groups > 128) most = up(all, 2 * kLeastShare) > up(128, groups) ? up(all, 2 * kLeastShare) : up(128, groups);
+    uint64_t shares = up(D > 128 ? 256 : 512, groups);
+    if (shares > most) shares = most;
+    return {(uint32_t)shares, (shares + B) * Hq * (D + 2) * 4 + (uint64_t)B * 8};
 }
 
 template <bool Q8, int DP, int NBLK, bool FULL>
 static int launch_form(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads) {
     static LdsLimit limit;
-    const uint32_t waves = 4, keys = waves * kTile * (Q8 ? DP + 4 * NBLK : 2 * DP), sums = (waves * 32 + waves * heads * (DP + 4)) * 4, lds = keys > sums ? keys : sums;
+    // keys, their scales and wide heads' queries; behind them the waves' sums, in the same place
+    constexpr uint32_t keys = kWaves * kTile * (Q8 ? DP + 4 * NBLK : 2 * DP) + (DP > 128 ? DP * 32 : 0), most = kWaves * (32 + 16 * (DP + 4)) * 4;
+    const uint32_t sums = kWaves * (32 + heads * (DP + 4)) * 4, lds = keys > sums ? keys : sums;
     if (lds > kLdsDefaultLimit)
-        if (int rc = raise_lds_limit(reinterpret_cast<const void*>(attn_decode_kernel<Q8, DP, NBLK, FULL>), limit, (4 * 32 + 4 * 16 * (DP + 4)) * 4)) return rc;
-    hipLaunchKernelGGL((attn_decode_kernel<Q8, DP, NBLK, FULL>), grid, dim3(waves * 64), lds, as_stream(s), a);
+        if (int rc = raise_lds_limit(reinterpret_cast<const void*>(attn_decode_kernel<Q8, DP, NBLK, FULL>), limit, keys > most ? keys : most)) return rc;
+    hipLaunchKernelGGL((attn_decode_kernel<Q8, DP, NBLK, FULL>), grid, dim3(kWaves * 64), lds, as_stream(s), a);
     return launch_status();
 }
 static int launch_attn(mx_stream_t s, const AttnArgs& a, bool q8, dim3 grid, uint32_t heads) {
@@ -495,16 +583,17 @@ static int attn_decode(mx_stream_t s, bool q8, const uint16_t* q, uint64_t q_str
     MX_REQUIRE_SHAPE(B > 0 && B <= 65535 && Hkv > 0 && Hkv <= 65535 && Hq > 0 && Hq <= 65535 && Hq % Hkv == 0);
     MX_REQUIRE_SHAPE(D > 0 && D <= 256 && D % (q8 ? 32 : 16) == 0 && q_stride % 8 == 0 && q_stride >= (uint64_t)Hq * D);
     MX_REQUIRE_SHAPE(n_pages > 0 && page_size > 0 && page_size % 16 == 0 && (uint64_t)n_pages * page_size < (1ull << 31) && max_pages > 0);
+    const uint64_t tiles = (uint64_t)max_pages * page_size / kTile + 1;
+    MX_REQUIRE_SHAPE(B * (tiles < (1u << 26) ? tiles : 1u << 26) < (1ull << 31));   // tiles of all sequences, counted in 32 bits
     MX_REQUIRE_SHAPE(!out_q8 || (uint64_t)Hq * D % 32 == 0);
     MX_REQUIRE_ALIGN(q, 16); MX_REQUIRE_ALIGN(k, 16); MX_REQUIRE_ALIGN(v, 16); MX_REQUIRE_ALIGN(out, 16); MX_REQUIRE_ALIGN(out_q8, 8);
     MX_REQUIRE_ALIGN(page_table, 4); MX_REQUIRE_ALIGN(seq_lens, 4); MX_REQUIRE_ALIGN(sinks, 4);
     if (q8) { MX_REQUIRE_ALIGN(k_d, 16); MX_REQUIRE_ALIGN(v_d, 16); }
-    const Plan p = plan_of(B, Hq, Hkv, max_len, window);
-    const uint64_t parts = p.splits > 1 ? (uint64_t)B * Hq * p.splits : 0, need = parts * (D + 2) * 4;
-    if (need) {
+    const Plan p = plan_of(B, Hq, Hkv, D, max_len, window);
+    if (p.shares) {
         MX_REQUIRE_PTR(ws);
         MX_REQUIRE_ALIGN(ws, 16);
-        if (ws_bytes < need) return MX_ERR_WORKSPACE;
+        if (ws_bytes < p.ws_bytes) return MX_ERR_WORKSPACE;
     }
     AttnArgs a = {};
     a.q = reinterpret_cast<const half_t*>(q); a.q_stride = q_stride;
@@ -512,17 +601,23 @@ static int attn_decode(mx_stream_t s, bool q8, const uint16_t* q, uint64_t q_str
     a.table = page_table; a.lens = seq_lens; a.sinks = sinks;
     a.out = reinterpret_cast<half_t*>(out);
     a.out_q8 = D % 32 == 0 ? static_cast<uint8_t*>(out_q8) : nullptr;   // heads of half a block: the quantizer, after the rows
-    a.part_o = static_cast<float*>(ws); a.part_ml = static_cast<float*>(ws) + parts * D;
-    a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.max_pages = max_pages; a.n_pages = n_pages; a.page_size = page_size;
+    if (p.shares) {
+        const uint64_t rows = ((uint64_t)p.shares + B) * Hq;
+        a.part_o = static_cast<float*>(ws);
+        a.part_ml = a.part_o + rows * D;
+        a.parts = reinterpret_cast<uint32_t*>(a.part_ml + rows * 2);
+    }
+    a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.max_pages = max_pages; a.n_pages = n_pages; a.page_size = page_size;
     a.page_shift = (page_size & (page_size - 1)) == 0 ? (uint32_t)__builtin_ctz(page_size) : 32u;
-    a.window = window; a.splits = p.splits; a.chunk_tiles = p.chunk_tiles;
+    a.window = window; a.shares = p.shares;
     a.scale = scale * kLog2e;
     const uint32_t G = Hq / Hkv, heads = G < 16 ? G : 16;
     const uint64_t groups = (uint64_t)Hkv * ((G + 15) / 16);
     MX_REQUIRE_SHAPE(groups <= 65535 && (uint64_t)B * Hq < (1ull << 31));
-    if (int rc = launch_attn(s, a, q8, dim3(p.splits, (uint32_t)groups, B), heads)) return rc;
-    if (p.splits > 1) {
-        uint32_t groups = (p.splits + 3) / 4;
+    if (int rc = launch_attn(s, a, q8, dim3(p.shares ? p.shares : B, (uint32_t)groups), heads)) return rc;
+    if (p.shares) {
+        // groups of parts: four parts a thread where a sequence has its even portion of them
+        uint32_t groups = (p.shares / B + 4) / 4;
         if (groups > 512 / (D / 4)) groups = 512 / (D / 4);
         const uint32_t threads = (groups * (D / 4) + 63) / 64 * 64;
         hipLaunchKernelGGL(attn_join_kernel, dim3(B * Hq), dim3(threads), groups * D * 4, as_stream(s), a, groups);
@@ -540,8 +635,7 @@ extern "C" {
 int mx_attn_decode_ws_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t max_len, uint32_t window, uint64_t* bytes) {
     MX_REQUIRE_PTR(bytes);
     MX_REQUIRE_SHAPE(B > 0 && B <= 65535 && Hkv > 0 && Hq > 0 && Hq <= 65535 && Hq % Hkv == 0 && D > 0 && D <= 256 && D % 16 == 0);
-    const Plan p = plan_of(B, Hq, Hkv, max_len, window);
-    *bytes = p.splits > 1 ? (uint64_t)B * Hq * p.splits * (D + 2) * 4 : 0;
+    *bytes = plan_of(B, Hq, Hkv, D, max_len, window).ws_bytes;
     return MX_OK;
 }
 

@@ -793,36 +793,47 @@ def _want(ok, what):
         raise ValueError(what)
 
 
-def _dev(t, dtype, what):
-    """Address of a contiguous tensor of this type on the current device."""
-    if t is None or t.dtype != dtype or not t.is_contiguous() or not t.is_cuda or t.get_device() != torch.cuda.current_device():
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+# These run before every launch of a decode step, so they ask for no more than they need: rope() into a given y takes 6.5 us, of
+# which the launch is 4.
+def _dev(t, dtype, dev, what):
+    """Address of a contiguous tensor of this type on the current device, whose number is `dev`."""
+    if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
         raise ValueError("%s must be a contiguous %s tensor on the current device" % (what, dtype))
     return t.data_ptr()
 
 
-def _rows(t, what):
+def _rows(t, shape, dev, what):
     """(address, elements from a row to the next) of fp16 rows [T, heads, D] whose heads lie side by side."""
-    if t.dtype != torch.float16 or t.dim() != 3 or not t.is_cuda or t.get_device() != torch.cuda.current_device():
-        raise ValueError("%s must be a fp16 tensor [T, heads, D] on the current device" % what)
-    T, H, D = t.shape
-    st = t.stride()
-    if (st[2] != 1 and D > 1) or (st[1] != D and H > 1):
+    if t.dtype is not torch.float16 or t.get_device() != dev or t.shape != shape:
+        raise ValueError("%s must be a fp16 tensor [%d, %d, %d] on the current device" % ((what,) + tuple(shape)))
+    T, H, D = shape
+    row, head, one = t.stride()
+    if (one != 1 and D > 1) or (head != D and H > 1):
         raise ValueError("%s: the heads of a row must lie side by side" % what)
-    return t.data_ptr(), st[0] if T > 1 else max(st[0], H * D + -(H * D) % 8)
+    return t.data_ptr(), row if T > 1 else max(row, H * D) + -max(row, H * D) % 8
 
 
-def _cache(cache):
-    """(format, plane addresses, pages, heads, page size, D) of a cache: (k, v) fp16 or (k_qs, k_d, v_qs, v_d) Q8_0 planes."""
-    n = len(cache)
-    _want(n in (2, 4), "a cache is (k, v) or (k_qs, k_d, v_qs, v_d)")
+def _new_rows(t):
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _cache(cache, dev):
+    """(plane addresses, shape) of a cache: (k, v) fp16 or (k_qs, k_d, v_qs, v_d) Q8_0 planes."""
     shape = cache[0].shape
-    _want(len(shape) == 4, "cache planes are [pages, heads, page size, D]")
-    if n == 2:
-        _want(cache[1].shape == shape, "the planes of a cache have one shape")
-        return "f16", (_dev(cache[0], torch.float16, "k"), _dev(cache[1], torch.float16, "v")), shape
+    if len(cache) == 2:
+        k, v = cache
+        if v.shape != shape or len(shape) != 4:
+            raise ValueError("the planes of a cache are [pages, heads, page size, D], both of one shape")
+        return (_dev(k, torch.float16, dev, "k"), _dev(v, torch.float16, dev, "v")), shape
+    _want(len(cache) == 4 and len(shape) == 4, "a cache is (k, v) or (k_qs, k_d, v_qs, v_d), planes [pages, heads, page size, D]")
     scales = shape[:3] + (shape[3] // 32,)
-    _want(cache[2].shape == shape and cache[1].shape == scales and cache[3].shape == scales, "the planes of a cache have one shape, its scales one for each 32")
-    return "q8_0", (_dev(cache[0], torch.int8, "k_qs"), _dev(cache[1], torch.float16, "k_d"), _dev(cache[2], torch.int8, "v_qs"), _dev(cache[3], torch.float16, "v_d")), shape
+    if cache[2].shape != shape or cache[1].shape != scales or cache[3].shape != scales:
+        raise ValueError("the planes of a cache have one shape, its scales one for each 32")
+    return (_dev(cache[0], torch.int8, dev, "k_qs"), _dev(cache[1], torch.float16, dev, "k_d"), _dev(cache[2], torch.int8, dev, "v_qs"),
+            _dev(cache[3], torch.float16, dev, "v_d")), shape
 
 
 def kv_cache(fmt, n_pages, n_kv_heads, page_size, head_dim, device="cuda"):
@@ -849,48 +860,70 @@ def rope_freqs(n_rot, base=10000.0, scale=1.0, ext_factor=0.0, attn_factor=1.0, 
 
 def rope(x, positions, freqs, interleaved=False, mscale=1.0, y=None):
     """x fp16 [T, heads, D] (any row stride), positions int32 [T], freqs float64 [n_rot / 2] -> y, the rotated rows (y=x: in place)."""
-    T, H, D = x.shape
+    dev, shape = _current_device(), x.shape
+    T, H, D = shape
     if y is None:
-        y = torch.empty((T, H, D), dtype=torch.float16, device=x.device)
-    _want(y.shape == x.shape and positions.shape == (T,), "y has x's shape, positions one entry for each row")
-    _call("mx_rope", *_rows(x, "x"), *_rows(y, "y"), _dev(positions, torch.int32, "positions"), _dev(freqs, torch.float64, "freqs"), T, H, D,
-          2 * freqs.numel(), int(interleaved), mscale)
+        y = _new_rows(x)
+    if positions.numel() != T:
+        raise ValueError("positions: one for each row")
+    rc = lib.mx_rope(_stream(), *_rows(x, shape, dev, "x"), *_rows(y, shape, dev, "y"), _dev(positions, torch.int32, dev, "positions"),
+                     _dev(freqs, torch.float64, dev, "freqs"), T, H, D, 2 * freqs.numel(), interleaved, mscale)
+    if rc != 0:
+        raise MxError("mx_rope", rc)
     return y
 
 
 def rope_kv_write(q, k, v, positions, slots, cache, freqs, interleaved=False, mscale=1.0, q_out=None):
-    """Rotates q [T, Hq, D] -> q_out (returned) and k [T, Hkv, D]; writes k and v to the cache's slots (int32 [T]; outside the cache: skipped)."""
-    fmt, planes, (n_pages, Hkv, page_size, D) = _cache(cache)
-    T, Hq = q.shape[0], q.shape[1]
+    """Rotates q [T, Hq, D] -> q_out (returned; q_out=q: in place) and k [T, Hkv, D]; writes k and v to the cache's slots (int32 [T]; outside the cache: skipped)."""
+    dev, q_shape = _current_device(), q.shape
+    planes, (n_pages, Hkv, page_size, D) = _cache(cache, dev)
+    T, Hq, Dq = q_shape
     if q_out is None:
-        q_out = torch.empty((T, Hq, D), dtype=torch.float16, device=q.device)
-    _want(q.shape == (T, Hq, D) and k.shape == (T, Hkv, D) and v.shape == k.shape and q_out.shape == q.shape, "q, k, v and the cache do not fit together")
-    _want(positions.shape == (T,) and slots.shape == (T,), "positions and slots have one entry for each row")
-    _call("mx_rope_kv_write_" + fmt, *_rows(q, "q"), *_rows(k, "k"), *_rows(v, "v"), *_rows(q_out, "q_out"), *planes, _dev(positions, torch.int32, "positions"),
-          _dev(slots, torch.int32, "slots"), _dev(freqs, torch.float64, "freqs"), T, Hq, Hkv, D, 2 * freqs.numel(), int(interleaved), mscale, n_pages, page_size)
+        q_out = _new_rows(q)
+    if Dq != D or positions.numel() != T or slots.numel() != T:
+        raise ValueError("q has the cache's D, positions and slots one entry for each row")
+    kv_shape = (T, Hkv, D)
+    fn = lib.mx_rope_kv_write_f16 if len(planes) == 2 else lib.mx_rope_kv_write_q8_0
+    rc = fn(_stream(), *_rows(q, q_shape, dev, "q"), *_rows(k, kv_shape, dev, "k"), *_rows(v, kv_shape, dev, "v"), *_rows(q_out, q_shape, dev, "q_out"), *planes,
+            _dev(positions, torch.int32, dev, "positions"), _dev(slots, torch.int32, dev, "slots"), _dev(freqs, torch.float64, dev, "freqs"), T, Hq, Hkv, D,
+            2 * freqs.numel(), interleaved, mscale, n_pages, page_size)
+    if rc != 0:
+        raise MxError("mx_rope_kv_write", rc)
     return q_out
 
 
 def kv_write(k, v, slots, cache):
     """k, v fp16 [T, Hkv, D] as they are into the cache's slots (int32 [T]; outside the cache: skipped)."""
-    fmt, planes, (n_pages, Hkv, page_size, D) = _cache(cache)
-    T = k.shape[0]
-    _want(k.shape == (T, Hkv, D) and v.shape == k.shape and slots.shape == (T,), "k, v, slots and the cache do not fit together")
-    _call("mx_kv_write_" + fmt, *_rows(k, "k"), *_rows(v, "v"), *planes, _dev(slots, torch.int32, "slots"), T, Hkv, D, n_pages, page_size)
+    dev = _current_device()
+    planes, (n_pages, Hkv, page_size, D) = _cache(cache, dev)
+    T = slots.numel()
+    fn = lib.mx_kv_write_f16 if len(planes) == 2 else lib.mx_kv_write_q8_0
+    rc = fn(_stream(), *_rows(k, (T, Hkv, D), dev, "k"), *_rows(v, (T, Hkv, D), dev, "v"), *planes, _dev(slots, torch.int32, dev, "slots"), T, Hkv, D, n_pages, page_size)
+    if rc != 0:
+        raise MxError("mx_kv_write", rc)
 
 
 def kv_read(cache, page_table, rows, total_rows, out=None):
     """The first rows[b + 1] - rows[b] tokens of every sequence b (rows int32 [B + 1], page_table int32 [B, max_pages]) -> k, v fp16 [total_rows, Hkv, D]."""
-    fmt, planes, (n_pages, Hkv, page_size, D) = _cache(cache)
+    dev = _current_device()
+    planes, (n_pages, Hkv, page_size, D) = _cache(cache, dev)
     B, max_pages = page_table.shape
-    _want(rows.shape == (B + 1,), "rows has one entry more than there are sequences")
-    k, v = out if out is not None else (torch.empty((total_rows, Hkv, D), dtype=torch.float16, device=rows.device) for _ in range(2))
-    _want(k.shape == (total_rows, Hkv, D) and v.shape == k.shape, "outputs are [total_rows, heads, D]")
-    _call("mx_kv_read_" + fmt, *planes, _dev(page_table, torch.int32, "page_table"), max_pages, _dev(rows, torch.int32, "rows"), _dev(k, torch.float16, "k_out"),
-          _dev(v, torch.float16, "v_out"), total_rows, B, Hkv, D, n_pages, page_size)
+    shape = (total_rows, Hkv, D)
+    if out is None:
+        k, v = torch.empty(shape, dtype=torch.float16, device=rows.device), torch.empty(shape, dtype=torch.float16, device=rows.device)
+    else:
+        k, v = out
+    if rows.numel() != B + 1 or k.shape != shape or v.shape != shape:
+        raise ValueError("rows has one entry more than there are sequences, outputs are [total_rows, heads, D]")
+    fn = lib.mx_kv_read_f16 if len(planes) == 2 else lib.mx_kv_read_q8_0
+    rc = fn(_stream(), *planes, _dev(page_table, torch.int32, dev, "page_table"), max_pages, _dev(rows, torch.int32, dev, "rows"), _dev(k, torch.float16, dev, "k_out"),
+            _dev(v, torch.float16, dev, "v_out"), total_rows, B, Hkv, D, n_pages, page_size)
+    if rc != 0:
+        raise MxError("mx_kv_read", rc)
     return k, v
 
 
+@functools.lru_cache(maxsize=1024)
 def attn_decode_ws_bytes(B, Hq, Hkv, D, max_len, window=0):
     n = ctypes.c_uint64()
     rc = lib.mx_attn_decode_ws_bytes(B, Hq, Hkv, D, max_len, window, ctypes.addressof(n))
@@ -903,23 +936,37 @@ def attn_decode(q, cache, page_table, seq_lens, scale=None, window=0, sinks=None
     """One query q [B, Hq, D] for each sequence over its seq_lens[b] (int32) tokens in the pages page_table[b] (int32 [B, max_pages]) -> fp16 [B, Hq, D].
     scale: D ** -0.5 unless given; window: the last tokens only; sinks: fp32 [Hq]; max_len: the longest sequence, where the host knows it; out_q8: uint8
     buffer for the block_q8_1x stream of the output rows; ws: a workspace of attn_decode_ws_bytes."""
-    fmt, planes, (n_pages, Hkv, page_size, D) = _cache(cache)
-    B, Hq = q.shape[0], q.shape[1]
-    max_pages = page_table.shape[1]
-    _want(q.shape == (B, Hq, D) and page_table.shape[0] == B and seq_lens.shape == (B,) and (sinks is None or sinks.shape == (Hq,)),
-          "q, page_table, seq_lens, sinks and the cache do not fit together")
+    dev, q_shape = _current_device(), q.shape
+    planes, (n_pages, Hkv, page_size, D) = _cache(cache, dev)
+    B, Hq, Dq = q_shape
+    rows, max_pages = page_table.shape
     if max_len is None:
-        max_len = max_pages * page_size
+        max_len = min(max_pages * page_size, 0x7FFFFFFF)
     if out is None:
-        out = torch.empty((B, Hq, D), dtype=torch.float16, device=q.device)
-    _want(out.shape == q.shape and (out_q8 is None or out_q8.numel() * out_q8.element_size() == B * Hq * D // 32 * Q81X_BYTES), "out or out_q8 has another size")
+        out = _new_rows(q)
+    if Dq != D or rows != B or seq_lens.numel() != B or out.shape != q_shape:
+        raise ValueError("q, out, page_table and seq_lens have one row for each sequence, q the cache's D")
+    ws_ptr, ws_size = None, 0
     if ws is None:
-        need = attn_decode_ws_bytes(B, Hq, Hkv, D, max_len, window)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _call("mx_attn_decode_" + fmt, *_rows(q, "q"), *planes, _dev(page_table, torch.int32, "page_table"), max_pages, _dev(seq_lens, torch.int32, "seq_lens"),
-          None if sinks is None else _dev(sinks, torch.float32, "sinks"), _dev(out, torch.float16, "out"), None if out_q8 is None else _dev(out_q8, torch.uint8, "out_q8"),
-          B, Hq, Hkv, D, n_pages, page_size, max_len, window, D ** -0.5 if scale is None else scale, None if ws is None else _dev(ws, ws.dtype, "ws"),
-          0 if ws is None else ws.numel() * ws.element_size())
+        ws_size = attn_decode_ws_bytes(B, Hq, Hkv, D, max_len, window)
+        if ws_size:
+            ws = torch.empty(ws_size, dtype=torch.uint8, device=q.device)
+            ws_ptr = ws.data_ptr()
+    else:
+        ws_ptr, ws_size = _dev(ws, ws.dtype, dev, "ws"), ws.numel() * ws.element_size()
+    sinks_ptr = q8_ptr = None
+    if sinks is not None:
+        _want(sinks.numel() == Hq, "sinks: one for each query head")
+        sinks_ptr = _dev(sinks, torch.float32, dev, "sinks")
+    if out_q8 is not None:
+        _want(out_q8.numel() * 32 == B * Hq * D * Q81X_BYTES, "out_q8: 40 bytes for each 32 elements of out")
+        q8_ptr = _dev(out_q8, torch.uint8, dev, "out_q8")
+    fn = lib.mx_attn_decode_f16 if len(planes) == 2 else lib.mx_attn_decode_q8_0
+    rc = fn(_stream(), *_rows(q, q_shape, dev, "q"), *planes, _dev(page_table, torch.int32, dev, "page_table"), max_pages, _dev(seq_lens, torch.int32, dev, "seq_lens"),
+            sinks_ptr, _dev(out, torch.float16, dev, "out"), q8_ptr, B, Hq, Hkv, D, n_pages, page_size, max_len, window, D ** -0.5 if scale is None else scale, ws_ptr,
+            ws_size)
+    if rc != 0:
+        raise MxError("mx_attn_decode", rc)
     return out
 
 
