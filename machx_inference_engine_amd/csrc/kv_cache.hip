@@ -7,6 +7,9 @@
 namespace mxq {
 
 constexpr int kRowThreads = 256;
+// Outputs that the L2s (8 x 4 MB) do not hold are written past them, which leaves those to what is read: a Q8_0 cache's
+// 32048 tokens of 4 heads of 128 read back 24.8 -> 19.4 us.
+constexpr uint64_t kStreamFrom = 32u << 20;
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float float8 __attribute__((ext_vector_type(8)));
 
@@ -46,60 +49,49 @@ __device__ __forceinline__ uint32_t max_bits4(uint32_t v) {  // over four adjace
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));
 }
 
-// One workgroup takes heads_per_wg heads (query, key, value heads in this order) of one token, one thread 8 consecutive elements of a head.  A thread
-// loads its own 8 and, in the half layout, the 8 that they are paired with before the barrier behind which the sines are ready, and stores after it:
-// rows may be rotated in place.
-template <bool ROPE, bool Q8, bool INTER>
-__global__ __launch_bounds__(kRowThreads) void rows_kernel(RowsArgs a) {
-    __shared__ float2 cs[128];
-    const uint32_t tid = threadIdx.x, t = blockIdx.x / a.groups, D = a.chunks * 8;
-    const uint32_t hw = tid / a.chunks, c = tid - hw * a.chunks, h = (blockIdx.x - t * a.groups) * a.heads_per_wg + hw;
-    const bool live = hw < a.heads_per_wg && h < a.Hq + 2 * a.Hkv;
-    const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hkv;
-    const uint32_t hk = is_q ? h : is_v ? h - a.Hq - a.Hkv : h - a.Hq;
-    half8 own = {}, other = {};
-    const bool turned = ROPE && !is_v && c * 8 < a.n_rot;
-    const uint32_t half_chunks = a.n_rot / 16;
-    const bool first = c < half_chunks;
-    if (live) {
-        const half_t* row = (is_q ? a.q + t * a.q_stride : is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride) + (size_t)hk * D;
-        own = *reinterpret_cast<const half8*>(row + c * 8);
-        if (!INTER && turned) other = *reinterpret_cast<const half8*>(row + (first ? c + half_chunks : c - half_chunks) * 8);
-    }
-    if (ROPE) {
-        if (tid < a.n_rot / 2) {
-            const float2 v = cos_sin_turns((double)a.positions[t] * (a.freqs[tid] * 0.15915494309189535));
-            cs[tid] = make_float2(v.x * a.mscale, v.y * a.mscale);
-        }
-        __syncthreads();
-    }
-    if (!live) return;   // whole groups of four lanes: chunks % 4 == 0 wherever they exchange values
-    half8 y = own;
-    if (turned) {
-        if (INTER) {
+// Eight elements of an interleaved chunk / the first and the second eight of a pair of chunks, turned by cs[0 ..]; products and sums in fp32, one rounding.
+__device__ __forceinline__ half8 turn_interleaved(half8 x, const float2* cs) {
+    half8 y;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 w = cs[c * 4 + i];
-                const float x0 = (float)own[2 * i], x1 = (float)own[2 * i + 1];
-                y[2 * i] = f32_to_f16_rne(fmaf(x0, w.x, -(x1 * w.y)));
-                y[2 * i + 1] = f32_to_f16_rne(fmaf(x0, w.y, x1 * w.x));
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float2 w = cs[(first ? c : c - half_chunks) * 8 + i];
-                const float x = (float)own[i], o = (float)other[i];
-                y[i] = f32_to_f16_rne(first ? fmaf(x, w.x, -(o * w.y)) : fmaf(o, w.y, x * w.x));
-            }
-        }
+    for (int i = 0; i < 4; ++i) {
+        const float2 w = cs[i];
+        const float x0 = (float)x[2 * i], x1 = (float)x[2 * i + 1];
+        y[2 * i] = f32_to_f16_rne(fmaf(x0, w.x, -(x1 * w.y)));
+        y[2 * i + 1] = f32_to_f16_rne(fmaf(x0, w.y, x1 * w.x));
     }
-    if (is_q) {
+    return y;
+}
+__device__ __forceinline__ half8 turn_first(half8 x0, half8 x1, const float2* cs) {
+    half8 y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = f32_to_f16_rne(fmaf((float)x0[i], cs[i].x, -((float)x1[i] * cs[i].y)));
+    return y;
+}
+__device__ __forceinline__ half8 turn_second(half8 x0, half8 x1, const float2* cs) {
+    half8 y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = f32_to_f16_rne(fmaf((float)x0[i], cs[i].y, (float)x1[i] * cs[i].x));
+    return y;
+}
+__device__ __forceinline__ float2 cs_of(const RowsArgs& a, uint32_t t, uint32_t i) {
+    const float2 v = cos_sin_turns((double)a.positions[t] * (a.freqs[i] * 0.15915494309189535));
+    return make_float2(v.x * a.mscale, v.y * a.mscale);
+}
+__device__ __forceinline__ const half_t* row_of(const RowsArgs& a, uint32_t t, uint32_t h, uint32_t D) {
+    return h < a.Hq ? a.q + t * a.q_stride + (size_t)h * D : h < a.Hq + a.Hkv ? a.k + t * a.k_stride + (size_t)(h - a.Hq) * D : a.v + t * a.v_stride + (size_t)(h - a.Hq - a.Hkv) * D;
+}
+
+// Chunk c of head h (query, key, value heads in this order) of token t to where it goes.  Q8: the four lanes of a block of 32 call together.
+template <bool Q8>
+__device__ __forceinline__ void put(const RowsArgs& a, uint32_t t, uint32_t slot, uint32_t h, uint32_t c, half8 y) {
+    const uint32_t D = a.chunks * 8;
+    if (h < a.Hq) {
         *reinterpret_cast<half8*>(a.q_out + t * a.q_out_stride + (size_t)h * D + c * 8) = y;
         return;
     }
-    const uint32_t slot = (uint32_t)a.slots[t];
     if (slot >= a.n_slots) return;
-    const uint32_t page = slot / a.page_size, at = slot - page * a.page_size;
+    const bool is_v = h >= a.Hq + a.Hkv;
+    const uint32_t hk = h - a.Hq - (is_v ? a.Hkv : 0), page = slot / a.page_size, at = slot - page * a.page_size;
     const size_t crow = ((size_t)page * a.Hkv + hk) * a.page_size + at;
     void* cache = is_v ? a.v_cache : a.k_cache;
     if (!Q8) {
@@ -118,11 +110,99 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(RowsArgs a) {
     }
 }
 
+// One workgroup takes heads_per_wg heads of one token, one thread 8 consecutive elements of a head.  A thread loads its own 8 and, in the half layout, the 8 that they
+// are paired with before the barrier behind which the sines are ready, and stores after it: rows may be rotated in place.
+template <bool ROPE, bool Q8, bool INTER>
+__global__ __launch_bounds__(kRowThreads) void rows_kernel(RowsArgs a) {
+    __shared__ float2 cs[128];
+    const uint32_t tid = threadIdx.x, t = blockIdx.x / a.groups, D = a.chunks * 8;
+    const uint32_t hw = tid / a.chunks, c = tid - hw * a.chunks, h = (blockIdx.x - t * a.groups) * a.heads_per_wg + hw;
+    const bool live = hw < a.heads_per_wg && h < a.Hq + 2 * a.Hkv;
+    half8 own = {}, other = {};
+    const bool turned = ROPE && h < a.Hq + a.Hkv && c * 8 < a.n_rot;
+    const uint32_t half_chunks = a.n_rot / 16;
+    const bool first = c < half_chunks;
+    if (live) {
+        const half_t* row = row_of(a, t, h, D);
+        own = *reinterpret_cast<const half8*>(row + c * 8);
+        if (!INTER && turned) other = *reinterpret_cast<const half8*>(row + (first ? c + half_chunks : c - half_chunks) * 8);
+    }
+    const uint32_t slot = a.slots ? (uint32_t)a.slots[t] : 0u;
+    if (ROPE) {
+        if (tid < a.n_rot / 2) cs[tid] = cs_of(a, t, tid);
+        __syncthreads();
+    }
+    if (!live) return;   // whole groups of four lanes: chunks % 4 == 0 wherever they exchange values
+    half8 y = own;
+    if (turned) y = INTER ? turn_interleaved(own, cs + c * 4) : first ? turn_first(own, other, cs + c * 8) : turn_second(other, own, cs + (c - half_chunks) * 8);
+    put<Q8>(a, t, slot, h, c, y);
+}
+
+// Prompts: a workgroup takes one token with all its heads, a thread two chunks at a time, in the half layout the two that are turned together: rows may be rotated
+// in place.  The chunks of a head that are not turned, and a value head's, are paired with the same distance between the two throughout.
+// Q8: that distance is a multiple of four chunks (D and n_rot multiples of 64), so that four lanes hold whole blocks.
+template <bool ROPE, bool Q8, bool INTER>
+__global__ __launch_bounds__(kRowThreads) void prompt_kernel(RowsArgs a) {
+    __shared__ float2 cs[128];
+    const uint32_t tid = threadIdx.x, t = blockIdx.x, D = a.chunks * 8, pairs = a.chunks / 2, items = (a.Hq + 2 * a.Hkv) * pairs, half_chunks = a.n_rot / 16;
+    struct Item {
+        uint32_t h, c0, c1;
+        bool together, angle;
+        half8 x0, x1;
+    };
+    auto load = [&](uint32_t i) {
+        Item m;
+        m.h = i / pairs;
+        const uint32_t p = i - m.h * pairs;
+        m.angle = ROPE && m.h < a.Hq + a.Hkv;
+        // (p, p + half_chunks) among the turned chunks of the half layout, then (p', p' + rest / 2) behind them
+        m.together = !INTER && m.angle && p < half_chunks;
+        m.c0 = !INTER && m.angle && !m.together ? p + half_chunks : p;
+        m.c1 = m.c0 + (INTER || !m.angle ? pairs : m.together ? half_chunks : pairs - half_chunks);
+        const half_t* row = row_of(a, t, m.h, D);
+        m.x0 = *reinterpret_cast<const half8*>(row + m.c0 * 8);
+        m.x1 = *reinterpret_cast<const half8*>(row + m.c1 * 8);
+        return m;
+    };
+    Item next;
+    if (tid < items) next = load(tid);
+    const uint32_t slot = a.slots ? (uint32_t)a.slots[t] : 0u;
+    if (ROPE) {
+        if (tid < a.n_rot / 2) cs[tid] = cs_of(a, t, tid);
+        __syncthreads();
+    }
+    for (uint32_t i = tid; i < items; i += kRowThreads) {
+        const Item m = next;
+        if (i + kRowThreads < items) next = load(i + kRowThreads);
+        half8 y0 = m.x0, y1 = m.x1;
+        if (m.together) {
+            y0 = turn_first(m.x0, m.x1, cs + m.c0 * 8);
+            y1 = turn_second(m.x0, m.x1, cs + m.c0 * 8);
+        } else if (INTER && m.angle) {
+            if (m.c0 * 8 < a.n_rot) y0 = turn_interleaved(m.x0, cs + m.c0 * 4);
+            if (m.c1 * 8 < a.n_rot) y1 = turn_interleaved(m.x1, cs + m.c1 * 4);
+        }
+        put<Q8>(a, t, slot, m.h, m.c0, y0);
+        put<Q8>(a, t, slot, m.h, m.c1, y1);
+    }
+}
+
+constexpr uint32_t kPromptTokens = 512;
 template <bool ROPE, bool Q8>
 static int launch_rows(mx_stream_t s, RowsArgs a, uint32_t T, int interleaved) {
     a.heads_per_wg = kRowThreads / a.chunks;
     a.groups = (a.Hq + 2 * a.Hkv + a.heads_per_wg - 1) / a.heads_per_wg;
     MX_REQUIRE_SHAPE((uint64_t)a.groups * T < (1ull << 31));
+    // Two chunks a thread load every row once where the half layout's other form loads turned rows twice: 8192 tokens of 72 heads of 64 35.9 -> 26.6 us (5.7 TB/s),
+    // 2047 tokens of 32 + 4 + 4 heads of 128 into a Q8_0 cache 14.5 -> 9.4; interleaved pairs are as fast either way.  Fewer tokens leave CUs without work: one
+    // token 2.2 -> 2.8 us, 333 (18 heads of 256) 3.9 -> 4.1.
+    if (T >= kPromptTokens && (!Q8 || (a.chunks % 8 == 0 && a.n_rot % 64 == 0))) {
+        auto launch = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(T), dim3(kRowThreads), 0, as_stream(s), a);
+            return launch_status();
+        };
+        return ROPE && interleaved ? launch(prompt_kernel<ROPE, Q8, ROPE>) : launch(prompt_kernel<ROPE, Q8, false>);
+    }
     const dim3 grid(a.groups * T);
     if (ROPE && interleaved) hipLaunchKernelGGL((rows_kernel<ROPE, Q8, ROPE>), grid, dim3(kRowThreads), 0, as_stream(s), a);
     else hipLaunchKernelGGL((rows_kernel<ROPE, Q8, false>), grid, dim3(kRowThreads), 0, as_stream(s), a);
@@ -131,7 +211,7 @@ static int launch_rows(mx_stream_t s, RowsArgs a, uint32_t T, int interleaved) {
 
 // Reading back: a workgroup takes 16 tokens of one sequence (they lie in one page) and all heads, a thread 8 elements at a time.
 // Tile numbers are dealt by floor(rows[b] / 16) + b, which leaves room for every sequence's ceil(length / 16).
-template <bool Q8>
+template <bool Q8, bool STREAM>
 __global__ __launch_bounds__(256) void kv_read_kernel(const void* k_cache, const half_t* k_d, const void* v_cache, const half_t* v_d, const int32_t* page_table,
                                                       uint32_t max_pages, const int32_t* rows, half_t* k_out, half_t* v_out, uint32_t total, uint32_t B,
                                                       uint32_t Hkv, uint32_t chunks, uint32_t n_pages, uint32_t page_size) {
@@ -170,7 +250,9 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const void* k_cache, const
                 for (int j = 0; j < 8; ++j) y[j] = f32_to_f16_rne((float)(int8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3))) * d);
             }
         }
-        *reinterpret_cast<half8*>((is_v ? v_out : k_out) + ((size_t)(row0 + t0 + tok) * Hkv + h) * D + c * 8) = y;
+        half8* const out = reinterpret_cast<half8*>((is_v ? v_out : k_out) + ((size_t)(row0 + t0 + tok) * Hkv + h) * D + c * 8);
+        if (STREAM) __builtin_nontemporal_store(y, out);
+        else *out = y;
     }
 }
 
@@ -239,7 +321,8 @@ static int kv_read(mx_stream_t s, bool q8, const void* k, const uint16_t* k_d, c
                            max_pages, rows, reinterpret_cast<half_t*>(k_out), reinterpret_cast<half_t*>(v_out), total_rows, B, Hkv, D / 8, n_pages, page_size);
         return launch_status();
     };
-    return q8 ? launch(kv_read_kernel<true>) : launch(kv_read_kernel<false>);
+    if ((uint64_t)total_rows * Hkv * D * 4 >= kStreamFrom) return q8 ? launch(kv_read_kernel<true, true>) : launch(kv_read_kernel<false, true>);
+    return q8 ? launch(kv_read_kernel<true, false>) : launch(kv_read_kernel<false, false>);
 }
 
 }  // namespace mxq

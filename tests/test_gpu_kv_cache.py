@@ -23,7 +23,8 @@ def near(got, want, tol, what):
 
 @pytest.mark.parametrize("inter", [False, True])
 @pytest.mark.parametrize("T,H,D,n_rot", [(1, 40, 128, 128), (3, 1, 16, 16), (7, 3, 64, 64), (5, 18, 256, 64), (2, 5, 80, 32), (33, 7, 96, 96), (4, 9, 112, 48),
-                                         (300, 40, 128, 128), (6, 2, 256, 256), (2, 65, 32, 16)])
+                                         (300, 40, 128, 128), (6, 2, 256, 256), (2, 65, 32, 16), (512, 3, 64, 64), (777, 5, 128, 32),
+                                         (600, 9, 80, 48), (513, 2, 256, 128)])
 def test_rope(mx, T, H, D, n_rot, inter):
     rng = np.random.default_rng(T * 1000 + D + n_rot)
     x, f = rows(rng, T, H, D), U.freqs(n_rot, 500000.0)
@@ -45,10 +46,11 @@ def test_rope_keeps_far_angles(mx, inter):
 
 
 @pytest.mark.parametrize("inter", [False, True])
-@pytest.mark.parametrize("H,D,n_rot", [(40, 128, 128), (70, 64, 32), (3, 256, 256)])
-def test_rope_in_place_and_strided(mx, H, D, n_rot, inter):
+@pytest.mark.parametrize("T", [37, 600])
+@pytest.mark.parametrize("H,D,n_rot", [(40, 128, 128), (70, 64, 32), (3, 256, 256), (5, 96, 48)])
+def test_rope_in_place_and_strided(mx, T, H, D, n_rot, inter):
     rng = np.random.default_rng(11)
-    T, wide = 37, (H + 5) * D + 8
+    wide = (H + 5) * D + 8
     buf = dev(rows(rng, T, 1, wide)).view(T, wide)
     f, pos = dev(U.freqs(n_rot)), dev(np.arange(100, 100 + T, dtype=np.int32))
     part = buf[:, 8 + 2 * D: 8 + (H + 2) * D].view(T, H, D)
@@ -79,7 +81,8 @@ def slots_for(rng, T, n_pages, ps):
 
 
 @pytest.mark.parametrize("fmt", ["f16", "q8_0"])
-@pytest.mark.parametrize("T,Hkv,D,ps", [(1, 8, 128, 16), (13, 1, 32, 48), (200, 3, 96, 16), (37, 8, 64, 256), (5, 2, 256, 32)])
+@pytest.mark.parametrize("T,Hkv,D,ps", [(1, 8, 128, 16), (13, 1, 32, 48), (200, 3, 96, 16), (37, 8, 64, 256), (5, 2, 256, 32), (700, 2, 64, 16), (512, 1, 96, 64),
+                                         (1000, 3, 128, 32)])
 def test_kv_write(mx, fmt, T, Hkv, D, ps):
     """The planes are the oracle's encoding of the rows bit for bit; every other slot is as it was."""
     rng = np.random.default_rng(T + D)
@@ -100,7 +103,8 @@ def test_kv_write(mx, fmt, T, Hkv, D, ps):
 
 @pytest.mark.parametrize("fmt", ["f16", "q8_0"])
 @pytest.mark.parametrize("inter", [False, True])
-@pytest.mark.parametrize("T,Hq,Hkv,D,n_rot,ps", [(1, 32, 8, 128, 128, 16), (9, 64, 8, 64, 64, 32), (50, 7, 1, 96, 48, 16), (21, 16, 2, 256, 64, 64), (3, 5, 5, 32, 16, 16)])
+@pytest.mark.parametrize("T,Hq,Hkv,D,n_rot,ps", [(1, 32, 8, 128, 128, 16), (9, 64, 8, 64, 64, 32), (50, 7, 1, 96, 48, 16), (21, 16, 2, 256, 64, 64), (3, 5, 5, 32, 16, 16), (700, 8, 2, 64, 64, 16),
+                                                  (530, 6, 3, 128, 64, 48), (512, 4, 1, 96, 96, 32), (600, 2, 2, 256, 64, 16)])
 def test_rope_kv_write_is_rope_then_write(mx, fmt, inter, T, Hq, Hkv, D, n_rot, ps):
     """One launch gives the bits of rope and kv_write, whether the rows are parts of a fused projection or not, and with q rotated in place."""
     rng = np.random.default_rng(T + Hq)
@@ -153,7 +157,7 @@ def test_q8_0_write_of_extremes(mx):
 
 @pytest.mark.parametrize("fmt", ["f16", "q8_0"])
 @pytest.mark.parametrize("Hkv,D,ps,lens", [(8, 128, 16, [1]), (2, 64, 48, [0, 5, 48, 0, 0, 97, 16]), (1, 256, 16, [333, 0]), (3, 96, 256, [17, 255, 256, 257, 1, 1, 1]),
-                                           (1, 32, 32, [(i * 7) % 23 for i in range(200)]), (1, 32, 16, [3] * 5000)])
+                                           (1, 32, 32, [(i * 7) % 23 for i in range(200)]), (1, 32, 16, [3] * 5000), (8, 128, 32, [8000, 300])])
 def test_kv_read(mx, fmt, Hkv, D, ps, lens):
     rng = np.random.default_rng(len(lens) + D)
     table, n_pages = U.pages_of(lens, ps, rng)
