@@ -482,34 +482,36 @@ __global__ __launch_bounds__(512) void attn_join_kernel(AttnArgs a, uint32_t gro
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)first * a.Hq + h;
     const float* po = a.part_o + ((size_t)first * a.Hq + h) * a.D + d;
     const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
-    // the first sums are requested before their weights are known
+    // everything that a sequence's even portion of the parts needs is requested at once
     constexpr uint32_t kAhead = 4;
     floatx4 ahead[kAhead];
+    float peak[kAhead];
 #pragma unroll
     for (uint32_t i = 0; i < kAhead; ++i) {
         const uint32_t s = part + i * groups;
-        ahead[i] = part < groups && s < n ? *reinterpret_cast<const floatx4*>(po + (size_t)s * a.Hq * a.D) : floatx4{0.f, 0.f, 0.f, 0.f};
+        const bool there = part < groups && s < n;
+        ahead[i] = there ? *reinterpret_cast<const floatx4*>(po + (size_t)s * a.Hq * a.D) : floatx4{0.f, 0.f, 0.f, 0.f};
+        peak[i] = there ? ml[(size_t)s * a.Hq].x : -INFINITY;
     }
     // every wave finds the maximum and the sum for itself
-    float top = sink;
-    for (uint32_t s = lane; s < n; s += 64) top = fmaxf(top, ml[(size_t)s * a.Hq].x);
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+    const float2 own = lane < n ? ml[(size_t)lane * a.Hq] : make_float2(-INFINITY, 0.f);
+    float top = fmaxf(own.x, sink);
+    for (uint32_t s = lane + 64; s < n; s += 64) top = fmaxf(top, ml[(size_t)s * a.Hq].x);
+    top = fmaxf(top, dpp_f<0xB1>(top));
+    top = fmaxf(top, dpp_f<0x4E>(top));
+    top = fmaxf(top, dpp_f<0x141>(top));
+    top = rows_max(fmaxf(top, dpp_f<0x140>(top)));
     const float ref = top == -INFINITY ? 0.f : top;
-    float total = 0.f;
-    for (uint32_t s = lane; s < n; s += 64) {
+    float total = __builtin_amdgcn_exp2f(own.x - ref) * own.y;
+    for (uint32_t s = lane + 64; s < n; s += 64) {
         const float2 v = ml[(size_t)s * a.Hq];
         total += __builtin_amdgcn_exp2f(v.x - ref) * v.y;
     }
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x);
+    total = rows_sum(group_sum<16>(total));
     floatx4 sum = {0.f, 0.f, 0.f, 0.f};
     if (part < groups) {
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            const uint32_t s = part + i * groups;
-            if (s < n) sum += __builtin_amdgcn_exp2f(ml[(size_t)s * a.Hq].x - ref) * ahead[i];
-        }
+        for (uint32_t i = 0; i < kAhead; ++i) sum += __builtin_amdgcn_exp2f(peak[i] - ref) * ahead[i];
         for (uint32_t s = part + kAhead * groups; s < n; s += groups)
             sum += __builtin_amdgcn_exp2f(ml[(size_t)s * a.Hq].x - ref) * *reinterpret_cast<const floatx4*>(po + (size_t)s * a.Hq * a.D);
         if (groups > 1) *reinterpret_cast<floatx4*>(sums + part * a.D + d) = sum;
@@ -523,9 +525,10 @@ __global__ __launch_bounds__(512) void attn_join_kernel(AttnArgs a, uint32_t gro
     store_rows(a, (size_t)row * a.D + d, y, true);
 }
 
-// Short sequences take a workgroup each.  Otherwise the tiles are shared equally by as many workgroups as stream the cache fastest, two for each CU (one where heads are
-// wide): 64 x 8192 fp16 tokens of 8 heads of 128, us by workgroups: 256 318, 512 321, 768 330, 2048 332; Q8_0 205, 176, 183 (768), ...; one Q8_0 sequence of 131071
-// 59, 54, 57, 66.  A share is two tiles a wave at least, but one where that leaves most CUs idle (one Q8_0 sequence of 2000: 11.1 -> 9.8 us; of 8000: 11.9, 12.8).
+// Short sequences take a workgroup each.  Otherwise the tiles are shared equally by as many workgroups as stream the cache fastest: 512, two for each CU; three where
+// heads are narrow, one where they are wide.  us by workgroups (256, 512, 768, 1024): 64 x 8192 tokens of 8 heads of 128, fp16 318, 321, 330, 328, Q8_0 201, 175, 183, 182;
+// one Q8_0 sequence of 131071 57, 52, 56, 58; 64 ragged ones of up to 6001 with heads of 64 72, 53, 49, 49; 16 fp16 ones of 16384 with 2 heads of 256 89 (256), 97 (512).
+// A share is two tiles a wave at least, but one where that leaves most CUs idle (one Q8_0 sequence of 2000: 11.1 -> 9.8 us; of 8000: 11.9, 12.8).
 struct Plan {
     uint32_t shares;         // 0: a workgroup for each sequence and group of heads
     uint64_t ws_bytes;
@@ -539,7 +542,7 @@ static Plan plan_of(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t 
     auto up = [](uint64_t x, uint64_t y) { return (x + y - 1) / y; };
     uint64_t most = up(all, kLeastShare);
     if (most * groups > 128) most = up(all, 2 * kLeastShare) > up(128, groups) ? up(all, 2 * kLeastShare) : up(128, groups);
-    uint64_t shares = up(D > 128 ? 256 : 512, groups);
+    uint64_t shares = up(D > 128 ? 256 : D > 64 ? 512 : 768, groups);
     if (shares > most) shares = most;
     return {(uint32_t)shares, (shares + B) * Hq * (D + 2) * 4 + (uint64_t)B * 8};
 }
