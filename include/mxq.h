@@ -703,17 +703,17 @@ int mx_swiglu_oai_q8(mx_stream_t s, const uint16_t* gate, const uint16_t* up, ui
  * ([total_rows][Hkv][D] fp16; rows: B + 1 non-decreasing int32 on the device, of at most total_rows).  Rows from rows[B] on are left as they were.
  * Tokens whose page is outside [0, n_pages) or past the table read as zeros.  */
 int mx_rope_freqs(uint32_t n_rot, double base, double scale, double ext_factor, double attn_factor, double beta_fast, double beta_slow,
-                  uint32_t n_ctx_orig, const float* factors, double* freqs, float* mscale);
+                  uint32_t n_ctx_orig, const float* factors, double* freqs, double* mscale);
 int mx_rope(mx_stream_t s, const uint16_t* x, uint64_t x_stride, uint16_t* y, uint64_t y_stride, const int32_t* positions, const double* freqs, uint32_t T,
-            uint32_t n_heads, uint32_t D, uint32_t n_rot, int interleaved, float mscale);
+            uint32_t n_heads, uint32_t D, uint32_t n_rot, int interleaved, double mscale);
 int mx_rope_kv_write_f16(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride,
                          uint16_t* q_out, uint64_t q_out_stride, uint16_t* k_cache, uint16_t* v_cache, const int32_t* positions, const int32_t* slots,
-                         const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved, float mscale,
+                         const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved, double mscale,
                          uint32_t n_pages, uint32_t page_size);
 int mx_rope_kv_write_q8_0(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride,
                           uint16_t* q_out, uint64_t q_out_stride, int8_t* k_qs, uint16_t* k_d, int8_t* v_qs, uint16_t* v_d, const int32_t* positions,
                           const int32_t* slots, const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved,
-                          float mscale, uint32_t n_pages, uint32_t page_size);
+                          double mscale, uint32_t n_pages, uint32_t page_size);
 int mx_kv_write_f16(mx_stream_t s, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride, uint16_t* k_cache, uint16_t* v_cache,
                     const int32_t* slots, uint32_t T, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size);
 int mx_kv_write_q8_0(mx_stream_t s, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride, int8_t* k_qs, uint16_t* k_d, int8_t* v_qs,

@@ -13,22 +13,22 @@ constexpr uint64_t kStreamFrom = 32u << 20;
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float float8 __attribute__((ext_vector_type(8)));
 
-// cos and sin of `turns` revolutions.  The angle is cut to a quarter turn in 64 bits (a position of 2^20 has 2^-12 radians left in 32), what is
-// left is rounded once, and the two Taylor polynomials below are good to 2^-26 on [-pi/4, pi/4].
-__device__ __forceinline__ float2 cos_sin_turns(double turns) {
-    const double quarters = turns * 4.0, k = rint(quarters);
-    const float a = (float)((quarters - k) * 1.5707963267948966), a2 = a * a;
-    float s = fmaf(a2, 2.7557319e-6f, -1.9841270e-4f);
-    s = fmaf(a2, s, 8.3333333e-3f);
-    s = fmaf(a2, s, -1.6666667e-1f);
-    s = fmaf(a * a2, s, a);
-    float c = fmaf(a2, -2.7557319e-7f, 2.4801587e-5f);
-    c = fmaf(a2, c, -1.3888889e-3f);
-    c = fmaf(a2, c, 4.1666667e-2f);
-    c = fmaf(a2, c, -0.5f);
-    c = fmaf(a2, c, 1.0f);
+// m cos and m sin of `turns` revolutions, each rounded once: the angle is cut to a quarter turn and the Taylor polynomials are summed in 64 bits (a position of 2^20 has
+// 2^-12 radians left in 32; one thread does this for each pair of a token, all heads use it).  On [-pi/4, pi/4] the next terms are below 2^-34.
+__device__ __forceinline__ float2 cos_sin_turns(double turns, double m) {
+    const double quarters = turns * 4.0, k = rint(quarters), a = (quarters - k) * 1.5707963267948966, a2 = a * a;
+    double s = fma(a2, -1.0 / 39916800.0, 1.0 / 362880.0);
+    s = fma(a2, s, -1.0 / 5040.0);
+    s = fma(a2, s, 1.0 / 120.0);
+    s = fma(a2, s, -1.0 / 6.0);
+    s = fma(a * a2, s, a) * m;
+    double c = fma(a2, -1.0 / 3628800.0, 1.0 / 40320.0);
+    c = fma(a2, c, -1.0 / 720.0);
+    c = fma(a2, c, 1.0 / 24.0);
+    c = fma(a2, c, -0.5);
+    c = fma(a2, c, 1.0) * m;
     const int q = (int)(k - 4.0 * floor(k * 0.25));
-    const float cc = (q & 1) ? s : c, ss = (q & 1) ? c : s;
+    const float cc = (float)((q & 1) ? s : c), ss = (float)((q & 1) ? c : s);
     return make_float2((q == 1 || q == 2) ? -cc : cc, (q & 2) ? -ss : ss);
 }
 
@@ -41,7 +41,7 @@ struct RowsArgs {
     const int32_t *positions, *slots;
     const double* freqs;
     uint32_t Hq, Hkv, chunks, n_rot, heads_per_wg, groups, page_size, n_slots;  // chunks = D / 8, groups: workgroups of a token
-    float mscale;
+    double mscale;
 };
 
 __device__ __forceinline__ uint32_t max_bits4(uint32_t v) {  // over four adjacent lanes
@@ -74,8 +74,7 @@ __device__ __forceinline__ half8 turn_second(half8 x0, half8 x1, const float2* c
     return y;
 }
 __device__ __forceinline__ float2 cs_of(const RowsArgs& a, uint32_t t, uint32_t i) {
-    const float2 v = cos_sin_turns((double)a.positions[t] * (a.freqs[i] * 0.15915494309189535));
-    return make_float2(v.x * a.mscale, v.y * a.mscale);
+    return cos_sin_turns((double)a.positions[t] * (a.freqs[i] * 0.15915494309189535), a.mscale);
 }
 __device__ __forceinline__ const half_t* row_of(const RowsArgs& a, uint32_t t, uint32_t h, uint32_t D) {
     return h < a.Hq ? a.q + t * a.q_stride + (size_t)h * D : h < a.Hq + a.Hkv ? a.k + t * a.k_stride + (size_t)(h - a.Hq) * D : a.v + t * a.v_stride + (size_t)(h - a.Hq - a.Hkv) * D;
@@ -282,7 +281,7 @@ static int check_rotation(const void* positions, const void* freqs, uint32_t D, 
 static int rope_kv_write(mx_stream_t s, bool q8, const uint16_t* q, uint64_t q_stride, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride,
                          uint16_t* q_out, uint64_t q_out_stride, void* k_cache, uint16_t* k_d, void* v_cache, uint16_t* v_d, const int32_t* positions,
                          const int32_t* slots, const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved,
-                         float mscale, uint32_t n_pages, uint32_t page_size) {
+                         double mscale, uint32_t n_pages, uint32_t page_size) {
     if (int rc = check_cache(q8, k_cache, k_d, v_cache, v_d, Hkv, D, n_pages, page_size)) return rc;
     if (int rc = check_rows(k, k_stride, (uint64_t)Hkv * D)) return rc;
     if (int rc = check_rows(v, v_stride, (uint64_t)Hkv * D)) return rc;
@@ -332,7 +331,7 @@ using namespace mxq;
 extern "C" {
 
 int mx_rope_freqs(uint32_t n_rot, double base, double scale, double ext_factor, double attn_factor, double beta_fast, double beta_slow, uint32_t n_ctx_orig,
-                  const float* factors, double* freqs, float* mscale) {
+                  const float* factors, double* freqs, double* mscale) {
     MX_REQUIRE_PTR(freqs); MX_REQUIRE_PTR(mscale);
     const bool yarn = ext_factor != 0.0;
     MX_REQUIRE_SHAPE(n_rot >= 16 && n_rot <= 256 && n_rot % 16 == 0 && base > 1.0 && scale > 0.0 && ext_factor >= 0.0 && ext_factor <= 1.0);
@@ -345,12 +344,12 @@ int mx_rope_freqs(uint32_t n_rot, double base, double scale, double ext_factor, 
         const double keep = yarn ? ext_factor * (1.0 - fmin(1.0, fmax(0.0, (i - low) / fmax(0.001, high - low)))) : 0.0;
         freqs[i] = f * scale * (1.0 - keep) + f * keep;
     }
-    *mscale = (float)(attn_factor * (yarn ? 1.0 + 0.1 * log(1.0 / scale) : 1.0));
+    *mscale = attn_factor * (yarn ? 1.0 + 0.1 * log(1.0 / scale) : 1.0);
     return MX_OK;
 }
 
 int mx_rope(mx_stream_t s, const uint16_t* x, uint64_t x_stride, uint16_t* y, uint64_t y_stride, const int32_t* positions, const double* freqs, uint32_t T,
-            uint32_t n_heads, uint32_t D, uint32_t n_rot, int interleaved, float mscale) {
+            uint32_t n_heads, uint32_t D, uint32_t n_rot, int interleaved, double mscale) {
     MX_REQUIRE_SHAPE(T > 0 && n_heads > 0 && n_heads <= 65535 && D > 0 && D <= 256 && D % 16 == 0);
     if (int rc = check_rows(x, x_stride, (uint64_t)n_heads * D)) return rc;
     if (int rc = check_rows(y, y_stride, (uint64_t)n_heads * D)) return rc;
@@ -365,7 +364,7 @@ int mx_rope(mx_stream_t s, const uint16_t* x, uint64_t x_stride, uint16_t* y, ui
 
 int mx_rope_kv_write_f16(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride,
                          uint16_t* q_out, uint64_t q_out_stride, uint16_t* k_cache, uint16_t* v_cache, const int32_t* positions, const int32_t* slots,
-                         const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved, float mscale,
+                         const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved, double mscale,
                          uint32_t n_pages, uint32_t page_size) {
     MX_REQUIRE_PTR(freqs);
     return rope_kv_write(s, false, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, k_cache, nullptr, v_cache, nullptr, positions, slots, freqs, T, Hq,
@@ -374,7 +373,7 @@ int mx_rope_kv_write_f16(mx_stream_t s, const uint16_t* q, uint64_t q_stride, co
 int mx_rope_kv_write_q8_0(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride,
                           uint16_t* q_out, uint64_t q_out_stride, int8_t* k_qs, uint16_t* k_d, int8_t* v_qs, uint16_t* v_d, const int32_t* positions,
                           const int32_t* slots, const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved,
-                          float mscale, uint32_t n_pages, uint32_t page_size) {
+                          double mscale, uint32_t n_pages, uint32_t page_size) {
     MX_REQUIRE_PTR(freqs);
     return rope_kv_write(s, true, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, k_qs, k_d, v_qs, v_d, positions, slots, freqs, T, Hq, Hkv, D, n_rot,
                          interleaved, mscale, n_pages, page_size);
@@ -382,11 +381,11 @@ int mx_rope_kv_write_q8_0(mx_stream_t s, const uint16_t* q, uint64_t q_stride, c
 int mx_kv_write_f16(mx_stream_t s, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride, uint16_t* k_cache, uint16_t* v_cache,
                     const int32_t* slots, uint32_t T, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size) {
     return rope_kv_write(s, false, nullptr, 0, k, k_stride, v, v_stride, nullptr, 0, k_cache, nullptr, v_cache, nullptr, nullptr, slots, nullptr, T, 0, Hkv, D, 0, 0,
-                         1.f, n_pages, page_size);
+                         1.0, n_pages, page_size);
 }
 int mx_kv_write_q8_0(mx_stream_t s, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride, int8_t* k_qs, uint16_t* k_d, int8_t* v_qs,
                      uint16_t* v_d, const int32_t* slots, uint32_t T, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size) {
-    return rope_kv_write(s, true, nullptr, 0, k, k_stride, v, v_stride, nullptr, 0, k_qs, k_d, v_qs, v_d, nullptr, slots, nullptr, T, 0, Hkv, D, 0, 0, 1.f, n_pages,
+    return rope_kv_write(s, true, nullptr, 0, k, k_stride, v, v_stride, nullptr, 0, k_qs, k_d, v_qs, v_d, nullptr, slots, nullptr, T, 0, Hkv, D, 0, 0, 1.0, n_pages,
                          page_size);
 }
 int mx_kv_read_f16(mx_stream_t s, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* page_table, uint32_t max_pages, const int32_t* rows,

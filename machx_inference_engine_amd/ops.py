@@ -850,7 +850,7 @@ def kv_cache(fmt, n_pages, n_kv_heads, page_size, head_dim, device="cuda"):
 def rope_freqs(n_rot, base=10000.0, scale=1.0, ext_factor=0.0, attn_factor=1.0, beta_fast=32.0, beta_slow=1.0, n_ctx_orig=0, factors=None):
     """-> (float64 [n_rot / 2] on the host: radians a position, mscale).  scale: 1 / the factor by which the context grows; ext_factor > 0: YaRN;
     factors: a divisor for every pair."""
-    freqs, mscale = np.empty(n_rot // 2, np.float64), np.empty(1, np.float32)
+    freqs, mscale = np.empty(n_rot // 2, np.float64), np.empty(1, np.float64)
     f = None if factors is None else np.ascontiguousarray(factors, np.float32)
     _want(f is None or f.shape == freqs.shape, "factors: one for every pair")
     _host("mx_rope_freqs", n_rot, float(base), float(scale), float(ext_factor), float(attn_factor), float(beta_fast), float(beta_slow), n_ctx_orig,
@@ -864,9 +864,12 @@ def rope(x, positions, freqs, interleaved=False, mscale=1.0, y=None):
     T, H, D = shape
     if y is None:
         y = _new_rows(x)
+        to = y.data_ptr(), H * D
+    else:
+        to = _rows(y, shape, dev, "y")
     if positions.numel() != T:
         raise ValueError("positions: one for each row")
-    rc = lib.mx_rope(_stream(), *_rows(x, shape, dev, "x"), *_rows(y, shape, dev, "y"), _dev(positions, torch.int32, dev, "positions"),
+    rc = lib.mx_rope(_stream(), *_rows(x, shape, dev, "x"), *to, _dev(positions, torch.int32, dev, "positions"),
                      _dev(freqs, torch.float64, dev, "freqs"), T, H, D, 2 * freqs.numel(), interleaved, mscale)
     if rc != 0:
         raise MxError("mx_rope", rc)
@@ -880,11 +883,14 @@ def rope_kv_write(q, k, v, positions, slots, cache, freqs, interleaved=False, ms
     T, Hq, Dq = q_shape
     if q_out is None:
         q_out = _new_rows(q)
+        to = q_out.data_ptr(), Hq * Dq
+    else:
+        to = _rows(q_out, q_shape, dev, "q_out")
     if Dq != D or positions.numel() != T or slots.numel() != T:
         raise ValueError("q has the cache's D, positions and slots one entry for each row")
     kv_shape = (T, Hkv, D)
     fn = lib.mx_rope_kv_write_f16 if len(planes) == 2 else lib.mx_rope_kv_write_q8_0
-    rc = fn(_stream(), *_rows(q, q_shape, dev, "q"), *_rows(k, kv_shape, dev, "k"), *_rows(v, kv_shape, dev, "v"), *_rows(q_out, q_shape, dev, "q_out"), *planes,
+    rc = fn(_stream(), *_rows(q, q_shape, dev, "q"), *_rows(k, kv_shape, dev, "k"), *_rows(v, kv_shape, dev, "v"), *to, *planes,
             _dev(positions, torch.int32, dev, "positions"), _dev(slots, torch.int32, dev, "slots"), _dev(freqs, torch.float64, dev, "freqs"), T, Hq, Hkv, D,
             2 * freqs.numel(), interleaved, mscale, n_pages, page_size)
     if rc != 0:

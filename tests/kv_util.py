@@ -24,14 +24,14 @@ def rope(x, pos, f, inter, mscale=1.0):
 
 
 def rope_tol(x, f, inter, mscale=1.0):
-    """A rounding to fp16 (half a step, 2^-11 of the value; 2^-25 below its normal range) and 32-bit sines and products: each of the two products has
-    its sine's error (2^-24 of the angle's rounding, 2^-24 of the polynomial's, 2^-24 of mscale's product), the product's and the sum's 2^-24."""
+    """Beside the rounding to fp16 (half a step, 2^-11 of the value; 2^-25 below its normal range), which the caller counts: each of the two products
+    has its sine's rounding (2^-24) and its own, the sum one more; the sines themselves are off by 2^-34."""
     x = np.abs(np.asarray(x, np.float64))
     n = 2 * len(f)
     i0, i1 = (np.arange(0, n, 2), np.arange(1, n, 2)) if inter else (np.arange(n // 2), np.arange(n // 2, n))
     size = np.zeros_like(x)
     size[..., i0] = size[..., i1] = mscale * (x[..., i0] + x[..., i1])
-    return size * 6 * 2.0 ** -24
+    return size * (3 * 2.0 ** -24 + 2.0 ** -33)
 
 
 def q8_0(x):
