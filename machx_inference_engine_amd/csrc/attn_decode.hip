@@ -143,15 +143,19 @@ __device__ __forceinline__ half2_t bytes_f16(uint32_t w, uint32_t sel) {
     return __builtin_bit_cast(half2_t, pick(w, 0x64646464u, sel)) + bias;
 }
 
-// One workgroup takes one key-value head of one sequence, up to 16 of the query heads that share it, and one chunk of the tokens; its waves take the
-// chunk's tiles of 32 tokens in turn, each with a running maximum and sum of its own.
+// A workgroup takes one key-value head, up to 16 of the query heads that share it, and a sequence or a share of the sequences' tiles; its waves take the tiles in turn,
+// each with a running maximum and sum of its own.  Bound by the cache's bytes: 64 x 8192 fp16 tokens of 8 heads of 128 in 322 us, 6.7 TB/s (a plain copy of that size moves 4.9, reads
+// alone reach 6.3 to 7.1); what a launch has beside them is 5 us from its start to its first tile and from its last one to its end.
 //
-// Scores: S^T[token][head] = K Q^T, mfma 16x16x32 with K's rows as they lie (a lane loads 8 elements of one token).  Row r of the two 16-row products of
-// a tile is token 8 (r / 4) + r % 4 (+ 4), so that a lane, which gets 4 rows of a product, ends up with the 8 consecutive tokens 8g .. 8g + 7 of one head (g = lane / 16):
-// exactly the operand layout of the second product, O^T[d][head] += V^T P^T, whose other operand is 8 tokens of one d a lane.  A
-// lane loads elements E c .. E c + E - 1 (c = lane % 16, E = DP / 16) of its 8 tokens, whole rows by 16 lanes, and turns them in registers by byte permutes;
-// nothing goes through LDS before the end.  The weights are two fp16 parts, the second what the first's rounding left (2^-21 of it), so only the result's rounding to
-// fp16 is felt.  Q8_0: keys are exact as fp16 integers and their scales are folded into the fp32 products of each block; values are rounded to fp16 as they are dequantised.
+// Scores: S^T[token][head] = K Q^T, mfma 16x16x32.  Keys come in whole rows, 16 bytes a lane (read as the operand wants them, 16 rows a load, they kept the address units
+// busy: Q8_0 99 -> 56 us for one sequence of 131071), and reach the operand through an LDS tile of the wave's own.  Row r of the two 16-row products of a tile is
+// token 8 (r / 4) + r % 4 (+ 4), so that a lane, which gets 4 rows of a product, ends up with the 8 consecutive tokens 8g .. 8g + 7 of one head (g = lane / 16): exactly
+// the operand layout of the second product, O^T[d][head] += V^T P^T, whose other operand is 8 tokens of one d a lane.  A lane loads elements E c .. E c + E - 1 (c = lane % 16,
+// E = DP / 16) of its 8 tokens, whole rows by 16 lanes, and turns them in registers by byte permutes.
+//
+// Only the result is rounded to fp16: scores, maxima and sums are fp32, and the matrix instruction's fp16 operands carry the weights in two parts, the second what the first's
+// rounding left (to 2^-22).  Q8_0: keys are exact as fp16 integers and their scales are folded into the fp32 products of each block; values are q d in two parts, which hold it
+// exactly (8 + 11 bits; d and so q d are multiples of 2^-24).  One part would be 3 % faster and 1.4 times as far off.
 template <bool Q8, int DP, int NBLK, bool FULL>
 __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 ? 3 : 2) void attn_decode_kernel(AttnArgs a) {
     constexpr int E = DP / 16, NB = DP / 32;
@@ -395,14 +399,18 @@ __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 
             // ---- values
 #pragma unroll
             for (int e = 0; e < E; e += 2) {
-                half8 f0, f1;   // elements e and e + 1 of 8 tokens
+                half8 f0, f1, g0, g1;   // elements e and e + 1 of 8 tokens; Q8_0: what their rounding to fp16 left
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     half2_t h0, h1;
                     if (Q8) {
                         const uint32_t both = pick(vr[2 * w + 1][e / 4] , vr[2 * w][e / 4], e & 2 ? 0x07030602u : 0x05010400u) ^ 0x80808080u;
-                        h0 = bytes_f16(both, 0x00050004u) * half2_t{sc[2 * w], sc[2 * w + 1]};
-                        h1 = bytes_f16(both, 0x00070006u) * half2_t{sc[2 * w], sc[2 * w + 1]};
+                        const half2_t d = {sc[2 * w], sc[2 * w + 1]}, q0 = bytes_f16(both, 0x00050004u), q1 = bytes_f16(both, 0x00070006u);
+                        h0 = q0 * d;
+                        h1 = q1 * d;
+                        const half2_t l0 = __builtin_elementwise_fma(q0, d, -h0), l1 = __builtin_elementwise_fma(q1, d, -h1);
+                        g0[2 * w] = l0[0]; g0[2 * w + 1] = l0[1];
+                        g1[2 * w] = l1[0]; g1[2 * w + 1] = l1[1];
                     } else {
                         h0 = __builtin_bit_cast(half2_t, pick(vr[2 * w + 1][e / 2], vr[2 * w][e / 2], 0x05040100u));
                         h1 = __builtin_bit_cast(half2_t, pick(vr[2 * w + 1][e / 2], vr[2 * w][e / 2], 0x07060302u));
@@ -414,6 +422,10 @@ __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 
                 o[e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f1, hi, o[e + 1], 0, 0, 0);
                 o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f0, lo, o[e], 0, 0, 0);
                 o[e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f1, lo, o[e + 1], 0, 0, 0);
+                if (Q8) {
+                    o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(g0, hi, o[e], 0, 0, 0);
+                    o[e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(g1, hi, o[e + 1], 0, 0, 0);
+                }
             }
             if (more) {
                 load_v(next);

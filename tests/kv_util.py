@@ -86,9 +86,9 @@ def keep_only(cache, table, lens, ps):
 
 
 def attention(q, cache, table, lens, ps, scale, window=0, sinks=None, k_rounded=None):
-    """-> (out, tolerance) in fp64 [B, Hq, D].  The tolerance: one rounding of the result to fp16 (2^-11 of it, 2^-25 below the normal range), one of the
-    values (a Q8_0 value becomes fp16 before its product: 2^-11 of it), 2^-20 for the weights' two fp16 parts and the sums, and what the
-    32-bit scores are off, e: D + 16 roundings of 2^-24 of the products' magnitudes, and 2^-21 of the score itself in its exponential."""
+    """-> (out, tolerance) in fp64 [B, Hq, D].  The tolerance: one rounding of the result to fp16 (2^-11 of it, 2^-25 below the normal range), 2^-20 for the weights' and
+    values' two fp16 parts and the sums, 2^-25 of the largest weight where a weight's second part is below fp16's range, and what the 32-bit scores are off,
+    e: D + 16 roundings of 2^-24 of the products' magnitudes, and 2^-21 of the score itself in its exponential."""
     q = np.asarray(q, np.float64)
     K, V = stored(cache)
     B, Hq, D = q.shape
@@ -111,5 +111,5 @@ def attention(q, cache, table, lens, ps, scale, window=0, sinks=None, k_rounded=
             total = p.sum() + (np.exp(sinks[h] - top) if sinks is not None else 0.0)
             out[b, h] = p @ v / total
             size = p @ np.abs(v) / total
-            tol[b, h] += 2.0 ** -11 * np.abs(out[b, h]) + size * ((2.0 ** -11 if len(cache) == 4 else 0.0) + 2.0 ** -20 + 3 * e)
+            tol[b, h] += 2.0 ** -11 * np.abs(out[b, h]) + size * (2.0 ** -20 + 3 * e) + 2.0 ** -25 * np.abs(v).sum(0) / total
     return out, tol
