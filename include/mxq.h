@@ -729,6 +729,7 @@ int mx_kv_read_q8_0(mx_stream_t s, const int8_t* k_qs, const uint16_t* k_d, cons
  * whose page is outside [0, n_pages) count as masked; what the cache holds behind a sequence's end is never used, whatever it is.
  * out: [B][Hq][D] fp16; out_q8 (may be NULL, Hq * D % 32 == 0): the block_q8_1x stream of the rounded out, as the output
  * projection's int-dot product takes it, bit-identical to mx_quantize_q8_1(out).
+ * B <= 65535; the tiles of 32 tokens that B full tables could hold must count less than 2^31.
  * max_len: no sequence is expected to be longer; it decides how the lengths are split over workgroups (longer ones are right, and slower).  ws: 16-byte aligned,
  * mx_attn_decode_ws_bytes of the same arguments (0 bytes: NULL will do); its contents on entry do not matter.  */
 int mx_attn_decode_ws_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t max_len, uint32_t window, uint64_t* bytes);

@@ -489,8 +489,8 @@ __global__ __launch_bounds__(512) void attn_join_kernel(AttnArgs a, uint32_t gro
     const uint32_t row = blockIdx.x, b = row / a.Hq, h = row - b * a.Hq, tid = threadIdx.x, lane = tid & 63u;
     const uint32_t per = a.D / 4, part = tid / per, d = (tid - part * per) * 4;
     const uint2 parts = *reinterpret_cast<const uint2*>(a.parts + 2 * b);
-    const uint32_t first = parts.x, n = parts.y;
-    if (n == 1) return;                      // the result is there
+    // the only sequence's parts begin at 0: they can be requested before their number is known, up to what there is room for
+    const uint32_t first = a.B == 1 ? 0u : parts.x, room = a.B == 1 ? a.shares : parts.y;
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)first * a.Hq + h;
     const float* po = a.part_o + ((size_t)first * a.Hq + h) * a.D + d;
     const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
@@ -501,12 +501,18 @@ __global__ __launch_bounds__(512) void attn_join_kernel(AttnArgs a, uint32_t gro
 #pragma unroll
     for (uint32_t i = 0; i < kAhead; ++i) {
         const uint32_t s = part + i * groups;
-        const bool there = part < groups && s < n;
+        const bool there = part < groups && s < room;
         ahead[i] = there ? *reinterpret_cast<const floatx4*>(po + (size_t)s * a.Hq * a.D) : floatx4{0.f, 0.f, 0.f, 0.f};
         peak[i] = there ? ml[(size_t)s * a.Hq].x : -INFINITY;
     }
     // every wave finds the maximum and the sum for itself
-    const float2 own = lane < n ? ml[(size_t)lane * a.Hq] : make_float2(-INFINITY, 0.f);
+    float2 own = lane < room ? ml[(size_t)lane * a.Hq] : make_float2(-INFINITY, 0.f);
+    const uint32_t n = parts.y;
+    if (n == 1) return;                      // the result is there
+    if (lane >= n) own = make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i)
+        if (part + i * groups >= n) peak[i] = -INFINITY;
     float top = fmaxf(own.x, sink);
     for (uint32_t s = lane + 64; s < n; s += 64) top = fmaxf(top, ml[(size_t)s * a.Hq].x);
     top = fmaxf(top, dpp_f<0xB1>(top));
@@ -523,7 +529,8 @@ __global__ __launch_bounds__(512) void attn_join_kernel(AttnArgs a, uint32_t gro
     floatx4 sum = {0.f, 0.f, 0.f, 0.f};
     if (part < groups) {
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) sum += __builtin_amdgcn_exp2f(peak[i] - ref) * ahead[i];
+        for (uint32_t i = 0; i < kAhead; ++i)
+            if (part + i * groups < n) sum += __builtin_amdgcn_exp2f(peak[i] - ref) * ahead[i];
         for (uint32_t s = part + kAhead * groups; s < n; s += groups)
             sum += __builtin_amdgcn_exp2f(ml[(size_t)s * a.Hq].x - ref) * *reinterpret_cast<const floatx4*>(po + (size_t)s * a.Hq * a.D);
         if (groups > 1) *reinterpret_cast<floatx4*>(sums + part * a.D + d) = sum;
@@ -548,7 +555,7 @@ struct Plan {
 constexpr uint32_t kDirectTiles = 4 * kWaves;
 static Plan plan_of(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t max_len, uint32_t window) {
     const uint32_t span = window && window < max_len ? window : max_len;
-    const uint64_t tiles = span / kTile + (window && window < max_len ? 2 : 1), all = B * tiles;
+    const uint64_t tiles = window && window < max_len ? span / kTile + 2 : (span + (uint64_t)kTile - 1) / kTile, all = B * tiles;   // a window may begin within a tile
     const uint64_t groups = (uint64_t)Hkv * ((Hq / Hkv + 15) / 16);
     if (tiles <= kDirectTiles) return {0, 0};
     auto up = [](uint64_t x, uint64_t y) { return (x + y - 1) / y; };

@@ -73,6 +73,60 @@ def test_window_and_sinks(mx, fmt, window, with_sinks):
 
 
 @pytest.mark.parametrize("fmt", ["f16", "q8_0"])
+@pytest.mark.parametrize("B,Hkv,G,D", [(150, 1, 4, 64), (70, 2, 24, 128), (65, 1, 2, 256), (300, 3, 1, 96)])
+def test_many_ragged_sequences_in_equal_shares(mx, fmt, B, Hkv, G, D):
+    """More sequences than a wave has lanes, empty ones among them (the first and the last too), shares that end in the middle of some and span others."""
+    rng = np.random.default_rng(B)
+    lens = [int(n) if rng.random() < 0.8 else 0 for n in np.exp(rng.uniform(0, np.log(900), B))]
+    lens[0] = lens[-1] = 0
+    lens[B // 2] = 2500
+    rng, table, cache, q = case(fmt, lens, Hkv, G, D, 16, B)
+    sinks = rng.standard_normal(Hkv * G).astype(np.float32)
+    y = mx.ops.attn_decode(dev(q), cache, dev(table), dev(np.array(lens, np.int32)), sinks=dev(sinks))
+    near(host(y), *U.attention(q, cache, table, lens, 16, D ** -0.5, sinks=sinks), "B=%d" % B)
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q8_0"])
+@pytest.mark.parametrize("n", [513, 544, 640, 1024, 1025, 4096, 16385])
+def test_one_sequence_in_shares(mx, fmt, n):
+    """Lengths around those at which the number of shares changes, with a length in front of what max_len says and behind it."""
+    rng, table, cache, q = case(fmt, [n], 2, 4, 64, 32, n)
+    for m in (n, n - 1, n // 2, 33, 1, 0):
+        lens = np.array([m], np.int32)
+        want, tol = U.attention(q, cache, table, lens, 32, 0.125)
+        for max_len in (n, 600):
+            near(host(mx.ops.attn_decode(dev(q), cache, dev(table), dev(lens), max_len=max_len)), want, tol, "%d of %d, max_len %d" % (m, n, max_len))
+
+
+def test_pages_of_sixteen_times_any_number(mx):
+    for ps in (16, 48, 80, 112, 1008, 4096):
+        lens = [700, 1001, 0, ps + 1]
+        rng, table, cache, q = case("q8_0", lens, 1, 4, 64, ps, ps)
+        y = mx.ops.attn_decode(dev(q), cache, dev(table), dev(np.array(lens, np.int32)), window=900)
+        near(host(y), *U.attention(q, cache, table, lens, ps, 0.125, 900), "pages of %d" % ps)
+
+
+def test_refusals(mx):
+    ops = mx.ops
+    cache, tab, lens = ops.kv_cache("f16", 4, 2, 16, 64), dev(np.zeros((3, 4), np.int32)), dev(np.ones(3, np.int32))
+    q = torch.zeros(3, 8, 64, dtype=torch.float16, device="cuda")
+    ok = dict(q=q, cache=cache, page_table=tab, seq_lens=lens)
+    ops.attn_decode(**ok)
+    for bad in (dict(q=q.float()), dict(q=q.cpu()), dict(q=q[:2]), dict(q=q[..., :48]), dict(q=q.transpose(1, 2).contiguous().transpose(1, 2)), dict(page_table=tab.long()),
+                dict(page_table=tab[:, ::2]), dict(page_table=tab[:2]), dict(seq_lens=lens[:2]), dict(seq_lens=lens.cpu()), dict(sinks=torch.zeros(7, device="cuda")),
+                dict(sinks=torch.zeros(8, device="cuda").half()), dict(out=q[:2]), dict(out=q.float()), dict(out=torch.zeros(3, 9, 64, device="cuda").half()[:, :8]),
+                dict(out_q8=torch.zeros(5, dtype=torch.uint8, device="cuda")), dict(cache=cache[:1]), dict(cache=(cache[0], cache[1][:3])),
+                dict(cache=(cache[0].transpose(1, 2), cache[1].transpose(1, 2))), dict(cache=(cache[0].float(), cache[1])), dict(cache=(cache[0].cpu(), cache[1])),
+                dict(cache=ops.kv_cache("q8_0", 4, 2, 16, 64)[:3])):
+        with pytest.raises(ValueError):
+            ops.attn_decode(**{**ok, **bad})
+    for bad in (dict(q=torch.zeros(3, 7, 64, dtype=torch.float16, device="cuda")), dict(max_len=100000, ws=torch.zeros(16, device="cuda")), dict(cache=ops.kv_cache("f16", 4, 2, 24, 64)),
+                dict(q=torch.zeros(3 * 516, dtype=torch.float16, device="cuda").as_strided((3, 8, 64), (516, 64, 1)))):
+        with pytest.raises(mx.ops.MxError):
+            ops.attn_decode(**{**ok, **bad})
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q8_0"])
 def test_what_the_window_left_behind_is_not_read(mx, fmt):
     """Pages in front of the window are given back: their entries name no page, and NaN lies in the slots in front of it."""
     ps, window, n = 16, 40, 203

@@ -220,3 +220,54 @@ def test_write_then_read_and_a_captured_step(mx):
             torch.cuda.synchronize()
             replayed = [t.clone() for t in out]
             assert all(torch.equal(a, b) for a, b in zip(replayed, step()))
+
+
+def test_refusals(mx):
+    ops = mx.ops
+    x, pos, f = torch.zeros(3, 4, 64, dtype=torch.float16, device="cuda"), dev(np.zeros(3, np.int32)), dev(U.freqs(64))
+    for bad in (dict(x=x.float()), dict(x=x.cpu()), dict(x=x.transpose(1, 2).contiguous().transpose(1, 2)),
+                dict(positions=pos.long()), dict(positions=pos[:2]), dict(freqs=f.float()), dict(freqs=f.cpu()), dict(y=x[:2]), dict(y=x.float())):
+        with pytest.raises(ValueError):
+            ops.rope(**{**dict(x=x, positions=pos, freqs=f), **bad})
+    for bad in (dict(freqs=dev(U.freqs(128))), dict(freqs=dev(U.freqs(24))), dict(x=x[:0], positions=pos[:0])):
+        with pytest.raises(mx.ops.MxError):
+            ops.rope(**{**dict(x=x, positions=pos, freqs=f), **bad})
+    cache, slots = ops.kv_cache("q8_0", 2, 4, 16, 64), dev(np.arange(3, dtype=np.int32))
+    ok = dict(q=x, k=x, v=x, positions=pos, slots=slots, cache=cache, freqs=f)
+    ops.rope_kv_write(**ok)
+    for bad in (dict(k=x[:, :2]), dict(v=x[:2]), dict(q=x[..., :32]), dict(slots=slots[:2]), dict(slots=slots.long()), dict(positions=pos[:1]), dict(cache=cache[:2]),
+                dict(cache=cache[:3]), dict(cache=(cache[0], cache[1], cache[2], cache[3][..., :1])), dict(q_out=x[:2]), dict(cache=tuple(t.cpu() for t in cache))):
+        with pytest.raises(ValueError):
+            ops.rope_kv_write(**{**ok, **bad})
+    with pytest.raises(ValueError):
+        ops.kv_write(x[:, :1], x, slots, cache)
+    tab, rows = dev(np.zeros((2, 1), np.int32)), dev(np.array([0, 3, 5], np.int32))
+    for bad in (dict(rows=rows[:2]), dict(rows=rows.long()), dict(page_table=tab.long()), dict(out=(x, x)), dict(cache=cache[:3])):
+        with pytest.raises(ValueError):
+            ops.kv_read(**{**dict(cache=cache, page_table=tab, rows=rows, total_rows=5), **bad})
+    with pytest.raises(mx.ops.MxError):
+        ops.kv_read(cache, tab, rows, 0)
+    with pytest.raises(ValueError):
+        ops.kv_cache("q8_0", 2, 4, 16, 80)
+    with pytest.raises(mx.ops.MxError):
+        ops.rope_freqs(24)
+
+
+@pytest.mark.parametrize("T", [5, 600])
+def test_rows_beside_each_other_keep_their_neighbours(mx, T):
+    """q, k and v as parts of wider rows, q_out as a part of another: what lies between them is neither read as theirs nor written."""
+    rng = np.random.default_rng(T)
+    Hq, Hkv, D, ps = 4, 2, 64, 16
+    wide = torch.full((T, 1024), float("nan"), dtype=torch.float16, device="cuda")
+    parts = [wide[:, 64: 64 + Hq * D], wide[:, 384: 384 + Hkv * D], wide[:, 640: 640 + Hkv * D]]
+    for p in parts:
+        p.copy_(dev(rows(rng, T, 1, p.shape[1])).view(T, -1))
+    q, k, v = (p.view(T, -1, D) for p in parts)
+    to = torch.full((T, 512), 3.0, dtype=torch.float16, device="cuda")
+    cache = mx.ops.kv_cache("f16", -(-T // ps), Hkv, ps, D)
+    pos, slots, f = dev(np.arange(T, dtype=np.int32)), dev(np.arange(T, dtype=np.int32)), dev(U.freqs(D))
+    mx.ops.rope_kv_write(q, k, v, pos, slots, cache, f, q_out=to[:, 128: 128 + Hq * D].view(T, Hq, D))
+    assert torch.equal(to[:, 128: 384].view(T, Hq, D), mx.ops.rope(q.contiguous(), pos, f))
+    assert (to[:, :128] == 3).all() and (to[:, 384:] == 3).all()
+    at = torch.arange(T, device="cuda")
+    assert torch.equal(cache[0][at // ps, :, at % ps], mx.ops.rope(k.contiguous(), pos, f)) and torch.equal(cache[1][at // ps, :, at % ps], v.contiguous())
