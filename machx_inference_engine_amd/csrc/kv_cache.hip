@@ -143,7 +143,7 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(RowsArgs a) {
 template <bool ROPE, bool Q8, bool INTER>
 __global__ __launch_bounds__(kRowThreads) void prompt_kernel(RowsArgs a) {
     __shared__ float2 cs[128];
-    const uint32_t tid = threadIdx.x, t = blockIdx.x, D = a.chunks * 8, pairs = a.chunks / 2, items = (a.Hq + 2 * a.Hkv) * pairs, half_chunks = a.n_rot / 16;
+    const uint32_t tid = threadIdx.x, threads = blockDim.x, t = blockIdx.x, D = a.chunks * 8, pairs = a.chunks / 2, items = (a.Hq + 2 * a.Hkv) * pairs, half_chunks = a.n_rot / 16;
     struct Item {
         uint32_t h, c0, c1;
         bool together, angle;
@@ -167,12 +167,12 @@ __global__ __launch_bounds__(kRowThreads) void prompt_kernel(RowsArgs a) {
     if (tid < items) next = load(tid);
     const uint32_t slot = a.slots ? (uint32_t)a.slots[t] : 0u;
     if (ROPE) {
-        if (tid < a.n_rot / 2) cs[tid] = cs_of(a, t, tid);
+        for (uint32_t i = tid; i < a.n_rot / 2; i += threads) cs[i] = cs_of(a, t, i);
         __syncthreads();
     }
-    for (uint32_t i = tid; i < items; i += kRowThreads) {
+    for (uint32_t i = tid; i < items; i += threads) {
         const Item m = next;
-        if (i + kRowThreads < items) next = load(i + kRowThreads);
+        if (i + threads < items) next = load(i + threads);
         half8 y0 = m.x0, y1 = m.x1;
         if (m.together) {
             y0 = turn_first(m.x0, m.x1, cs + m.c0 * 8);
@@ -196,8 +196,10 @@ static int launch_rows(mx_stream_t s, RowsArgs a, uint32_t T, int interleaved) {
     // 2047 tokens of 32 + 4 + 4 heads of 128 into a Q8_0 cache 14.5 -> 9.4; interleaved pairs are as fast either way.  Fewer tokens leave CUs without work: one
     // token 2.2 -> 2.8 us, 333 (18 heads of 256) 3.9 -> 4.1.
     if (T >= kPromptTokens && (!Q8 || (a.chunks % 8 == 0 && a.n_rot % 64 == 0))) {
+        // as many waves as the token's pairs of chunks fill evenly
+        const uint32_t items = (a.Hq + 2 * a.Hkv) * (a.chunks / 2), turns = (items + kRowThreads - 1) / kRowThreads, threads = ((items + turns - 1) / turns + 63) / 64 * 64;
         auto launch = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(T), dim3(kRowThreads), 0, as_stream(s), a);
+            hipLaunchKernelGGL(kernel, dim3(T), dim3(threads), 0, as_stream(s), a);
             return launch_status();
         };
         return ROPE && interleaved ? launch(prompt_kernel<ROPE, Q8, ROPE>) : launch(prompt_kernel<ROPE, Q8, false>);
@@ -208,8 +210,11 @@ static int launch_rows(mx_stream_t s, RowsArgs a, uint32_t T, int interleaved) {
     return launch_status();
 }
 
-// Reading back: a workgroup takes 16 tokens of one sequence (they lie in one page) and all heads, a thread 8 elements at a time.
+// Reading back: a workgroup takes 16 tokens of one sequence (they lie in one page) and 1024 pieces of 8 elements of their keys and values, a thread four, which it
+// requests before it writes the first (4 ragged sequences of 300 tokens with 8 heads of 128, with their write: 11.8 us one after the other, 6.3; long ones run at a
+// copy's rate: 10 k tokens of them in 15.9 us, 5.1 TB/s).
 // Tile numbers are dealt by floor(rows[b] / 16) + b, which leaves room for every sequence's ceil(length / 16).
+constexpr int kReadPieces = 4;
 template <bool Q8, bool STREAM>
 __global__ __launch_bounds__(256) void kv_read_kernel(const void* k_cache, const half_t* k_d, const void* v_cache, const half_t* v_d, const int32_t* page_table,
                                                       uint32_t max_pages, const int32_t* rows, half_t* k_out, half_t* v_out, uint32_t total, uint32_t B,
@@ -230,26 +235,43 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const void* k_cache, const
     const uint32_t count = min(16u, end - row0 - t0), col = t0 / page_size, D = chunks * 8;
     const uint32_t page = col < max_pages ? (uint32_t)page_table[(size_t)b * max_pages + col] : 0xFFFFFFFFu;
     const bool good = page < n_pages;
-    const uint32_t per_head = 16 * chunks, items = 2 * Hkv * per_head;
-    for (uint32_t i = threadIdx.x; i < items; i += 256) {
-        const uint32_t hh = i / per_head, r = i - hh * per_head, tok = r / chunks, c = r - tok * chunks;
-        if (tok >= count) continue;
-        const bool is_v = hh >= Hkv;
-        const uint32_t h = is_v ? hh - Hkv : hh;
-        half8 y = {};
-        if (good) {
+    const uint32_t per_head = 16 * chunks, items = 2 * Hkv * per_head, i0 = blockIdx.y * (256 * kReadPieces) + threadIdx.x;
+    constexpr int U = kReadPieces;
+    uint4 got[U];
+    half_t d[U];
+    uint32_t at[U];                      // token * heads * chunks + head * chunks + chunk, from the tile's first row
+    bool is_v[U], live[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t i = i0 + 256 * u, hh = i / per_head, r = i - hh * per_head, tok = r / chunks, c = r - tok * chunks;
+        live[u] = i < items && tok < count;
+        is_v[u] = hh >= Hkv;
+        const uint32_t h = is_v[u] ? hh - Hkv : hh;
+        at[u] = (tok * Hkv + h) * chunks + c;
+        got[u] = make_uint4(0, 0, 0, 0);
+        d[u] = (half_t)0.f;
+        if (live[u] && good) {
             const size_t crow = ((size_t)page * Hkv + h) * page_size + (t0 - col * page_size) + tok;
-            const void* cache = is_v ? v_cache : k_cache;
+            const void* cache = is_v[u] ? v_cache : k_cache;
             if (!Q8) {
-                y = *reinterpret_cast<const half8*>(static_cast<const half_t*>(cache) + crow * D + c * 8);
+                got[u] = *reinterpret_cast<const uint4*>(static_cast<const half_t*>(cache) + crow * D + c * 8);
             } else {
                 const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(cache) + crow * D + c * 8);
-                const float d = (float)(is_v ? v_d : k_d)[crow * (D / 32) + c / 4];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = f32_to_f16_rne((float)(int8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3))) * d);
+                got[u].x = w.x;
+                got[u].y = w.y;
+                d[u] = (is_v[u] ? v_d : k_d)[crow * (D / 32) + c / 4];
             }
         }
-        half8* const out = reinterpret_cast<half8*>((is_v ? v_out : k_out) + ((size_t)(row0 + t0 + tok) * Hkv + h) * D + c * 8);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (!live[u]) continue;
+        half8 y = __builtin_bit_cast(half8, got[u]);
+        if (Q8) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = f32_to_f16_rne((float)(int8_t)((j < 4 ? got[u].x : got[u].y) >> (8 * (j & 3))) * (float)d[u]);
+        }
+        half8* const out = reinterpret_cast<half8*>((is_v[u] ? v_out : k_out) + (size_t)(row0 + t0) * Hkv * D) + at[u];
         if (STREAM) __builtin_nontemporal_store(y, out);
         else *out = y;
     }
@@ -314,7 +336,7 @@ static int kv_read(mx_stream_t s, bool q8, const void* k, const uint16_t* k_d, c
     MX_REQUIRE_PTR(page_table); MX_REQUIRE_PTR(rows); MX_REQUIRE_PTR(k_out); MX_REQUIRE_PTR(v_out);
     MX_REQUIRE_SHAPE(B > 0 && B <= (1u << 24) && max_pages > 0 && total_rows > 0 && total_rows < (1u << 31));
     MX_REQUIRE_ALIGN(page_table, 4); MX_REQUIRE_ALIGN(rows, 4); MX_REQUIRE_ALIGN(k_out, 16); MX_REQUIRE_ALIGN(v_out, 16);
-    const dim3 grid(total_rows / 16 + B);
+    const dim3 grid(total_rows / 16 + B, (2 * Hkv * 16 * (D / 8) + 256 * kReadPieces - 1) / (256 * kReadPieces));
     auto launch = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, as_stream(s), k, reinterpret_cast<const half_t*>(k_d), v, reinterpret_cast<const half_t*>(v_d), page_table,
                            max_pages, rows, reinterpret_cast<half_t*>(k_out), reinterpret_cast<half_t*>(v_out), total_rows, B, Hkv, D / 8, n_pages, page_size);
