@@ -24,7 +24,7 @@ def near(got, want, tol, what):
 @pytest.mark.parametrize("inter", [False, True])
 @pytest.mark.parametrize("T,H,D,n_rot", [(1, 40, 128, 128), (3, 1, 16, 16), (7, 3, 64, 64), (5, 18, 256, 64), (2, 5, 80, 32), (33, 7, 96, 96), (4, 9, 112, 48),
                                          (300, 40, 128, 128), (6, 2, 256, 256), (2, 65, 32, 16), (512, 3, 64, 64), (777, 5, 128, 32),
-                                         (600, 9, 80, 48), (513, 2, 256, 128)])
+                                         (600, 9, 80, 48), (513, 2, 256, 128), (70001, 2, 16, 16)])
 def test_rope(mx, T, H, D, n_rot, inter):
     rng = np.random.default_rng(T * 1000 + D + n_rot)
     x, f = rows(rng, T, H, D), U.freqs(n_rot, 500000.0)
