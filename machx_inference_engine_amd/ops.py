@@ -794,9 +794,11 @@ def _want(ok, what):
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_F16, _F32, _F64, _I32, _I8 = torch.float16, torch.float32, torch.float64, torch.int32, torch.int8
 
 
-# These run before every launch of a decode step, so they ask for no more than they need: rope() into a given y takes 6.5 us, of
+# These run before every launch of a decode step, so they ask for no more than they need: rope() into a given y takes 5.9 us, of
 # which the launch is 4.
 def _dev(t, dtype, dev, what):
     """Address of a contiguous tensor of this type on the current device, whose number is `dev`."""
@@ -807,13 +809,15 @@ def _dev(t, dtype, dev, what):
 
 def _rows(t, shape, dev, what):
     """(address, elements from a row to the next) of fp16 rows [T, heads, D] whose heads lie side by side."""
-    if t.dtype is not torch.float16 or t.get_device() != dev or t.shape != shape:
+    if t.dtype is not _F16 or t.get_device() != dev or t.shape != shape:
         raise ValueError("%s must be a fp16 tensor [%d, %d, %d] on the current device" % ((what,) + tuple(shape)))
     T, H, D = shape
+    if t.is_contiguous():
+        return t.data_ptr(), H * D
     row, head, one = t.stride()
     if (one != 1 and D > 1) or (head != D and H > 1):
         raise ValueError("%s: the heads of a row must lie side by side" % what)
-    return t.data_ptr(), row if T > 1 else max(row, H * D) + -max(row, H * D) % 8
+    return t.data_ptr(), row
 
 
 def _new_rows(t):
@@ -827,13 +831,13 @@ def _cache(cache, dev):
         k, v = cache
         if v.shape != shape or len(shape) != 4:
             raise ValueError("the planes of a cache are [pages, heads, page size, D], both of one shape")
-        return (_dev(k, torch.float16, dev, "k"), _dev(v, torch.float16, dev, "v")), shape
+        return (_dev(k, _F16, dev, "k"), _dev(v, _F16, dev, "v")), shape
     _want(len(cache) == 4 and len(shape) == 4, "a cache is (k, v) or (k_qs, k_d, v_qs, v_d), planes [pages, heads, page size, D]")
     scales = shape[:3] + (shape[3] // 32,)
     if cache[2].shape != shape or cache[1].shape != scales or cache[3].shape != scales:
         raise ValueError("the planes of a cache have one shape, its scales one for each 32")
-    return (_dev(cache[0], torch.int8, dev, "k_qs"), _dev(cache[1], torch.float16, dev, "k_d"), _dev(cache[2], torch.int8, dev, "v_qs"),
-            _dev(cache[3], torch.float16, dev, "v_d")), shape
+    return (_dev(cache[0], _I8, dev, "k_qs"), _dev(cache[1], _F16, dev, "k_d"), _dev(cache[2], _I8, dev, "v_qs"),
+            _dev(cache[3], _F16, dev, "v_d")), shape
 
 
 def kv_cache(fmt, n_pages, n_kv_heads, page_size, head_dim, device="cuda"):
@@ -841,9 +845,9 @@ def kv_cache(fmt, n_pages, n_kv_heads, page_size, head_dim, device="cuda"):
     int8 of that shape with fp16 scales [..., head_dim / 32].  A token's slot is page * page_size + offset."""
     shape = (n_pages, n_kv_heads, page_size, head_dim)
     if fmt == "f16":
-        return tuple(torch.zeros(shape, dtype=torch.float16, device=device) for _ in range(2))
+        return tuple(torch.zeros(shape, dtype=_F16, device=device) for _ in range(2))
     _want(fmt == "q8_0" and head_dim % 32 == 0, "a cache is f16, or q8_0 with heads of whole blocks of 32")
-    plane = lambda: (torch.zeros(shape, dtype=torch.int8, device=device), torch.zeros(shape[:3] + (head_dim // 32,), dtype=torch.float16, device=device))  # noqa: E731
+    plane = lambda: (torch.zeros(shape, dtype=_I8, device=device), torch.zeros(shape[:3] + (head_dim // 32,), dtype=_F16, device=device))  # noqa: E731
     return plane() + plane()
 
 
@@ -869,8 +873,8 @@ def rope(x, positions, freqs, interleaved=False, mscale=1.0, y=None):
         to = _rows(y, shape, dev, "y")
     if positions.numel() != T:
         raise ValueError("positions: one for each row")
-    rc = lib.mx_rope(_stream(), *_rows(x, shape, dev, "x"), *to, _dev(positions, torch.int32, dev, "positions"),
-                     _dev(freqs, torch.float64, dev, "freqs"), T, H, D, 2 * freqs.numel(), interleaved, mscale)
+    rc = lib.mx_rope(_stream_of(dev), *_rows(x, shape, dev, "x"), *to, _dev(positions, _I32, dev, "positions"),
+                     _dev(freqs, _F64, dev, "freqs"), T, H, D, 2 * freqs.numel(), interleaved, mscale)
     if rc != 0:
         raise MxError("mx_rope", rc)
     return y
@@ -890,8 +894,8 @@ def rope_kv_write(q, k, v, positions, slots, cache, freqs, interleaved=False, ms
         raise ValueError("q has the cache's D, positions and slots one entry for each row")
     kv_shape = (T, Hkv, D)
     fn = lib.mx_rope_kv_write_f16 if len(planes) == 2 else lib.mx_rope_kv_write_q8_0
-    rc = fn(_stream(), *_rows(q, q_shape, dev, "q"), *_rows(k, kv_shape, dev, "k"), *_rows(v, kv_shape, dev, "v"), *to, *planes,
-            _dev(positions, torch.int32, dev, "positions"), _dev(slots, torch.int32, dev, "slots"), _dev(freqs, torch.float64, dev, "freqs"), T, Hq, Hkv, D,
+    rc = fn(_stream_of(dev), *_rows(q, q_shape, dev, "q"), *_rows(k, kv_shape, dev, "k"), *_rows(v, kv_shape, dev, "v"), *to, *planes,
+            _dev(positions, _I32, dev, "positions"), _dev(slots, _I32, dev, "slots"), _dev(freqs, _F64, dev, "freqs"), T, Hq, Hkv, D,
             2 * freqs.numel(), interleaved, mscale, n_pages, page_size)
     if rc != 0:
         raise MxError("mx_rope_kv_write", rc)
@@ -904,7 +908,7 @@ def kv_write(k, v, slots, cache):
     planes, (n_pages, Hkv, page_size, D) = _cache(cache, dev)
     T = slots.numel()
     fn = lib.mx_kv_write_f16 if len(planes) == 2 else lib.mx_kv_write_q8_0
-    rc = fn(_stream(), *_rows(k, (T, Hkv, D), dev, "k"), *_rows(v, (T, Hkv, D), dev, "v"), *planes, _dev(slots, torch.int32, dev, "slots"), T, Hkv, D, n_pages, page_size)
+    rc = fn(_stream_of(dev), *_rows(k, (T, Hkv, D), dev, "k"), *_rows(v, (T, Hkv, D), dev, "v"), *planes, _dev(slots, _I32, dev, "slots"), T, Hkv, D, n_pages, page_size)
     if rc != 0:
         raise MxError("mx_kv_write", rc)
 
@@ -916,14 +920,14 @@ def kv_read(cache, page_table, rows, total_rows, out=None):
     B, max_pages = page_table.shape
     shape = (total_rows, Hkv, D)
     if out is None:
-        k, v = torch.empty(shape, dtype=torch.float16, device=rows.device), torch.empty(shape, dtype=torch.float16, device=rows.device)
+        k, v = torch.empty(shape, dtype=_F16, device=rows.device), torch.empty(shape, dtype=_F16, device=rows.device)
     else:
         k, v = out
     if rows.numel() != B + 1 or k.shape != shape or v.shape != shape:
         raise ValueError("rows has one entry more than there are sequences, outputs are [total_rows, heads, D]")
     fn = lib.mx_kv_read_f16 if len(planes) == 2 else lib.mx_kv_read_q8_0
-    rc = fn(_stream(), *planes, _dev(page_table, torch.int32, dev, "page_table"), max_pages, _dev(rows, torch.int32, dev, "rows"), _dev(k, torch.float16, dev, "k_out"),
-            _dev(v, torch.float16, dev, "v_out"), total_rows, B, Hkv, D, n_pages, page_size)
+    rc = fn(_stream_of(dev), *planes, _dev(page_table, _I32, dev, "page_table"), max_pages, _dev(rows, _I32, dev, "rows"), _dev(k, _F16, dev, "k_out"),
+            _dev(v, _F16, dev, "v_out"), total_rows, B, Hkv, D, n_pages, page_size)
     if rc != 0:
         raise MxError("mx_kv_read", rc)
     return k, v
@@ -963,13 +967,13 @@ def attn_decode(q, cache, page_table, seq_lens, scale=None, window=0, sinks=None
     sinks_ptr = q8_ptr = None
     if sinks is not None:
         _want(sinks.numel() == Hq, "sinks: one for each query head")
-        sinks_ptr = _dev(sinks, torch.float32, dev, "sinks")
+        sinks_ptr = _dev(sinks, _F32, dev, "sinks")
     if out_q8 is not None:
         _want(out_q8.numel() * 32 == B * Hq * D * Q81X_BYTES, "out_q8: 40 bytes for each 32 elements of out")
         q8_ptr = _dev(out_q8, torch.uint8, dev, "out_q8")
     fn = lib.mx_attn_decode_f16 if len(planes) == 2 else lib.mx_attn_decode_q8_0
-    rc = fn(_stream(), *_rows(q, q_shape, dev, "q"), *planes, _dev(page_table, torch.int32, dev, "page_table"), max_pages, _dev(seq_lens, torch.int32, dev, "seq_lens"),
-            sinks_ptr, _dev(out, torch.float16, dev, "out"), q8_ptr, B, Hq, Hkv, D, n_pages, page_size, max_len, window, D ** -0.5 if scale is None else scale, ws_ptr,
+    rc = fn(_stream_of(dev), *_rows(q, q_shape, dev, "q"), *planes, _dev(page_table, _I32, dev, "page_table"), max_pages, _dev(seq_lens, _I32, dev, "seq_lens"),
+            sinks_ptr, _dev(out, _F16, dev, "out"), q8_ptr, B, Hq, Hkv, D, n_pages, page_size, max_len, window, D ** -0.5 if scale is None else scale, ws_ptr,
             ws_size)
     if rc != 0:
         raise MxError("mx_attn_decode", rc)
