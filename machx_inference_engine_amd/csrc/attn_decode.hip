@@ -6,6 +6,7 @@ namespace mxq {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kTile = 32, kWaves = 4, kLeastShare = kWaves;   // tokens of a tile, waves of a workgroup, tiles of a share at least
+constexpr float kShift = 15.f, kMostShifted = 1 << 20;   // what a running maximum lies below the largest score, scores for which it does (log2 units)
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -154,7 +155,8 @@ __device__ __forceinline__ half2_t bytes_f16(uint32_t w, uint32_t sel) {
 // E = DP / 16) of its 8 tokens, whole rows by 16 lanes, and turns them in registers by byte permutes.
 //
 // Only the result is rounded to fp16: scores, maxima and sums are fp32, and the matrix instruction's fp16 operands carry the weights in two parts, the second what the first's
-// rounding left (to 2^-22).  Q8_0: keys are exact as fp16 integers and their scales are folded into the fp32 products of each block; values are q d in two parts, which hold it
+// rounding left (to 2^-22, or 2^-40 of the largest weight: that is 2^15, not 1, so that the many small weights of a long sequence lie above fp16's smallest step; where
+// scores are so large that 15 of them could round to 16, it is 1).  Q8_0: keys are exact as fp16 integers and their scales are folded into the fp32 products of each block; values are q d in two parts, which hold it
 // exactly (8 + 11 bits; d and so q d are multiples of 2^-24).  One part would be 3 % faster and 1.4 times as far off.
 template <bool Q8, int DP, int NBLK, bool FULL>
 __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 ? 3 : 2) void attn_decode_kernel(AttnArgs a) {
@@ -377,7 +379,8 @@ __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 
             }
             // ---- running maximum and sum
             float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-            top = fmaxf(m, rows_max(top));
+            top = rows_max(top);
+            top = fmaxf(m, fabsf(top) < kMostShifted ? top - kShift : top);
             const float ref = top == -INFINITY ? 0.f : top;
             if (__any(top > m)) {
                 const float keep = __builtin_amdgcn_exp2f(m - ref);

@@ -206,6 +206,45 @@ def test_small_values_keep_their_precision(mx, fmt):
     near(host(mx.ops.attn_decode(dev(q), cache, dev(table), dev(np.array(lens, np.int32)))), want, tol, "small values")
 
 
+@pytest.mark.parametrize("fmt", ["f16", "q8_0"])
+@pytest.mark.parametrize("n", [480, 6000])
+@pytest.mark.parametrize("gap", [17.5, 20.0])
+def test_many_small_weights_are_not_lost(mx, fmt, n, gap):
+    """The first token of every tile outweighs each of the others by e^gap, which is below fp16's smallest step, but only they have values.  Of a value: its rounding,
+    2^-20 for the parts and sums and the score's error as elsewhere (one product, 2^-24 of it, and 2^-21 in its exponential); of all values 2^-40 of the largest weight."""
+    kv = np.zeros((2, 1, 1, -(-n // 16) * 16, 64), np.float32)
+    kv[0, ..., 0] = -gap
+    kv[0, 0, 0, ::32, 0] = 0.0
+    kv[1] = 512.0
+    kv[1, 0, 0, ::32] = 0.0
+    cache = tuple(dev(t.astype(np.float16)) for t in kv) if fmt == "f16" else tuple(dev(p) for t in kv for p in U.q8_0(t))
+    q = np.zeros((1, 2, 64), np.float16)
+    q[..., 0] = 8.0
+    table, lens, ps = np.zeros((1, 1), np.int32), np.array([n], np.int32), kv.shape[3]
+    want, _ = U.attention(q, cache, table, lens, ps, 0.125)
+    tol = want * (2.0 ** -11 + 2.0 ** -20 + 3 * gap * (2.0 ** -21 + 80 * 2.0 ** -24)) + 2.0 ** -25 + 2.0 ** -40 * 512 * 32
+    near(host(mx.ops.attn_decode(dev(q), cache, dev(table), dev(lens))), want, tol, "small weights")
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q8_0"])
+def test_scores_of_many_sizes(mx, fmt):
+    """Scores from 2^-8 to 2^29, of either sign, one sequence each: around them the distance between neighbouring 32-bit numbers passes 1.  All of a sequence are equal, so the
+    result is the mean of its values; a score's rounding is the same for all."""
+    B, n, ps = 76, 520, 544
+    size = np.concatenate([s * 2.0 ** np.arange(-8, 30) for s in (1, -1)])
+    kv = np.zeros((2, 1, 1, ps, 64), np.float32)
+    kv[0, ..., 0] = 127.0 * 128
+    kv[1] = np.random.default_rng(5).integers(-127, 128, (ps, 64))
+    kv[1, ..., ::32] = 127.0
+    cache = tuple(dev(t.astype(np.float16)) for t in kv) if fmt == "f16" else tuple(dev(p) for t in kv for p in U.q8_0(t))
+    q = np.zeros((B, 2, 64), np.float16)
+    q[..., 0] = (size * 2.0 ** -14 / (127.0 / 128))[:, None]
+    table, lens = np.zeros((B, 1), np.int32), np.full(B, n, np.int32)
+    want = U.stored(cache)[1][0, 0, :n].mean(0)
+    y = host(mx.ops.attn_decode(dev(q), cache, dev(table), dev(lens), scale=1.0)).astype(np.float64)
+    near(y, np.broadcast_to(want, y.shape), np.abs(want) * 2.0 ** -11 + 2.0 ** -20 * 127, "equal scores")
+
+
 def test_nan_and_infinity_of_a_sequence_stay_with_it(mx):
     lens = [70, 70, 70]
     for fmt in ("f16", "q8_0"):
