@@ -689,7 +689,8 @@ int mx_swiglu_oai_q8(mx_stream_t s, const uint16_t* gate, const uint16_t* up, ui
  * it quantises the fp16 values that the fp16 cache would hold.  A block that holds a NaN or an infinity reads back as NaN; one whose amax is
  * above 65471 has a scale whose 127-fold passes fp16 and reads back with infinities.  n_pages * page_size < 2^31; offsets into a plane take 64 bits.
  *
- * All row pointers and planes 16-byte aligned, strides multiples of 8.
+ * All row pointers and planes 16-byte aligned, strides multiples of 8.  What one launch cannot hold (2^32 threads) is refused: never T < 2^22 with
+ * T * D * (all heads, key and value heads too) < 2^34, nor total_rows / 16 + B < 2^24.
  *
  * mx_rope_freqs (host): freqs[i] = base^(-2i / n_rot) / factors[i] (factors: n_rot / 2 floats or NULL), slowed down by `scale` (1 / the
  * factor by which the context grows; 1: as trained).  ext_factor 0: every pair alike (linear).  ext_factor > 0 (YaRN): with dim(r) = n_rot ln(n_ctx_orig / (2 pi r)) / (2 ln base),
@@ -729,7 +730,7 @@ int mx_kv_read_q8_0(mx_stream_t s, const int8_t* k_qs, const uint16_t* k_d, cons
  * whose page is outside [0, n_pages) count as masked; what the cache holds behind a sequence's end is never used, whatever it is.
  * out: [B][Hq][D] fp16; out_q8 (may be NULL, Hq * D % 32 == 0): the block_q8_1x stream of the rounded out, as the output
  * projection's int-dot product takes it, bit-identical to mx_quantize_q8_1(out).
- * B <= 65535; the tiles of 32 tokens that B full tables could hold must count less than 2^31.
+ * B <= 65535, B * Hq < 2^26 (2^31 where ws_bytes is 0); the tiles of 32 tokens that B full tables could hold must count less than 2^31.
  * max_len: no sequence is expected to be longer; it decides how the lengths are split over workgroups (longer ones are right, and slower).  ws: 16-byte aligned,
  * mx_attn_decode_ws_bytes of the same arguments (0 bytes: NULL will do); its contents on entry do not matter.  */
 int mx_attn_decode_ws_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t max_len, uint32_t window, uint64_t* bytes);

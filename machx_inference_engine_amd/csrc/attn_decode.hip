@@ -639,13 +639,14 @@ static int attn_decode(mx_stream_t s, bool q8, const uint16_t* q, uint64_t q_str
     const uint32_t G = Hq / Hkv, heads = G < 16 ? G : 16;
     const uint64_t groups = (uint64_t)Hkv * ((G + 15) / 16);
     MX_REQUIRE_SHAPE(groups <= 65535 && (uint64_t)B * Hq < (1ull << 31));
+    // the join's groups of parts: four parts a thread where a sequence has its even portion of them; a launch holds fewer than 2^32 threads
+    uint32_t join_groups = (p.shares / B + 4) / 4;
+    if (join_groups > 512 / (D / 4)) join_groups = 512 / (D / 4);
+    const uint32_t join_threads = (join_groups * (D / 4) + 63) / 64 * 64;
+    MX_REQUIRE_SHAPE(!p.shares || (uint64_t)B * Hq * join_threads < (1ull << 32));
     if (int rc = launch_attn(s, a, q8, dim3(p.shares ? p.shares : B, (uint32_t)groups), heads)) return rc;
     if (p.shares) {
-        // groups of parts: four parts a thread where a sequence has its even portion of them
-        uint32_t groups = (p.shares / B + 4) / 4;
-        if (groups > 512 / (D / 4)) groups = 512 / (D / 4);
-        const uint32_t threads = (groups * (D / 4) + 63) / 64 * 64;
-        hipLaunchKernelGGL(attn_join_kernel, dim3(B * Hq), dim3(threads), groups * D * 4, as_stream(s), a, groups);
+        hipLaunchKernelGGL(attn_join_kernel, dim3(B * Hq), dim3(join_threads), join_groups * D * 4, as_stream(s), a, join_groups);
         if (int rc = launch_status()) return rc;
     }
     return out_q8 && !a.out_q8 ? mx_quantize_q8_1(s, out, out_q8, (uint64_t)B * Hq * D) : MX_OK;

@@ -186,24 +186,28 @@ __global__ __launch_bounds__(kRowThreads) void prompt_kernel(RowsArgs a) {
     }
 }
 
+// A launch holds fewer than 2^32 threads in a row of its grid.
+static bool fits(uint64_t workgroups, uint32_t threads) { return workgroups * threads < (1ull << 32); }
+
 constexpr uint32_t kPromptTokens = 512;
 template <bool ROPE, bool Q8>
 static int launch_rows(mx_stream_t s, RowsArgs a, uint32_t T, int interleaved) {
     a.heads_per_wg = kRowThreads / a.chunks;
     a.groups = (a.Hq + 2 * a.Hkv + a.heads_per_wg - 1) / a.heads_per_wg;
-    MX_REQUIRE_SHAPE((uint64_t)a.groups * T < (1ull << 31));
     // Two chunks a thread load every row once where the half layout's other form loads turned rows twice: 8192 tokens of 72 heads of 64 35.9 -> 26.6 us (5.7 TB/s),
     // 2047 tokens of 32 + 4 + 4 heads of 128 into a Q8_0 cache 14.5 -> 9.4; interleaved pairs are as fast either way.  Fewer tokens leave CUs without work: one
     // token 2.2 -> 2.8 us, 333 (18 heads of 256) 3.9 -> 4.1.
     if (T >= kPromptTokens && (!Q8 || (a.chunks % 8 == 0 && a.n_rot % 64 == 0))) {
         // as many waves as the token's pairs of chunks fill evenly
         const uint32_t items = (a.Hq + 2 * a.Hkv) * (a.chunks / 2), turns = (items + kRowThreads - 1) / kRowThreads, threads = ((items + turns - 1) / turns + 63) / 64 * 64;
+        MX_REQUIRE_SHAPE(fits(T, threads));
         auto launch = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3(T), dim3(threads), 0, as_stream(s), a);
             return launch_status();
         };
         return ROPE && interleaved ? launch(prompt_kernel<ROPE, Q8, ROPE>) : launch(prompt_kernel<ROPE, Q8, false>);
     }
+    MX_REQUIRE_SHAPE(fits((uint64_t)a.groups * T, kRowThreads));
     const dim3 grid(a.groups * T);
     if (ROPE && interleaved) hipLaunchKernelGGL((rows_kernel<ROPE, Q8, ROPE>), grid, dim3(kRowThreads), 0, as_stream(s), a);
     else hipLaunchKernelGGL((rows_kernel<ROPE, Q8, false>), grid, dim3(kRowThreads), 0, as_stream(s), a);
@@ -334,7 +338,7 @@ static int kv_read(mx_stream_t s, bool q8, const void* k, const uint16_t* k_d, c
                    uint32_t page_size) {
     if (int rc = check_cache(q8, k, k_d, v, v_d, Hkv, D, n_pages, page_size)) return rc;
     MX_REQUIRE_PTR(page_table); MX_REQUIRE_PTR(rows); MX_REQUIRE_PTR(k_out); MX_REQUIRE_PTR(v_out);
-    MX_REQUIRE_SHAPE(B > 0 && B <= (1u << 24) && max_pages > 0 && total_rows > 0 && total_rows < (1u << 31));
+    MX_REQUIRE_SHAPE(B > 0 && B <= (1u << 24) && max_pages > 0 && total_rows > 0 && total_rows < (1u << 31) && fits(total_rows / 16 + (uint64_t)B, 256));
     MX_REQUIRE_ALIGN(page_table, 4); MX_REQUIRE_ALIGN(rows, 4); MX_REQUIRE_ALIGN(k_out, 16); MX_REQUIRE_ALIGN(v_out, 16);
     const dim3 grid(total_rows / 16 + B, (2 * Hkv * 16 * (D / 8) + 256 * kReadPieces - 1) / (256 * kReadPieces));
     auto launch = [&](auto kernel) {

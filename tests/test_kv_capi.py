@@ -60,6 +60,22 @@ def test_write_refusals(lib, fmt):
 
 
 @pytest.mark.parametrize("fmt", ["f16", "q8_0"])
+def test_launches_of_too_many_threads(lib, fmt):
+    r = Call(lib, "mx_rope", T=1 << 26, n_heads=8, D=128, x_stride=1024, y_stride=1024, n_rot=128, interleaved=0, mscale=1.0)
+    assert r.with_() == r.with_(T=0xFFFFFFFF) == r.with_(n_heads=1, D=16, n_rot=16, T=1 << 31) == SHAPE
+    c, w = Call(lib, "mx_rope_kv_write_" + fmt, **HEADS), Call(lib, "mx_kv_write_" + fmt, **HEADS)
+    for bad in (dict(T=1 << 26), dict(T=0xFFFFFFFF), dict(T=1 << 26, D=96)):
+        assert c.with_(n_rot=96, **bad) == w.with_(**bad) == SHAPE, bad
+    if fmt == "q8_0":                                          # three workgroups a token
+        assert c.with_(T=1 << 23, D=96, n_rot=96) == SHAPE
+    k = Call(lib, "mx_kv_read_" + fmt, max_pages=4, total_rows=1 << 28, B=1, Hkv=8, D=128, n_pages=10, page_size=16)
+    assert k.with_() == k.with_(total_rows=1 << 27, B=1 << 23) == SHAPE
+    a = Call(lib, "mx_attn_decode_" + fmt, q_stride=1 << 20, max_pages=4, B=65535, Hq=8192, Hkv=1, D=128, n_pages=10, page_size=16, max_len=2048, window=0, scale=0.1, out_q8=None,
+             ws_bytes=1 << 60)
+    assert a.with_() == a.with_(Hq=2048, Hkv=2048) == SHAPE
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q8_0"])
 def test_read_refusals(lib, fmt):
     planes = ("k_cache", "v_cache") if fmt == "f16" else ("k_qs", "k_d", "v_qs", "v_d")
     c = Call(lib, "mx_kv_read_" + fmt, max_pages=4, total_rows=60, B=2, Hkv=8, D=128, n_pages=10, page_size=16)
