@@ -686,8 +686,8 @@ int mx_swiglu_oai_q8(mx_stream_t s, const uint16_t* gate, const uint16_t* up, ui
  * Cache: pages of `page_size` tokens (a multiple of 16; one page for each sequence makes it a plain cache), each [Hkv][page_size][D], of fp16
  * (D % 16 == 0) or of Q8_0 planes, int8 values and an fp16 scale for each 32 of a head (D % 32 == 0; scales [Hkv][page_size][D / 32]); D <= 256.
  * A token's slot is page * page_size + offset.  Q8_0 is the weight format's arithmetic: d = fp16(amax / 127), q = round-half-away(x * (127 / amax));
- * it quantises the fp16 values that the fp16 cache would hold.  A block that holds a NaN or an infinity reads back as NaN; one whose amax is
- * above 65471 has a scale whose 127-fold passes fp16 and reads back with infinities.  n_pages * page_size < 2^31; offsets into a plane take 64 bits.
+ * it quantises the fp16 values that the fp16 cache would hold.  A block that holds a NaN or an infinity reads back as NaN.
+ * 65504, fp16's largest number, is stored as 127 * 516: it reads back as an infinity, and attention weighs it as 65532.  Scales written elsewhere may be as large as that, 516.  n_pages * page_size < 2^31; offsets into a plane take 64 bits.
  *
  * All row pointers and planes 16-byte aligned, strides multiples of 8.  What one launch cannot hold (2^32 threads) is refused: never T < 2^22 with
  * T * D * (all heads, key and value heads too) < 2^34, nor total_rows / 16 + B < 2^24.

@@ -137,6 +137,14 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// Whether an fp16 result of finite operands that passes fp16 becomes its largest number (or, as usual, an infinity): FP16_OVFL, bit 23 of the wave's mode register.
+template <bool LARGEST>
+__device__ __forceinline__ void f16_overflow_to_largest() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_s_setreg(1 | 23 << 6, LARGEST);
+#endif
+}
+
 __device__ __forceinline__ uint32_t pick(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
 // Two unsigned bytes u (bytes `sel` of w) as the fp16 pair u - 128: 0x6400 + u is 1024 + u.
 __device__ __forceinline__ half2_t bytes_f16(uint32_t w, uint32_t sel) {
@@ -157,7 +165,8 @@ __device__ __forceinline__ half2_t bytes_f16(uint32_t w, uint32_t sel) {
 // Only the result is rounded to fp16: scores, maxima and sums are fp32, and the matrix instruction's fp16 operands carry the weights in two parts, the second what the first's
 // rounding left (to 2^-22, or 2^-40 of the largest weight: that is 2^15, not 1, so that the many small weights of a long sequence lie above fp16's smallest step; where
 // scores are so large that 15 of them could round to 16, it is 1).  Q8_0: keys are exact as fp16 integers and their scales are folded into the fp32 products of each block; values are q d in two parts, which hold it
-// exactly (8 + 11 bits; d and so q d are multiples of 2^-24).  One part would be 3 % faster and 1.4 times as far off.
+// exactly (8 + 11 bits; d and so q d are multiples of 2^-24; 127 * 516, as which 65504 is stored, is 65504 and 28, since the products' overflow is set to end at
+// the largest number).  One part would be 3 % faster and 1.4 times as far off.
 template <bool Q8, int DP, int NBLK, bool FULL>
 __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 ? 3 : 2) void attn_decode_kernel(AttnArgs a) {
     constexpr int E = DP / 16, NB = DP / 32;
@@ -303,6 +312,7 @@ __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 
             for (int w = 0; w < VW; ++w) vr[t][w] = 0;
     }
 
+    if (Q8) f16_overflow_to_largest<true>();   // the products q d
     float m = -INFINITY, l = 0.f;
     floatx4 o[E];
 #pragma unroll
@@ -441,6 +451,7 @@ __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 
     // ---- the waves' sums: lane (r, g) holds elements 4 E g .. 4 E g + 4 E - 1 of head r
     l = rows_sum(l);
     __syncthreads();                         // the key tiles' place is taken
+    if (Q8) f16_overflow_to_largest<false>();   // the result's rounding
     float* ml = lds;                         // [waves][16] (maximum, sum)
     float* os = lds + kWaves * 32;            // [waves][heads][OS]
     if (g == 0) {

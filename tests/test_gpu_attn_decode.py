@@ -381,3 +381,25 @@ def test_a_decode_step_between_its_projections(mx, fmt):
         # fp16: half a step of it, twice (rotation, and the reference's 32-bit part of it far below); Q8_0: half a step of the block, its scale's rounding, and
         # the value's own two roundings to fp16
         assert (np.abs(g - w) <= 2.0 ** -10 * np.abs(w) + 2.0 ** -24 + (0.5 * step * (1 + 2.0 ** -9) + 2.0 ** -10 * np.abs(w) if fmt == "q8_0" else 0)).all()
+
+
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 160, 256])
+def test_largest_values_of_a_q8_0_cache(mx, D):
+    """65504 is stored as 127 * 516 = 65532, which fp16 does not hold: weighed with others it counts as that, alone it rounds to infinity, and the block's other values are
+    what they are.  Signs alternate from token to token and weights are nearly equal, so that sums of two or more are finite."""
+    lens, Hkv, G, ps = [1000, 3, 40, 2], 2, 4, 16
+    rng = np.random.default_rng(81 + D)
+    table, n_pages = U.pages_of(lens + [1], ps, rng)
+    cache = mx.ops.kv_cache("q8_0", n_pages, Hkv, ps, D)
+    for b, n in enumerate(lens + [1]):
+        t = np.arange(n)
+        k, v = ((rng.uniform(-1, 1, (n, Hkv, D)) * s).astype(np.float16) for s in (0.05, 30000))
+        v[..., ::5] = np.where(t % 2, -65504, 65504)[:, None, None]
+        mx.ops.kv_write(dev(k), dev(v), dev((table[b, t // ps] * ps + t % ps).astype(np.int32)), cache)
+    q = rng.standard_normal((5, Hkv * G, D)).astype(np.float16)
+    want, tol = U.attention(q, cache, table, lens + [1], ps, D ** -0.5)
+    y = host(mx.ops.attn_decode(dev(q), cache, dev(table), dev(np.array(lens + [1], np.int32))))
+    near(y[:4], want[:4], tol[:4], "largest values")
+    assert (want[4, :, ::5] == 65532).all() and (y[4, :, ::5] == np.inf).all()
+    y[4, :, ::5] = want[4, :, ::5] = 0
+    near(y[4], want[4], tol[4], "beside the largest values")
