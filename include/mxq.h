@@ -728,6 +728,7 @@ int mx_kv_read_q8_0(mx_stream_t s, const int8_t* k_qs, const uint16_t* k_d, cons
  * t of [max(0, len - window), len) (window 0: all), len = seq_lens[b] cut to what page_table[b][max_pages] holds; query head h reads
  * key-value head h / (Hq / Hkv) (Hq % Hkv == 0).  sinks: Hq floats or NULL.  Scores, softmax and sums are fp32.  A sequence without tokens (len <= 0) gives zeros; tokens
  * whose page is outside [0, n_pages) count as masked; what the cache holds behind a sequence's end is never used, whatever it is.
+ * An infinite value in an fp16 cache makes its element infinite, whatever its token's weight; infinities of either sign, or a NaN, make it NaN.
  * out: [B][Hq][D] fp16; out_q8 (may be NULL, Hq * D % 32 == 0): the block_q8_1x stream of the rounded out, as the output
  * projection's int-dot product takes it, bit-identical to mx_quantize_q8_1(out).
  * B <= 65535, B * Hq < 2^26 (2^31 where ws_bytes is 0); the tiles of 32 tokens that B full tables could hold must count less than 2^31.

@@ -403,3 +403,21 @@ def test_largest_values_of_a_q8_0_cache(mx, D):
     assert (want[4, :, ::5] == 65532).all() and (y[4, :, ::5] == np.inf).all()
     y[4, :, ::5] = want[4, :, ::5] = 0
     near(y[4], want[4], tol[4], "beside the largest values")
+
+
+@pytest.mark.parametrize("steep", [1.0, 15.0])
+@pytest.mark.parametrize("D,G,ps", [(64, 8, 16), (48, 3, 32), (128, 4, 16), (112, 2, 48), (256, 2, 16), (128, 17, 64)])
+def test_infinite_values_of_an_fp16_cache(mx, D, G, ps, steep):
+    """An element is infinite where one token's value is, whatever that token's weight, and NaN where infinities of either sign or a NaN are; all others are what they were."""
+    lens = [900, 40, 5, 1, 0, 130]
+    rng, table, cache, q = case("f16", lens, 2, G, D, ps, 83 + D, k_scale=steep)
+    for b, n in enumerate(lens):
+        for t in rng.integers(0, max(n, 1), 6) if n else ():
+            for i, x in enumerate((np.inf, -np.inf, np.inf if rng.random() < 0.5 else -np.inf, np.nan)):
+                cache[1][int(table[b, t // ps]), int(rng.integers(0, 2)), int(t) % ps, 4 * i + int(rng.integers(0, 2))] = float(x)
+    with np.errstate(invalid="ignore"):
+        want, tol = U.attention(q, cache, table, lens, ps, D ** -0.5)
+    y = host(mx.ops.attn_decode(dev(q), cache, dev(table), dev(np.array(lens, np.int32)))).astype(np.float64)
+    bad = ~np.isfinite(want)
+    assert bad.any() and np.array_equal(y[bad], want[bad], equal_nan=True)
+    near(np.where(bad, 0, y), np.where(bad, 0, want), np.where(bad, 1, tol), "beside infinities")
