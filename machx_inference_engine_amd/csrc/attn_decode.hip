@@ -152,15 +152,30 @@ __device__ __forceinline__ half2_t bytes_f16(uint32_t w, uint32_t sel) {
     return __builtin_bit_cast(half2_t, pick(w, 0x64646464u, sel)) + bias;
 }
 
-// What of two fp16 values is no number, zeros in the place of the others.
-__device__ __forceinline__ half2_t no_numbers(half2_t v) {
-    const uint32_t w = __builtin_bit_cast(uint32_t, v);
-    return __builtin_bit_cast(half2_t, ((w & 0x7C00u) == 0x7C00u ? w & 0xFFFFu : 0u) | ((w & 0x7C000000u) == 0x7C000000u ? w & 0xFFFF0000u : 0u));
+// Four sums of which some are NaN, over fp16 values.  An infinity times a weight's part, or times what a running sum is scaled by, is NaN where that is zero or where the two
+// parts differ in sign: what is NaN is made again of the values alone that are no numbers, each once, so that infinities of one sign give one and others NaN.  (A weight that is
+// NaN is in the sum of weights too.)  v: the elements in token 0 of head 0 of page 0.  A function of its own, since its registers would cost every call 2 % of a short sequence.
+__device__ __attribute__((noinline)) floatx4 without_numbers(floatx4 sum, const half_t* v, const int32_t* table, uint32_t n_pages, uint32_t page_size, uint32_t hk, uint32_t Hkv, uint32_t D,
+                                                             uint32_t from, uint32_t to) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] = sum[j] == sum[j] ? sum[j] : 0.f;
+    for (uint32_t t0 = from / 8 * 8; t0 < to; t0 += 8) {      // 8 tokens, of one page
+        const uint32_t col = t0 / page_size, page = (uint32_t)table[col];
+        if (page >= n_pages) continue;
+        const half_t* row = v + (((size_t)page * Hkv + hk) * page_size + t0 - col * page_size) * D;
+        uint2 w[8];
+#pragma unroll
+        for (uint32_t t = 0; t < 8; ++t) w[t] = *reinterpret_cast<const uint2*>(row + t * D);
+#pragma unroll
+        for (uint32_t t = 0; t < 8; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t bits = (j < 2 ? w[t].x : w[t].y) >> (16 * (j & 1)) & 0xFFFFu;
+                if (t0 + t >= from && t0 + t < to && (bits & 0x7C00u) == 0x7C00u) sum[j] += h2f(bits);
+            }
+    }
+    return sum;
 }
-// A part's weight in the sum of parts, never zero: an infinite sum stays one.  (What 2^-126 of a finite one adds is far below fp16.)
-__device__ __forceinline__ float part_weight(float x) { return fmaxf(__builtin_amdgcn_exp2f(x), 0x1p-126f); }
-// The result: zero where no token has a weight, an infinity all the same.
-__device__ __forceinline__ float divided(float sum, float total, float inv) { return total == 0.f && fabsf(sum) < INFINITY ? 0.f : sum * inv; }
 
 // A workgroup takes one key-value head, up to 16 of the query heads that share it, and a sequence or a share of the sequences' tiles; its waves take the tiles in turn,
 // each with a running maximum and sum of its own.  Bound by the cache's bytes: 64 x 8192 fp16 tokens of 8 heads of 128 in 322 us, 6.7 TB/s (a plain copy of that size moves 4.9, reads
@@ -244,10 +259,6 @@ __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 
         f.page[0] = (uint32_t)table[c0];                          // c0 < max_pages: the tile's first token is in front of the sequence's end
         f.page[1] = (uint32_t)table[min(c1, a.max_pages - 1)];
         return f;
-    };
-    auto counts = [&](const Ref& f, int i) {                      // the i-th of a lane's 8 tokens: not masked
-        const uint32_t t = f.token + 8 * g + i;
-        return t >= sp.start && t < sp.end && (g >> 1 ? f.page[1] : f.page[0]) < a.n_pages;
     };
     auto row_of = [&](const Ref& f, int h) { return ((size_t)(f.page[h] < a.n_pages ? f.page[h] : 0u) * a.Hkv + hk) * a.page_size + f.off[h]; };
 
@@ -393,7 +404,8 @@ __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 
             if (!full) {   // masked tokens: no weight, and values of zero, since what lies there may be no number
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const bool ok = counts(cur, i);
+                    const uint32_t t = cur.token + 8 * g + i;
+                    const bool ok = t >= sp.start && t < sp.end && (g >> 1 ? ok1 : ok0);
                     x[i] = ok ? x[i] : -INFINITY;
                     sc[i] = ok ? sc[i] : (half_t)0.f;
 #pragma unroll
@@ -460,44 +472,6 @@ __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 
             }
         }
     }
-    // An infinite value times a weight's part, or times what a sum is scaled by, makes a NaN where that is zero or where its parts differ in sign.  Sums that have become
-    // NaN are made again of the values alone that are no numbers, each once: infinities of one sign are one, others NaN.  A weight that is NaN is in l too.
-    if (!Q8) {
-        floatx4 all = o[0];
-#pragma unroll
-        for (int e = 1; e < E; ++e) all += o[e];
-        const float sum = all[0] + all[1] + all[2] + all[3];
-        if (__any(sum != sum)) {
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[e][j] = o[e][j] == o[e][j] ? o[e][j] : 0.f;
-            const half_t one = (half_t)1.f;
-            const half8 ones = {one, one, one, one, one, one, one, one};
-#pragma unroll 1
-            for (tile = first + wave; tile < last; tile += kWaves) {
-                const Ref f = locate(tile);
-                load_v(f);
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-#pragma unroll
-                    for (int w = 0; w < VW; ++w) vr[i][w] = counts(f, i) ? vr[i][w] : 0u;
-#pragma unroll
-                for (int e = 0; e < E; e += 2) {
-                    half8 f0, f1;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const half2_t h0 = no_numbers(__builtin_bit_cast(half2_t, pick(vr[2 * w + 1][e / 2], vr[2 * w][e / 2], 0x05040100u)));
-                        const half2_t h1 = no_numbers(__builtin_bit_cast(half2_t, pick(vr[2 * w + 1][e / 2], vr[2 * w][e / 2], 0x07060302u)));
-                        f0[2 * w] = h0[0]; f0[2 * w + 1] = h0[1];
-                        f1[2 * w] = h1[0]; f1[2 * w + 1] = h1[1];
-                    }
-                    o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f0, ones, o[e], 0, 0, 0);
-                    o[e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f1, ones, o[e + 1], 0, 0, 0);
-                }
-            }
-        }
-    }
 
     // ---- the waves' sums: lane (r, g) holds elements 4 E g .. 4 E g + 4 E - 1 of head r
     l = rows_sum(l);
@@ -528,13 +502,20 @@ __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 
         const float ref = top == -INFINITY ? 0.f : top;
         floatx4 sum = {0.f, 0.f, 0.f, 0.f};
         for (uint32_t w = 0; w < kWaves; ++w) {
-            const float x = ml[(w * 16 + h) * 2] - ref;
-            total += __builtin_amdgcn_exp2f(x) * ml[(w * 16 + h) * 2 + 1];
-            sum += part_weight(x) * *reinterpret_cast<const floatx4*>(os + (w * heads + h) * OS + d);
+            const float f = __builtin_amdgcn_exp2f(ml[(w * 16 + h) * 2] - ref);
+            total += f * ml[(w * 16 + h) * 2 + 1];
+            sum += f * *reinterpret_cast<const floatx4*>(os + (w * heads + h) * OS + d);
+        }
+        const float four = sum[0] + sum[1] + sum[2] + sum[3];
+        if (!Q8 && __builtin_expect(four != four, 0)) {
+            sum = without_numbers(sum, static_cast<const half_t*>(a.v) + d, a.table + (size_t)b * a.max_pages, a.n_pages, a.page_size, hk, a.Hkv, D, max(sp.start, (sp.tile0 + first) * kTile),
+                                  min(sp.end, (sp.tile0 + last) * kTile));
+            total = total == 0.f ? 0x1p-126f : total;   // however little weight a sink has left the tokens
         }
         if (whole) {
             const float all = total + __builtin_amdgcn_exp2f(sink - ref), inv = 1.0f / all;
-            const float y[4] = {divided(sum[0], total, inv), divided(sum[1], total, inv), divided(sum[2], total, inv), divided(sum[3], total, inv)};
+            const bool none = total == 0.f;
+            const float y[4] = {none ? 0.f : sum[0] * inv, none ? 0.f : sum[1] * inv, none ? 0.f : sum[2] * inv, none ? 0.f : sum[3] * inv};
             store_rows(a, out0 + i, y, live);
         } else if (live) {
             const size_t at = (size_t)(share + b) * a.Hq + hq;
@@ -546,6 +527,11 @@ __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 
     if (left) __syncthreads();               // the sums have been read
     }
 }
+
+// A part's weight in the sum of parts, never zero: an infinite sum stays one.  (What 2^-126 of a finite one adds is far below fp16.)
+__device__ __forceinline__ float part_weight(float x) { return fmaxf(__builtin_amdgcn_exp2f(x), 0x1p-126f); }
+// The result: zero where no token has a weight, an infinity all the same.
+__device__ __forceinline__ float divided(float sum, float total, float inv) { return total == 0.f && fabsf(sum) < INFINITY ? 0.f : sum * inv; }
 
 // Joins the parts of one head of one sequence: D / 4 threads for each of `groups` groups of parts, each thread four elements.
 __global__ __launch_bounds__(512) void attn_join_kernel(AttnArgs a, uint32_t groups) {
