@@ -696,8 +696,9 @@ int mx_swiglu_oai_q8(mx_stream_t s, const uint16_t* gate, const uint16_t* up, ui
  * factor by which the context grows; 1: as trained).  ext_factor 0: every pair alike (linear).  ext_factor > 0 (YaRN): with dim(r) = n_rot ln(n_ctx_orig / (2 pi r)) / (2 ln base),
  * pairs up to floor(dim(beta_fast)) keep ext_factor of their own frequency, those from ceil(dim(beta_slow)) on are slowed down, those between are mixed
  * linearly, and mscale = attn_factor * (1 + 0.1 ln(1 / scale)); otherwise mscale = attn_factor.
- * mx_rope: x and y are [T] rows of n_heads heads; y may be x (same stride).
- * mx_rope_kv_write_*: q -> q_out rotated; k rotated and v as it is into the cache at slots[t]; q rows may be rotated in place.  A slot outside [0, n_pages * page_size)
+ * mx_rope: x and y are [T] rows of n_heads heads; y may be x (same stride: another is refused).
+ * mx_rope_kv_write_*: q -> q_out rotated; k rotated and v as it is into the cache at slots[t]; q rows may be rotated in place (q_out = q
+ * with the same stride: another is refused).  Outputs overlap no other input.  A slot outside [0, n_pages * page_size)
  * (a padded token) writes nothing to the cache.  The slots of one call must be distinct.
  * mx_kv_write_*: the same without rotation and queries.
  * mx_kv_read_*: tokens 0 .. rows[b + 1] - rows[b] - 1 of every sequence b, by the pages of page_table[b][max_pages], to rows rows[b] ... of k_out and v_out

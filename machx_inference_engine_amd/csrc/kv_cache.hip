@@ -297,6 +297,11 @@ static int check_rows(const void* p, uint64_t stride, uint64_t width) {
     MX_REQUIRE_ALIGN(p, 16);
     return MX_OK;
 }
+// In place is row by row: the same rows with other strides lie in each other's way.
+static int check_in_place(const void* from, uint64_t from_stride, const void* to, uint64_t to_stride, uint32_t T) {
+    MX_REQUIRE_SHAPE(from != to || from_stride == to_stride || T == 1);
+    return MX_OK;
+}
 static int check_rotation(const void* positions, const void* freqs, uint32_t D, uint32_t n_rot) {
     MX_REQUIRE_PTR(positions); MX_REQUIRE_PTR(freqs);
     MX_REQUIRE_SHAPE(n_rot >= 16 && n_rot <= D && n_rot % 16 == 0);
@@ -318,6 +323,7 @@ static int rope_kv_write(mx_stream_t s, bool q8, const uint16_t* q, uint64_t q_s
         MX_REQUIRE_SHAPE(Hq > 0);
         if (int rc = check_rows(q, q_stride, (uint64_t)Hq * D)) return rc;
         if (int rc = check_rows(q_out, q_out_stride, (uint64_t)Hq * D)) return rc;
+        if (int rc = check_in_place(q, q_stride, q_out, q_out_stride, T)) return rc;
         if (int rc = check_rotation(positions, freqs, D, n_rot)) return rc;
     }
     RowsArgs a = {};
@@ -379,6 +385,7 @@ int mx_rope(mx_stream_t s, const uint16_t* x, uint64_t x_stride, uint16_t* y, ui
     MX_REQUIRE_SHAPE(T > 0 && n_heads > 0 && n_heads <= 65535 && D > 0 && D <= 256 && D % 16 == 0);
     if (int rc = check_rows(x, x_stride, (uint64_t)n_heads * D)) return rc;
     if (int rc = check_rows(y, y_stride, (uint64_t)n_heads * D)) return rc;
+    if (int rc = check_in_place(x, x_stride, y, y_stride, T)) return rc;
     if (int rc = check_rotation(positions, freqs, D, n_rot)) return rc;
     RowsArgs a = {};
     a.q = reinterpret_cast<const half_t*>(x); a.q_out = reinterpret_cast<half_t*>(y);

@@ -158,3 +158,12 @@ def test_frequency_refusals(lib):
                 dict(ext=1.0, ctx=4096, fast=0.5), dict(ext=1.0, ctx=4096, slow=0.0)):
         args = {"n_rot": 64, **bad}
         assert freqs(lib, args.pop("n_rot"), **args)[0] == SHAPE, bad
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q8_0"])
+def test_in_place_needs_one_stride(lib, fmt):
+    """Rows that are read with one stride and written from the same address with another would be overwritten before they are read."""
+    r = Call(lib, "mx_rope", T=2, n_heads=8, D=128, x_stride=2048, y_stride=1024, n_rot=128, interleaved=0, mscale=1.0)
+    assert r.with_() == r.with_(x_stride=1024, y_stride=2048) == r.with_(T=600, x_stride=1032) == SHAPE
+    c = Call(lib, "mx_rope_kv_write_" + fmt, **{**HEADS, "q_stride": 6144})
+    assert c.with_() == c.with_(T=600) == c.with_(q_stride=4096, q_out_stride=4104) == SHAPE
