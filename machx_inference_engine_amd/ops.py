@@ -30,14 +30,15 @@ class MxError(RuntimeError):
 # The current device's current stream as an address.  torch.cuda.current_stream() builds a Stream object for it, 2.7 of the 9 us that a
 # small call costs the host; the raw handle of the same stream takes 0.2 (one token, Q4_K 4096 -> 4096, quantizer and product, called one after
 # the other: 13.4 us, 18.9 before).
-def _stream_handle():
+def _stream_lookup():
+    """(number of the current device, address of a device's current stream)"""
     raw, device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
     if raw is None or device is None:   # a torch built without a device
-        return lambda: torch.cuda.current_stream().cuda_stream
-    return lambda: raw(device())
+        return torch.cuda.current_device, lambda dev: torch.cuda.current_stream(dev).cuda_stream
+    return device, raw
 
 
-_stream = _stream_handle()
+_current_device, _stream_of = _stream_lookup()
 
 
 def _ptr(t):
@@ -51,7 +52,7 @@ def _ptr(t):
 
 
 def _call(name, *args):
-    rc = getattr(lib, name)(_stream(), *args)
+    rc = getattr(lib, name)(_stream_of(_current_device()), *args)
     if rc != 0:
         raise MxError(name, rc)
 
@@ -793,8 +794,6 @@ def _want(ok, what):
         raise ValueError(what)
 
 
-_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 _F16, _F32, _F64, _I32, _I8 = torch.float16, torch.float32, torch.float64, torch.int32, torch.int8
 
 
