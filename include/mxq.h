@@ -730,11 +730,13 @@ int mx_kv_read_q8_0(mx_stream_t s, const int8_t* k_qs, const uint16_t* k_d, cons
  * key-value head h / (Hq / Hkv) (Hq % Hkv == 0).  sinks: Hq floats or NULL.  Scores, softmax and sums are fp32.  A sequence without tokens (len <= 0) gives zeros; tokens
  * whose page is outside [0, n_pages) count as masked; what the cache holds behind a sequence's end is never used, whatever it is.
  * An infinite value in an fp16 cache makes its element infinite, whatever its token's weight; infinities of either sign, or a NaN, make it NaN.
+ * A sequence whose tokens' scores are all -infinity gives zeros.
  * out: [B][Hq][D] fp16; out_q8 (may be NULL, Hq * D % 32 == 0): the block_q8_1x stream of the rounded out, as the output
  * projection's int-dot product takes it, bit-identical to mx_quantize_q8_1(out).
  * B <= 65535, B * Hq < 2^26 (2^31 where ws_bytes is 0); the tiles of 32 tokens that B full tables could hold must count less than 2^31.
  * max_len: no sequence is expected to be longer; it decides how the lengths are split over workgroups (longer ones are right, and slower).  ws: 16-byte aligned,
- * mx_attn_decode_ws_bytes of the same arguments (0 bytes: NULL will do); its contents on entry do not matter.  */
+ * mx_attn_decode_ws_bytes of the same arguments (0 bytes: NULL will do); its contents on entry do not matter.  Calls that may run at the same time, captured ones too, need one each.  Equal arguments
+ * (lengths of all sequences, max_len and window among them) give equal bits; another max_len, or other sequences beside it, may change a sequence's last bit.  */
 int mx_attn_decode_ws_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t max_len, uint32_t window, uint64_t* bytes);
 int mx_attn_decode_f16(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* page_table,
                        uint32_t max_pages, const int32_t* seq_lens, const float* sinks, uint16_t* out, void* out_q8, uint32_t B, uint32_t Hq,

@@ -178,8 +178,8 @@ __device__ __attribute__((noinline)) floatx4 without_numbers(floatx4 sum, const 
 }
 
 // A workgroup takes one key-value head, up to 16 of the query heads that share it, and a sequence or a share of the sequences' tiles; its waves take the tiles in turn,
-// each with a running maximum and sum of its own.  Bound by the cache's bytes: 64 x 8192 fp16 tokens of 8 heads of 128 in 322 us, 6.7 TB/s (a plain copy of that size moves 4.9, reads
-// alone reach 6.3 to 7.1); what a launch has beside them is 5 us from its start to its first tile and from its last one to its end.
+// each with a running maximum and sum of its own.  Bound by the cache's bytes: 64 x 8192 fp16 tokens of 8 heads of 128 in 322 us one after another,
+// 6.7 TB/s, 328 to 334 each by itself under the tracer (a plain copy of that size moves 4.95, reads alone reach 6.3 to 7.1); what a launch has beside them is 5 us from its start to its first tile and from its last one to its end.
 //
 // Scores: S^T[token][head] = K Q^T, mfma 16x16x32.  Keys come in whole rows, 16 bytes a lane (read as the operand wants them, 16 rows a load, they kept the address units
 // busy: Q8_0 99 -> 56 us for one sequence of 131071), and reach the operand through an LDS tile of the wave's own.  Row r of the two 16-row products of a tile is
@@ -597,6 +597,9 @@ __global__ __launch_bounds__(512) void attn_join_kernel(AttnArgs a, uint32_t gro
 // heads are narrow, one where they are wide.  us by workgroups (256, 512, 768, 1024): 64 x 8192 tokens of 8 heads of 128, fp16 318, 321, 330, 328, Q8_0 201, 175, 183, 182;
 // one Q8_0 sequence of 131071 57, 52, 56, 58; 64 ragged ones of up to 6001 with heads of 64 72, 53, 49, 49; 16 fp16 ones of 16384 with 2 heads of 256 89 (256), 97 (512).
 // A share is two tiles a wave at least, but one where that leaves most CUs idle (one Q8_0 sequence of 2000: 11.1 -> 9.8 us; of 8000: 11.9, 12.8).
+// The figures are of fp16 for wide heads, which one workgroup fills a CU with; Q8_0's, of which two fit, have not been measured with more than one.  Shares are rounded up, so that
+// with a number of heads that does not divide these there are a few workgroups more, which wait for a place: 16384 fp16 tokens of 3, 5 and 6 heads of 256 4.6, 4.4 and 4.9 TB/s where
+// 2, 4 and 8 reach 6.2 to 6.3, Q8_0 3.8 to 3.9 where they reach 5.5.
 struct Plan {
     uint32_t shares;         // 0: a workgroup for each sequence and group of heads
     uint64_t ws_bytes;

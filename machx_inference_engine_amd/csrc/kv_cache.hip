@@ -11,10 +11,9 @@ constexpr int kRowThreads = 256;
 // 32048 tokens of 4 heads of 128 read back 24.8 -> 19.4 us.
 constexpr uint64_t kStreamFrom = 32u << 20;
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef float float8 __attribute__((ext_vector_type(8)));
 
 // m cos and m sin of `turns` revolutions, each rounded once: the angle is cut to a quarter turn and the Taylor polynomials are summed in 64 bits (a position of 2^20 has
-// 2^-12 radians left in 32; one thread does this for each pair of a token, all heads use it).  On [-pi/4, pi/4] the next terms are below 2^-34.
+// 2^-4 radians left in 32; one thread does this for each pair of a token, all heads use it).  On [-pi/4, pi/4] the sine's next term is below 2^-37, the cosine's 2^-33.
 __device__ __forceinline__ float2 cos_sin_turns(double turns, double m) {
     const double quarters = turns * 4.0, k = rint(quarters), a = (quarters - k) * 1.5707963267948966, a2 = a * a;
     double s = fma(a2, -1.0 / 39916800.0, 1.0 / 362880.0);
