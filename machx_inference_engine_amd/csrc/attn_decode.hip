@@ -137,14 +137,6 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// Whether an fp16 result of finite operands that passes fp16 becomes its largest number (or, as usual, an infinity): FP16_OVFL, bit 23 of the wave's mode register.
-template <bool LARGEST>
-__device__ __forceinline__ void f16_overflow_to_largest() {
-#if defined(__HIP_DEVICE_COMPILE__)
-    __builtin_amdgcn_s_setreg(1 | 23 << 6, LARGEST);
-#endif
-}
-
 __device__ __forceinline__ uint32_t pick(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
 // Two unsigned bytes u (bytes `sel` of w) as the fp16 pair u - 128: 0x6400 + u is 1024 + u.
 __device__ __forceinline__ half2_t bytes_f16(uint32_t w, uint32_t sel) {
@@ -177,6 +169,12 @@ __device__ __attribute__((noinline)) floatx4 without_numbers(floatx4 sum, const 
     return sum;
 }
 
+// Scales of at most 511.5, whose products with -128 .. 127 fp16 holds.  Their bits' order as signed integers is theirs as numbers; a NaN may become 511.5.
+__device__ __forceinline__ half8 at_most_511(half8 d) {
+    typedef short short8 __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(half8, __builtin_elementwise_min(__builtin_bit_cast(short8, d), (short8)(short)0x5FFE));
+}
+
 // A workgroup takes one key-value head, up to 16 of the query heads that share it, and a sequence or a share of the sequences' tiles; its waves take the tiles in turn,
 // each with a running maximum and sum of its own.  Bound by the cache's bytes: 64 x 8192 fp16 tokens of 8 heads of 128 in 322 us one after another,
 // 6.7 TB/s, 328 to 334 each by itself under the tracer (a plain copy of that size moves 4.95, reads alone reach 6.3 to 7.1); what a launch has beside them is 5 us from its start to its first tile and from its last one to its end.
@@ -190,10 +188,11 @@ __device__ __attribute__((noinline)) floatx4 without_numbers(floatx4 sum, const 
 // Only the result is rounded to fp16: scores, maxima and sums are fp32, and the matrix instruction's fp16 operands carry the weights in two parts, the second what the first's
 // rounding left (to 2^-22, or 2^-40 of the largest weight: that is 2^15, not 1, so that the many small weights of a long sequence lie above fp16's smallest step; where
 // scores are so large that 15 of them could round to 16, it is 1).  Q8_0: keys are exact as fp16 integers and their scales are folded into the fp32 products of each block; values are q d in two parts, which hold it
-// exactly (8 + 11 bits; d and so q d are multiples of 2^-24; 127 * 516, as which 65504 is stored, is 65504 and 28, since the products' overflow is set to end at
-// the largest number).  One part would be 3 % faster and 1.4 times as far off.
+// exactly (8 + 11 bits; d and so q d are multiples of 2^-24; the first part is that of a scale of at most 511.5, since 127 * 516, as which 65504 is stored, passes fp16: 64960 and
+// 572).  One part would be 3 % faster and 1.4 times as far off.
+// Registers: narrow Q8_0 heads take at most 128, so that four workgroups fit a CU (with 130: 126 sequences of up to 60 tokens of 8 heads of 64 6.5 -> 8.7 us).
 template <bool Q8, int DP, int NBLK, bool FULL>
-__global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 ? 3 : 2) void attn_decode_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : Q8 && DP == 64 ? 4 : FULL || Q8 ? 3 : 2) void attn_decode_kernel(AttnArgs a) {
     constexpr int E = DP / 16, NB = DP / 32;
     constexpr int VW = Q8 ? E / 4 : E / 2;                     // dwords of a lane's part of one value row, in VP pieces (wide fp16 heads: 8 of each half)
     constexpr int VP = !Q8 && E == 16 ? 2 : 1;
@@ -337,7 +336,6 @@ __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 
             for (int w = 0; w < VW; ++w) vr[t][w] = 0;
     }
 
-    if (Q8) f16_overflow_to_largest<true>();   // the products q d
     float m = -INFINITY, l = 0.f;
     floatx4 o[E];
 #pragma unroll
@@ -435,6 +433,7 @@ __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 
                 lo[i] = (half_t)(p - (float)hi[i]);
             }
             // ---- values
+            const half8 sm = at_most_511(sc);       // of the first parts
 #pragma unroll
             for (int e = 0; e < E; e += 2) {
                 half8 f0, f1, g0, g1;   // elements e and e + 1 of 8 tokens; Q8_0: what their rounding to fp16 left
@@ -444,8 +443,8 @@ __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 
                     if (Q8) {
                         const uint32_t both = pick(vr[2 * w + 1][e / 4] , vr[2 * w][e / 4], e & 2 ? 0x07030602u : 0x05010400u) ^ 0x80808080u;
                         const half2_t d = {sc[2 * w], sc[2 * w + 1]}, q0 = bytes_f16(both, 0x00050004u), q1 = bytes_f16(both, 0x00070006u);
-                        h0 = q0 * d;
-                        h1 = q1 * d;
+                        h0 = q0 * half2_t{sm[2 * w], sm[2 * w + 1]};
+                        h1 = q1 * half2_t{sm[2 * w], sm[2 * w + 1]};
                         const half2_t l0 = __builtin_elementwise_fma(q0, d, -h0), l1 = __builtin_elementwise_fma(q1, d, -h1);
                         g0[2 * w] = l0[0]; g0[2 * w + 1] = l0[1];
                         g1[2 * w] = l1[0]; g1[2 * w + 1] = l1[1];
@@ -476,7 +475,6 @@ __global__ __launch_bounds__(kWaves * 64, DP == 256 ? (Q8 ? 2 : 1) : FULL || Q8 
     // ---- the waves' sums: lane (r, g) holds elements 4 E g .. 4 E g + 4 E - 1 of head r
     l = rows_sum(l);
     __syncthreads();                         // the key tiles' place is taken
-    if (Q8) f16_overflow_to_largest<false>();   // the result's rounding
     float* ml = lds;                         // [waves][16] (maximum, sum)
     float* os = lds + kWaves * 32;            // [waves][heads][OS]
     if (g == 0) {

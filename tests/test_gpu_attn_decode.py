@@ -421,3 +421,25 @@ def test_infinite_values_of_an_fp16_cache(mx, D, G, ps, steep):
     bad = ~np.isfinite(want)
     assert bad.any() and np.array_equal(y[bad], want[bad], equal_nan=True)
     near(np.where(bad, 0, y), np.where(bad, 0, want), np.where(bad, 1, tol), "beside infinities")
+
+
+@pytest.mark.parametrize("D", [64, 96, 256])
+def test_a_q8_0_block_that_holds_no_number(mx, D):
+    """A value block written with a NaN or an infinity is NaN for every head that reads it; the blocks beside it and the other heads are what they were."""
+    lens, Hkv, G, ps = [700, 20], 2, 3, 16
+    rng = np.random.default_rng(91 + D)
+    table, n_pages = U.pages_of(lens, ps, rng)
+    cache = mx.ops.kv_cache("q8_0", n_pages, Hkv, ps, D)
+    bad = np.zeros((2, Hkv * G, D), bool)
+    for b, n in enumerate(lens):
+        t = np.arange(n)
+        k, v = (rng.standard_normal((n, Hkv, D)).astype(np.float16) for _ in range(2))
+        v[n // 2, b, 33 * b + 5] = (np.nan, -np.inf)[b]
+        bad[b, b * G: (b + 1) * G, 32 * b: 32 * b + 32] = True
+        mx.ops.kv_write(dev(k), dev(v), dev((table[b, t // ps] * ps + t % ps).astype(np.int32)), cache)
+    q = rng.standard_normal((2, Hkv * G, D)).astype(np.float16)
+    with np.errstate(invalid="ignore"):
+        want, tol = U.attention(q, cache, table, lens, ps, D ** -0.5)
+    y = host(mx.ops.attn_decode(dev(q), cache, dev(table), dev(np.array(lens, np.int32))))
+    assert np.isnan(y[bad]).all()
+    near(np.where(bad, 0, y), np.where(bad, 0, want), np.where(bad, 1, tol), "beside the block")
