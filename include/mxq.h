@@ -649,6 +649,21 @@ int mx_moe_router(mx_stream_t s, const uint16_t* x, const float* W_gate, int32_t
                   uint32_t n_tokens, uint32_t hidden, uint32_t n_experts, uint32_t k, float* logits_ws);
 int mx_moe_topk_from_logits(mx_stream_t s, const uint16_t* logits, int32_t* topk_idx, uint16_t* topk_w, uint32_t E,
                             uint32_t K, uint32_t n_tokens);
+/* Routing by other scores than the softmax's (no counterpart in the reference, whose routers are the two above).
+ *   mx_moe_router_logits: the logits of mx_moe_router by themselves, the same bits: logits[t][e] fp32.
+ *   mx_moe_route: from logits (fp16, or fp32 with MX_ROUTE_F32) to topk_idx (k distinct ids, ascending) and topk_w.
+ *     score s = softmax(logits), or 1 / (1 + exp(-logit)) with MX_ROUTE_SIGMOID; choice c = s + bias[e] (bias: n_experts floats or NULL).
+ *     n_groups > 1: the experts lie in n_groups groups of n_experts / n_groups; a group's worth is its largest c, or the sum of its two largest with MX_ROUTE_TOP2; the topk_groups of
+ *     largest worth are kept.  Of the kept experts those of the k largest c are chosen; of equal ones the lowest id (or group) is.
+ *     topk_w = half(scale * s / (sum of the chosen s + 1e-20)) with MX_ROUTE_RENORM, half(scale * s) without; the bias is no part of it.
+ *     Scores, worths and comparisons are 64 bits, so that what is chosen is that of the exact scores, next to ties too; weights are rounded once.
+ *     An expert of logit -infinity has score 0 (a softmax over nothing else: all scores 0).  A c that is NaN lies below every number, and is then taken by id; so does a group with one for its worth.
+ *     n_experts <= 1024, k <= 64, n_experts % n_groups == 0, n_groups <= 64, 1 <= topk_groups <= n_groups, k <= topk_groups * n_experts / n_groups, n_tokens < 2^26.
+ *     MX_ROUTE_TOP2 over groups of one expert: its c.  A token's result is the same bits in every call.  */
+enum { MX_ROUTE_SIGMOID = 1, MX_ROUTE_RENORM = 2, MX_ROUTE_TOP2 = 4, MX_ROUTE_F32 = 8 };
+int mx_moe_router_logits(mx_stream_t s, const uint16_t* x, const float* W_gate, float* logits, uint32_t n_tokens, uint32_t hidden, uint32_t n_experts);
+int mx_moe_route(mx_stream_t s, const void* logits, const float* bias, int32_t* topk_idx, uint16_t* topk_w, uint32_t n_tokens, uint32_t n_experts, uint32_t k,
+                 uint32_t n_groups, uint32_t topk_groups, uint32_t flags, float scale);
 int mx_moe_build_pack_decode(mx_stream_t s, const int32_t* topk_idx, const uint16_t* topk_w, uint32_t* expert_offsets,
                              int32_t* sorted_idx, int32_t* tk_to_packed, uint16_t* weights_packed, uint32_t E, uint32_t K);
 int mx_moe_build_packing_device(mx_stream_t s, const int32_t* topk_idx, const uint16_t* topk_w, uint32_t T, uint32_t K,
@@ -666,6 +681,13 @@ int mx_rms_norm_f32w_q8(mx_stream_t s, const uint16_t* x, const float* w, uint16
                         uint32_t hidden, float eps);
 int mx_gated_rms_norm_q8(mx_stream_t s, const float* x, const uint16_t* z, const uint16_t* weight, uint16_t* y,
                          void* q8_out, uint32_t n_rows, uint32_t hidden, float eps);
+/* The residual's addition in front of it (the reference: residual_add_rms_norm_fused, then quantize_q8_1, src/model/dense_transformer.cpp:617-705):
+ *   sum = half(x + residual); y of the rounded sum, the bits of mx_rms_norm_f32w_q8's; q8_out the block_q8_1x stream of y, the bits of
+ *   mx_quantize_q8_1(y) (halves = 0), or the block_q8_1s stream, those of mx_quantize_q8_1s(y) (halves != 0), as the int-dot products of a prompt take it.
+ *   sum may be residual or x (in place, the whole matrix), y may be NULL when only the stream is wanted; outputs overlap nothing else.  All 16-byte
+ *   aligned (q8_out without halves 8); hidden % 32 == 0, n_rows < 2^25.  A row that holds a NaN or an infinity gives NaN where the norm does, and stream blocks of it that mean nothing.  */
+int mx_add_rms_norm_f32w_q8(mx_stream_t s, const uint16_t* x, const uint16_t* residual, const float* w, uint16_t* sum, uint16_t* y, void* q8_out, uint32_t n_rows,
+                            uint32_t hidden, float eps, int halves);
 /* Gated activations with the same fused emitter (no counterpart in the reference, which runs swiglu /
  * swiglu_oai and then quantize_q8_1): y = half(silu(gate) * up) (swiglu, src/ops/elementwise.cpp:449-467)
  * or the clamped gpt-oss form (swiglu_oai, :469-492; alpha 1.702, limit 7.0 there), and q8_out = the
@@ -688,6 +710,9 @@ int mx_swiglu_oai_q8(mx_stream_t s, const uint16_t* gate, const uint16_t* up, ui
  * A token's slot is page * page_size + offset.  Q8_0 is the weight format's arithmetic: d = fp16(amax / 127), q = round-half-away(x * (127 / amax));
  * it quantises the fp16 values that the fp16 cache would hold.  A block that holds a NaN or an infinity reads back as NaN.
  * 65504, fp16's largest number, is stored as 127 * 516: it reads back as an infinity, and attention weighs it as 65532.  Scales written elsewhere may be as large as that, 516.  n_pages * page_size < 2^31; offsets into a plane take 64 bits.
+ * Or of Q4_0 planes (D % 32 == 0), [Hkv][page_size][D / 2] bytes and scales as Q8_0's: of a block of 32 the weight format's 16 bytes, elements j and j + 16 in the low and high half of byte j, value = d * (code - 8),
+ * d = fp16(m / -8) with m the value of largest magnitude, the first of equal ones, code = min(15, floor(8 x / -m + 8.5)) of the exact quotient.  A block of a NaN or an infinity reads back as NaN.  Any scale
+ * may stand in a plane that was written elsewhere; one that is no number makes its block NaN.
  *
  * All row pointers and planes 16-byte aligned, strides multiples of 8.  What one launch cannot hold (2^32 threads) is refused: never T < 2^22 with
  * T * D * (all heads, key and value heads too) < 2^34, nor total_rows / 16 + B < 2^24.
@@ -716,13 +741,22 @@ int mx_rope_kv_write_q8_0(mx_stream_t s, const uint16_t* q, uint64_t q_stride, c
                           uint16_t* q_out, uint64_t q_out_stride, int8_t* k_qs, uint16_t* k_d, int8_t* v_qs, uint16_t* v_d, const int32_t* positions,
                           const int32_t* slots, const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved,
                           double mscale, uint32_t n_pages, uint32_t page_size);
+int mx_rope_kv_write_q4_0(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride,
+                          uint16_t* q_out, uint64_t q_out_stride, uint8_t* k_qs, uint16_t* k_d, uint8_t* v_qs, uint16_t* v_d, const int32_t* positions,
+                          const int32_t* slots, const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved,
+                          double mscale, uint32_t n_pages, uint32_t page_size);
 int mx_kv_write_f16(mx_stream_t s, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride, uint16_t* k_cache, uint16_t* v_cache,
                     const int32_t* slots, uint32_t T, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size);
 int mx_kv_write_q8_0(mx_stream_t s, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride, int8_t* k_qs, uint16_t* k_d, int8_t* v_qs,
                      uint16_t* v_d, const int32_t* slots, uint32_t T, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size);
+int mx_kv_write_q4_0(mx_stream_t s, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride, uint8_t* k_qs, uint16_t* k_d, uint8_t* v_qs,
+                     uint16_t* v_d, const int32_t* slots, uint32_t T, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size);
 int mx_kv_read_f16(mx_stream_t s, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* page_table, uint32_t max_pages, const int32_t* rows,
                    uint16_t* k_out, uint16_t* v_out, uint32_t total_rows, uint32_t B, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size);
 int mx_kv_read_q8_0(mx_stream_t s, const int8_t* k_qs, const uint16_t* k_d, const int8_t* v_qs, const uint16_t* v_d, const int32_t* page_table,
+                    uint32_t max_pages, const int32_t* rows, uint16_t* k_out, uint16_t* v_out, uint32_t total_rows, uint32_t B, uint32_t Hkv, uint32_t D,
+                    uint32_t n_pages, uint32_t page_size);
+int mx_kv_read_q4_0(mx_stream_t s, const uint8_t* k_qs, const uint16_t* k_d, const uint8_t* v_qs, const uint16_t* v_d, const int32_t* page_table,
                     uint32_t max_pages, const int32_t* rows, uint16_t* k_out, uint16_t* v_out, uint32_t total_rows, uint32_t B, uint32_t Hkv, uint32_t D,
                     uint32_t n_pages, uint32_t page_size);
 /* mx_attn_decode_*: one query token for each of B sequences: out[b][h] = sum_t p_t v_t / (sum_t p_t + exp(sink_h - m)), p_t = exp(scale q . k_t - m), over the tokens
@@ -730,7 +764,7 @@ int mx_kv_read_q8_0(mx_stream_t s, const int8_t* k_qs, const uint16_t* k_d, cons
  * key-value head h / (Hq / Hkv) (Hq % Hkv == 0).  sinks: Hq floats or NULL.  Scores, softmax and sums are fp32.  A sequence without tokens (len <= 0) gives zeros; tokens
  * whose page is outside [0, n_pages) count as masked; what the cache holds behind a sequence's end is never used, whatever it is.
  * An infinite value in an fp16 cache makes its element infinite, whatever its token's weight; infinities of either sign, or a NaN, make it NaN.
- * A sequence whose tokens' scores are all -infinity gives zeros.
+ * A sequence whose tokens' scores are all -infinity gives zeros.  Over a Q4_0 cache a query head with an infinity or a NaN gives NaN.
  * out: [B][Hq][D] fp16; out_q8 (may be NULL, Hq * D % 32 == 0): the block_q8_1x stream of the rounded out, as the output
  * projection's int-dot product takes it, bit-identical to mx_quantize_q8_1(out).
  * B <= 65535, B * Hq < 2^26 (2^31 where ws_bytes is 0); the tiles of 32 tokens that B full tables could hold must count less than 2^31.
@@ -743,6 +777,10 @@ int mx_attn_decode_f16(mx_stream_t s, const uint16_t* q, uint64_t q_stride, cons
                        uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size, uint32_t max_len, uint32_t window, float scale, void* ws,
                        uint64_t ws_bytes);
 int mx_attn_decode_q8_0(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const int8_t* k_qs, const uint16_t* k_d, const int8_t* v_qs,
+                        const uint16_t* v_d, const int32_t* page_table, uint32_t max_pages, const int32_t* seq_lens, const float* sinks, uint16_t* out,
+                        void* out_q8, uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size, uint32_t max_len,
+                        uint32_t window, float scale, void* ws, uint64_t ws_bytes);
+int mx_attn_decode_q4_0(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint8_t* k_qs, const uint16_t* k_d, const uint8_t* v_qs,
                         const uint16_t* v_d, const int32_t* page_table, uint32_t max_pages, const int32_t* seq_lens, const float* sinks, uint16_t* out,
                         void* out_q8, uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size, uint32_t max_len,
                         uint32_t window, float scale, void* ws, uint64_t ws_bytes);

@@ -1,4 +1,4 @@
-// attn_decode.hip — attention of one new token over a paged key-value cache (fp16 or Q8_0 planes).
+// attn_decode.hip — attention of one new token over a paged key-value cache (fp16, Q8_0 or Q4_0 planes).
 #include "mxq_device.h"
 #include "mxq_host.h"
 
@@ -14,8 +14,8 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 struct AttnArgs {
     const half_t* q;
     uint64_t q_stride;
-    const void *k, *v;              // fp16, or int8
-    const half_t *k_d, *v_d;        // Q8_0 scales
+    const void *k, *v;              // fp16, int8, or two 4-bit codes a byte
+    const half_t *k_d, *v_d;        // scales
     const int32_t *table, *lens;
     const float* sinks;
     half_t* out;
@@ -616,6 +616,345 @@ static Plan plan_of(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t 
     return {(uint32_t)shares, (shares + B) * Hq * (D + 2) * 4 + (uint64_t)B * 8};
 }
 
+// ---------------------------------------------------------------- Q4_0
+// Shares, tiles, running maxima and the join as above; one wave's tile is 32 tokens of one key-value head, 18 bytes for each 32 values.  What the fp16 operands of the two products
+// are made of differs, since at a quarter of fp16's bytes the vector unit is what would bound a kernel that widens every value and multiplies it by its scale:
+//   * A 4-bit code in the low bits of a half is n 2^-24, in bits 4 .. 7 it is 16 n 2^-24: numbers below fp16's normal range, which the matrix instruction multiplies exactly.  One `and`
+//     gives two operands, none converts.  The codes' offset, value = d (n - 8), is taken out of the sums.
+//   * Keys: a query's values that meet high codes are divided by 16, and the product of a block starts from -8 times the sum of its query values; its four rows are then multiplied by their tokens' scales.
+//     Queries are scaled by a power of two to a largest element of 2^14 .. 2^15, so that neither division nor small queries lose bits.
+//   * Values: the scales multiply the weights instead, for each block of 32 (p d in two fp16 parts, from p's two: three packed operations for two tokens, and the products of a block share
+//     them), and the offset is 8 times sum p d, one matrix product of the scales' tile with the weights for all blocks, in which a row of ones gives the sum of weights too.
+//     For that every product's 16 rows are the low or the high codes of one block: the bytes of a block's column of 8 tokens come from LDS by the transposing read.
+//   * p d must stay in fp16's range: the largest weight is 2^(15 - k), 2^k above every scale that this wave has met (k > 0 only for values beyond 8).
+// Precision as above: p d is held to 2^-22, or 2^-39 + k of the largest weight's; what the offsets cancel in the fp32 sums is at most 15 / 8 of the values' own size.
+
+// Eight codes' operand: the low or high codes (mask 0x000f000f, 0x00f000f0) of the bytes of two words, even bytes of a word in front of its odd ones.
+__device__ __forceinline__ half8 codes_f16(uint32_t a, uint32_t b, uint32_t mask) {
+    typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(half8, uint4_t{a & mask, a >> 8 & mask, b & mask, b >> 8 & mask});
+}
+
+template <int NB>
+__global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void attn_decode_q4_kernel(AttnArgs a) {
+    constexpr uint32_t D = 32 * NB, ROW = 16 * (NB | 1);        // LDS bytes of a token's codes: an odd number of 16-byte pieces, so that 16 rows meet all banks
+    constexpr uint32_t CODES = kTile * ROW, KS = kTile * NB * 2, VS = kTile * (NB + 1) * 2, WAVE = 2 * CODES + KS + VS;
+    constexpr uint32_t OS = D + 4;
+    constexpr int LP = (NB + 1) / 2, SL = (16 * NB + 63) / 64;  // a lane's 16-byte pieces of a tile's codes, dwords of its scales
+    extern __shared__ float lds[];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15u, g = lane >> 4;
+    const uint32_t G = a.Hq / a.Hkv, tiles_of_heads = (G + 15) / 16;
+    const uint32_t hk = blockIdx.y / tiles_of_heads, head0 = (blockIdx.y - hk * tiles_of_heads) * 16, heads = min(16u, G - head0);
+    const bool shared = a.shares != 0;
+    const uint32_t share = blockIdx.x;
+    char* const keys = reinterpret_cast<char*>(lds) + wave * WAVE;
+    char* const values = keys + CODES;
+    half_t* const k_scales = reinterpret_cast<half_t*>(values + CODES);               // [token][block]
+    half_t* const v_scales = reinterpret_cast<half_t*>(values + CODES + KS);          // [block][token], tokens of four in the order 0 2 1 3; a row of ones behind them
+    Share sh = {1, 1, blockIdx.x, 0, 0};
+    if (shared) sh = share_of(a, share, lane);
+    else sh.len = a.lens[sh.b];
+    uint32_t b = sh.b, first = sh.from, left = sh.left;
+    int32_t len = __builtin_amdgcn_readfirstlane(sh.len);
+    for (; left; len = __builtin_amdgcn_readfirstlane(left ? a.lens[b + 1] : 0), ++b) {
+    const Span sp = span_of(a, len);
+    const uint32_t last = shared ? min(sp.tiles, first + left) : sp.tiles;
+    const bool whole = first == 0 && last == sp.tiles;     // the result itself, not a part of it
+    const size_t out0 = ((size_t)b * a.Hq + hk * G + head0) * D;
+    if (shared) {
+        if (sp.tiles == 0) continue;
+        if (first == 0 && blockIdx.y == 0 && threadIdx.x == 0) *reinterpret_cast<uint2*>(a.parts + 2 * b) = make_uint2(share + b, (sh.per - left + sp.tiles - 1) / sh.per + 1);
+        left -= last - first;
+    } else {
+        left = 0;
+    }
+
+    typedef const __attribute__((address_space(4))) int32_t* table_t;
+    const table_t table = (table_t)(uintptr_t)(a.table + (size_t)b * a.max_pages);
+    struct Ref {             // a tile's first token and, for its two halves, page and place in the page
+        uint32_t token, page[2], off[2];
+    };
+    auto page_of = [&](uint32_t t) { return a.page_shift < 32 ? t >> a.page_shift : t / a.page_size; };
+    auto locate = [&](uint32_t tile) {
+        Ref f;
+        f.token = (sp.tile0 + tile) * kTile;
+        const uint32_t c0 = page_of(f.token), o0 = f.token - c0 * a.page_size;
+        const bool next = o0 + 16 >= a.page_size;
+        f.off[0] = o0;
+        f.off[1] = next ? 0 : o0 + 16;
+        f.page[0] = (uint32_t)table[c0];                          // c0 < max_pages: the tile's first token is in front of the sequence's end
+        f.page[1] = (uint32_t)table[min(next ? c0 + 1 : c0, a.max_pages - 1)];
+        return f;
+    };
+    auto row_of = [&](const Ref& f, int h) { return ((size_t)(f.page[h] < a.n_pages ? f.page[h] : 0u) * a.Hkv + hk) * a.page_size + f.off[h]; };
+
+    uint4 kr[LP], vr[LP];
+    uint32_t ks[SL], vs[SL];
+    auto load = [&](const Ref& f) {      // a half's codes lie in one piece, as its scales do
+        const size_t row0 = row_of(f, 0), row1 = row_of(f, 1);
+#pragma unroll
+        for (int i = 0; i < LP; ++i) {
+            const uint32_t w = i * 64 + lane;
+            if (NB % 2 == 0 || w < 32 * NB) {
+                const size_t at = w < 16 * NB ? row0 * (D / 2) + w * 16 : row1 * (D / 2) + (w - 16 * NB) * 16;
+                kr[i] = load_once<uint4>(static_cast<const char*>(a.k) + at);
+                vr[i] = load_once<uint4>(static_cast<const char*>(a.v) + at);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < SL; ++i) {
+            const uint32_t w = i * 64 + lane;
+            if (SL * 64 == 16 * NB || w < 16 * NB) {
+                const size_t at = w < 8 * NB ? row0 * NB + 2 * w : row1 * NB + 2 * (w - 8 * NB);
+                ks[i] = *reinterpret_cast<const uint32_t*>(a.k_d + at);
+                vs[i] = *reinterpret_cast<const uint32_t*>(a.v_d + at);
+            }
+        }
+    };
+    auto stage = [&]() {
+#pragma unroll
+        for (int i = 0; i < LP; ++i) {
+            const uint32_t w = i * 64 + lane;
+            if (NB % 2 == 0 || w < 32 * NB) {
+                const uint32_t at = w / NB * ROW + w % NB * 16;
+                *reinterpret_cast<uint4*>(keys + at) = kr[i];
+                *reinterpret_cast<uint4*>(values + at) = vr[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < SL; ++i) {
+            const uint32_t w = i * 64 + lane;
+            if (SL * 64 == 16 * NB || w < 16 * NB) {
+                reinterpret_cast<uint32_t*>(k_scales)[w] = ks[i];
+                auto place = [&](uint32_t s) { return s % NB * kTile + ((s / NB & ~3u) | (s / NB & 1u) << 1 | (s / NB >> 1 & 1u)); };
+                reinterpret_cast<uint16_t*>(v_scales)[place(2 * w)] = (uint16_t)vs[i];
+                reinterpret_cast<uint16_t*>(v_scales)[place(2 * w + 1)] = (uint16_t)(vs[i] >> 16);
+            }
+        }
+    };
+
+    uint32_t tile = first + wave;
+    Ref cur = {}, next = {};
+    if (tile < last) {
+        cur = locate(tile);
+        load(cur);
+        if (tile + kWaves < last) next = locate(tile + kWaves);
+    }
+    // ---- queries: lane (r, g) has head r, of every block elements 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3, in the order of a word's codes
+    half8 qf[NB];
+    float off[NB];
+    float unit;              // of the scores
+    {
+        float top = 0.f;
+        uint2 lo[NB], hi[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            lo[n] = hi[n] = make_uint2(0, 0);
+            if (r < heads) {
+                const half_t* p = a.q + b * a.q_stride + (size_t)(hk * G + head0 + r) * D + n * 32 + 4 * g;
+                lo[n] = *reinterpret_cast<const uint2*>(p);
+                hi[n] = *reinterpret_cast<const uint2*>(p + 16);
+            }
+            top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(h2f(lo[n].x & 0xFFFFu)), fabsf(h2f(lo[n].x >> 16))), fmaxf(fabsf(h2f(lo[n].y & 0xFFFFu)), fabsf(h2f(lo[n].y >> 16)))),
+                                   fmaxf(fmaxf(fabsf(h2f(hi[n].x & 0xFFFFu)), fabsf(h2f(hi[n].x >> 16))), fmaxf(fabsf(h2f(hi[n].y & 0xFFFFu)), fabsf(h2f(hi[n].y >> 16))))));
+        }
+        top = rows_max(top);
+        const uint32_t e = f2u(top) >> 23;                                 // 2^(e - 127) <= top < 2^(e - 126)
+        const uint32_t up = e == 0 ? 0u : 141u - min(e, 141u);             // by 2^up to 2^14 and more (at most 38; from 2^15 on as it is)
+        const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f, by = sign * u2f((127u + up) << 23);
+        unit = a.scale == 0.f ? 1.f : fabsf(a.scale) * 0x1p24f * u2f((127u - up) << 23);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const float v[8] = {h2f(lo[n].x & 0xFFFFu), h2f(lo[n].y & 0xFFFFu), h2f(hi[n].x & 0xFFFFu), h2f(hi[n].y & 0xFFFFu),
+                                h2f(lo[n].x >> 16),     h2f(lo[n].y >> 16),     h2f(hi[n].x >> 16),     h2f(hi[n].y >> 16)};
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                sum += v[i] * by;
+                qf[n][i] = (half_t)(v[i] * by * (i & 2 ? 0.0625f : 1.f));
+            }
+            off[n] = rows_sum(sum) * -0x1p-21f;
+        }
+    }
+    if (lane < 16) reinterpret_cast<uint32_t*>(v_scales + NB * kTile)[lane] = 0x3C003C00u;
+
+    float m = -INFINITY, room = 15.f;          // room: log2 of the largest weight
+    uint32_t most = 15u << 10;                  // scales below this, as bits, leave it as it is
+    floatx4 o[2 * NB], z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 2 * NB; ++e) o[e] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (; tile < last; tile += kWaves) {
+        const bool more = tile + kWaves < last;
+        const bool ok0 = cur.page[0] < a.n_pages, ok1 = cur.page[1] < a.n_pages, full = cur.token >= sp.start && cur.token + kTile <= sp.end && ok0 && ok1;
+        auto live = [&](uint32_t t) { return cur.token + t >= sp.start && cur.token + t < sp.end && (t >> 4 ? ok1 : ok0); };
+        if (!full) {         // masked tokens' values have no scale, since what lies there may be no number
+#pragma unroll
+            for (int i = 0; i < SL; ++i) {
+                const uint32_t w = i * 64 + lane;
+                vs[i] = (live(2 * w / NB) ? vs[i] & 0xFFFFu : 0u) | (live((2 * w + 1) / NB) ? vs[i] & 0xFFFF0000u : 0u);
+            }
+        }
+        uint32_t big = 0;
+#pragma unroll
+        for (int i = 0; i < SL; ++i)
+            if (SL * 64 == 16 * NB || i * 64 + lane < 16 * NB) big = max(big, max(vs[i] & 0x7FFFu, vs[i] >> 16 & 0x7FFFu));
+        if (__any(big >= most)) {
+            // a scale of 2^(e - 15) .. 2^(e - 14), e its exponent's bits: weights up to 2^(29 - e), where they are 2^15 otherwise; an infinity or a NaN asks for no more than the largest scale
+            uint32_t e = 15;
+            for (uint32_t t = 16; t < 31; ++t) e = __any(big >= t << 10) ? t : e;
+            const float down = 29.f - (float)e, to = fabsf(m) < kMostShifted ? m + (room - down) : m, keep = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
+            z *= keep;
+#pragma unroll
+            for (int i = 0; i < 2 * NB; ++i) o[i] *= keep;
+            m = to;
+            room = down;
+            most = e >= 30 ? 0xFFFFu : (e + 1) << 10;
+        }
+        wave_sync();                     // the tile before has been read
+        stage();
+        wave_sync();
+        if (more) {
+            load(next);
+        }
+        // ---- scores: row r of product t is token 8 (r / 4) + r % 4 + 4 t, so that lane (r, g) gets tokens 8 g + 4 t + 0 .. 3 of head r
+        floatx4 score[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        uint4 kd[NB];                    // scales of the lane's 8 tokens: [token][block]
+#pragma unroll
+        for (int n = 0; n < NB; ++n) kd[n] = reinterpret_cast<const uint4*>(k_scales + 8 * g * NB)[n];
+        const char* const key_row = keys + (8 * (r >> 2) + (r & 3u)) * ROW + 4 * g;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(key_row + t * 4 * ROW + n * 16);
+                typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
+                const half8 kf = __builtin_bit_cast(half8, uint4_t{w & 0x000F000Fu, w & 0x00F000F0u, w >> 8 & 0x000F000Fu, w >> 8 & 0x00F000F0u});
+                const floatx4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[n], floatx4{off[n], off[n], off[n], off[n]}, 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int i = (4 * t + j) * NB + n;
+                    const uint32_t two = i / 2 % 4 == 0 ? kd[i / 8].x : i / 2 % 4 == 1 ? kd[i / 8].y : i / 2 % 4 == 2 ? kd[i / 8].z : kd[i / 8].w;
+                    score[t][j] = fmaf(p[j], h2f((i & 1 ? two >> 16 : two) & 0xFFFFu), score[t][j]);
+                }
+            }
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x[i] = score[i / 4][i % 4] * unit;
+            if (!full) x[i] = live(8 * g + i) ? x[i] : -INFINITY;
+        }
+        // ---- running maximum, weights
+        float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        top = rows_max(top);
+        top = fmaxf(m, fabsf(top) < kMostShifted ? top - room : top);
+        const float ref = top == -INFINITY ? 0.f : top;
+        if (__any(top > m)) {
+            const float keep = __builtin_amdgcn_exp2f(m - ref);
+            z *= keep;
+#pragma unroll
+            for (int e = 0; e < 2 * NB; ++e) o[e] *= keep;
+            m = top;
+        }
+        half8 hi, lo;        // in the order of a column's bytes: 0 2 1 3, 4 6 5 7
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int at = (i & 4) | (i & 1) << 1 | (i >> 1 & 1);
+            const float p = __builtin_amdgcn_exp2f(x[i] - ref);
+            hi[at] = (half_t)p;
+            lo[at] = (half_t)(p - (float)hi[at]);
+        }
+        // ---- sums of weights and of weights times scales
+        const half8 sc = *reinterpret_cast<const half8*>(v_scales + min(r, (uint32_t)NB) * kTile + 8 * g);
+        z = __builtin_amdgcn_mfma_f32_16x16x32_f16(sc, hi, z, 0, 0, 0);
+        z = __builtin_amdgcn_mfma_f32_16x16x32_f16(sc, lo, z, 0, 0, 0);
+        // ---- values
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            typedef int int2_t __attribute__((ext_vector_type(2)));
+            const int2_t w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((int2_t __attribute__((address_space(3)))*)(values + (8 * g + (r >> 1)) * ROW + n * 16 + (r & 1u) * 8));
+            const half8 d = *reinterpret_cast<const half8*>(v_scales + n * kTile + 8 * g);
+            const half8 p = hi * d, rest = __builtin_elementwise_fma(lo, d, __builtin_elementwise_fma(hi, d, -p));
+            const half8 v0 = codes_f16((uint32_t)w.x, (uint32_t)w.y, 0x000F000Fu), v1 = codes_f16((uint32_t)w.x, (uint32_t)w.y, 0x00F000F0u);
+            o[2 * n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p, o[2 * n], 0, 0, 0);
+            o[2 * n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p, o[2 * n + 1], 0, 0, 0);
+            o[2 * n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, rest, o[2 * n], 0, 0, 0);
+            o[2 * n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, rest, o[2 * n + 1], 0, 0, 0);
+        }
+        if (more) {
+            cur = next;
+            if (tile + 2 * kWaves < last) next = locate(tile + 2 * kWaves);
+        }
+    }
+
+    // ---- the waves' sums: lane (r, g) holds elements 32 n + 16 h + 4 g + 0 .. 3 of head r in o[2 n + h]; sum p d of block n is in row n of z, the sum of weights in row NB
+    __syncthreads();                         // the tiles' place is taken
+    float* ml = lds;                         // [waves][16] (maximum, sum)
+    float* os = lds + kWaves * 32;            // [waves][heads][OS]
+    const float l = __shfl(z[NB % 4], NB / 4 * 16 + r);
+    if (g == 0) {
+        ml[(wave * 16 + r) * 2] = m;
+        ml[(wave * 16 + r) * 2 + 1] = l;
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        const float eight = -8.f * __shfl(z[n % 4], n / 4 * 16 + r);
+        if (r < heads) {
+            float* row = os + (wave * heads + r) * OS + n * 32 + 4 * g;
+            floatx4 s0, s1;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s0[j] = fmaf(o[2 * n][j], 0x1p24f, eight);
+                s1[j] = fmaf(o[2 * n + 1][j], 0x1p20f, eight);
+            }
+            *reinterpret_cast<floatx4*>(row) = s0;
+            *reinterpret_cast<floatx4*>(row + 16) = s1;
+        }
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x * 4; i < (heads * D + kWaves * 256 - 1) / (kWaves * 256) * (kWaves * 256); i += kWaves * 256) {
+        const bool live = i < heads * D;
+        const uint32_t h = live ? i / D : 0, d = live ? i - h * D : 0;
+        const uint32_t hq = hk * G + head0 + h;
+        const float sink = whole && a.sinks ? a.sinks[hq] * kLog2e : -INFINITY;
+        float top = sink, total = 0.f;
+        for (uint32_t w = 0; w < kWaves; ++w) top = fmaxf(top, ml[(w * 16 + h) * 2]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+        for (uint32_t w = 0; w < kWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(ml[(w * 16 + h) * 2] - ref);
+            total += f * ml[(w * 16 + h) * 2 + 1];
+            sum += f * *reinterpret_cast<const floatx4*>(os + (w * heads + h) * OS + d);
+        }
+        if (whole) {
+            const float all = total + __builtin_amdgcn_exp2f(sink - ref), inv = 1.0f / all;
+            const bool none = total == 0.f;
+            const float y[4] = {none ? 0.f : sum[0] * inv, none ? 0.f : sum[1] * inv, none ? 0.f : sum[2] * inv, none ? 0.f : sum[3] * inv};
+            store_rows(a, out0 + i, y, live);
+        } else if (live) {
+            const size_t at = (size_t)(share + b) * a.Hq + hq;
+            *reinterpret_cast<floatx4*>(a.part_o + at * D + d) = sum;
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(top, total);
+        }
+    }
+    first = 0;
+    if (left) __syncthreads();               // the sums have been read
+    }
+}
+
+// ---------------------------------------------------------------- launches
+enum { kF16 = 0, kQ8 = 1, kQ4 = 2 };   // what a cache holds
+
+template <int NB>
+static int launch_q4(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads) {
+    static LdsLimit limit;
+    constexpr uint32_t tiles = kWaves * (2 * kTile * 16 * (NB | 1) + kTile * (2 * NB + 1) * 2), most = kWaves * (32 + 16 * (32 * NB + 4)) * 4;
+    const uint32_t sums = kWaves * (32 + heads * (32 * NB + 4)) * 4, lds = tiles > sums ? tiles : sums;
+    if (lds > kLdsDefaultLimit)
+        if (int rc = raise_lds_limit(reinterpret_cast<const void*>(attn_decode_q4_kernel<NB>), limit, tiles > most ? tiles : most)) return rc;
+    hipLaunchKernelGGL((attn_decode_q4_kernel<NB>), grid, dim3(kWaves * 64), lds, as_stream(s), a);
+    return launch_status();
+}
 template <bool Q8, int DP, int NBLK, bool FULL>
 static int launch_form(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads) {
     static LdsLimit limit;
@@ -627,8 +966,18 @@ static int launch_form(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t hea
     hipLaunchKernelGGL((attn_decode_kernel<Q8, DP, NBLK, FULL>), grid, dim3(kWaves * 64), lds, as_stream(s), a);
     return launch_status();
 }
-static int launch_attn(mx_stream_t s, const AttnArgs& a, bool q8, dim3 grid, uint32_t heads) {
-    if (q8) switch (a.D / 32) {
+static int launch_attn(mx_stream_t s, const AttnArgs& a, int fmt, dim3 grid, uint32_t heads) {
+    if (fmt == kQ4) switch (a.D / 32) {
+        case 1: return launch_q4<1>(s, a, grid, heads);
+        case 2: return launch_q4<2>(s, a, grid, heads);
+        case 3: return launch_q4<3>(s, a, grid, heads);
+        case 4: return launch_q4<4>(s, a, grid, heads);
+        case 5: return launch_q4<5>(s, a, grid, heads);
+        case 6: return launch_q4<6>(s, a, grid, heads);
+        case 7: return launch_q4<7>(s, a, grid, heads);
+        default: return launch_q4<8>(s, a, grid, heads);
+    }
+    if (fmt == kQ8) switch (a.D / 32) {
         case 1: return launch_form<true, 64, 1, false>(s, a, grid, heads);
         case 2: return launch_form<true, 64, 2, true>(s, a, grid, heads);
         case 3: return launch_form<true, 128, 3, false>(s, a, grid, heads);
@@ -646,21 +995,21 @@ static int launch_attn(mx_stream_t s, const AttnArgs& a, bool q8, dim3 grid, uin
     return launch_form<false, 256, 8, false>(s, a, grid, heads);
 }
 
-static int attn_decode(mx_stream_t s, bool q8, const uint16_t* q, uint64_t q_stride, const void* k, const uint16_t* k_d, const void* v, const uint16_t* v_d,
+static int attn_decode(mx_stream_t s, int fmt, const uint16_t* q, uint64_t q_stride, const void* k, const uint16_t* k_d, const void* v, const uint16_t* v_d,
                        const int32_t* page_table, uint32_t max_pages, const int32_t* seq_lens, const float* sinks, uint16_t* out, void* out_q8, uint32_t B,
                        uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size, uint32_t max_len, uint32_t window, float scale, void* ws,
                        uint64_t ws_bytes) {
     MX_REQUIRE_PTR(q); MX_REQUIRE_PTR(k); MX_REQUIRE_PTR(v); MX_REQUIRE_PTR(page_table); MX_REQUIRE_PTR(seq_lens); MX_REQUIRE_PTR(out);
-    if (q8) { MX_REQUIRE_PTR(k_d); MX_REQUIRE_PTR(v_d); }
+    if (fmt != kF16) { MX_REQUIRE_PTR(k_d); MX_REQUIRE_PTR(v_d); }
     MX_REQUIRE_SHAPE(B > 0 && B <= 65535 && Hkv > 0 && Hkv <= 65535 && Hq > 0 && Hq <= 65535 && Hq % Hkv == 0);
-    MX_REQUIRE_SHAPE(D > 0 && D <= 256 && D % (q8 ? 32 : 16) == 0 && q_stride % 8 == 0 && q_stride >= (uint64_t)Hq * D);
+    MX_REQUIRE_SHAPE(D > 0 && D <= 256 && D % (fmt != kF16 ? 32 : 16) == 0 && q_stride % 8 == 0 && q_stride >= (uint64_t)Hq * D);
     MX_REQUIRE_SHAPE(n_pages > 0 && page_size > 0 && page_size % 16 == 0 && (uint64_t)n_pages * page_size < (1ull << 31) && max_pages > 0);
     const uint64_t tiles = (uint64_t)max_pages * page_size / kTile + 1;
     MX_REQUIRE_SHAPE(B * (tiles < (1u << 26) ? tiles : 1u << 26) < (1ull << 31));   // tiles of all sequences, counted in 32 bits
     MX_REQUIRE_SHAPE(!out_q8 || (uint64_t)Hq * D % 32 == 0);
     MX_REQUIRE_ALIGN(q, 16); MX_REQUIRE_ALIGN(k, 16); MX_REQUIRE_ALIGN(v, 16); MX_REQUIRE_ALIGN(out, 16); MX_REQUIRE_ALIGN(out_q8, 8);
     MX_REQUIRE_ALIGN(page_table, 4); MX_REQUIRE_ALIGN(seq_lens, 4); MX_REQUIRE_ALIGN(sinks, 4);
-    if (q8) { MX_REQUIRE_ALIGN(k_d, 16); MX_REQUIRE_ALIGN(v_d, 16); }
+    if (fmt != kF16) { MX_REQUIRE_ALIGN(k_d, 16); MX_REQUIRE_ALIGN(v_d, 16); }
     const Plan p = plan_of(B, Hq, Hkv, D, max_len, window);
     if (p.shares) {
         MX_REQUIRE_PTR(ws);
@@ -691,7 +1040,7 @@ static int attn_decode(mx_stream_t s, bool q8, const uint16_t* q, uint64_t q_str
     if (join_groups > 512 / (D / 4)) join_groups = 512 / (D / 4);
     const uint32_t join_threads = (join_groups * (D / 4) + 63) / 64 * 64;
     MX_REQUIRE_SHAPE(!p.shares || (uint64_t)B * Hq * join_threads < (1ull << 32));
-    if (int rc = launch_attn(s, a, q8, dim3(p.shares ? p.shares : B, (uint32_t)groups), heads)) return rc;
+    if (int rc = launch_attn(s, a, fmt, dim3(p.shares ? p.shares : B, (uint32_t)groups), heads)) return rc;
     if (p.shares) {
         hipLaunchKernelGGL(attn_join_kernel, dim3(B * Hq), dim3(join_threads), join_groups * D * 4, as_stream(s), a, join_groups);
         if (int rc = launch_status()) return rc;
@@ -715,14 +1064,21 @@ int mx_attn_decode_ws_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, u
 int mx_attn_decode_f16(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* page_table,
                        uint32_t max_pages, const int32_t* seq_lens, const float* sinks, uint16_t* out, void* out_q8, uint32_t B, uint32_t Hq, uint32_t Hkv,
                        uint32_t D, uint32_t n_pages, uint32_t page_size, uint32_t max_len, uint32_t window, float scale, void* ws, uint64_t ws_bytes) {
-    return attn_decode(s, false, q, q_stride, k_cache, nullptr, v_cache, nullptr, page_table, max_pages, seq_lens, sinks, out, out_q8, B, Hq, Hkv, D, n_pages,
+    return attn_decode(s, kF16, q, q_stride, k_cache, nullptr, v_cache, nullptr, page_table, max_pages, seq_lens, sinks, out, out_q8, B, Hq, Hkv, D, n_pages,
                        page_size, max_len, window, scale, ws, ws_bytes);
 }
 int mx_attn_decode_q8_0(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const int8_t* k_qs, const uint16_t* k_d, const int8_t* v_qs, const uint16_t* v_d,
                         const int32_t* page_table, uint32_t max_pages, const int32_t* seq_lens, const float* sinks, uint16_t* out, void* out_q8, uint32_t B,
                         uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size, uint32_t max_len, uint32_t window, float scale, void* ws,
                         uint64_t ws_bytes) {
-    return attn_decode(s, true, q, q_stride, k_qs, k_d, v_qs, v_d, page_table, max_pages, seq_lens, sinks, out, out_q8, B, Hq, Hkv, D, n_pages, page_size, max_len,
+    return attn_decode(s, kQ8, q, q_stride, k_qs, k_d, v_qs, v_d, page_table, max_pages, seq_lens, sinks, out, out_q8, B, Hq, Hkv, D, n_pages, page_size, max_len,
+                       window, scale, ws, ws_bytes);
+}
+int mx_attn_decode_q4_0(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint8_t* k_qs, const uint16_t* k_d, const uint8_t* v_qs,
+                        const uint16_t* v_d, const int32_t* page_table, uint32_t max_pages, const int32_t* seq_lens, const float* sinks, uint16_t* out,
+                        void* out_q8, uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size, uint32_t max_len,
+                        uint32_t window, float scale, void* ws, uint64_t ws_bytes) {
+    return attn_decode(s, kQ4, q, q_stride, k_qs, k_d, v_qs, v_d, page_table, max_pages, seq_lens, sinks, out, out_q8, B, Hq, Hkv, D, n_pages, page_size, max_len,
                        window, scale, ws, ws_bytes);
 }
 

@@ -1,4 +1,4 @@
-// kv_cache.hip — rotary positions and the paged key-value cache: rotation of query and key rows, writing (with Q8_0 quantisation) and reading back.
+// kv_cache.hip — rotary positions and the paged key-value cache: rotation of query and key rows, writing (with Q8_0 or Q4_0 quantisation) and reading back.
 #include <math.h>
 
 #include "mxq_device.h"
@@ -7,6 +7,7 @@
 namespace mxq {
 
 constexpr int kRowThreads = 256;
+enum { kF16 = 0, kQ8 = 1, kQ4 = 2 };   // what a cache holds
 // Outputs that the L2s (8 x 4 MB) do not hold are written past them, which leaves those to what is read: a Q8_0 cache's
 // 32048 tokens of 4 heads of 128 read back 24.8 -> 19.4 us.
 constexpr uint64_t kStreamFrom = 32u << 20;
@@ -35,8 +36,8 @@ struct RowsArgs {
     const half_t *q, *k, *v;
     uint64_t q_stride, k_stride, v_stride, q_out_stride;
     half_t* q_out;
-    void *k_cache, *v_cache;       // fp16, or int8
-    half_t *k_d, *v_d;             // Q8_0 scales
+    void *k_cache, *v_cache;       // fp16, int8, or two 4-bit codes a byte
+    half_t *k_d, *v_d;             // scales
     const int32_t *positions, *slots;
     const double* freqs;
     uint32_t Hq, Hkv, chunks, n_rot, heads_per_wg, groups, page_size, n_slots;  // chunks = D / 8, groups: workgroups of a token
@@ -79,8 +80,37 @@ __device__ __forceinline__ const half_t* row_of(const RowsArgs& a, uint32_t t, u
     return h < a.Hq ? a.q + t * a.q_stride + (size_t)h * D : h < a.Hq + a.Hkv ? a.k + t * a.k_stride + (size_t)(h - a.Hq) * D : a.v + t * a.v_stride + (size_t)(h - a.Hq - a.Hkv) * D;
 }
 
-// Chunk c of head h (query, key, value heads in this order) of token t to where it goes.  Q8: the four lanes of a block of 32 call together.
-template <bool Q8>
+// A quarter of a Q4_0 block, elements 8 l .. 8 l + 7 of its 32 in lane l = lane % 4; the four lanes call together.  d = m / -8 with m the value of largest magnitude, the first
+// of equal ones, code = min(15, floor(8 x / -m + 8.5)).  Gives the lane's dword of the block, the one at Q4Part::at, and d.
+// m is found as the largest of keys magnitude | 31 - element | sign.  A multiply-add with the reciprocal is off by less than 2^-20; 8 x / m + 8.5 is a whole number or at least 2^-13 from one (next
+// to one, 16 x is a multiple of half of m's last place, as is (2 k - 17) m), so that 2^-14 added makes every code that of the exact quotient.
+struct Q4Part {
+    uint32_t word, at;
+    half_t d;
+};
+__device__ __forceinline__ Q4Part q4_part(half8 y, uint32_t l) {
+    uint32_t top = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        const half_t e = y[i];               // of a vector's element itself the cast takes the first
+        const uint32_t bits = __builtin_bit_cast(uint16_t, e);
+        top = max(top, (bits & 0x7FFFu) << 6 | (31u - 8u * l - i) << 1 | bits >> 15);
+    }
+    top = max_bits4(top);
+    const uint32_t size = top >> 6;
+    const bool number = size < 0x7C00u;      // a NaN or an infinity: the scale is NaN, and with it the block
+    const float m = size == 0 ? 0.f : h2f(size | top << 15), inv = number && size != 0 ? -8.0f / m : 0.f;
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i / 4] |= (number ? (uint32_t)min(15, (int)fmaf((float)y[i], inv, 8.5f + 0x1p-14f)) : 8u) << (8 * (i % 4));
+    // lanes 0 and 1 hold the low, lanes 2 and 3 the high halves of the bytes: each gives away four codes and gets those that its own are paired with
+    const bool high = l >= 2;
+    const uint32_t own = high ? w[1] : w[0], other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(high ? w[0] : w[1]), 0x4E, 0xF, 0xF, true);
+    return {high ? other | own << 4 : own | other << 4, (l & 1) * 2 + (l >> 1), number ? f32_to_f16_rne(m * -0.125f) : (half_t)NAN};
+}
+
+// Chunk c of head h (query, key, value heads in this order) of token t to where it goes.  Quantised: the four lanes of a block of 32 call together.
+template <int FMT>
 __device__ __forceinline__ void put(const RowsArgs& a, uint32_t t, uint32_t slot, uint32_t h, uint32_t c, half8 y) {
     const uint32_t D = a.chunks * 8;
     if (h < a.Hq) {
@@ -92,8 +122,12 @@ __device__ __forceinline__ void put(const RowsArgs& a, uint32_t t, uint32_t slot
     const uint32_t hk = h - a.Hq - (is_v ? a.Hkv : 0), page = slot / a.page_size, at = slot - page * a.page_size;
     const size_t crow = ((size_t)page * a.Hkv + hk) * a.page_size + at;
     void* cache = is_v ? a.v_cache : a.k_cache;
-    if (!Q8) {
+    if (FMT == kF16) {
         *reinterpret_cast<half8*>(static_cast<half_t*>(cache) + crow * D + c * 8) = y;
+    } else if (FMT == kQ4) {
+        const Q4Part p = q4_part(y, c & 3u);
+        reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(cache) + crow * (D / 2) + c / 4 * 16)[p.at] = p.word;
+        if ((c & 3) == 0) (is_v ? a.v_d : a.k_d)[crow * (D / 32) + c / 4] = p.d;
     } else {
         // the largest magnitude by its bits: a NaN's are above all others, so that it reaches the scale
         uint32_t top = 0;
@@ -110,7 +144,7 @@ __device__ __forceinline__ void put(const RowsArgs& a, uint32_t t, uint32_t slot
 
 // One workgroup takes heads_per_wg heads of one token, one thread 8 consecutive elements of a head.  A thread loads its own 8 and, in the half layout, the 8 that they
 // are paired with before the barrier behind which the sines are ready, and stores after it: rows may be rotated in place.
-template <bool ROPE, bool Q8, bool INTER>
+template <bool ROPE, int FMT, bool INTER>
 __global__ __launch_bounds__(kRowThreads) void rows_kernel(RowsArgs a) {
     __shared__ float2 cs[128];
     const uint32_t tid = threadIdx.x, t = blockIdx.x / a.groups, D = a.chunks * 8;
@@ -133,13 +167,13 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(RowsArgs a) {
     if (!live) return;   // whole groups of four lanes: chunks % 4 == 0 wherever they exchange values
     half8 y = own;
     if (turned) y = INTER ? turn_interleaved(own, cs + c * 4) : first ? turn_first(own, other, cs + c * 8) : turn_second(other, own, cs + (c - half_chunks) * 8);
-    put<Q8>(a, t, slot, h, c, y);
+    put<FMT>(a, t, slot, h, c, y);
 }
 
 // Prompts: a workgroup takes one token with all its heads, a thread two chunks at a time, in the half layout the two that are turned together: rows may be rotated
 // in place.  The chunks of a head that are not turned, and a value head's, are paired with the same distance between the two throughout.
-// Q8: that distance is a multiple of four chunks (D and n_rot multiples of 64), so that four lanes hold whole blocks.
-template <bool ROPE, bool Q8, bool INTER>
+// Quantised: that distance is a multiple of four chunks (D and n_rot multiples of 64), so that four lanes hold whole blocks.
+template <bool ROPE, int FMT, bool INTER>
 __global__ __launch_bounds__(kRowThreads) void prompt_kernel(RowsArgs a) {
     __shared__ float2 cs[128];
     const uint32_t tid = threadIdx.x, threads = blockDim.x, t = blockIdx.x, D = a.chunks * 8, pairs = a.chunks / 2, items = (a.Hq + 2 * a.Hkv) * pairs, half_chunks = a.n_rot / 16;
@@ -180,8 +214,8 @@ __global__ __launch_bounds__(kRowThreads) void prompt_kernel(RowsArgs a) {
             if (m.c0 * 8 < a.n_rot) y0 = turn_interleaved(m.x0, cs + m.c0 * 4);
             if (m.c1 * 8 < a.n_rot) y1 = turn_interleaved(m.x1, cs + m.c1 * 4);
         }
-        put<Q8>(a, t, slot, m.h, m.c0, y0);
-        put<Q8>(a, t, slot, m.h, m.c1, y1);
+        put<FMT>(a, t, slot, m.h, m.c0, y0);
+        put<FMT>(a, t, slot, m.h, m.c1, y1);
     }
 }
 
@@ -189,14 +223,14 @@ __global__ __launch_bounds__(kRowThreads) void prompt_kernel(RowsArgs a) {
 static bool fits(uint64_t workgroups, uint32_t threads) { return workgroups * threads < (1ull << 32); }
 
 constexpr uint32_t kPromptTokens = 512;
-template <bool ROPE, bool Q8>
+template <bool ROPE, int FMT>
 static int launch_rows(mx_stream_t s, RowsArgs a, uint32_t T, int interleaved) {
     a.heads_per_wg = kRowThreads / a.chunks;
     a.groups = (a.Hq + 2 * a.Hkv + a.heads_per_wg - 1) / a.heads_per_wg;
     // Two chunks a thread load every row once where the half layout's other form loads turned rows twice: 8192 tokens of 72 heads of 64 35.9 -> 26.6 us (5.7 TB/s),
     // 2047 tokens of 32 + 4 + 4 heads of 128 into a Q8_0 cache 14.5 -> 9.4; interleaved pairs are as fast either way.  Fewer tokens leave CUs without work: one
     // token 2.2 -> 2.8 us, 333 (18 heads of 256) 3.9 -> 4.1.
-    if (T >= kPromptTokens && (!Q8 || (a.chunks % 8 == 0 && a.n_rot % 64 == 0))) {
+    if (T >= kPromptTokens && (FMT == kF16 || (a.chunks % 8 == 0 && a.n_rot % 64 == 0))) {
         // as many waves as the token's pairs of chunks fill evenly
         const uint32_t items = (a.Hq + 2 * a.Hkv) * (a.chunks / 2), turns = (items + kRowThreads - 1) / kRowThreads, threads = ((items + turns - 1) / turns + 63) / 64 * 64;
         MX_REQUIRE_SHAPE(fits(T, threads));
@@ -204,12 +238,12 @@ static int launch_rows(mx_stream_t s, RowsArgs a, uint32_t T, int interleaved) {
             hipLaunchKernelGGL(kernel, dim3(T), dim3(threads), 0, as_stream(s), a);
             return launch_status();
         };
-        return ROPE && interleaved ? launch(prompt_kernel<ROPE, Q8, ROPE>) : launch(prompt_kernel<ROPE, Q8, false>);
+        return ROPE && interleaved ? launch(prompt_kernel<ROPE, FMT, ROPE>) : launch(prompt_kernel<ROPE, FMT, false>);
     }
     MX_REQUIRE_SHAPE(fits((uint64_t)a.groups * T, kRowThreads));
     const dim3 grid(a.groups * T);
-    if (ROPE && interleaved) hipLaunchKernelGGL((rows_kernel<ROPE, Q8, ROPE>), grid, dim3(kRowThreads), 0, as_stream(s), a);
-    else hipLaunchKernelGGL((rows_kernel<ROPE, Q8, false>), grid, dim3(kRowThreads), 0, as_stream(s), a);
+    if (ROPE && interleaved) hipLaunchKernelGGL((rows_kernel<ROPE, FMT, ROPE>), grid, dim3(kRowThreads), 0, as_stream(s), a);
+    else hipLaunchKernelGGL((rows_kernel<ROPE, FMT, false>), grid, dim3(kRowThreads), 0, as_stream(s), a);
     return launch_status();
 }
 
@@ -218,7 +252,7 @@ static int launch_rows(mx_stream_t s, RowsArgs a, uint32_t T, int interleaved) {
 // copy's rate: 10 k tokens of them in 15.9 us, 5.1 TB/s).
 // Tile numbers are dealt by floor(rows[b] / 16) + b, which leaves room for every sequence's ceil(length / 16).
 constexpr int kReadPieces = 4;
-template <bool Q8, bool STREAM>
+template <int FMT, bool STREAM>
 __global__ __launch_bounds__(256) void kv_read_kernel(const void* k_cache, const half_t* k_d, const void* v_cache, const half_t* v_d, const int32_t* page_table,
                                                       uint32_t max_pages, const int32_t* rows, half_t* k_out, half_t* v_out, uint32_t total, uint32_t B,
                                                       uint32_t Hkv, uint32_t chunks, uint32_t n_pages, uint32_t page_size) {
@@ -256,12 +290,14 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const void* k_cache, const
         if (live[u] && good) {
             const size_t crow = ((size_t)page * Hkv + h) * page_size + (t0 - col * page_size) + tok;
             const void* cache = is_v[u] ? v_cache : k_cache;
-            if (!Q8) {
+            if (FMT == kF16) {
                 got[u] = *reinterpret_cast<const uint4*>(static_cast<const half_t*>(cache) + crow * D + c * 8);
             } else {
-                const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(cache) + crow * D + c * 8);
-                got[u].x = w.x;
-                got[u].y = w.y;
+                // Q4_0: the 8 bytes that hold the chunk's codes in their low halves and those of the chunk two further in their high ones, or the other way about
+                const size_t byte = FMT == kQ8 ? crow * D + c * 8 : crow * (D / 2) + c / 4 * 16 + (c & 1) * 8;
+                const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(cache) + byte);
+                got[u].x = FMT == kQ4 ? w.x >> (c & 2) * 2 : w.x;
+                got[u].y = FMT == kQ4 ? w.y >> (c & 2) * 2 : w.y;
                 d[u] = (is_v[u] ? v_d : k_d)[crow * (D / 32) + c / 4];
             }
         }
@@ -270,9 +306,12 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const void* k_cache, const
     for (int u = 0; u < U; ++u) {
         if (!live[u]) continue;
         half8 y = __builtin_bit_cast(half8, got[u]);
-        if (Q8) {
+        if (FMT != kF16) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = f32_to_f16_rne((float)(int8_t)((j < 4 ? got[u].x : got[u].y) >> (8 * (j & 3))) * (float)d[u]);
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t code = (j < 4 ? got[u].x : got[u].y) >> (8 * (j & 3));
+                y[j] = f32_to_f16_rne((FMT == kQ8 ? (float)(int8_t)code : (float)(int)(code & 15u) - 8.f) * (float)d[u]);
+            }
         }
         half8* const out = reinterpret_cast<half8*>((is_v[u] ? v_out : k_out) + (size_t)(row0 + t0) * Hkv * D) + at[u];
         if (STREAM) __builtin_nontemporal_store(y, out);
@@ -281,13 +320,13 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const void* k_cache, const
 }
 
 // ---------------------------------------------------------------- argument checks (before any HIP call)
-static int check_cache(bool q8, const void* k, const void* k_d, const void* v, const void* v_d, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size) {
+static int check_cache(int fmt, const void* k, const void* k_d, const void* v, const void* v_d, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size) {
     MX_REQUIRE_PTR(k); MX_REQUIRE_PTR(v);
-    if (q8) { MX_REQUIRE_PTR(k_d); MX_REQUIRE_PTR(v_d); }
-    MX_REQUIRE_SHAPE(Hkv > 0 && Hkv <= 65535 && D > 0 && D <= 256 && D % (q8 ? 32 : 16) == 0);
+    if (fmt != kF16) { MX_REQUIRE_PTR(k_d); MX_REQUIRE_PTR(v_d); }
+    MX_REQUIRE_SHAPE(Hkv > 0 && Hkv <= 65535 && D > 0 && D <= 256 && D % (fmt != kF16 ? 32 : 16) == 0);
     MX_REQUIRE_SHAPE(n_pages > 0 && page_size > 0 && page_size % 16 == 0 && (uint64_t)n_pages * page_size < (1ull << 31));
     MX_REQUIRE_ALIGN(k, 16); MX_REQUIRE_ALIGN(v, 16);
-    if (q8) { MX_REQUIRE_ALIGN(k_d, 16); MX_REQUIRE_ALIGN(v_d, 16); }
+    if (fmt != kF16) { MX_REQUIRE_ALIGN(k_d, 16); MX_REQUIRE_ALIGN(v_d, 16); }
     return MX_OK;
 }
 static int check_rows(const void* p, uint64_t stride, uint64_t width) {
@@ -308,11 +347,11 @@ static int check_rotation(const void* positions, const void* freqs, uint32_t D, 
     return MX_OK;
 }
 
-static int rope_kv_write(mx_stream_t s, bool q8, const uint16_t* q, uint64_t q_stride, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride,
+static int rope_kv_write(mx_stream_t s, int fmt, const uint16_t* q, uint64_t q_stride, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride,
                          uint16_t* q_out, uint64_t q_out_stride, void* k_cache, uint16_t* k_d, void* v_cache, uint16_t* v_d, const int32_t* positions,
                          const int32_t* slots, const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved,
                          double mscale, uint32_t n_pages, uint32_t page_size) {
-    if (int rc = check_cache(q8, k_cache, k_d, v_cache, v_d, Hkv, D, n_pages, page_size)) return rc;
+    if (int rc = check_cache(fmt, k_cache, k_d, v_cache, v_d, Hkv, D, n_pages, page_size)) return rc;
     if (int rc = check_rows(k, k_stride, (uint64_t)Hkv * D)) return rc;
     if (int rc = check_rows(v, v_stride, (uint64_t)Hkv * D)) return rc;
     MX_REQUIRE_PTR(slots);
@@ -334,14 +373,14 @@ static int rope_kv_write(mx_stream_t s, bool q8, const uint16_t* q, uint64_t q_s
     a.positions = positions; a.slots = slots; a.freqs = freqs;
     a.Hq = Hq; a.Hkv = Hkv; a.chunks = D / 8; a.n_rot = n_rot; a.page_size = page_size; a.n_slots = n_pages * page_size;
     a.mscale = mscale;
-    if (freqs) return q8 ? launch_rows<true, true>(s, a, T, interleaved) : launch_rows<true, false>(s, a, T, interleaved);
-    return q8 ? launch_rows<false, true>(s, a, T, 0) : launch_rows<false, false>(s, a, T, 0);
+    if (freqs) return fmt == kQ4 ? launch_rows<true, kQ4>(s, a, T, interleaved) : fmt == kQ8 ? launch_rows<true, kQ8>(s, a, T, interleaved) : launch_rows<true, kF16>(s, a, T, interleaved);
+    return fmt == kQ4 ? launch_rows<false, kQ4>(s, a, T, 0) : fmt == kQ8 ? launch_rows<false, kQ8>(s, a, T, 0) : launch_rows<false, kF16>(s, a, T, 0);
 }
 
-static int kv_read(mx_stream_t s, bool q8, const void* k, const uint16_t* k_d, const void* v, const uint16_t* v_d, const int32_t* page_table, uint32_t max_pages,
+static int kv_read(mx_stream_t s, int fmt, const void* k, const uint16_t* k_d, const void* v, const uint16_t* v_d, const int32_t* page_table, uint32_t max_pages,
                    const int32_t* rows, uint16_t* k_out, uint16_t* v_out, uint32_t total_rows, uint32_t B, uint32_t Hkv, uint32_t D, uint32_t n_pages,
                    uint32_t page_size) {
-    if (int rc = check_cache(q8, k, k_d, v, v_d, Hkv, D, n_pages, page_size)) return rc;
+    if (int rc = check_cache(fmt, k, k_d, v, v_d, Hkv, D, n_pages, page_size)) return rc;
     MX_REQUIRE_PTR(page_table); MX_REQUIRE_PTR(rows); MX_REQUIRE_PTR(k_out); MX_REQUIRE_PTR(v_out);
     MX_REQUIRE_SHAPE(B > 0 && B <= (1u << 24) && max_pages > 0 && total_rows > 0 && total_rows < (1u << 31) && fits(total_rows / 16 + (uint64_t)B, 256));
     MX_REQUIRE_ALIGN(page_table, 4); MX_REQUIRE_ALIGN(rows, 4); MX_REQUIRE_ALIGN(k_out, 16); MX_REQUIRE_ALIGN(v_out, 16);
@@ -351,8 +390,9 @@ static int kv_read(mx_stream_t s, bool q8, const void* k, const uint16_t* k_d, c
                            max_pages, rows, reinterpret_cast<half_t*>(k_out), reinterpret_cast<half_t*>(v_out), total_rows, B, Hkv, D / 8, n_pages, page_size);
         return launch_status();
     };
-    if ((uint64_t)total_rows * Hkv * D * 4 >= kStreamFrom) return q8 ? launch(kv_read_kernel<true, true>) : launch(kv_read_kernel<false, true>);
-    return q8 ? launch(kv_read_kernel<true, false>) : launch(kv_read_kernel<false, false>);
+    if ((uint64_t)total_rows * Hkv * D * 4 >= kStreamFrom)
+        return fmt == kQ4 ? launch(kv_read_kernel<kQ4, true>) : fmt == kQ8 ? launch(kv_read_kernel<kQ8, true>) : launch(kv_read_kernel<kF16, true>);
+    return fmt == kQ4 ? launch(kv_read_kernel<kQ4, false>) : fmt == kQ8 ? launch(kv_read_kernel<kQ8, false>) : launch(kv_read_kernel<kF16, false>);
 }
 
 }  // namespace mxq
@@ -391,7 +431,7 @@ int mx_rope(mx_stream_t s, const uint16_t* x, uint64_t x_stride, uint16_t* y, ui
     a.q_stride = x_stride; a.q_out_stride = y_stride;
     a.positions = positions; a.freqs = freqs;
     a.Hq = n_heads; a.chunks = D / 8; a.n_rot = n_rot; a.mscale = mscale;
-    return launch_rows<true, false>(s, a, T, interleaved);
+    return launch_rows<true, kF16>(s, a, T, interleaved);
 }
 
 int mx_rope_kv_write_f16(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride,
@@ -399,7 +439,7 @@ int mx_rope_kv_write_f16(mx_stream_t s, const uint16_t* q, uint64_t q_stride, co
                          const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved, double mscale,
                          uint32_t n_pages, uint32_t page_size) {
     MX_REQUIRE_PTR(freqs);
-    return rope_kv_write(s, false, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, k_cache, nullptr, v_cache, nullptr, positions, slots, freqs, T, Hq,
+    return rope_kv_write(s, kF16, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, k_cache, nullptr, v_cache, nullptr, positions, slots, freqs, T, Hq,
                          Hkv, D, n_rot, interleaved, mscale, n_pages, page_size);
 }
 int mx_rope_kv_write_q8_0(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride,
@@ -407,27 +447,45 @@ int mx_rope_kv_write_q8_0(mx_stream_t s, const uint16_t* q, uint64_t q_stride, c
                           const int32_t* slots, const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved,
                           double mscale, uint32_t n_pages, uint32_t page_size) {
     MX_REQUIRE_PTR(freqs);
-    return rope_kv_write(s, true, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, k_qs, k_d, v_qs, v_d, positions, slots, freqs, T, Hq, Hkv, D, n_rot,
+    return rope_kv_write(s, kQ8, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, k_qs, k_d, v_qs, v_d, positions, slots, freqs, T, Hq, Hkv, D, n_rot,
+                         interleaved, mscale, n_pages, page_size);
+}
+int mx_rope_kv_write_q4_0(mx_stream_t s, const uint16_t* q, uint64_t q_stride, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride,
+                          uint16_t* q_out, uint64_t q_out_stride, uint8_t* k_qs, uint16_t* k_d, uint8_t* v_qs, uint16_t* v_d, const int32_t* positions,
+                          const int32_t* slots, const double* freqs, uint32_t T, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t n_rot, int interleaved,
+                          double mscale, uint32_t n_pages, uint32_t page_size) {
+    MX_REQUIRE_PTR(freqs);
+    return rope_kv_write(s, kQ4, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, k_qs, k_d, v_qs, v_d, positions, slots, freqs, T, Hq, Hkv, D, n_rot,
                          interleaved, mscale, n_pages, page_size);
 }
 int mx_kv_write_f16(mx_stream_t s, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride, uint16_t* k_cache, uint16_t* v_cache,
                     const int32_t* slots, uint32_t T, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size) {
-    return rope_kv_write(s, false, nullptr, 0, k, k_stride, v, v_stride, nullptr, 0, k_cache, nullptr, v_cache, nullptr, nullptr, slots, nullptr, T, 0, Hkv, D, 0, 0,
+    return rope_kv_write(s, kF16, nullptr, 0, k, k_stride, v, v_stride, nullptr, 0, k_cache, nullptr, v_cache, nullptr, nullptr, slots, nullptr, T, 0, Hkv, D, 0, 0,
                          1.0, n_pages, page_size);
 }
 int mx_kv_write_q8_0(mx_stream_t s, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride, int8_t* k_qs, uint16_t* k_d, int8_t* v_qs,
                      uint16_t* v_d, const int32_t* slots, uint32_t T, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size) {
-    return rope_kv_write(s, true, nullptr, 0, k, k_stride, v, v_stride, nullptr, 0, k_qs, k_d, v_qs, v_d, nullptr, slots, nullptr, T, 0, Hkv, D, 0, 0, 1.0, n_pages,
+    return rope_kv_write(s, kQ8, nullptr, 0, k, k_stride, v, v_stride, nullptr, 0, k_qs, k_d, v_qs, v_d, nullptr, slots, nullptr, T, 0, Hkv, D, 0, 0, 1.0, n_pages,
+                         page_size);
+}
+int mx_kv_write_q4_0(mx_stream_t s, const uint16_t* k, uint64_t k_stride, const uint16_t* v, uint64_t v_stride, uint8_t* k_qs, uint16_t* k_d, uint8_t* v_qs,
+                     uint16_t* v_d, const int32_t* slots, uint32_t T, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size) {
+    return rope_kv_write(s, kQ4, nullptr, 0, k, k_stride, v, v_stride, nullptr, 0, k_qs, k_d, v_qs, v_d, nullptr, slots, nullptr, T, 0, Hkv, D, 0, 0, 1.0, n_pages,
                          page_size);
 }
 int mx_kv_read_f16(mx_stream_t s, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* page_table, uint32_t max_pages, const int32_t* rows,
                    uint16_t* k_out, uint16_t* v_out, uint32_t total_rows, uint32_t B, uint32_t Hkv, uint32_t D, uint32_t n_pages, uint32_t page_size) {
-    return kv_read(s, false, k_cache, nullptr, v_cache, nullptr, page_table, max_pages, rows, k_out, v_out, total_rows, B, Hkv, D, n_pages, page_size);
+    return kv_read(s, kF16, k_cache, nullptr, v_cache, nullptr, page_table, max_pages, rows, k_out, v_out, total_rows, B, Hkv, D, n_pages, page_size);
 }
 int mx_kv_read_q8_0(mx_stream_t s, const int8_t* k_qs, const uint16_t* k_d, const int8_t* v_qs, const uint16_t* v_d, const int32_t* page_table,
                     uint32_t max_pages, const int32_t* rows, uint16_t* k_out, uint16_t* v_out, uint32_t total_rows, uint32_t B, uint32_t Hkv, uint32_t D,
                     uint32_t n_pages, uint32_t page_size) {
-    return kv_read(s, true, k_qs, k_d, v_qs, v_d, page_table, max_pages, rows, k_out, v_out, total_rows, B, Hkv, D, n_pages, page_size);
+    return kv_read(s, kQ8, k_qs, k_d, v_qs, v_d, page_table, max_pages, rows, k_out, v_out, total_rows, B, Hkv, D, n_pages, page_size);
+}
+int mx_kv_read_q4_0(mx_stream_t s, const uint8_t* k_qs, const uint16_t* k_d, const uint8_t* v_qs, const uint16_t* v_d, const int32_t* page_table,
+                    uint32_t max_pages, const int32_t* rows, uint16_t* k_out, uint16_t* v_out, uint32_t total_rows, uint32_t B, uint32_t Hkv, uint32_t D,
+                    uint32_t n_pages, uint32_t page_size) {
+    return kv_read(s, kQ4, k_qs, k_d, v_qs, v_d, page_table, max_pages, rows, k_out, v_out, total_rows, B, Hkv, D, n_pages, page_size);
 }
 
 }  // extern "C"

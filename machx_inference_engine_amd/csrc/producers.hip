@@ -68,6 +68,86 @@ __global__ __launch_bounds__(kNormThreads) void norm_q8_kernel(const XT* x, cons
     }
 }
 
+// The residual's addition, the norm of the rounded sum and the 8-bit stream of the rounded norm.  A workgroup takes a row, thread u of pass p elements 8 (128 p + u) .. + 7, which are what threads
+// 2 u and 2 u + 1 of norm_q8_kernel<false> own: their squares are summed apart and in that kernel's order, so that rows normalised here have the bits of those normalised there.
+// P passes keep the row in registers between the sum and the norm (P = 0: rows that are longer read the sum back).
+// Bound by memory: 8 bytes and the stream's 1.25 or 1.5 an element.
+constexpr int kSumThreads = 128;
+template <int P, bool HALVES>
+__global__ __launch_bounds__(kSumThreads) void add_norm_q8_kernel(const half_t* x, const half_t* residual, const float* w, half_t* total, half_t* y, uint8_t* q8, uint32_t hidden, float eps) {
+    typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+    __shared__ float red[kSumThreads / 32];
+    const uint32_t tid = threadIdx.x;
+    const size_t row = (size_t)blockIdx.x * hidden;
+    const uint32_t passes = (hidden + kSumThreads * 8 - 1) / (kSumThreads * 8);
+    half8 h[P ? P : 1];
+    float even = 0.f, odd = 0.f;
+    auto add = [&](uint32_t p) {
+        half8 v = {};
+        const uint32_t i = (p * kSumThreads + tid) * 8;
+        if (i < hidden) {
+            const half8 a = *reinterpret_cast<const half8*>(x + row + i), b = *reinterpret_cast<const half8*>(residual + row + i);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = f32_to_f16_rne((float)a[j] + (float)b[j]);
+            *reinterpret_cast<half8*>(total + row + i) = v;
+        }
+        return v;
+    };
+    auto square = [&](const half8& v) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            even = fmaf((float)v[j], (float)v[j], even);
+            odd = fmaf((float)v[j + 4], (float)v[j + 4], odd);
+        }
+    };
+    if constexpr (P > 0) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) h[p] = add(p);
+#pragma unroll
+        for (int p = 0; p < P; ++p) square(h[p]);
+    } else {
+        for (uint32_t p = 0; p < passes; ++p) square(add(p));
+    }
+    // what block_sum adds, lane by lane of twice as many
+    const float part = group_sum<32>(even + odd);
+    if ((tid & 31u) == 31) red[tid >> 5] = part;
+    __syncthreads();
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < kSumThreads / 32; ++k) sum += red[k];
+    const float r = rsqrtf(sum / (float)hidden + eps);
+    auto norm = [&](uint32_t p, const half8& v) {
+        const uint32_t i = (p * kSumThreads + tid) * 8;
+        const bool live = i < hidden;
+        float f[8];
+        half8 o = {};
+        if (live) {
+            const float4 w0 = *reinterpret_cast<const float4*>(w + i), w1 = *reinterpret_cast<const float4*>(w + i + 4);
+            const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = (half_t)(((float)v[j] * r) * ww[j]);
+            // the stream goes by what is stored: without this the compiler may round a product twice over, to fp16 at once for the one and by way of fp32 for the other
+            typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
+            uint4_t bits = __builtin_bit_cast(uint4_t, o);
+            asm("" : "+v"(bits));
+            o = __builtin_bit_cast(half8, bits);
+            if (y) *reinterpret_cast<half8*>(y + row + i) = o;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = (float)o[j];
+        emit_q8_wide<HALVES>(f, tid & 3u, live, q8 + (row + i) / 32 * (HALVES ? kQ81sBytes : kQ81xBytes));
+    };
+    if constexpr (P > 0) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) norm(p, h[p]);
+    } else {
+        for (uint32_t p = 0; p < passes; ++p) {
+            const uint32_t i = (p * kSumThreads + tid) * 8;
+            norm(p, i < hidden ? *reinterpret_cast<const half8*>(total + row + i) : half8{});     // the thread's own stores
+        }
+    }
+}
+
 // y = half(silu(gate) * up) (swiglu, src/ops/elementwise.cpp:449-467) or, OAI = true, the clamped
 // gpt-oss form x = min(gate, limit), z = clamp(up, -limit, limit), y = half(x * sigmoid(alpha x) * (z + 1))
 // (swiglu_oai, :469-492), written as fp16 (when y != NULL) and as the block_q8_1x stream of the rounded
@@ -148,6 +228,32 @@ int mx_gated_rms_norm_q8(mx_stream_t s, const float* x, const uint16_t* z, const
     hipLaunchKernelGGL((norm_q8_kernel<true, float, half_t>), dim3(n_rows), dim3(kNormThreads), 0, as_stream(s), x, reinterpret_cast<const half_t*>(z),
                        reinterpret_cast<const half_t*>(weight), reinterpret_cast<half_t*>(y), static_cast<uint8_t*>(q8_out), hidden, eps);
     return launch_status();
+}
+
+int mx_add_rms_norm_f32w_q8(mx_stream_t s, const uint16_t* x, const uint16_t* residual, const float* w, uint16_t* sum, uint16_t* y, void* q8_out, uint32_t n_rows,
+                            uint32_t hidden, float eps, int halves) {
+    MX_REQUIRE_PTR(x); MX_REQUIRE_PTR(residual); MX_REQUIRE_PTR(w); MX_REQUIRE_PTR(sum); MX_REQUIRE_PTR(q8_out);
+    MX_REQUIRE_SHAPE(n_rows > 0 && n_rows < (1u << 25) && hidden > 0 && hidden % 32 == 0);
+    MX_REQUIRE_ALIGN(x, 16); MX_REQUIRE_ALIGN(residual, 16); MX_REQUIRE_ALIGN(w, 16); MX_REQUIRE_ALIGN(sum, 16); MX_REQUIRE_ALIGN(y, 16);
+    MX_REQUIRE_ALIGN(q8_out, halves ? 16 : 8);
+    auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(n_rows), dim3(kSumThreads), 0, as_stream(s), reinterpret_cast<const half_t*>(x), reinterpret_cast<const half_t*>(residual), w,
+                           reinterpret_cast<half_t*>(sum), reinterpret_cast<half_t*>(y), static_cast<uint8_t*>(q8_out), hidden, eps);
+        return launch_status();
+    };
+    const uint32_t passes = (hidden + kSumThreads * 8 - 1) / (kSumThreads * 8);
+#define MX_SUM(P) (halves ? launch(add_norm_q8_kernel<P, true>) : launch(add_norm_q8_kernel<P, false>))
+    switch (passes) {
+        case 1: return MX_SUM(1);
+        case 2: return MX_SUM(2);
+        case 3: return MX_SUM(3);
+        case 4: return MX_SUM(4);
+        case 5: return MX_SUM(5);
+        case 6: return MX_SUM(6);
+        case 7: case 8: return MX_SUM(8);
+        default: return MX_SUM(0);
+    }
+#undef MX_SUM
 }
 
 int mx_swiglu_q8(mx_stream_t s, const uint16_t* gate, const uint16_t* up, uint16_t* y, void* q8_out, uint64_t n) {

@@ -4,6 +4,7 @@
 //   softmax + top-k from logits already on the device                     src/ops/moe.cpp:366-412
 //   packing arrays for one token                                          src/ops/moe.cpp:423-446
 //   packing arrays for T tokens: stable counting sort by expert           src/model/qwen3moe_pack.cpp:5-31
+//   softmax or sigmoid scores, a bias, groups, top-k from logits          (no counterpart)
 #include "mxq_device.h"
 #include "mxq_host.h"
 
@@ -233,6 +234,143 @@ static int launch_topk(hipStream_t st, const LogitT* logits, int32_t* topk_idx, 
     return launch_status();
 }
 
+// ---------------------------------------------------------------- scores, bias, groups, top-k
+// A 64-bit number as an unsigned one of the same order; every NaN is 1, below all numbers, and 0 is left for experts that are out.
+__device__ __forceinline__ uint64_t order_of(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return v == v ? (b >> 63 ? ~b : b | 1ull << 63) : 1ull;
+}
+__device__ __forceinline__ double number_of(uint64_t k) {
+    return k == 1ull ? __builtin_nan("") : __builtin_bit_cast(double, k >> 63 ? k & ~(1ull << 63) : ~k);
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
+struct RouteArgs {
+    const void* logits;
+    const float* bias;
+    int32_t* topk_idx;
+    half_t* topk_w;
+    uint32_t n_tokens, E, K, n_groups, size, size_inv, kept, lanes, flags;   // size: experts of a group, size_inv = ceil(2^32 / size); lanes: of a wave for each group
+    float scale;
+};
+
+// One wave a token, lane l holds experts l, l + 64, .. (NJ of them): scores in 64 bits and, as integers of the same order, what they are chosen by.
+template <int NJ>
+__global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
+    __shared__ uint64_t choice[4][NJ * 64];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, t = blockIdx.x * 4u + wave;
+    if (t >= a.n_tokens) return;          // no barriers: a wave's LDS is its own
+    float x[NJ];
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const uint32_t e = lane + 64u * j;
+        const size_t at = (size_t)t * a.E + e;
+        x[j] = e >= a.E ? -INFINITY : a.flags & MX_ROUTE_F32 ? static_cast<const float*>(a.logits)[at] : (float)static_cast<const half_t*>(a.logits)[at];
+        m = fmaxf(m, x[j]);
+    }
+    double score[NJ];
+    if (a.flags & MX_ROUTE_SIGMOID) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) score[j] = 1.0 / (1.0 + exp(-(double)x[j]));
+    } else {
+        m = wave_max_f(m);
+        double sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            score[j] = x[j] == -INFINITY ? 0.0 : exp((double)x[j] - (double)m);
+            sum += score[j];
+        }
+        sum = wave_sum_f64(sum);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) score[j] = sum == 0.0 ? 0.0 : score[j] / sum;
+    }
+    uint64_t key[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const uint32_t e = lane + 64u * j;
+        key[j] = e < a.E ? order_of(a.bias ? score[j] + (double)a.bias[e] : score[j]) : 0ull;
+    }
+    if (a.n_groups > 1) {
+        // a group's two largest, by `lanes` lanes each, from LDS
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) choice[wave][lane + 64u * j] = key[j];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        uint64_t first = 0, second = 0;
+        const uint32_t group = lane / a.lanes;
+        if (group < a.n_groups)
+            for (uint32_t i = lane - group * a.lanes; i < a.size; i += a.lanes) {
+                const uint64_t k = choice[wave][group * a.size + i];
+                second = k > first ? first : k > second ? k : second;
+                first = k > first ? k : first;
+            }
+        for (uint32_t d = 1; d < a.lanes; d <<= 1) {
+            const uint64_t f = __shfl_xor(first, d), s = __shfl_xor(second, d);
+            const uint64_t low = f < first ? f : first, more = s > second ? s : second;
+            first = f > first ? f : first;
+            second = low > more ? low : more;
+        }
+        const uint64_t own = a.flags & MX_ROUTE_TOP2 && a.size > 1 ? order_of(number_of(first) + number_of(second)) : first;
+        const uint64_t worth = __shfl(own, lane * a.lanes & 63u);        // lane g: of group g
+        uint32_t better = 0;
+        for (uint32_t g = 0; g < a.n_groups; ++g) {
+            const uint64_t other = __shfl(worth, g);
+            better += other > worth || (other == worth && g < lane) ? 1u : 0u;
+        }
+        const uint64_t kept = __ballot(lane < a.n_groups && better < a.kept);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const uint32_t g = a.size == 1u ? lane + 64u * j : __umulhi(lane + 64u * j, a.size_inv);
+            if (!(kept >> (g & 63u) & 1ull)) key[j] = 0ull;
+        }
+    }
+    // K rounds of the largest key, the lowest id among equal ones
+    unsigned long long taken[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) taken[j] = 0ull;
+    for (uint32_t kk = 0; kk < a.K; ++kk) {
+        uint64_t best = key[0];
+#pragma unroll
+        for (int j = 1; j < NJ; ++j) best = key[j] > best ? key[j] : best;
+        const uint32_t high = wave_max_u32((uint32_t)(best >> 32)), low = wave_max_u32((uint32_t)(best >> 32) == high ? (uint32_t)best : 0u);
+        const uint64_t win = (uint64_t)high << 32 | low;
+        bool open = true;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const unsigned long long hit = open ? __ballot(key[j] == win) : 0ull;
+            if (hit) {
+                const uint32_t l = (uint32_t)__ffsll(hit) - 1u;
+                taken[j] |= 1ull << l;
+                if (lane == l) key[j] = 0ull;
+                open = false;
+            }
+        }
+    }
+    double factor = (double)a.scale;
+    if (a.flags & MX_ROUTE_RENORM) {
+        double sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) sum += (taken[j] >> lane) & 1ull ? score[j] : 0.0;
+        factor /= wave_sum_f64(sum) + 1e-20;
+    }
+    uint32_t below = 0;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        if ((taken[j] >> lane) & 1ull) {
+            const size_t at = (size_t)t * a.K + below + (uint32_t)__builtin_popcountll(taken[j] & ((1ull << lane) - 1ull));
+            a.topk_idx[at] = (int32_t)(lane + 64u * j);
+            a.topk_w[at] = (half_t)(score[j] * factor);
+        }
+        below += (uint32_t)__builtin_popcountll(taken[j]);
+    }
+}
+
 // ---------------------------------------------------------------- packing
 // One token (src/ops/moe.cpp:423-446): offsets by counting, identity order.
 __global__ void pack_decode_kernel(const int32_t* topk_idx, const half_t* topk_w, uint32_t* expert_offsets, int32_t* sorted_idx, int32_t* tk_to_packed,
@@ -373,6 +511,32 @@ int mx_moe_router(mx_stream_t s, const uint16_t* x, const float* W_gate, int32_t
     hipStream_t st = as_stream(s);
     if (int rc = launch_router_logits(st, reinterpret_cast<const half_t*>(x), W_gate, logits_ws, n_tokens, hidden, n_experts)) return rc;
     return launch_topk(st, (const float*)logits_ws, topk_idx, reinterpret_cast<half_t*>(topk_w), n_experts, k, n_tokens);
+}
+
+int mx_moe_router_logits(mx_stream_t s, const uint16_t* x, const float* W_gate, float* logits, uint32_t n_tokens, uint32_t hidden, uint32_t n_experts) {
+    MX_REQUIRE_PTR(x); MX_REQUIRE_PTR(W_gate); MX_REQUIRE_PTR(logits);
+    MX_REQUIRE_SHAPE(n_tokens > 0 && n_tokens <= 65535 && hidden > 0 && hidden % 4 == 0 && n_experts > 0 && n_experts <= 1024);
+    MX_REQUIRE_ALIGN(x, 8); MX_REQUIRE_ALIGN(W_gate, 16); MX_REQUIRE_ALIGN(logits, 4);
+    return launch_router_logits(as_stream(s), reinterpret_cast<const half_t*>(x), W_gate, logits, n_tokens, hidden, n_experts);
+}
+
+int mx_moe_route(mx_stream_t s, const void* logits, const float* bias, int32_t* topk_idx, uint16_t* topk_w, uint32_t n_tokens, uint32_t n_experts, uint32_t k,
+                 uint32_t n_groups, uint32_t topk_groups, uint32_t flags, float scale) {
+    MX_REQUIRE_PTR(logits); MX_REQUIRE_PTR(topk_idx); MX_REQUIRE_PTR(topk_w);
+    MX_REQUIRE_SHAPE(n_tokens > 0 && n_tokens < (1u << 26) && n_experts > 0 && n_experts <= 1024 && n_groups > 0 && n_groups <= 64 && n_experts % n_groups == 0);
+    const uint32_t size = n_experts / n_groups;
+    MX_REQUIRE_SHAPE(topk_groups > 0 && topk_groups <= n_groups && k > 0 && k <= (uint32_t)kMaxTopK && k <= topk_groups * size && flags < 16u);
+    MX_REQUIRE_ALIGN(logits, flags & MX_ROUTE_F32 ? 4 : 2); MX_REQUIRE_ALIGN(bias, 4); MX_REQUIRE_ALIGN(topk_idx, 4); MX_REQUIRE_ALIGN(topk_w, 2);
+    RouteArgs a = {logits, bias, topk_idx, reinterpret_cast<half_t*>(topk_w), n_tokens, n_experts, k, n_groups, size, size > 1 ? 0xFFFFFFFFu / size + 1u : 0u, topk_groups, 1, flags, scale};
+    while (a.lanes * 2 * n_groups <= 64) a.lanes *= 2;
+    const dim3 grid((n_tokens + 3) / 4), block(256);
+    hipStream_t st = as_stream(s);
+    if (n_experts <= 64) hipLaunchKernelGGL((route_kernel<1>), grid, block, 0, st, a);
+    else if (n_experts <= 128) hipLaunchKernelGGL((route_kernel<2>), grid, block, 0, st, a);
+    else if (n_experts <= 256) hipLaunchKernelGGL((route_kernel<4>), grid, block, 0, st, a);
+    else if (n_experts <= 512) hipLaunchKernelGGL((route_kernel<8>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((route_kernel<16>), grid, block, 0, st, a);
+    return launch_status();
 }
 
 int mx_moe_build_pack_decode(mx_stream_t s, const int32_t* topk_idx, const uint16_t* topk_w, uint32_t* expert_offsets, int32_t* sorted_idx,

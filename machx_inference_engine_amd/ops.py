@@ -57,6 +57,14 @@ def _call(name, *args):
         raise MxError(name, rc)
 
 
+def _want(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+_F16, _F32, _F64, _I32, _I8, _U8 = torch.float16, torch.float32, torch.float64, torch.int32, torch.int8, torch.uint8
+
+
 def _f16(t):
     assert t.dtype == torch.float16, t.dtype
     return _ptr(t)
@@ -737,6 +745,41 @@ def moe_topk_from_logits(logits, k):
     return idx, w
 
 
+def moe_router_logits(x, W_gate):
+    """x fp16 [T, H], W_gate fp32 [E, H] -> fp32 [T, E], the logits that moe_router goes by."""
+    T, H = x.shape
+    E = W_gate.shape[0]
+    _want(W_gate.dtype is _F32 and W_gate.shape == (E, H), "W_gate is fp32 [experts, H]")
+    logits = torch.empty((T, E), dtype=_F32, device=x.device)
+    _call("mx_moe_router_logits", _f16(x), _ptr(W_gate), _ptr(logits), T, H, E)
+    return logits
+
+
+_ROUTE_SCORE, _ROUTE_GROUP = {"softmax": 0, "sigmoid": 1}, {"max": 0, "top2": 4}
+
+
+def moe_route(logits, k, score="softmax", bias=None, n_groups=1, topk_groups=1, group_score="max", renormalize=True, scale=1.0):
+    """logits fp16 or fp32 [T, E] -> (topk_idx int32 [T, k] ascending, topk_w fp16 [T, k]).  score: "softmax" or "sigmoid"; the k largest score + bias (fp32 [E]) of the topk_groups
+    best of n_groups groups, by a group's largest ("max") or the sum of its two largest ("top2"); equal ones: the lowest id.  Weights: the scores without the bias, over
+    their sum (renormalize), times scale."""
+    dev = _current_device()
+    T, E = logits.shape
+    f32 = logits.dtype is _F32
+    _want(score in _ROUTE_SCORE and group_score in _ROUTE_GROUP, "score is softmax or sigmoid, group_score max or top2")
+    flags = _ROUTE_SCORE[score] | (2 if renormalize else 0) | _ROUTE_GROUP[group_score] | (8 if f32 else 0)
+    logits_ptr = _dev(logits, _F32 if f32 else _F16, dev, "logits")
+    bias_ptr = None
+    if bias is not None:
+        _want(bias.numel() == E, "bias: one for each expert")
+        bias_ptr = _dev(bias, _F32, dev, "bias")
+    idx = torch.empty((T, k), dtype=_I32, device=logits.device)
+    w = torch.empty((T, k), dtype=_F16, device=logits.device)
+    rc = lib.mx_moe_route(_stream_of(dev), logits_ptr, bias_ptr, idx.data_ptr(), w.data_ptr(), T, E, k, n_groups, topk_groups, flags, scale)
+    if rc != 0:
+        raise MxError("mx_moe_route", rc)
+    return idx, w
+
+
 def moe_build_packing_device(topk_idx, topk_w, E, decode=False):
     """Device arrays (expert_offsets uint32-as-int32 [E+1], sorted_idx, weights_packed fp16, tk_to_packed)."""
     T, K = topk_idx.shape
@@ -761,6 +804,26 @@ def rms_norm_f32w_q8(x, w, eps):
     assert w.dtype == torch.float32
     _call("mx_rms_norm_f32w_q8", _f16(x), _ptr(w), _ptr(y), _ptr(q8), n_rows, hidden, float(eps))
     return y, q8
+
+
+def add_rms_norm_f32w_q8(x, residual, w, eps, halves=False, want_y=True, out=None):
+    """x, residual fp16 [rows, hidden] -> (half(x + residual), its norm times w (fp32) as fp16 or None, that norm's block_q8_1x stream, block_q8_1s with halves).
+    out = (sum, y, q8) reuses caller buffers; sum may be residual or x, y None where want_y is false."""
+    dev, shape = _current_device(), x.shape
+    n_rows, hidden = shape
+    size = n_rows * (hidden // 32) * (Q81S_BYTES if halves else Q81X_BYTES)
+    if out is not None:
+        total, y, q8 = out
+    else:
+        total, y = torch.empty_like(x), torch.empty_like(x) if want_y else None
+        q8 = torch.empty(size, dtype=torch.uint8, device=x.device)
+    if residual.shape != shape or total.shape != shape or w.numel() != hidden or q8.numel() != size or (y is not None and y.shape != shape):
+        raise ValueError("x, residual, sum and y are [rows, hidden], w has hidden elements, q8 40 (halves: 48) bytes for each 32")
+    rc = lib.mx_add_rms_norm_f32w_q8(_stream_of(dev), _dev(x, _F16, dev, "x"), _dev(residual, _F16, dev, "residual"), _dev(w, _F32, dev, "w"), _dev(total, _F16, dev, "sum"),
+                                     None if y is None else _dev(y, _F16, dev, "y"), _dev(q8, torch.uint8, dev, "q8"), n_rows, hidden, eps, halves)
+    if rc != 0:
+        raise MxError("mx_add_rms_norm_f32w_q8", rc)
+    return total, y, q8
 
 
 def swiglu_q8(gate, up, oai=False, alpha=1.702, limit=7.0, want_y=True, out=None):
@@ -789,12 +852,6 @@ def gated_rms_norm_q8(x, z, weight, eps):
 
 
 # ---------------------------------------------------------------- rotary positions, the key-value cache, the attention of one token
-def _want(ok, what):
-    if not ok:
-        raise ValueError(what)
-
-
-_F16, _F32, _F64, _I32, _I8 = torch.float16, torch.float32, torch.float64, torch.int32, torch.int8
 
 
 # These run before every launch of a decode step, so they ask for no more than they need: rope() into a given y takes 5.9 us, of
@@ -824,29 +881,35 @@ def _new_rows(t):
 
 
 def _cache(cache, dev):
-    """(plane addresses, shape) of a cache: (k, v) fp16 or (k_qs, k_d, v_qs, v_d) Q8_0 planes."""
+    """(plane addresses, shape, format) of a cache: (k, v) fp16 or (k_qs, k_d, v_qs, v_d), int8 codes of Q8_0 or uint8 pairs of Q4_0."""
     shape = cache[0].shape
     if len(cache) == 2:
         k, v = cache
         if v.shape != shape or len(shape) != 4:
             raise ValueError("the planes of a cache are [pages, heads, page size, D], both of one shape")
-        return (_dev(k, _F16, dev, "k"), _dev(v, _F16, dev, "v")), shape
-    _want(len(cache) == 4 and len(shape) == 4, "a cache is (k, v) or (k_qs, k_d, v_qs, v_d), planes [pages, heads, page size, D]")
-    scales = shape[:3] + (shape[3] // 32,)
+        return (_dev(k, _F16, dev, "k"), _dev(v, _F16, dev, "v")), shape, "f16"
+    _want(len(cache) == 4 and len(shape) == 4, "a cache is (k, v) or (k_qs, k_d, v_qs, v_d), planes [pages, heads, page size, D], of Q4_0 D / 2 bytes")
+    codes, fmt, whole = (_U8, "q4_0", (*shape[:3], 2 * shape[3])) if cache[0].dtype is _U8 else (_I8, "q8_0", shape)
+    scales = shape[:3] + (whole[3] // 32,)
     if cache[2].shape != shape or cache[1].shape != scales or cache[3].shape != scales:
         raise ValueError("the planes of a cache have one shape, its scales one for each 32")
-    return (_dev(cache[0], _I8, dev, "k_qs"), _dev(cache[1], _F16, dev, "k_d"), _dev(cache[2], _I8, dev, "v_qs"),
-            _dev(cache[3], _F16, dev, "v_d")), shape
+    return (_dev(cache[0], codes, dev, "k_qs"), _dev(cache[1], _F16, dev, "k_d"), _dev(cache[2], codes, dev, "v_qs"),
+            _dev(cache[3], _F16, dev, "v_d")), whole, fmt
+
+
+_ROPE_KV_WRITE, _KV_WRITE, _KV_READ, _ATTN_DECODE = ({fmt: getattr(lib, "mx_%s_%s" % (name, fmt)) for fmt in ("f16", "q8_0", "q4_0")}
+                                                     for name in ("rope_kv_write", "kv_write", "kv_read", "attn_decode"))
 
 
 def kv_cache(fmt, n_pages, n_kv_heads, page_size, head_dim, device="cuda"):
     """The planes of an empty paged cache: fmt "f16" -> (k, v) fp16 [n_pages, n_kv_heads, page_size, head_dim]; "q8_0" -> (k_qs, k_d, v_qs, v_d),
-    int8 of that shape with fp16 scales [..., head_dim / 32].  A token's slot is page * page_size + offset."""
+    int8 of that shape with fp16 scales [..., head_dim / 32]; "q4_0" -> the same, uint8 [..., head_dim / 2].  A token's slot is page * page_size + offset."""
     shape = (n_pages, n_kv_heads, page_size, head_dim)
     if fmt == "f16":
         return tuple(torch.zeros(shape, dtype=_F16, device=device) for _ in range(2))
-    _want(fmt == "q8_0" and head_dim % 32 == 0, "a cache is f16, or q8_0 with heads of whole blocks of 32")
-    plane = lambda: (torch.zeros(shape, dtype=_I8, device=device), torch.zeros(shape[:3] + (head_dim // 32,), dtype=_F16, device=device))  # noqa: E731
+    _want(fmt in ("q8_0", "q4_0") and head_dim % 32 == 0, "a cache is f16, or q8_0 or q4_0 with heads of whole blocks of 32")
+    codes = torch.zeros(shape, dtype=_I8, device=device) if fmt == "q8_0" else torch.zeros(shape[:3] + (head_dim // 2,), dtype=_U8, device=device)
+    plane = lambda: (codes.clone(), torch.zeros(shape[:3] + (head_dim // 32,), dtype=_F16, device=device))  # noqa: E731
     return plane() + plane()
 
 
@@ -882,7 +945,7 @@ def rope(x, positions, freqs, interleaved=False, mscale=1.0, y=None):
 def rope_kv_write(q, k, v, positions, slots, cache, freqs, interleaved=False, mscale=1.0, q_out=None):
     """Rotates q [T, Hq, D] -> q_out (returned; q_out=q: in place) and k [T, Hkv, D]; writes k and v to the cache's slots (int32 [T]; outside the cache: skipped)."""
     dev, q_shape = _current_device(), q.shape
-    planes, (n_pages, Hkv, page_size, D) = _cache(cache, dev)
+    planes, (n_pages, Hkv, page_size, D), fmt = _cache(cache, dev)
     T, Hq, Dq = q_shape
     if q_out is None:
         q_out = _new_rows(q)
@@ -892,7 +955,7 @@ def rope_kv_write(q, k, v, positions, slots, cache, freqs, interleaved=False, ms
     if Dq != D or positions.numel() != T or slots.numel() != T:
         raise ValueError("q has the cache's D, positions and slots one entry for each row")
     kv_shape = (T, Hkv, D)
-    fn = lib.mx_rope_kv_write_f16 if len(planes) == 2 else lib.mx_rope_kv_write_q8_0
+    fn = _ROPE_KV_WRITE[fmt]
     rc = fn(_stream_of(dev), *_rows(q, q_shape, dev, "q"), *_rows(k, kv_shape, dev, "k"), *_rows(v, kv_shape, dev, "v"), *to, *planes,
             _dev(positions, _I32, dev, "positions"), _dev(slots, _I32, dev, "slots"), _dev(freqs, _F64, dev, "freqs"), T, Hq, Hkv, D,
             2 * freqs.numel(), interleaved, mscale, n_pages, page_size)
@@ -904,9 +967,9 @@ def rope_kv_write(q, k, v, positions, slots, cache, freqs, interleaved=False, ms
 def kv_write(k, v, slots, cache):
     """k, v fp16 [T, Hkv, D] as they are into the cache's slots (int32 [T]; outside the cache: skipped)."""
     dev = _current_device()
-    planes, (n_pages, Hkv, page_size, D) = _cache(cache, dev)
+    planes, (n_pages, Hkv, page_size, D), fmt = _cache(cache, dev)
     T = slots.numel()
-    fn = lib.mx_kv_write_f16 if len(planes) == 2 else lib.mx_kv_write_q8_0
+    fn = _KV_WRITE[fmt]
     rc = fn(_stream_of(dev), *_rows(k, (T, Hkv, D), dev, "k"), *_rows(v, (T, Hkv, D), dev, "v"), *planes, _dev(slots, _I32, dev, "slots"), T, Hkv, D, n_pages, page_size)
     if rc != 0:
         raise MxError("mx_kv_write", rc)
@@ -915,7 +978,7 @@ def kv_write(k, v, slots, cache):
 def kv_read(cache, page_table, rows, total_rows, out=None):
     """The first rows[b + 1] - rows[b] tokens of every sequence b (rows int32 [B + 1], page_table int32 [B, max_pages]) -> k, v fp16 [total_rows, Hkv, D]."""
     dev = _current_device()
-    planes, (n_pages, Hkv, page_size, D) = _cache(cache, dev)
+    planes, (n_pages, Hkv, page_size, D), fmt = _cache(cache, dev)
     B, max_pages = page_table.shape
     shape = (total_rows, Hkv, D)
     if out is None:
@@ -924,7 +987,7 @@ def kv_read(cache, page_table, rows, total_rows, out=None):
         k, v = out
     if rows.numel() != B + 1 or k.shape != shape or v.shape != shape:
         raise ValueError("rows has one entry more than there are sequences, outputs are [total_rows, heads, D]")
-    fn = lib.mx_kv_read_f16 if len(planes) == 2 else lib.mx_kv_read_q8_0
+    fn = _KV_READ[fmt]
     rc = fn(_stream_of(dev), *planes, _dev(page_table, _I32, dev, "page_table"), max_pages, _dev(rows, _I32, dev, "rows"), _dev(k, _F16, dev, "k_out"),
             _dev(v, _F16, dev, "v_out"), total_rows, B, Hkv, D, n_pages, page_size)
     if rc != 0:
@@ -946,7 +1009,7 @@ def attn_decode(q, cache, page_table, seq_lens, scale=None, window=0, sinks=None
     scale: D ** -0.5 unless given; window: the last tokens only; sinks: fp32 [Hq]; max_len: the longest sequence, where the host knows it; out_q8: uint8
     buffer for the block_q8_1x stream of the output rows; ws: a workspace of attn_decode_ws_bytes."""
     dev, q_shape = _current_device(), q.shape
-    planes, (n_pages, Hkv, page_size, D) = _cache(cache, dev)
+    planes, (n_pages, Hkv, page_size, D), fmt = _cache(cache, dev)
     B, Hq, Dq = q_shape
     rows, max_pages = page_table.shape
     if max_len is None:
@@ -970,7 +1033,7 @@ def attn_decode(q, cache, page_table, seq_lens, scale=None, window=0, sinks=None
     if out_q8 is not None:
         _want(out_q8.numel() * 32 == B * Hq * D * Q81X_BYTES, "out_q8: 40 bytes for each 32 elements of out")
         q8_ptr = _dev(out_q8, torch.uint8, dev, "out_q8")
-    fn = lib.mx_attn_decode_f16 if len(planes) == 2 else lib.mx_attn_decode_q8_0
+    fn = _ATTN_DECODE[fmt]
     rc = fn(_stream_of(dev), *_rows(q, q_shape, dev, "q"), *planes, _dev(page_table, _I32, dev, "page_table"), max_pages, _dev(seq_lens, _I32, dev, "seq_lens"),
             sinks_ptr, _dev(out, _F16, dev, "out"), q8_ptr, B, Hq, Hkv, D, n_pages, page_size, max_len, window, D ** -0.5 if scale is None else scale, ws_ptr,
             ws_size)
