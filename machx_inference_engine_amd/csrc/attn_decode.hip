@@ -621,11 +621,15 @@ static Plan plan_of(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t 
 // are made of differs, since at a quarter of fp16's bytes the vector unit is what would bound a kernel that widens every value and multiplies it by its scale:
 //   * A 4-bit code in the low bits of a half is n 2^-24, in bits 4 .. 7 it is 16 n 2^-24: numbers below fp16's normal range, which the matrix instruction multiplies exactly.  One `and`
 //     gives two operands, none converts.  The codes' offset, value = d (n - 8), is taken out of the sums.
-//   * Keys: a query's values that meet high codes are divided by 16, and the product of a block starts from -8 times the sum of its query values; its four rows are then multiplied by their tokens' scales.
+//   * The products have 16 columns and a group has G query heads, mostly 1 to 8: the columns are C groups of 16 / C >= G heads, the same heads in each, and column group c is
+//     block c's (then c + C's, ..).  A set is C blocks; there are S = ceil(NB / C) of them.
+//   * Keys: the operand of block n holds the queries in the columns of its group and zeros elsewhere, so that the products of a set add up in one accumulator, block by block in columns of their own:
+//     one multiplication by the scales for each set and token, and the groups are added up across lanes.
+//     A query's values that meet high codes are divided by 16, and the sum starts from -8 times the sum of a block's query values.
 //     Queries are scaled by a power of two to a largest element of 2^14 .. 2^15, so that neither division nor small queries lose bits.
-//   * Values: the scales multiply the weights instead, for each block of 32 (p d in two fp16 parts, from p's two: three packed operations for two tokens, and the products of a block share
-//     them), and the offset is 8 times sum p d, one matrix product of the scales' tile with the weights for all blocks, in which a row of ones gives the sum of weights too.
-//     For that every product's 16 rows are the low or the high codes of one block: the bytes of a block's column of 8 tokens come from LDS by the transposing read.
+//   * Values: the scales multiply the weights instead, each column's those of its block (p d in two fp16 parts, from p's two: three packed operations for two tokens of a set), and
+//     a block's products are right in its columns.  The offset is 8 times sum p d, one matrix product of the scales' tile with the weights for all blocks, in which a row of ones gives the
+//     sum of weights too.  Every product's 16 rows are the low or the high codes of one block: the bytes of a block's column of 8 tokens come from LDS by the transposing read.
 //   * p d must stay in fp16's range: the largest weight is 2^(15 - k), 2^k above every scale that this wave has met (k > 0 only for values beyond 8).
 // Precision as above: p d is held to 2^-22, or 2^-39 + k of the largest weight's; what the offsets cancel in the fp32 sums is at most 15 / 8 of the values' own size.
 
@@ -635,10 +639,13 @@ __device__ __forceinline__ half8 codes_f16(uint32_t a, uint32_t b, uint32_t mask
     return __builtin_bit_cast(half8, uint4_t{a & mask, a >> 8 & mask, b & mask, b >> 8 & mask});
 }
 
-template <int NB>
+template <int NB, int C>
 __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void attn_decode_q4_kernel(AttnArgs a) {
-    constexpr uint32_t D = 32 * NB, ROW = 16 * (NB | 1);        // LDS bytes of a token's codes: an odd number of 16-byte pieces, so that 16 rows meet all banks
-    constexpr uint32_t CODES = kTile * ROW, KS = kTile * NB * 2, VS = kTile * (NB + 1) * 2, WAVE = 2 * CODES + KS + VS;
+    constexpr uint32_t D = 32 * NB, GP = 16 / C;
+    // LDS of a token's codes: an odd number of 16-byte pieces, so that 16 rows meet all banks; the second half of a tile lies four rows further, for the keys' rows 0 .. 3, 8 .. 11, 16 .. 19, 24 .. 27
+    constexpr uint32_t ROW = 16 * (NB | 1), HALF = 20 * ROW;
+    constexpr uint32_t CODES = HALF + 16 * ROW, KS = kTile * NB * 2, VS = kTile * (NB + 1) * 2, WAVE = 2 * CODES + KS + VS;
+    constexpr int S = (NB + C - 1) / C;
     constexpr uint32_t OS = D + 4;
     constexpr int LP = (NB + 1) / 2, SL = (16 * NB + 63) / 64;  // a lane's 16-byte pieces of a tile's codes, dwords of its scales
     extern __shared__ float lds[];
@@ -649,8 +656,9 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
     const uint32_t share = blockIdx.x;
     char* const keys = reinterpret_cast<char*>(lds) + wave * WAVE;
     char* const values = keys + CODES;
-    half_t* const k_scales = reinterpret_cast<half_t*>(values + CODES);               // [token][block]
-    half_t* const v_scales = reinterpret_cast<half_t*>(values + CODES + KS);          // [block][token], tokens of four in the order 0 2 1 3; a row of ones behind them
+    half_t* const k_scales = reinterpret_cast<half_t*>(values + CODES);               // [block][token]
+    half_t* const v_scales = reinterpret_cast<half_t*>(values + CODES + KS);          // the same, and a row of ones behind them
+    const uint32_t head = r % GP, group = r / GP;
     Share sh = {1, 1, blockIdx.x, 0, 0};
     if (shared) sh = share_of(a, share, lane);
     else sh.len = a.lens[sh.b];
@@ -716,7 +724,7 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
         for (int i = 0; i < LP; ++i) {
             const uint32_t w = i * 64 + lane;
             if (NB % 2 == 0 || w < 32 * NB) {
-                const uint32_t at = w / NB * ROW + w % NB * 16;
+                const uint32_t at = w / NB * ROW + w % NB * 16 + (w < 16 * NB ? 0 : HALF - 16 * ROW);
                 *reinterpret_cast<uint4*>(keys + at) = kr[i];
                 *reinterpret_cast<uint4*>(values + at) = vr[i];
             }
@@ -725,10 +733,11 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
         for (int i = 0; i < SL; ++i) {
             const uint32_t w = i * 64 + lane;
             if (SL * 64 == 16 * NB || w < 16 * NB) {
-                reinterpret_cast<uint32_t*>(k_scales)[w] = ks[i];
-                auto place = [&](uint32_t s) { return s % NB * kTile + ((s / NB & ~3u) | (s / NB & 1u) << 1 | (s / NB >> 1 & 1u)); };
-                reinterpret_cast<uint16_t*>(v_scales)[place(2 * w)] = (uint16_t)vs[i];
-                reinterpret_cast<uint16_t*>(v_scales)[place(2 * w + 1)] = (uint16_t)(vs[i] >> 16);
+                const uint32_t p0 = 2 * w % NB * kTile + 2 * w / NB, p1 = (2 * w + 1) % NB * kTile + (2 * w + 1) / NB;
+                reinterpret_cast<uint16_t*>(k_scales)[p0] = (uint16_t)ks[i];
+                reinterpret_cast<uint16_t*>(k_scales)[p1] = (uint16_t)(ks[i] >> 16);
+                reinterpret_cast<uint16_t*>(v_scales)[p0] = (uint16_t)vs[i];
+                reinterpret_cast<uint16_t*>(v_scales)[p1] = (uint16_t)(vs[i] >> 16);
             }
         }
     };
@@ -740,44 +749,53 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
         load(cur);
         if (tile + kWaves < last) next = locate(tile + kWaves);
     }
-    // ---- queries: lane (r, g) has head r, of every block elements 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3, in the order of a word's codes
+    // ---- queries: lane (r, g) has the head and the blocks of its column, of a block elements 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3, in the order of a word's codes
     half8 qf[NB];
-    float off[NB];
+    float off[S];
     float unit;              // of the scores
     {
         float top = 0.f;
-        uint2 lo[NB], hi[NB];
+        uint2 lo[S], hi[S];
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            lo[n] = hi[n] = make_uint2(0, 0);
-            if (r < heads) {
-                const half_t* p = a.q + b * a.q_stride + (size_t)(hk * G + head0 + r) * D + n * 32 + 4 * g;
-                lo[n] = *reinterpret_cast<const uint2*>(p);
-                hi[n] = *reinterpret_cast<const uint2*>(p + 16);
+        for (int s = 0; s < S; ++s) {
+            const uint32_t n = s * C + group;
+            lo[s] = hi[s] = make_uint2(0, 0);
+            if (head < heads && n < NB) {
+                const half_t* p = a.q + b * a.q_stride + (size_t)(hk * G + head0 + head) * D + n * 32 + 4 * g;
+                lo[s] = *reinterpret_cast<const uint2*>(p);
+                hi[s] = *reinterpret_cast<const uint2*>(p + 16);
             }
-            top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(h2f(lo[n].x & 0xFFFFu)), fabsf(h2f(lo[n].x >> 16))), fmaxf(fabsf(h2f(lo[n].y & 0xFFFFu)), fabsf(h2f(lo[n].y >> 16)))),
-                                   fmaxf(fmaxf(fabsf(h2f(hi[n].x & 0xFFFFu)), fabsf(h2f(hi[n].x >> 16))), fmaxf(fabsf(h2f(hi[n].y & 0xFFFFu)), fabsf(h2f(hi[n].y >> 16))))));
+            top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(h2f(lo[s].x & 0xFFFFu)), fabsf(h2f(lo[s].x >> 16))), fmaxf(fabsf(h2f(lo[s].y & 0xFFFFu)), fabsf(h2f(lo[s].y >> 16)))),
+                                   fmaxf(fmaxf(fabsf(h2f(hi[s].x & 0xFFFFu)), fabsf(h2f(hi[s].x >> 16))), fmaxf(fabsf(h2f(hi[s].y & 0xFFFFu)), fabsf(h2f(hi[s].y >> 16))))));
         }
+        if (C >= 2) top = fmaxf(top, dpp_f<0x128>(top));                     // over the column groups: rotations by 8, 4, 2 within 16 lanes
+        if (C >= 4) top = fmaxf(top, dpp_f<0x124>(top));
+        if (C >= 8) top = fmaxf(top, dpp_f<0x122>(top));
         top = rows_max(top);
         const uint32_t e = f2u(top) >> 23;                                 // 2^(e - 127) <= top < 2^(e - 126)
         const uint32_t up = e == 0 ? 0u : 141u - min(e, 141u);             // by 2^up to 2^14 and more (at most 38; from 2^15 on as it is)
         const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f, by = sign * u2f((127u + up) << 23);
         unit = a.scale == 0.f ? 1.f : fabsf(a.scale) * 0x1p24f * u2f((127u - up) << 23);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            const float v[8] = {h2f(lo[n].x & 0xFFFFu), h2f(lo[n].y & 0xFFFFu), h2f(hi[n].x & 0xFFFFu), h2f(hi[n].y & 0xFFFFu),
-                                h2f(lo[n].x >> 16),     h2f(lo[n].y >> 16),     h2f(hi[n].x >> 16),     h2f(hi[n].y >> 16)};
+        for (int s = 0; s < S; ++s) {
+            const float v[8] = {h2f(lo[s].x & 0xFFFFu), h2f(lo[s].y & 0xFFFFu), h2f(hi[s].x & 0xFFFFu), h2f(hi[s].y & 0xFFFFu),
+                                h2f(lo[s].x >> 16),     h2f(lo[s].y >> 16),     h2f(hi[s].x >> 16),     h2f(hi[s].y >> 16)};
             float sum = 0.f;
+            half8 q;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 sum += v[i] * by;
-                qf[n][i] = (half_t)(v[i] * by * (i & 2 ? 0.0625f : 1.f));
+                q[i] = (half_t)(v[i] * by * (i & 2 ? 0.0625f : 1.f));
             }
-            off[n] = rows_sum(sum) * -0x1p-21f;
+            off[s] = rows_sum(sum) * -0x1p-21f;
+#pragma unroll
+            for (int n = s * C; n < s * C + C && n < NB; ++n) qf[n] = group == (uint32_t)(n - s * C) ? q : half8{};
         }
     }
     if (lane < 16) reinterpret_cast<uint32_t*>(v_scales + NB * kTile)[lane] = 0x3C003C00u;
 
+    float minus = -1.f;                        // unknown to the compiler, which would subtract a converted half in two instructions where a mixed multiply-add takes one
+    asm("" : "+s"(minus));
     float m = -INFINITY, room = 15.f;          // room: log2 of the largest weight
     uint32_t most = 15u << 10;                  // scales below this, as bits, leave it as it is
     floatx4 o[2 * NB], z = {0.f, 0.f, 0.f, 0.f};
@@ -818,35 +836,38 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
             load(next);
         }
         // ---- scores: row r of product t is token 8 (r / 4) + r % 4 + 4 t, so that lane (r, g) gets tokens 8 g + 4 t + 0 .. 3 of head r
-        floatx4 score[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        uint4 kd[NB];                    // scales of the lane's 8 tokens: [token][block]
-#pragma unroll
-        for (int n = 0; n < NB; ++n) kd[n] = reinterpret_cast<const uint4*>(k_scales + 8 * g * NB)[n];
-        const char* const key_row = keys + (8 * (r >> 2) + (r & 3u)) * ROW + 4 * g;
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(key_row + t * 4 * ROW + n * 16);
-                typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
-                const half8 kf = __builtin_bit_cast(half8, uint4_t{w & 0x000F000Fu, w & 0x00F000F0u, w >> 8 & 0x000F000Fu, w >> 8 & 0x00F000F0u});
-                const floatx4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[n], floatx4{off[n], off[n], off[n], off[n]}, 0, 0, 0);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int i = (4 * t + j) * NB + n;
-                    const uint32_t two = i / 2 % 4 == 0 ? kd[i / 8].x : i / 2 % 4 == 1 ? kd[i / 8].y : i / 2 % 4 == 2 ? kd[i / 8].z : kd[i / 8].w;
-                    score[t][j] = fmaf(p[j], h2f((i & 1 ? two >> 16 : two) & 0xFFFFu), score[t][j]);
-                }
-            }
         float x[8];
+        const char* const key_row = keys + (8 * (r >> 2) + (r & 3u)) * ROW + (r >> 3) * (HALF - 16 * ROW) + 4 * g;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const half8 kd = *reinterpret_cast<const half8*>(k_scales + min((uint32_t)(s * C) + group, NB - 1u) * kTile + 8 * g);
+            floatx4 p[2] = {{off[s], off[s], off[s], off[s]}, {off[s], off[s], off[s], off[s]}};
+#pragma unroll
+            for (int n = s * C; n < s * C + C && n < NB; ++n)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const uint32_t w = *reinterpret_cast<const uint32_t*>(key_row + t * 4 * ROW + n * 16);
+                    typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
+                    const half8 kf = __builtin_bit_cast(half8, uint4_t{w & 0x000F000Fu, w & 0x00F000F0u, w >> 8 & 0x000F000Fu, w >> 8 & 0x00F000F0u});
+                    p[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[n], p[t], 0, 0, 0);
+                }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = fmaf(p[i / 4][i % 4], (float)kd[i], s == 0 ? 0.f : x[i]);
+        }
+        // over the column groups: rotations by 8, 4, 2 within 16 lanes, in this order, so that every lane adds the same pairs
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            x[i] = score[i / 4][i % 4] * unit;
-            if (!full) x[i] = live(8 * g + i) ? x[i] : -INFINITY;
+            if (C >= 2) x[i] += dpp_f<0x128>(x[i]);
+            if (C >= 4) x[i] += dpp_f<0x124>(x[i]);
+            if (C >= 8) x[i] += dpp_f<0x122>(x[i]);
         }
-        // ---- running maximum, weights
+        if (!full) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = live(8 * g + i) ? x[i] : -INFINITY;
+        }
+        // ---- running maximum, weights (unit is positive)
         float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-        top = rows_max(top);
+        top = rows_max(top) * unit;
         top = fmaxf(m, fabsf(top) < kMostShifted ? top - room : top);
         const float ref = top == -INFINITY ? 0.f : top;
         if (__any(top > m)) {
@@ -856,30 +877,36 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
             for (int e = 0; e < 2 * NB; ++e) o[e] *= keep;
             m = top;
         }
-        half8 hi, lo;        // in the order of a column's bytes: 0 2 1 3, 4 6 5 7
+        half8 hi, lo;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int at = (i & 4) | (i & 1) << 1 | (i >> 1 & 1);
-            const float p = __builtin_amdgcn_exp2f(x[i] - ref);
-            hi[at] = (half_t)p;
-            lo[at] = (half_t)(p - (float)hi[at]);
+        for (int i = 0; i < 8; i += 2) {
+            typedef float float2_t __attribute__((ext_vector_type(2)));
+            const float2_t p = {__builtin_amdgcn_exp2f(fmaf(x[i], unit, -ref)), __builtin_amdgcn_exp2f(fmaf(x[i + 1], unit, -ref))};
+            const half2_t h = __builtin_convertvector(p, half2_t);
+            const half2_t rest = __builtin_convertvector((float2_t{fmaf((float)h[0], minus, p[0]), fmaf((float)h[1], minus, p[1])}), half2_t);
+            hi[i] = h[0]; hi[i + 1] = h[1];
+            lo[i] = rest[0]; lo[i + 1] = rest[1];
         }
         // ---- sums of weights and of weights times scales
         const half8 sc = *reinterpret_cast<const half8*>(v_scales + min(r, (uint32_t)NB) * kTile + 8 * g);
         z = __builtin_amdgcn_mfma_f32_16x16x32_f16(sc, hi, z, 0, 0, 0);
         z = __builtin_amdgcn_mfma_f32_16x16x32_f16(sc, lo, z, 0, 0, 0);
-        // ---- values
+        // ---- values: bytes 0 1 2 3 of a word of the transposing read are tokens 0 2 1 3 of four, so that an `and` leaves two consecutive ones; lane r of 16 brings 8 bytes of row r / 2
+        const char* const value_row = values + (8 * g + ((r >> 1 & 4u) | (r >> 1 & 1u) << 1 | (r >> 2 & 1u))) * ROW + (g >> 1) * (HALF - 16 * ROW) + (r & 1u) * 8;
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            typedef int int2_t __attribute__((ext_vector_type(2)));
-            const int2_t w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((int2_t __attribute__((address_space(3)))*)(values + (8 * g + (r >> 1)) * ROW + n * 16 + (r & 1u) * 8));
-            const half8 d = *reinterpret_cast<const half8*>(v_scales + n * kTile + 8 * g);
+        for (int s = 0; s < S; ++s) {
+            const half8 d = *reinterpret_cast<const half8*>(v_scales + min((uint32_t)(s * C) + group, NB - 1u) * kTile + 8 * g);
             const half8 p = hi * d, rest = __builtin_elementwise_fma(lo, d, __builtin_elementwise_fma(hi, d, -p));
-            const half8 v0 = codes_f16((uint32_t)w.x, (uint32_t)w.y, 0x000F000Fu), v1 = codes_f16((uint32_t)w.x, (uint32_t)w.y, 0x00F000F0u);
-            o[2 * n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p, o[2 * n], 0, 0, 0);
-            o[2 * n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p, o[2 * n + 1], 0, 0, 0);
-            o[2 * n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, rest, o[2 * n], 0, 0, 0);
-            o[2 * n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, rest, o[2 * n + 1], 0, 0, 0);
+#pragma unroll
+            for (int n = s * C; n < s * C + C && n < NB; ++n) {
+                typedef int int2_t __attribute__((ext_vector_type(2)));
+                const int2_t w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((int2_t __attribute__((address_space(3)))*)(value_row + n * 16));
+                const half8 v0 = codes_f16((uint32_t)w.x, (uint32_t)w.y, 0x000F000Fu), v1 = codes_f16((uint32_t)w.x, (uint32_t)w.y, 0x00F000F0u);
+                o[2 * n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p, o[2 * n], 0, 0, 0);
+                o[2 * n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p, o[2 * n + 1], 0, 0, 0);
+                o[2 * n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, rest, o[2 * n], 0, 0, 0);
+                o[2 * n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, rest, o[2 * n + 1], 0, 0, 0);
+            }
         }
         if (more) {
             cur = next;
@@ -887,20 +914,20 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
         }
     }
 
-    // ---- the waves' sums: lane (r, g) holds elements 32 n + 16 h + 4 g + 0 .. 3 of head r in o[2 n + h]; sum p d of block n is in row n of z, the sum of weights in row NB
+    // ---- the waves' sums: lane (r, g) holds elements 32 n + 16 h + 4 g + 0 .. 3 of its head in o[2 n + h], of the blocks of its column; sum p d of block n is in row n of z, the sum of weights in row NB
     __syncthreads();                         // the tiles' place is taken
     float* ml = lds;                         // [waves][16] (maximum, sum)
     float* os = lds + kWaves * 32;            // [waves][heads][OS]
     const float l = __shfl(z[NB % 4], NB / 4 * 16 + r);
-    if (g == 0) {
+    if (g == 0 && group == 0) {
         ml[(wave * 16 + r) * 2] = m;
         ml[(wave * 16 + r) * 2 + 1] = l;
     }
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
         const float eight = -8.f * __shfl(z[n % 4], n / 4 * 16 + r);
-        if (r < heads) {
-            float* row = os + (wave * heads + r) * OS + n * 32 + 4 * g;
+        if (head < heads && group == (uint32_t)(n % C)) {
+            float* row = os + (wave * heads + head) * OS + n * 32 + 4 * g;
             floatx4 s0, s1;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -945,15 +972,23 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
 // ---------------------------------------------------------------- launches
 enum { kF16 = 0, kQ8 = 1, kQ4 = 2 };   // what a cache holds
 
-template <int NB>
+template <int NB, int C>
 static int launch_q4(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads) {
     static LdsLimit limit;
-    constexpr uint32_t tiles = kWaves * (2 * kTile * 16 * (NB | 1) + kTile * (2 * NB + 1) * 2), most = kWaves * (32 + 16 * (32 * NB + 4)) * 4;
+    constexpr uint32_t tiles = kWaves * (2 * 36 * 16 * (NB | 1) + kTile * (2 * NB + 1) * 2), most = kWaves * (32 + 16 / C * (32 * NB + 4)) * 4;
     const uint32_t sums = kWaves * (32 + heads * (32 * NB + 4)) * 4, lds = tiles > sums ? tiles : sums;
     if (lds > kLdsDefaultLimit)
-        if (int rc = raise_lds_limit(reinterpret_cast<const void*>(attn_decode_q4_kernel<NB>), limit, tiles > most ? tiles : most)) return rc;
-    hipLaunchKernelGGL((attn_decode_q4_kernel<NB>), grid, dim3(kWaves * 64), lds, as_stream(s), a);
+        if (int rc = raise_lds_limit(reinterpret_cast<const void*>(attn_decode_q4_kernel<NB, C>), limit, tiles > most ? tiles : most)) return rc;
+    hipLaunchKernelGGL((attn_decode_q4_kernel<NB, C>), grid, dim3(kWaves * 64), lds, as_stream(s), a);
     return launch_status();
+}
+// As many column groups as the heads leave room for and the blocks can use.
+template <int NB>
+static int launch_q4_columns(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads) {
+    if (NB > 4 && heads <= 2) return launch_q4<NB, (NB > 4 ? 8 : 1)>(s, a, grid, heads);
+    if (NB > 2 && heads <= 4) return launch_q4<NB, (NB > 2 ? 4 : 1)>(s, a, grid, heads);
+    if (NB > 1 && heads <= 8) return launch_q4<NB, (NB > 1 ? 2 : 1)>(s, a, grid, heads);
+    return launch_q4<NB, 1>(s, a, grid, heads);
 }
 template <bool Q8, int DP, int NBLK, bool FULL>
 static int launch_form(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads) {
@@ -968,14 +1003,14 @@ static int launch_form(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t hea
 }
 static int launch_attn(mx_stream_t s, const AttnArgs& a, int fmt, dim3 grid, uint32_t heads) {
     if (fmt == kQ4) switch (a.D / 32) {
-        case 1: return launch_q4<1>(s, a, grid, heads);
-        case 2: return launch_q4<2>(s, a, grid, heads);
-        case 3: return launch_q4<3>(s, a, grid, heads);
-        case 4: return launch_q4<4>(s, a, grid, heads);
-        case 5: return launch_q4<5>(s, a, grid, heads);
-        case 6: return launch_q4<6>(s, a, grid, heads);
-        case 7: return launch_q4<7>(s, a, grid, heads);
-        default: return launch_q4<8>(s, a, grid, heads);
+        case 1: return launch_q4_columns<1>(s, a, grid, heads);
+        case 2: return launch_q4_columns<2>(s, a, grid, heads);
+        case 3: return launch_q4_columns<3>(s, a, grid, heads);
+        case 4: return launch_q4_columns<4>(s, a, grid, heads);
+        case 5: return launch_q4_columns<5>(s, a, grid, heads);
+        case 6: return launch_q4_columns<6>(s, a, grid, heads);
+        case 7: return launch_q4_columns<7>(s, a, grid, heads);
+        default: return launch_q4_columns<8>(s, a, grid, heads);
     }
     if (fmt == kQ8) switch (a.D / 32) {
         case 1: return launch_form<true, 64, 1, false>(s, a, grid, heads);

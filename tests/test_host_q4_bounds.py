@@ -23,15 +23,21 @@ template <class V> static V shim_tr8(V* p) {
     return v;
 }
 #define __builtin_amdgcn_ds_read_tr8_b64_v2i32 shim_tr8
+static int shim_dpp_or_rotation(int old, int v, int ctrl, int row_mask, int bank_mask, bool bound) {
+    if (ctrl > 0x120 && ctrl <= 0x12F) return from_lane(v, 3, 16, ((lane_id() & 15) + ctrl - 0x120) & 15);
+    return shim_dpp(old, v, ctrl, row_mask, bank_mask, bound);
+}
+#undef __builtin_amdgcn_update_dpp
+#define __builtin_amdgcn_update_dpp shim_dpp_or_rotation
 """
 
 ATTENTION = r"""
-template <int NB> static void one(uint32_t Hkv, uint32_t G, uint32_t ps, uint32_t window, uint32_t shares, std::vector<int32_t> lens, float scale = 0.3f, float q_size = 1.f, int plant = 0) {
+template <int NB, int C> static void one(uint32_t Hkv, uint32_t G, uint32_t ps, uint32_t window, uint32_t shares, std::vector<int32_t> lens, float scale = 0.3f, float q_size = 1.f, int plant = 0) {
     const uint32_t D = 32 * NB, B = (uint32_t)lens.size(), Hq = Hkv * G;
     uint32_t most = 1, pages = 0;
     for (int32_t n : lens) { const uint32_t need = n > 0 ? (n + ps - 1) / ps : 0; most = std::max(most, need); pages += need; }
     if (pages == 0) pages = 1;
-    snprintf(what, sizeof what, "attention, Q4_0 D=%u Hkv=%u G=%u pages of %u, window %u, %u shares, %u sequences of %d.., scale %g, queries of %g, plant %d\n", D, Hkv, G, ps, window, shares, B, lens[0], scale, q_size, plant);
+    snprintf(what, sizeof what, "attention, Q4_0 D=%u, %d column groups, Hkv=%u G=%u pages of %u, window %u, %u shares, %u sequences of %d.., scale %g, queries of %g, plant %d\n", D, C, Hkv, G, ps, window, shares, B, lens[0], scale, q_size, plant);
     const size_t values = (size_t)pages * Hkv * ps * D;
     Held q(2 * (size_t)B * Hq * D), k(values / 2), v(values / 2), kd(values / 16), vd(values / 16), table(4 * (size_t)B * most), len(4 * B), sinks(4 * Hq),
         out(2 * (size_t)B * Hq * D), q8((size_t)B * Hq * D / 32 * 40 + 8), ws((((size_t)shares + B) * Hq * (D + 2) * 4 + B * 8 + 15) / 16 * 16);
@@ -68,8 +74,8 @@ template <int NB> static void one(uint32_t Hkv, uint32_t G, uint32_t ps, uint32_
     a.page_shift = (ps & (ps - 1)) == 0 ? (uint32_t)__builtin_ctz(ps) : 32u;
     a.scale = scale * kLog2e;
     const uint32_t heads = std::min(G, 16u);
-    const size_t tiles = kWaves * (2 * kTile * 16 * (NB | 1) + kTile * (2 * NB + 1) * 2), sums = kWaves * (32 + heads * (D + 4)) * 4;   // as the launch asks for
-    run(kWaves * 64, shares ? shares : B, Hkv * ((G + 15) / 16), std::max(tiles, sums), [&] { attn_decode_q4_kernel<NB>(a); });
+    const size_t tiles = kWaves * (2 * 36 * 16 * (NB | 1) + kTile * (2 * NB + 1) * 2), sums = kWaves * (32 + heads * (D + 4)) * 4;   // as the launch asks for
+    run(kWaves * 64, shares ? shares : B, Hkv * ((G + 15) / 16), std::max(tiles, sums), [&] { attn_decode_q4_kernel<NB, C>(a); });
     if (shares) {
         uint32_t groups = std::min((shares / B + 4) / 4, 512 / (D / 4));
         run((groups * (D / 4) + 63) / 64 * 64, B * Hq, 1, groups * D * 4, [&] { attn_join_kernel(a, groups); });
@@ -118,18 +124,23 @@ int main() {
 
 # lengths that end within a tile, at its end, at a page's end, in the last page of the cache; every width of head, short and in shares; other sizes of queries and scales; planes with no numbers
 ATTENTION_CASES = {
-    "32": "one<1>(2, 2, 16, 0, 0, {1, 33, 0}); one<1>(1, 17, 48, 33, 3, {250, 0, 0, 48, 96});",
-    "64": "one<2>(1, 8, 16, 0, 0, {16, 129}); one<2>(2, 1, 48, 33, 3, {250, 0, 0, 48, 96}); one<2>(1, 4, 16, 0, 0, {300}, -0.3f, 1e-4f); one<2>(1, 2, 16, 7, 0, {40, 7}, 0.f);",
-    "96": "one<3>(1, 2, 16, 0, 0, {31, 32}); one<3>(1, 1, 32, 40, 2, {200});",
-    "128": "one<4>(1, 4, 64, 0, 0, {65}); one<4>(1, 2, 16, 0, 3, {300, 1, 0, 128}); one<4>(1, 16, 16, 0, 0, {47}, 0.1f, 30.f);",
-    "wide": "one<5>(1, 1, 16, 0, 0, {17}); one<6>(1, 2, 16, 0, 0, {32}); one<7>(1, 1, 48, 0, 2, {140}); one<8>(1, 2, 16, 0, 2, {150, 0, 31}); one<8>(1, 1, 32, 9, 0, {64});",
-    "scales": "one<2>(1, 3, 16, 0, 0, {333, 5}, 0.3f, 1.f, 1); one<4>(1, 2, 32, 0, 3, {400, 31}, 0.3f, 1.f, 1); one<2>(2, 1, 48, 0, 0, {17, 100, 1}, 0.3f, 1.f, 2); one<3>(1, 1, 16, 20, 2, {333, 18}, 0.3f, 1.f, 2);",
-    "no_numbers": "one<2>(1, 3, 16, 0, 0, {133, 5}, 0.3f, 1.f, 3); one<4>(1, 2, 32, 0, 3, {300, 31}, 0.3f, 1.f, 3);",
+    "32": "one<1, 1>(2, 2, 16, 0, 0, {1, 33, 0}); one<1, 1>(1, 17, 48, 33, 3, {250, 0, 0, 48, 96});",
+    "64": """one<2, 2>(1, 8, 16, 0, 0, {16, 129}); one<2, 2>(2, 1, 48, 33, 3, {250, 0, 0, 48, 96}); one<2, 2>(1, 4, 16, 0, 0, {300}, -0.3f, 1e-4f); one<2, 1>(1, 9, 16, 0, 0, {100, 33});
+             one<2, 2>(1, 2, 16, 7, 0, {40, 7}, 0.f);""",
+    "96": "one<3, 4>(1, 2, 16, 0, 0, {31, 32}); one<3, 4>(1, 1, 32, 40, 2, {200}); one<3, 2>(1, 5, 16, 0, 0, {45}); one<3, 1>(1, 10, 16, 0, 0, {45});",
+    "128": "one<4, 4>(1, 4, 64, 0, 0, {65}); one<4, 4>(1, 2, 16, 0, 3, {300, 1, 0, 128}); one<4, 1>(1, 16, 16, 0, 0, {47}, 0.1f, 30.f); one<4, 2>(1, 7, 16, 0, 2, {300, 64});",
+    "wide": """one<5, 8>(1, 1, 16, 0, 0, {17}); one<6, 8>(1, 2, 16, 0, 0, {32}); one<7, 8>(1, 1, 48, 0, 2, {140}); one<8, 8>(1, 2, 16, 0, 2, {150, 0, 31}); one<8, 8>(1, 1, 32, 9, 0, {64});
+               one<5, 4>(1, 3, 16, 0, 0, {40}); one<6, 2>(1, 6, 16, 0, 0, {70}); one<7, 4>(1, 4, 16, 0, 0, {33}); one<8, 4>(1, 4, 16, 0, 2, {150}); one<8, 2>(1, 8, 16, 0, 0, {50}); one<8, 1>(1, 9, 16, 0, 0, {40});
+               one<5, 1>(1, 12, 16, 0, 0, {20}); one<7, 2>(1, 5, 16, 0, 0, {20});""",
+    "scales": """one<2, 2>(1, 3, 16, 0, 0, {333, 5}, 0.3f, 1.f, 1); one<4, 4>(1, 2, 32, 0, 3, {400, 31}, 0.3f, 1.f, 1); one<2, 2>(2, 1, 48, 0, 0, {17, 100, 1}, 0.3f, 1.f, 2);
+                 one<3, 4>(1, 1, 16, 20, 2, {333, 18}, 0.3f, 1.f, 2);""",
+    "no_numbers": "one<2, 2>(1, 3, 16, 0, 0, {133, 5}, 0.3f, 1.f, 3); one<4, 4>(1, 2, 32, 0, 3, {300, 31}, 0.3f, 1.f, 3); one<4, 2>(1, 5, 32, 0, 0, {100}, 0.3f, 1.f, 3);",
 }
 
 
 def attention_source():
-    return B.source("attn_decode.hip", "// ---------------------------------------------------------------- launches").replace("__attribute__((address_space(3)))", "")
+    return B.source("attn_decode.hip", "// ---------------------------------------------------------------- launches").replace("__attribute__((address_space(3)))", "").replace(
+        'asm("" : "+s"(minus));', "")
 
 
 @pytest.mark.parametrize("form", sorted(ATTENTION_CASES))
