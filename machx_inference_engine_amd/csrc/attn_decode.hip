@@ -625,6 +625,8 @@ static Plan plan_of(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t 
 //     block c's (then c + C's, ..).  A set is C blocks; there are S = ceil(NB / C) of them.
 //   * Keys: the operand of block n holds the queries in the columns of its group and zeros elsewhere, so that the products of a set add up in one accumulator, block by block in columns of their own:
 //     one multiplication by the scales for each set and token, and the groups are added up across lanes.
+//   * The order of a lane's 8 tokens is the block's own: that of column group c begins c mod R quarters (R = min(C, 4); halves, for C = 2) further on, in rows of the first product, in the scales' tile and in the depth
+//     of the second.  So a rotation across lanes adds one group's tokens to another's, every lane ends with 8 / R scores, whose exponentials only it takes, and rotations give the other weights back.
 //     A query's values that meet high codes are divided by 16, and the sum starts from -8 times the sum of a block's query values.
 //     Queries are scaled by a power of two to a largest element of 2^14 .. 2^15, so that neither division nor small queries lose bits.
 //   * Values: the scales multiply the weights instead, each column's those of its block (p d in two fp16 parts, from p's two: three packed operations for two tokens of a set), and
@@ -638,6 +640,11 @@ __device__ __forceinline__ half8 codes_f16(uint32_t a, uint32_t b, uint32_t mask
     typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
     return __builtin_bit_cast(half8, uint4_t{a & mask, a >> 8 & mask, b & mask, b >> 8 & mask});
 }
+
+template <int N>
+struct Int {
+    static constexpr int value = N;
+};
 
 template <int NB, int C>
 __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void attn_decode_q4_kernel(AttnArgs a) {
@@ -656,9 +663,20 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
     const uint32_t share = blockIdx.x;
     char* const keys = reinterpret_cast<char*>(lds) + wave * WAVE;
     char* const values = keys + CODES;
-    half_t* const k_scales = reinterpret_cast<half_t*>(values + CODES);               // [block][token]
+    half_t* const k_scales = reinterpret_cast<half_t*>(values + CODES);               // [block][token], eight tokens in their block's order
     half_t* const v_scales = reinterpret_cast<half_t*>(values + CODES + KS);          // the same, and a row of ones behind them
     const uint32_t head = r % GP, group = r / GP;
+    // a lane's 8 tokens are 4 pairs; place q of column group c (and of its blocks) has pair (q + turn) % 4, turn = PS * (c % R)
+    constexpr int R = C < 4 ? C : 4, PS = 4 / R, V = 8 / R;      // PS pairs and V tokens whose weights a lane finds
+    auto turn_of = [](uint32_t n) { return n % C % R * PS; };
+    const uint32_t turn = turn_of(group);
+    // rows of the products: row r of product t of a block that is turned by u is token 8 (r / 4) + 2 ((2 t + r / 2 % 2 + u) % 4) + r % 2, so that lane (r, g) gets tokens of 8 g .. 8 g + 7 in its order
+    uint32_t key_at[R == 4 ? 4 : 2], value_at[R];
+#pragma unroll
+    for (int k = 0; k < (R == 4 ? 4 : 2); ++k) key_at[k] = (8 * (r >> 2) + 2 * (((r >> 1 & 1u) + k * (R == 4 ? 1 : 2)) & 3u) + (r & 1u)) * ROW + (r >> 3) * (HALF - 16 * ROW) + 4 * g;
+    // bytes 0 1 2 3 of a word of the transposing read are tokens 0 2 1 3 of four places, so that an `and` leaves two consecutive ones; lane r of 16 brings 8 bytes of row r / 2
+#pragma unroll
+    for (int k = 0; k < R; ++k) value_at[k] = (8 * g + 2 * (((r >> 2 & 2u) + (r >> 1 & 1u) + k * PS) & 3u) + (r >> 2 & 1u)) * ROW + (g >> 1) * (HALF - 16 * ROW) + (r & 1u) * 8;
     Share sh = {1, 1, blockIdx.x, 0, 0};
     if (shared) sh = share_of(a, share, lane);
     else sh.len = a.lens[sh.b];
@@ -733,7 +751,11 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
         for (int i = 0; i < SL; ++i) {
             const uint32_t w = i * 64 + lane;
             if (SL * 64 == 16 * NB || w < 16 * NB) {
-                const uint32_t p0 = 2 * w % NB * kTile + 2 * w / NB, p1 = (2 * w + 1) % NB * kTile + (2 * w + 1) / NB;
+                auto place = [&](uint32_t i) {
+                    const uint32_t n = i % NB, t = i / NB;
+                    return n * kTile + (t & 24u) + (((t >> 1) - turn_of(n)) & 3u) * 2 + (t & 1u);
+                };
+                const uint32_t p0 = place(2 * w), p1 = place(2 * w + 1);
                 reinterpret_cast<uint16_t*>(k_scales)[p0] = (uint16_t)ks[i];
                 reinterpret_cast<uint16_t*>(k_scales)[p1] = (uint16_t)(ks[i] >> 16);
                 reinterpret_cast<uint16_t*>(v_scales)[p0] = (uint16_t)vs[i];
@@ -742,29 +764,34 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
         }
     };
 
-    uint32_t tile = first + wave;
-    Ref cur = {}, next = {};
-    if (tile < last) {
-        cur = locate(tile);
-        load(cur);
-        if (tile + kWaves < last) next = locate(tile + kWaves);
-    }
+    float m = -INFINITY;
+    floatx4 o[2 * NB], z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 2 * NB; ++e) o[e] = floatx4{0.f, 0.f, 0.f, 0.f};
+    if (first + wave < last) {
     // ---- queries: lane (r, g) has the head and the blocks of its column, of a block elements 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3, in the order of a word's codes
+    uint2 lo[S], hi[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const uint32_t n = s * C + group;
+        lo[s] = hi[s] = make_uint2(0, 0);
+        if (head < heads && n < NB) {
+            const half_t* p = a.q + b * a.q_stride + (size_t)(hk * G + head0 + head) * D + n * 32 + 4 * g;
+            lo[s] = *reinterpret_cast<const uint2*>(p);
+            hi[s] = *reinterpret_cast<const uint2*>(p + 16);
+        }
+    }
+    uint32_t tile = first + wave;
+    Ref cur = locate(tile), next = cur;
+    load(cur);
+    if (tile + kWaves < last) next = locate(tile + kWaves);
     half8 qf[NB];
     float off[S];
     float unit;              // of the scores
     {
         float top = 0.f;
-        uint2 lo[S], hi[S];
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const uint32_t n = s * C + group;
-            lo[s] = hi[s] = make_uint2(0, 0);
-            if (head < heads && n < NB) {
-                const half_t* p = a.q + b * a.q_stride + (size_t)(hk * G + head0 + head) * D + n * 32 + 4 * g;
-                lo[s] = *reinterpret_cast<const uint2*>(p);
-                hi[s] = *reinterpret_cast<const uint2*>(p + 16);
-            }
             top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(h2f(lo[s].x & 0xFFFFu)), fabsf(h2f(lo[s].x >> 16))), fmaxf(fabsf(h2f(lo[s].y & 0xFFFFu)), fabsf(h2f(lo[s].y >> 16)))),
                                    fmaxf(fmaxf(fabsf(h2f(hi[s].x & 0xFFFFu)), fabsf(h2f(hi[s].x >> 16))), fmaxf(fabsf(h2f(hi[s].y & 0xFFFFu)), fabsf(h2f(hi[s].y >> 16))))));
         }
@@ -796,11 +823,8 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
 
     float minus = -1.f;                        // unknown to the compiler, which would subtract a converted half in two instructions where a mixed multiply-add takes one
     asm("" : "+s"(minus));
-    float m = -INFINITY, room = 15.f;          // room: log2 of the largest weight
+    float room = 15.f;                         // log2 of the largest weight
     uint32_t most = 15u << 10;                  // scales below this, as bits, leave it as it is
-    floatx4 o[2 * NB], z = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int e = 0; e < 2 * NB; ++e) o[e] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
     for (; tile < last; tile += kWaves) {
         const bool more = tile + kWaves < last;
@@ -832,21 +856,19 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
         wave_sync();                     // the tile before has been read
         stage();
         wave_sync();
-        if (more) {
-            load(next);
-        }
-        // ---- scores: row r of product t is token 8 (r / 4) + r % 4 + 4 t, so that lane (r, g) gets tokens 8 g + 4 t + 0 .. 3 of head r
-        float x[8];
-        const char* const key_row = keys + (8 * (r >> 2) + (r & 3u)) * ROW + (r >> 3) * (HALF - 16 * ROW) + 4 * g;
+        if (more) load(next);
+        // ---- scores: x in the lane's order, of its column's blocks; y of its own tokens
+        float x[8], y[V];
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const half8 kd = *reinterpret_cast<const half8*>(k_scales + min((uint32_t)(s * C) + group, NB - 1u) * kTile + 8 * g);
+            const half8 kd = *reinterpret_cast<const half8*>(k_scales + (s * C + group < NB ? s * C + group : 2u * NB) * kTile + 8 * g);   // columns of no block: the ones
             floatx4 p[2] = {{off[s], off[s], off[s], off[s]}, {off[s], off[s], off[s], off[s]}};
 #pragma unroll
             for (int n = s * C; n < s * C + C && n < NB; ++n)
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    const uint32_t w = *reinterpret_cast<const uint32_t*>(key_row + t * 4 * ROW + n * 16);
+                    const int u = (2 * t + n % C % R * PS) & 3;
+                    const uint32_t w = *reinterpret_cast<const uint32_t*>(keys + key_at[R == 4 ? u : u / 2] + n * 16);
                     typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
                     const half8 kf = __builtin_bit_cast(half8, uint4_t{w & 0x000F000Fu, w & 0x00F000F0u, w >> 8 & 0x000F000Fu, w >> 8 & 0x00F000F0u});
                     p[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[n], p[t], 0, 0, 0);
@@ -854,19 +876,29 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = fmaf(p[i / 4][i % 4], (float)kd[i], s == 0 ? 0.f : x[i]);
         }
-        // over the column groups: rotations by 8, 4, 2 within 16 lanes, in this order, so that every lane adds the same pairs
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (C >= 2) x[i] += dpp_f<0x128>(x[i]);
-            if (C >= 4) x[i] += dpp_f<0x124>(x[i]);
-            if (C >= 8) x[i] += dpp_f<0x122>(x[i]);
+        for (int i = 0; i < V; ++i) {
+            // from the group that is j further (lane r from r - N): its place of the same pair
+            auto from = [&](int j) { return x[2 * ((i / 2 - j * PS) & 3) + (i & 1)]; };
+            y[i] = from(0);
+            if (C >= 2) y[i] += dpp_f<0x120 + 16 - GP>(from(1));
+            if (C >= 4) y[i] += dpp_f<0x120 + (32 - 2 * GP) % 16>(from(2));
+            if (C >= 4) y[i] += dpp_f<0x120 + (48 - 3 * GP) % 16>(from(3));
+            if (C >= 8) y[i] += dpp_f<0x120 + (64 - 4 * GP) % 16>(from(4));
+            if (C >= 8) y[i] += dpp_f<0x120 + (80 - 5 * GP) % 16>(from(5));
+            if (C >= 8) y[i] += dpp_f<0x120 + (96 - 6 * GP) % 16>(from(6));
+            if (C >= 8) y[i] += dpp_f<0x120 + (112 - 7 * GP) % 16>(from(7));
         }
         if (!full) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = live(8 * g + i) ? x[i] : -INFINITY;
+            for (int i = 0; i < V; ++i) y[i] = live(8 * g + 2 * ((i / 2 + turn) & 3u) + (i & 1)) ? y[i] : -INFINITY;
         }
         // ---- running maximum, weights (unit is positive)
-        float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        float top = y[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) top = fmaxf(top, y[i]);
+        if (R >= 2) top = fmaxf(top, dpp_f<0x120 + GP % 16>(top));
+        if (R >= 4) top = fmaxf(top, dpp_f<0x120 + 2 * GP % 16>(top));
         top = rows_max(top) * unit;
         top = fmaxf(m, fabsf(top) < kMostShifted ? top - room : top);
         const float ref = top == -INFINITY ? 0.f : top;
@@ -877,30 +909,46 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
             for (int e = 0; e < 2 * NB; ++e) o[e] *= keep;
             m = top;
         }
-        half8 hi, lo;
+        union Weights {
+            half2_t pair[4];
+            uint32_t word[4];
+            half8 all;
+        } hi, lo;
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
+        for (int i = 0; i < PS; ++i) {
             typedef float float2_t __attribute__((ext_vector_type(2)));
-            const float2_t p = {__builtin_amdgcn_exp2f(fmaf(x[i], unit, -ref)), __builtin_amdgcn_exp2f(fmaf(x[i + 1], unit, -ref))};
+            const float2_t p = {__builtin_amdgcn_exp2f(fmaf(y[2 * i], unit, -ref)), __builtin_amdgcn_exp2f(fmaf(y[2 * i + 1], unit, -ref))};
             const half2_t h = __builtin_convertvector(p, half2_t);
-            const half2_t rest = __builtin_convertvector((float2_t{fmaf((float)h[0], minus, p[0]), fmaf((float)h[1], minus, p[1])}), half2_t);
-            hi[i] = h[0]; hi[i + 1] = h[1];
-            lo[i] = rest[0]; lo[i + 1] = rest[1];
+            hi.pair[i] = h;
+            lo.pair[i] = __builtin_convertvector((float2_t{fmaf((float)h[0], minus, p[0]), fmaf((float)h[1], minus, p[1])}), half2_t);
+        }
+#pragma unroll
+        for (int i = 0; i < PS; ++i) {
+            auto turned = [](uint32_t v, auto by) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + decltype(by)::value, 0xF, 0xF, true); };
+            if constexpr (R >= 2) {
+                hi.word[PS + i] = turned(hi.word[i], Int<16 - GP>());
+                lo.word[PS + i] = turned(lo.word[i], Int<16 - GP>());
+            }
+            if constexpr (R >= 4) {
+                hi.word[2 + i] = turned(hi.word[i], Int<16 - 2 * GP>());
+                lo.word[2 + i] = turned(lo.word[i], Int<16 - 2 * GP>());
+                hi.word[3 + i] = turned(hi.word[i], Int<16 - 3 * GP>());
+                lo.word[3 + i] = turned(lo.word[i], Int<16 - 3 * GP>());
+            }
         }
         // ---- sums of weights and of weights times scales
         const half8 sc = *reinterpret_cast<const half8*>(v_scales + min(r, (uint32_t)NB) * kTile + 8 * g);
-        z = __builtin_amdgcn_mfma_f32_16x16x32_f16(sc, hi, z, 0, 0, 0);
-        z = __builtin_amdgcn_mfma_f32_16x16x32_f16(sc, lo, z, 0, 0, 0);
-        // ---- values: bytes 0 1 2 3 of a word of the transposing read are tokens 0 2 1 3 of four, so that an `and` leaves two consecutive ones; lane r of 16 brings 8 bytes of row r / 2
-        const char* const value_row = values + (8 * g + ((r >> 1 & 4u) | (r >> 1 & 1u) << 1 | (r >> 2 & 1u))) * ROW + (g >> 1) * (HALF - 16 * ROW) + (r & 1u) * 8;
+        z = __builtin_amdgcn_mfma_f32_16x16x32_f16(sc, hi.all, z, 0, 0, 0);
+        z = __builtin_amdgcn_mfma_f32_16x16x32_f16(sc, lo.all, z, 0, 0, 0);
+        // ---- values
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const half8 d = *reinterpret_cast<const half8*>(v_scales + min((uint32_t)(s * C) + group, NB - 1u) * kTile + 8 * g);
-            const half8 p = hi * d, rest = __builtin_elementwise_fma(lo, d, __builtin_elementwise_fma(hi, d, -p));
+            const half8 d = *reinterpret_cast<const half8*>(v_scales + min((uint32_t)(s * C) + group, (uint32_t)NB) * kTile + 8 * g);
+            const half8 p = hi.all * d, rest = __builtin_elementwise_fma(lo.all, d, __builtin_elementwise_fma(hi.all, d, -p));
 #pragma unroll
             for (int n = s * C; n < s * C + C && n < NB; ++n) {
                 typedef int int2_t __attribute__((ext_vector_type(2)));
-                const int2_t w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((int2_t __attribute__((address_space(3)))*)(value_row + n * 16));
+                const int2_t w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((int2_t __attribute__((address_space(3)))*)(values + value_at[n % C % R] + n * 16));
                 const half8 v0 = codes_f16((uint32_t)w.x, (uint32_t)w.y, 0x000F000Fu), v1 = codes_f16((uint32_t)w.x, (uint32_t)w.y, 0x00F000F0u);
                 o[2 * n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p, o[2 * n], 0, 0, 0);
                 o[2 * n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p, o[2 * n + 1], 0, 0, 0);
@@ -912,6 +960,7 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
             cur = next;
             if (tile + 2 * kWaves < last) next = locate(tile + 2 * kWaves);
         }
+    }
     }
 
     // ---- the waves' sums: lane (r, g) holds elements 32 n + 16 h + 4 g + 0 .. 3 of its head in o[2 n + h], of the blocks of its column; sum p d of block n is in row n of z, the sum of weights in row NB

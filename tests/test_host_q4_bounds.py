@@ -24,7 +24,7 @@ template <class V> static V shim_tr8(V* p) {
 }
 #define __builtin_amdgcn_ds_read_tr8_b64_v2i32 shim_tr8
 static int shim_dpp_or_rotation(int old, int v, int ctrl, int row_mask, int bank_mask, bool bound) {
-    if (ctrl > 0x120 && ctrl <= 0x12F) return from_lane(v, 3, 16, ((lane_id() & 15) + ctrl - 0x120) & 15);
+    if (ctrl > 0x120 && ctrl <= 0x12F) return from_lane(v, 3, 16, ((lane_id() & 15) - (ctrl - 0x120)) & 15);
     return shim_dpp(old, v, ctrl, row_mask, bank_mask, bound);
 }
 #undef __builtin_amdgcn_update_dpp
