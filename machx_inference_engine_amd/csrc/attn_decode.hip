@@ -602,8 +602,11 @@ struct Plan {
     uint32_t shares;         // 0: a workgroup for each sequence and group of heads
     uint64_t ws_bytes;
 };
+// Q4_0: as many as are resident, four workgroups a CU for heads of up to 64, three up to 128, two beyond, rounded down.  us by workgroups (256, 512, 768, 1024): 64 x 8192 tokens of 8 heads of 64 115, 73, 66, 59, of
+// 128 104, 105, 98, 118; 16 x 8192 of 8 heads of 256 67, 53, 75, 58; 16 x 8192 of 3 heads of 128 21.8, 18.4 (513 of them), 15.8, 20.1.
+enum { kF16 = 0, kQ8 = 1, kQ4 = 2 };   // what a cache holds
 constexpr uint32_t kDirectTiles = 4 * kWaves;
-static Plan plan_of(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t max_len, uint32_t window) {
+static Plan plan_of(int fmt, uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t max_len, uint32_t window) {
     const uint32_t span = window && window < max_len ? window : max_len;
     const uint64_t tiles = window && window < max_len ? span / kTile + 2 : (span + (uint64_t)kTile - 1) / kTile, all = B * tiles;   // a window may begin within a tile
     const uint64_t groups = (uint64_t)Hkv * ((Hq / Hkv + 15) / 16);
@@ -611,7 +614,8 @@ static Plan plan_of(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t 
     auto up = [](uint64_t x, uint64_t y) { return (x + y - 1) / y; };
     uint64_t most = up(all, kLeastShare);
     if (most * groups > 128) most = up(all, 2 * kLeastShare) > up(128, groups) ? up(all, 2 * kLeastShare) : up(128, groups);
-    uint64_t shares = up(D > 128 ? 256 : D > 64 ? 512 : 768, groups);
+    uint64_t shares = fmt == kQ4 ? (D > 128 ? 512 : D > 64 ? 768 : 1024) / groups : up(D > 128 ? 256 : D > 64 ? 512 : 768, groups);
+    if (shares == 0) shares = 1;
     if (shares > most) shares = most;
     return {(uint32_t)shares, (shares + B) * Hq * (D + 2) * 4 + (uint64_t)B * 8};
 }
@@ -653,6 +657,7 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
     constexpr uint32_t ROW = 16 * (NB | 1), HALF = 20 * ROW;
     constexpr uint32_t CODES = HALF + 16 * ROW, KS = kTile * NB * 2, VS = kTile * (NB + 1) * 2, WAVE = 2 * CODES + KS + VS;
     constexpr int S = (NB + C - 1) / C;
+    constexpr bool EARLY = NB <= 4 && C > 1;                    // a tile's values leave LDS before its scores are found, where there are registers for them: 64 x 8192 tokens of 8 heads of 128 98.3 -> 97.0 us
     constexpr uint32_t OS = D + 4;
     constexpr int LP = (NB + 1) / 2, SL = (16 * NB + 63) / 64;  // a lane's 16-byte pieces of a tile's codes, dwords of its scales
     extern __shared__ float lds[];
@@ -857,6 +862,17 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
         stage();
         wave_sync();
         if (more) load(next);
+        typedef int int2_t __attribute__((ext_vector_type(2)));
+        auto codes_of = [&](int n) { return __builtin_amdgcn_ds_read_tr8_b64_v2i32((int2_t __attribute__((address_space(3)))*)(values + value_at[n % C % R] + n * 16)); };
+        auto scales_of = [&](int s) { return *reinterpret_cast<const half8*>(v_scales + min((uint32_t)(s * C) + group, (uint32_t)NB) * kTile + 8 * g); };
+        int2_t vw[NB];                   // the values' codes, and their scales by set
+        half8 vd[S];
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n) vw[n] = codes_of(n);
+#pragma unroll
+            for (int s = 0; s < S; ++s) vd[s] = scales_of(s);
+        }
         // ---- scores: x in the lane's order, of its column's blocks; y of its own tokens
         float x[8], y[V];
 #pragma unroll
@@ -943,12 +959,11 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
         // ---- values
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const half8 d = *reinterpret_cast<const half8*>(v_scales + min((uint32_t)(s * C) + group, (uint32_t)NB) * kTile + 8 * g);
+            const half8 d = EARLY ? vd[s] : scales_of(s);
             const half8 p = hi.all * d, rest = __builtin_elementwise_fma(lo.all, d, __builtin_elementwise_fma(hi.all, d, -p));
 #pragma unroll
             for (int n = s * C; n < s * C + C && n < NB; ++n) {
-                typedef int int2_t __attribute__((ext_vector_type(2)));
-                const int2_t w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((int2_t __attribute__((address_space(3)))*)(values + value_at[n % C % R] + n * 16));
+                const int2_t w = EARLY ? vw[n] : codes_of(n);
                 const half8 v0 = codes_f16((uint32_t)w.x, (uint32_t)w.y, 0x000F000Fu), v1 = codes_f16((uint32_t)w.x, (uint32_t)w.y, 0x00F000F0u);
                 o[2 * n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p, o[2 * n], 0, 0, 0);
                 o[2 * n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p, o[2 * n + 1], 0, 0, 0);
@@ -1019,8 +1034,6 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
 }
 
 // ---------------------------------------------------------------- launches
-enum { kF16 = 0, kQ8 = 1, kQ4 = 2 };   // what a cache holds
-
 template <int NB, int C>
 static int launch_q4(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads) {
     static LdsLimit limit;
@@ -1094,7 +1107,7 @@ static int attn_decode(mx_stream_t s, int fmt, const uint16_t* q, uint64_t q_str
     MX_REQUIRE_ALIGN(q, 16); MX_REQUIRE_ALIGN(k, 16); MX_REQUIRE_ALIGN(v, 16); MX_REQUIRE_ALIGN(out, 16); MX_REQUIRE_ALIGN(out_q8, 8);
     MX_REQUIRE_ALIGN(page_table, 4); MX_REQUIRE_ALIGN(seq_lens, 4); MX_REQUIRE_ALIGN(sinks, 4);
     if (fmt != kF16) { MX_REQUIRE_ALIGN(k_d, 16); MX_REQUIRE_ALIGN(v_d, 16); }
-    const Plan p = plan_of(B, Hq, Hkv, D, max_len, window);
+    const Plan p = plan_of(fmt, B, Hq, Hkv, D, max_len, window);
     if (p.shares) {
         MX_REQUIRE_PTR(ws);
         MX_REQUIRE_ALIGN(ws, 16);
@@ -1141,7 +1154,8 @@ extern "C" {
 int mx_attn_decode_ws_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t max_len, uint32_t window, uint64_t* bytes) {
     MX_REQUIRE_PTR(bytes);
     MX_REQUIRE_SHAPE(B > 0 && B <= 65535 && Hkv > 0 && Hq > 0 && Hq <= 65535 && Hq % Hkv == 0 && D > 0 && D <= 256 && D % 16 == 0);
-    *bytes = plan_of(B, Hq, Hkv, D, max_len, window).ws_bytes;
+    const uint64_t wide = plan_of(kF16, B, Hq, Hkv, D, max_len, window).ws_bytes, narrow = D % 32 == 0 ? plan_of(kQ4, B, Hq, Hkv, D, max_len, window).ws_bytes : 0;
+    *bytes = wide > narrow ? wide : narrow;      // for a cache of any format
     return MX_OK;
 }
 
