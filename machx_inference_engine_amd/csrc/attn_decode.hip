@@ -1154,8 +1154,13 @@ extern "C" {
 int mx_attn_decode_ws_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t max_len, uint32_t window, uint64_t* bytes) {
     MX_REQUIRE_PTR(bytes);
     MX_REQUIRE_SHAPE(B > 0 && B <= 65535 && Hkv > 0 && Hq > 0 && Hq <= 65535 && Hq % Hkv == 0 && D > 0 && D <= 256 && D % 16 == 0);
-    const uint64_t wide = plan_of(kF16, B, Hq, Hkv, D, max_len, window).ws_bytes, narrow = D % 32 == 0 ? plan_of(kQ4, B, Hq, Hkv, D, max_len, window).ws_bytes : 0;
-    *bytes = wide > narrow ? wide : narrow;      // for a cache of any format
+    *bytes = plan_of(kF16, B, Hq, Hkv, D, max_len, window).ws_bytes;
+    return MX_OK;
+}
+int mx_attn_decode_q4_0_ws_bytes(uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t max_len, uint32_t window, uint64_t* bytes) {
+    MX_REQUIRE_PTR(bytes);
+    MX_REQUIRE_SHAPE(B > 0 && B <= 65535 && Hkv > 0 && Hq > 0 && Hq <= 65535 && Hq % Hkv == 0 && D > 0 && D <= 256 && D % 32 == 0);
+    *bytes = plan_of(kQ4, B, Hq, Hkv, D, max_len, window).ws_bytes;
     return MX_OK;
 }
 

@@ -996,9 +996,11 @@ def kv_read(cache, page_table, rows, total_rows, out=None):
 
 
 @functools.lru_cache(maxsize=1024)
-def attn_decode_ws_bytes(B, Hq, Hkv, D, max_len, window=0):
+def attn_decode_ws_bytes(B, Hq, Hkv, D, max_len, window=0, fmt="f16"):
+    """fmt: the cache's format, as kv_cache has it."""
     n = ctypes.c_uint64()
-    rc = lib.mx_attn_decode_ws_bytes(B, Hq, Hkv, D, max_len, window, ctypes.addressof(n))
+    query = lib.mx_attn_decode_q4_0_ws_bytes if fmt == "q4_0" else lib.mx_attn_decode_ws_bytes
+    rc = query(B, Hq, Hkv, D, max_len, window, ctypes.addressof(n))
     if rc != 0:
         raise MxError("mx_attn_decode_ws_bytes", rc)
     return n.value
@@ -1020,7 +1022,7 @@ def attn_decode(q, cache, page_table, seq_lens, scale=None, window=0, sinks=None
         raise ValueError("q, out, page_table and seq_lens have one row for each sequence, q the cache's D")
     ws_ptr, ws_size = None, 0
     if ws is None:
-        ws_size = attn_decode_ws_bytes(B, Hq, Hkv, D, max_len, window)
+        ws_size = attn_decode_ws_bytes(B, Hq, Hkv, D, max_len, window, fmt)
         if ws_size:
             ws = torch.empty(ws_size, dtype=torch.uint8, device=q.device)
             ws_ptr = ws.data_ptr()

@@ -384,7 +384,7 @@ def test_streams_and_captured_graphs(mx):
     lens = [3000, 700, 1, 1200]
     rng, table, cache, q = case(lens, 2, 8, 128, 16, 71)
     tab, n, f = dev(table), dev(np.array(lens, np.int32)), dev(U.freqs(128))
-    size = mx.ops.attn_decode_ws_bytes(4, 16, 2, 128, 3000)
+    size = mx.ops.attn_decode_ws_bytes(4, 16, 2, 128, 3000, fmt="q4_0")
     assert size > 0
     qs = [dev(rows(rng, 4, 16, 128)) for _ in range(2)]
     want = [mx.ops.attn_decode(t, cache, tab, n, max_len=3000) for t in qs]

@@ -41,6 +41,14 @@ def test_attention_refusals(lib):  # noqa: F811
     for bad in (dict(q=P8), dict(out=P8), dict(out_q8=0x1004), dict(page_table=P2), dict(seq_lens=P2), dict(sinks=P2), dict(k_qs=P8), dict(k_d=P8)):
         assert c.with_(**bad) == ALIGN, bad
     assert c.with_(max_len=100000, ws_bytes=100) == WORKSPACE
+    import ctypes
+    n, query = ctypes.c_uint64(), lib[0].mx_attn_decode_q4_0_ws_bytes
+    assert query(2, 32, 8, 128, 512, 0, ctypes.addressof(n)) == 0 and n.value == 0
+    assert query(2, 32, 8, 128, 100000, 0, ctypes.addressof(n)) == 0 and n.value > 0
+    assert c.with_(max_len=100000, ws_bytes=n.value - 1) == WORKSPACE
+    assert query(2, 32, 8, 128, 100000, 0, None) == NULL
+    for bad in ((0, 32, 8, 128), (65536, 32, 8, 128), (2, 33, 8, 128), (2, 32, 0, 128), (2, 32, 8, 48), (2, 32, 8, 288)):
+        assert query(*bad, 1000, 0, ctypes.addressof(n)) == SHAPE, bad
     assert c.with_(max_len=100000, ws=None) == NULL
 
 
