@@ -272,16 +272,19 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const void* k_cache, const
     const uint32_t count = min(16u, end - row0 - t0), col = t0 / page_size, D = chunks * 8;
     const uint32_t page = col < max_pages ? (uint32_t)page_table[(size_t)b * max_pages + col] : 0xFFFFFFFFu;
     const bool good = page < n_pages;
-    const uint32_t per_head = 16 * chunks, items = 2 * Hkv * per_head, i0 = blockIdx.y * (256 * kReadPieces) + threadIdx.x;
+    const uint32_t items = 2 * Hkv * 16 * chunks, i0 = blockIdx.y * (256 * kReadPieces) + threadIdx.x;
     constexpr int U = kReadPieces;
+    // piece i is chunk i % chunks of token (i / chunks) % 16 of head i / chunks / 16; 256 pieces on are `tokens` tokens and `more` chunks on
+    uint32_t q = i0 / chunks, c = i0 - q * chunks;
+    const uint32_t tokens = 256 / chunks, more = 256 - tokens * chunks;
     uint4 got[U];
     half_t d[U];
     uint32_t at[U];                      // token * heads * chunks + head * chunks + chunk, from the tile's first row
     bool is_v[U], live[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const uint32_t i = i0 + 256 * u, hh = i / per_head, r = i - hh * per_head, tok = r / chunks, c = r - tok * chunks;
-        live[u] = i < items && tok < count;
+        const uint32_t hh = q >> 4, tok = q & 15u;
+        live[u] = i0 + 256 * u < items && tok < count;
         is_v[u] = hh >= Hkv;
         const uint32_t h = is_v[u] ? hh - Hkv : hh;
         at[u] = (tok * Hkv + h) * chunks + c;
@@ -300,6 +303,12 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const void* k_cache, const
                 got[u].y = FMT == kQ4 ? w.y >> (c & 2) * 2 : w.y;
                 d[u] = (is_v[u] ? v_d : k_d)[crow * (D / 32) + c / 4];
             }
+        }
+        q += tokens;
+        c += more;
+        if (c >= chunks) {
+            c -= chunks;
+            ++q;
         }
     }
 #pragma unroll

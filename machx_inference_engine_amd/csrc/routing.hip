@@ -243,10 +243,32 @@ __device__ __forceinline__ uint64_t order_of(double v) {
 __device__ __forceinline__ double number_of(uint64_t k) {
     return k == 1ull ? __builtin_nan("") : __builtin_bit_cast(double, k >> 63 ? k & ~(1ull << 63) : ~k);
 }
+template <int CTRL, int ROW_MASK = 0xF, bool BOUND = true>
+__device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROW_MASK, 0xF, BOUND), hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROW_MASK, 0xF, BOUND);
+    return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
 __device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
-    return v;
+    auto step = [&](uint64_t o) { v += __builtin_bit_cast(double, o); };
+    step(dpp_u64<0xB1>(__builtin_bit_cast(uint64_t, v)));
+    step(dpp_u64<0x4E>(__builtin_bit_cast(uint64_t, v)));
+    step(dpp_u64<0x141>(__builtin_bit_cast(uint64_t, v)));
+    step(dpp_u64<0x140>(__builtin_bit_cast(uint64_t, v)));
+    step(dpp_u64<0x142, 0xA, false>(__builtin_bit_cast(uint64_t, v)));
+    step(dpp_u64<0x143, 0xC, false>(__builtin_bit_cast(uint64_t, v)));
+    return __builtin_bit_cast(double, lane_u64(__builtin_bit_cast(uint64_t, v), 63));
+}
+__device__ __forceinline__ float wave_max_dpp(float v) {
+    v = fmaxf(v, dpp_f<0xB1>(v));
+    v = fmaxf(v, dpp_f<0x4E>(v));
+    v = fmaxf(v, dpp_f<0x141>(v));
+    v = fmaxf(v, dpp_f<0x140>(v));
+    v = fmaxf(v, u2f((uint32_t)__builtin_amdgcn_update_dpp((int)f2u(-INFINITY), (int)f2u(v), 0x142, 0xA, 0xF, false)));
+    v = fmaxf(v, u2f((uint32_t)__builtin_amdgcn_update_dpp((int)f2u(-INFINITY), (int)f2u(v), 0x143, 0xC, 0xF, false)));
+    return u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(v), 63));
 }
 
 struct RouteArgs {
@@ -256,29 +278,58 @@ struct RouteArgs {
     half_t* topk_w;
     uint32_t n_tokens, E, K, n_groups, size, size_inv, kept, lanes, flags;   // size: experts of a group, size_inv = ceil(2^32 / size); lanes: of a wave for each group
     float scale;
+    bool wide;               // a lane's logits are loaded at once
 };
 
-// One wave a token, lane l holds experts l, l + 64, .. (NJ of them): scores in 64 bits and, as integers of the same order, what they are chosen by.
+// The two largest of two pairs (first >= second).
+__device__ __forceinline__ void merge_two(uint64_t& first, uint64_t& second, uint64_t f, uint64_t s) {
+    const uint64_t low = f < first ? f : first, more = s > second ? s : second;
+    first = f > first ? f : first;
+    second = low > more ? low : more;
+}
+
+// One wave a token, lane l holds experts NJ l .. NJ l + NJ - 1: scores in 64 bits and, as integers of the same order, what they are chosen by.  K rounds of a wave-wide maximum, of the upper halves
+// first and of the lower ones where these are equal; the lowest lane of equal keys has the lowest id.  Bound by the vector instructions and, for few tokens, by their latency one after the other.
 template <int NJ>
 __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
     __shared__ uint64_t choice[4][NJ * 64];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, t = blockIdx.x * 4u + wave;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, t = blockIdx.x * 4u + wave, e0 = lane * NJ;
     if (t >= a.n_tokens) return;          // no barriers: a wave's LDS is its own
     float x[NJ];
-    float m = -INFINITY;
+    const size_t row = (size_t)t * a.E + e0;
+    typedef float floats __attribute__((ext_vector_type(NJ)));
+    typedef _Float16 halves __attribute__((ext_vector_type(NJ)));
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-        const uint32_t e = lane + 64u * j;
-        const size_t at = (size_t)t * a.E + e;
-        x[j] = e >= a.E ? -INFINITY : a.flags & MX_ROUTE_F32 ? static_cast<const float*>(a.logits)[at] : (float)static_cast<const half_t*>(a.logits)[at];
-        m = fmaxf(m, x[j]);
+    for (int j = 0; j < NJ; ++j) x[j] = -INFINITY;
+    if (a.wide) {            // E is a multiple of NJ
+        if (e0 < a.E) {
+            if (a.flags & MX_ROUTE_F32) {
+                const floats v = *reinterpret_cast<const floats*>(static_cast<const float*>(a.logits) + row);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) x[j] = v[j];
+            } else {
+                const halves v = *reinterpret_cast<const halves*>(static_cast<const half_t*>(a.logits) + row);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) x[j] = (float)v[j];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+            if (e0 + j < a.E) x[j] = a.flags & MX_ROUTE_F32 ? static_cast<const float*>(a.logits)[row + j] : (float)static_cast<const half_t*>(a.logits)[row + j];
     }
+    float add[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) add[j] = a.bias && e0 + j < a.E ? a.bias[e0 + j] : 0.f;
     double score[NJ];
     if (a.flags & MX_ROUTE_SIGMOID) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) score[j] = 1.0 / (1.0 + exp(-(double)x[j]));
     } else {
-        m = wave_max_f(m);
+        float m = x[0];
+#pragma unroll
+        for (int j = 1; j < NJ; ++j) m = fmaxf(m, x[j]);
+        m = wave_max_dpp(m);
         double sum = 0.0;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
@@ -286,89 +337,99 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
             sum += score[j];
         }
         sum = wave_sum_f64(sum);
+        const double inv = sum == 0.0 ? 0.0 : 1.0 / sum;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) score[j] = sum == 0.0 ? 0.0 : score[j] / sum;
+        for (int j = 0; j < NJ; ++j) score[j] *= inv;
     }
     uint64_t key[NJ];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-        const uint32_t e = lane + 64u * j;
-        key[j] = e < a.E ? order_of(a.bias ? score[j] + (double)a.bias[e] : score[j]) : 0ull;
-    }
+    for (int j = 0; j < NJ; ++j) key[j] = e0 + j < a.E ? order_of(a.bias ? score[j] + (double)add[j] : score[j]) : 0ull;
     if (a.n_groups > 1) {
-        // a group's two largest, by `lanes` lanes each, from LDS
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) choice[wave][lane + 64u * j] = key[j];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         uint64_t first = 0, second = 0;
-        const uint32_t group = lane / a.lanes;
-        if (group < a.n_groups)
-            for (uint32_t i = lane - group * a.lanes; i < a.size; i += a.lanes) {
-                const uint64_t k = choice[wave][group * a.size + i];
-                second = k > first ? first : k > second ? k : second;
-                first = k > first ? k : first;
-            }
-        for (uint32_t d = 1; d < a.lanes; d <<= 1) {
-            const uint64_t f = __shfl_xor(first, d), s = __shfl_xor(second, d);
-            const uint64_t low = f < first ? f : first, more = s > second ? s : second;
-            first = f > first ? f : first;
-            second = low > more ? low : more;
+        const bool whole = a.size % NJ == 0 && (a.size / NJ & (a.size / NJ - 1)) == 0;    // groups of whole lanes, a power of two of them
+        if (whole) {
+            const uint32_t of = a.size / NJ;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) merge_two(first, second, key[j], 0ull);
+            // equal within 2, 4, 8 lanes, a mirror brings the other half of twice as many
+            if (of > 1) merge_two(first, second, dpp_u64<0xB1>(first), dpp_u64<0xB1>(second));
+            if (of > 2) merge_two(first, second, dpp_u64<0x4E>(first), dpp_u64<0x4E>(second));
+            if (of > 4) merge_two(first, second, dpp_u64<0x141>(first), dpp_u64<0x141>(second));
+            if (of > 8) merge_two(first, second, dpp_u64<0x140>(first), dpp_u64<0x140>(second));
+            if (of > 16) merge_two(first, second, __shfl_xor(first, 16), __shfl_xor(second, 16));
+        } else {
+            // by `lanes` lanes each, from LDS
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) choice[wave][e0 + j] = key[j];
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            const uint32_t group = lane / a.lanes;
+            if (group < a.n_groups)
+                for (uint32_t i = lane - group * a.lanes; i < a.size; i += a.lanes) merge_two(first, second, choice[wave][group * a.size + i], 0ull);
+            for (uint32_t d = 1; d < a.lanes; d <<= 1) merge_two(first, second, __shfl_xor(first, d), __shfl_xor(second, d));
         }
-        const uint64_t own = a.flags & MX_ROUTE_TOP2 && a.size > 1 ? order_of(number_of(first) + number_of(second)) : first;
-        const uint64_t worth = __shfl(own, lane * a.lanes & 63u);        // lane g: of group g
+        const uint32_t of = whole ? a.size / NJ : a.lanes, own = lane / of;               // lanes of a group
+        const uint64_t worth = a.flags & MX_ROUTE_TOP2 && a.size > 1 ? order_of(number_of(first) + number_of(second)) : first;
         uint32_t better = 0;
         for (uint32_t g = 0; g < a.n_groups; ++g) {
-            const uint64_t other = __shfl(worth, g);
-            better += other > worth || (other == worth && g < lane) ? 1u : 0u;
+            const uint64_t other = lane_u64(worth, (int)(g * of));
+            better += other > worth || (other == worth && g < own) ? 1u : 0u;
         }
-        const uint64_t kept = __ballot(lane < a.n_groups && better < a.kept);
+        const bool in = own < a.n_groups && better < a.kept;
+        if (whole) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const uint32_t g = a.size == 1u ? lane + 64u * j : __umulhi(lane + 64u * j, a.size_inv);
-            if (!(kept >> (g & 63u) & 1ull)) key[j] = 0ull;
+            for (int j = 0; j < NJ; ++j) key[j] = in ? key[j] : 0ull;
+        } else {
+            const uint64_t kept = __ballot(in && lane % of == 0);                          // bit g * of
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const uint32_t g = a.size == 1u ? e0 + j : __umulhi(e0 + j, a.size_inv);
+                if (!(kept >> (g * of & 63u) & 1ull)) key[j] = 0ull;
+            }
         }
     }
-    // K rounds of the largest key, the lowest id among equal ones
-    unsigned long long taken[NJ];
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) taken[j] = 0ull;
+    uint32_t taken = 0;      // bit j
     for (uint32_t kk = 0; kk < a.K; ++kk) {
         uint64_t best = key[0];
 #pragma unroll
         for (int j = 1; j < NJ; ++j) best = key[j] > best ? key[j] : best;
-        const uint32_t high = wave_max_u32((uint32_t)(best >> 32)), low = wave_max_u32((uint32_t)(best >> 32) == high ? (uint32_t)best : 0u);
-        const uint64_t win = (uint64_t)high << 32 | low;
-        bool open = true;
+        const uint32_t high = wave_max_u32((uint32_t)(best >> 32));
+        bool top = (uint32_t)(best >> 32) == high;
+        uint64_t hit = __ballot(top);
+        if (hit & (hit - 1)) {
+            const uint32_t low = wave_max_u32(top ? (uint32_t)best : 0u);
+            hit = __ballot(top && (uint32_t)best == low);
+        }
+        bool open = lane == (uint32_t)__ffsll((unsigned long long)hit) - 1u;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const unsigned long long hit = open ? __ballot(key[j] == win) : 0ull;
-            if (hit) {
-                const uint32_t l = (uint32_t)__ffsll(hit) - 1u;
-                taken[j] |= 1ull << l;
-                if (lane == l) key[j] = 0ull;
-                open = false;
-            }
+            const bool it = open && key[j] == best;
+            key[j] = it ? 0ull : key[j];
+            taken |= it ? 1u << j : 0u;
+            open = open && !it;
         }
     }
     double factor = (double)a.scale;
     if (a.flags & MX_ROUTE_RENORM) {
         double sum = 0.0;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) sum += (taken[j] >> lane) & 1ull ? score[j] : 0.0;
+        for (int j = 0; j < NJ; ++j) sum += taken >> j & 1u ? score[j] : 0.0;
         factor /= wave_sum_f64(sum) + 1e-20;
     }
-    uint32_t below = 0;
+    uint32_t at = 0;         // chosen experts of lower lanes
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-        if ((taken[j] >> lane) & 1ull) {
-            const size_t at = (size_t)t * a.K + below + (uint32_t)__builtin_popcountll(taken[j] & ((1ull << lane) - 1ull));
-            a.topk_idx[at] = (int32_t)(lane + 64u * j);
-            a.topk_w[at] = (half_t)(score[j] * factor);
-        }
-        below += (uint32_t)__builtin_popcountll(taken[j]);
+        const uint64_t m = __ballot(taken >> j & 1u);
+        at += (uint32_t)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
     }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+        if (taken >> j & 1u) {
+            a.topk_idx[(size_t)t * a.K + at] = (int32_t)(e0 + j);
+            a.topk_w[(size_t)t * a.K + at] = (half_t)(score[j] * factor);
+            ++at;
+        }
 }
 
 // ---------------------------------------------------------------- packing
@@ -527,8 +588,10 @@ int mx_moe_route(mx_stream_t s, const void* logits, const float* bias, int32_t* 
     const uint32_t size = n_experts / n_groups;
     MX_REQUIRE_SHAPE(topk_groups > 0 && topk_groups <= n_groups && k > 0 && k <= (uint32_t)kMaxTopK && k <= topk_groups * size && flags < 16u);
     MX_REQUIRE_ALIGN(logits, flags & MX_ROUTE_F32 ? 4 : 2); MX_REQUIRE_ALIGN(bias, 4); MX_REQUIRE_ALIGN(topk_idx, 4); MX_REQUIRE_ALIGN(topk_w, 2);
-    RouteArgs a = {logits, bias, topk_idx, reinterpret_cast<half_t*>(topk_w), n_tokens, n_experts, k, n_groups, size, size > 1 ? 0xFFFFFFFFu / size + 1u : 0u, topk_groups, 1, flags, scale};
+    RouteArgs a = {logits, bias, topk_idx, reinterpret_cast<half_t*>(topk_w), n_tokens, n_experts, k, n_groups, size, size > 1 ? 0xFFFFFFFFu / size + 1u : 0u, topk_groups, 1, flags, scale, false};
     while (a.lanes * 2 * n_groups <= 64) a.lanes *= 2;
+    const uint32_t per_lane = n_experts <= 64 ? 1 : n_experts <= 128 ? 2 : n_experts <= 256 ? 4 : n_experts <= 512 ? 8 : 16;
+    a.wide = n_experts % per_lane == 0 && aligned(logits, per_lane * (flags & MX_ROUTE_F32 ? 4 : 2));
     const dim3 grid((n_tokens + 3) / 4), block(256);
     hipStream_t st = as_stream(s);
     if (n_experts <= 64) hipLaunchKernelGGL((route_kernel<1>), grid, block, 0, st, a);

@@ -8,6 +8,8 @@ MORE = r"""
 #include <cmath>
 template <class T> static T __shfl(T v, int l) { return from_lane(v, 9, 64, l & 63); }
 template <class T> static T __shfl_xor(T v, int m) { return from_lane(v, 9, 64, lane_id() ^ m); }
+#define __builtin_amdgcn_mbcnt_lo(m, c) ((uint32_t)__builtin_popcount((m) & (lane_id() < 32 ? (1u << lane_id()) - 1u : 0xFFFFFFFFu)) + (c))
+#define __builtin_amdgcn_mbcnt_hi(m, c) ((uint32_t)__builtin_popcount((m) & (lane_id() < 32 ? 0u : (1u << (lane_id() - 32)) - 1u)) + (c))
 static uint32_t __umulhi(uint32_t a, uint32_t b) { return (uint32_t)((uint64_t)a * b >> 32); }
 // sixteen lanes bring the halves of eight rows of 16 bytes; lane r gets byte r of each
 template <class V> static V shim_tr8(V* p) {
@@ -327,7 +329,7 @@ template <int NJ> static void route(uint32_t T, uint32_t E, uint32_t K, uint32_t
     }
     for (uint32_t e = 0; e < E; ++e) bias.as<float>()[e] = plant == 1 ? 0.f : real() * 0.1f;
     const uint32_t size = E / groups;
-    RouteArgs a = {logits.p, with_bias ? bias.as<float>() : nullptr, idx.as<int32_t>(), w.as<half_t>(), T, E, K, groups, size, size > 1 ? 0xFFFFFFFFu / size + 1u : 0u, kept, 1, flags, 2.5f};
+    RouteArgs a = {logits.p, with_bias ? bias.as<float>() : nullptr, idx.as<int32_t>(), w.as<half_t>(), T, E, K, groups, size, size > 1 ? 0xFFFFFFFFu / size + 1u : 0u, kept, 1, flags, 2.5f, E % NJ == 0};
     while (a.lanes * 2 * groups <= 64) a.lanes *= 2;
     memset(idx.p, 0xFF, idx.n);
     run(256, (T + 3) / 4, 1, 0, [&] { route_kernel<NJ>(a); });
