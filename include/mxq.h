@@ -685,7 +685,7 @@ int mx_gated_rms_norm_q8(mx_stream_t s, const float* x, const uint16_t* z, const
  *   sum = half(x + residual); y of the rounded sum, the bits of mx_rms_norm_f32w_q8's; q8_out the block_q8_1x stream of y, the bits of
  *   mx_quantize_q8_1(y) (halves = 0), or the block_q8_1s stream, those of mx_quantize_q8_1s(y) (halves != 0), as the int-dot products of a prompt take it.
  *   sum may be residual or x (in place, the whole matrix), y may be NULL when only the stream is wanted; outputs overlap nothing else.  All 16-byte
- *   aligned (q8_out without halves 8); hidden % 32 == 0, n_rows < 2^25.  A row that holds a NaN or an infinity gives NaN where the norm does, and stream blocks of it that mean nothing.  */
+ *   aligned (q8_out without halves 8); hidden % 32 == 0, n_rows * min(8, ceil(hidden / 1024)) < 2^25.  A row that holds a NaN or an infinity gives NaN where the norm does, and stream blocks of it that mean nothing.  */
 int mx_add_rms_norm_f32w_q8(mx_stream_t s, const uint16_t* x, const uint16_t* residual, const float* w, uint16_t* sum, uint16_t* y, void* q8_out, uint32_t n_rows,
                             uint32_t hidden, float eps, int halves);
 /* Gated activations with the same fused emitter (no counterpart in the reference, which runs swiglu /

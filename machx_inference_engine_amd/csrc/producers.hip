@@ -68,84 +68,115 @@ __global__ __launch_bounds__(kNormThreads) void norm_q8_kernel(const XT* x, cons
     }
 }
 
-// The residual's addition, the norm of the rounded sum and the 8-bit stream of the rounded norm.  A workgroup takes a row, thread u of pass p elements 8 (128 p + u) .. + 7, which are what threads
-// 2 u and 2 u + 1 of norm_q8_kernel<false> own: their squares are summed apart and in that kernel's order, so that rows normalised here have the bits of those normalised there.
-// P passes keep the row in registers between the sum and the norm (P = 0: rows that are longer read the sum back).
-// Bound by memory: 8 bytes and the stream's 1.25 or 1.5 an element.
-constexpr int kSumThreads = 128;
-template <int P, bool HALVES>
-__global__ __launch_bounds__(kSumThreads) void add_norm_q8_kernel(const half_t* x, const half_t* residual, const float* w, half_t* total, half_t* y, uint8_t* q8, uint32_t hidden, float eps) {
-    typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+// The residual's addition, the norm of the rounded sum and the 8-bit stream of the rounded norm.  A thread owns 8 consecutive elements, those of threads 2 u and 2 u + 1 of norm_q8_kernel<false>: their
+// squares are summed apart and in that kernel's order, so that rows normalised here have the bits of those normalised there.
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+struct SumArgs {
+    const half_t *x, *residual;
+    const float* w;
+    half_t *total, *y;
+    uint8_t* q8;
+    uint32_t n_rows, hidden;
+    float eps;
+};
+__device__ __forceinline__ half8 added(const SumArgs& a, size_t at) {
+    const half8 x = *reinterpret_cast<const half8*>(a.x + at), r = *reinterpret_cast<const half8*>(a.residual + at);
+    half8 v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = f32_to_f16_rne((float)x[j] + (float)r[j]);
+    *reinterpret_cast<half8*>(a.total + at) = v;
+    return v;
+}
+__device__ __forceinline__ void square(const half8& v, float& even, float& odd) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        even = fmaf((float)v[j], (float)v[j], even);
+        odd = fmaf((float)v[j + 4], (float)v[j + 4], odd);
+    }
+}
+struct Weights {
+    float4 lo, hi;
+};
+__device__ __forceinline__ Weights weights_at(const SumArgs& a, uint32_t i) { return {*reinterpret_cast<const float4*>(a.w + i), *reinterpret_cast<const float4*>(a.w + i + 4)}; }
+// All threads call (four share a block of 32); those that are not live store nothing.
+template <bool HALVES>
+__device__ __forceinline__ void normed(const SumArgs& a, size_t at, const half8& v, const Weights& w, float r, bool live) {
+    const float ww[8] = {w.lo.x, w.lo.y, w.lo.z, w.lo.w, w.hi.x, w.hi.y, w.hi.z, w.hi.w};
+    float f[8];
+    half8 o = {};
+    if (live) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = (half_t)(((float)v[j] * r) * ww[j]);
+        // the stream goes by what is stored: without this the compiler may round a product twice over, to fp16 at once for the one and by way of fp32 for the other
+        typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
+        uint4_t bits = __builtin_bit_cast(uint4_t, o);
+        asm("" : "+v"(bits));
+        o = __builtin_bit_cast(half8, bits);
+        if (a.y) *reinterpret_cast<half8*>(a.y + at) = o;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (float)o[j];
+    emit_q8_wide<HALVES>(f, threadIdx.x & 3u, live, a.q8 + at / 32 * (HALVES ? kQ81sBytes : kQ81xBytes));
+}
+
+// A workgroup takes a row, 128 threads each 1024 elements of it (a pass), up to eight passes at once; they meet in LDS (FAR, for rows beyond it: in the sum that they wrote), where 128 threads sum
+// the squares in the order above, lane by lane of half as many as block_sum has.
+// Bound by memory, 8 bytes and the stream's 1.25 or 1.5 an element: 8192 x 4096 51.6 us, 6.0 TB/s; one row of 4096 2.5 us.  With 128 threads for the whole row, which keep it in registers: 61.9 and
+// 3.6; 2048 x 16384 68 for 56, 333 x 2880 5.6 for 4.8.
+constexpr uint32_t kSumThreads = 128, kSumPasses = 8, kSumLds = 32768;      // elements that LDS holds
+template <bool HALVES, bool FAR>
+__global__ __launch_bounds__(kSumThreads * kSumPasses) void add_norm_kernel(SumArgs a) {
+    extern __shared__ char sums[];
     __shared__ float red[kSumThreads / 32];
-    const uint32_t tid = threadIdx.x;
-    const size_t row = (size_t)blockIdx.x * hidden;
-    const uint32_t passes = (hidden + kSumThreads * 8 - 1) / (kSumThreads * 8);
-    half8 h[P ? P : 1];
-    float even = 0.f, odd = 0.f;
-    auto add = [&](uint32_t p) {
-        half8 v = {};
-        const uint32_t i = (p * kSumThreads + tid) * 8;
-        if (i < hidden) {
-            const half8 a = *reinterpret_cast<const half8*>(x + row + i), b = *reinterpret_cast<const half8*>(residual + row + i);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = f32_to_f16_rne((float)a[j] + (float)b[j]);
-            *reinterpret_cast<half8*>(total + row + i) = v;
-        }
-        return v;
-    };
-    auto square = [&](const half8& v) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            even = fmaf((float)v[j], (float)v[j], even);
-            odd = fmaf((float)v[j + 4], (float)v[j + 4], odd);
-        }
-    };
-    if constexpr (P > 0) {
-#pragma unroll
-        for (int p = 0; p < P; ++p) h[p] = add(p);
-#pragma unroll
-        for (int p = 0; p < P; ++p) square(h[p]);
-    } else {
-        for (uint32_t p = 0; p < passes; ++p) square(add(p));
+    const uint32_t tid = threadIdx.x, threads = blockDim.x, last = (a.hidden + kSumThreads * 8 - 1) / (kSumThreads * 8) * kSumThreads;
+    const size_t row = (size_t)blockIdx.x * a.hidden;
+    half8* const rows = reinterpret_cast<half8*>(sums);      // [passes][128]
+    auto sum_at = [&](uint32_t i) { return !FAR ? rows[i] : i * 8 < a.hidden ? *reinterpret_cast<const half8*>(a.total + row + i * 8) : half8{}; };
+    Weights w;
+    if (tid * 8 < a.hidden) w = weights_at(a, tid * 8);
+    for (uint32_t i = tid; i < last; i += threads) {
+        const half8 v = i * 8 < a.hidden ? added(a, row + i * 8) : half8{};
+        if (!FAR) rows[i] = v;
     }
-    // what block_sum adds, lane by lane of twice as many
-    const float part = group_sum<32>(even + odd);
-    if ((tid & 31u) == 31) red[tid >> 5] = part;
     __syncthreads();
-    float sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < kSumThreads / 32; ++k) sum += red[k];
-    const float r = rsqrtf(sum / (float)hidden + eps);
-    auto norm = [&](uint32_t p, const half8& v) {
-        const uint32_t i = (p * kSumThreads + tid) * 8;
-        const bool live = i < hidden;
-        float f[8];
-        half8 o = {};
-        if (live) {
-            const float4 w0 = *reinterpret_cast<const float4*>(w + i), w1 = *reinterpret_cast<const float4*>(w + i + 4);
-            const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] = (half_t)(((float)v[j] * r) * ww[j]);
-            // the stream goes by what is stored: without this the compiler may round a product twice over, to fp16 at once for the one and by way of fp32 for the other
-            typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
-            uint4_t bits = __builtin_bit_cast(uint4_t, o);
-            asm("" : "+v"(bits));
-            o = __builtin_bit_cast(half8, bits);
-            if (y) *reinterpret_cast<half8*>(y + row + i) = o;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = (float)o[j];
-        emit_q8_wide<HALVES>(f, tid & 3u, live, q8 + (row + i) / 32 * (HALVES ? kQ81sBytes : kQ81xBytes));
-    };
-    if constexpr (P > 0) {
-#pragma unroll
-        for (int p = 0; p < P; ++p) norm(p, h[p]);
-    } else {
-        for (uint32_t p = 0; p < passes; ++p) {
-            const uint32_t i = (p * kSumThreads + tid) * 8;
-            norm(p, i < hidden ? *reinterpret_cast<const half8*>(total + row + i) : half8{});     // the thread's own stores
-        }
+    if (tid < kSumThreads) {
+        float even = 0.f, odd = 0.f;
+        for (uint32_t i = tid; i < last; i += kSumThreads) square(sum_at(i), even, odd);
+        const float part = group_sum<32>(even + odd);
+        if ((tid & 31u) == 31) red[tid >> 5] = part;
     }
+    __syncthreads();
+    const float r = rsqrtf((((red[0] + red[1]) + red[2]) + red[3]) / (float)a.hidden + a.eps);
+    for (uint32_t i = tid; i < last; i += threads) {
+        const bool live = i * 8 < a.hidden;
+        if (live && i != tid) w = weights_at(a, i * 8);
+        normed<HALVES>(a, row + i * 8, sum_at(i), w, r, live);
+    }
+}
+
+// Short rows: LANES lanes take one, up to 8 LANES elements; no barrier: 100000 x 128 19 us, where a workgroup a row takes 53.
+template <int LANES, bool HALVES>
+__global__ __launch_bounds__(256) void add_norm_short_kernel(SumArgs a) {
+    const uint32_t lane = threadIdx.x % LANES, n = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const bool live = n < a.n_rows && lane * 8 < a.hidden;
+    const size_t at = (size_t)n * a.hidden + lane * 8;
+    half8 v = {};
+    Weights w;
+    if (live) {
+        v = added(a, at);
+        w = weights_at(a, lane * 8);
+    }
+    float even = 0.f, odd = 0.f;
+    square(v, even, odd);
+    float sum;
+    if constexpr (LANES <= 16) {
+        sum = group_sum<LANES>(even + odd);
+    } else {                 // the halves of a wave
+        const float part = group_sum<32>(even + odd), low = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(part), 31)), high = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(part), 63));
+        sum = LANES == 64 ? low + high : (threadIdx.x & 32u) ? high : low;
+    }
+    const float r = rsqrtf(sum / (float)a.hidden + a.eps);
+    normed<HALVES>(a, at, v, w, r, live);
 }
 
 // y = half(silu(gate) * up) (swiglu, src/ops/elementwise.cpp:449-467) or, OAI = true, the clamped
@@ -201,6 +232,11 @@ static int act_q8(mx_stream_t s, const uint16_t* gate, const uint16_t* up, uint1
     return launch_status();
 }
 
+template <bool B>
+struct Bool {
+    static constexpr bool value = B;
+};
+
 static int check_norm(const void* x, const void* w, const void* y, const void* q8, uint32_t n_rows, uint32_t hidden) {
     MX_REQUIRE_PTR(x); MX_REQUIRE_PTR(w); MX_REQUIRE_PTR(y); MX_REQUIRE_PTR(q8);
     MX_REQUIRE_SHAPE(n_rows > 0 && hidden > 0 && hidden % 32 == 0);
@@ -233,27 +269,26 @@ int mx_gated_rms_norm_q8(mx_stream_t s, const float* x, const uint16_t* z, const
 int mx_add_rms_norm_f32w_q8(mx_stream_t s, const uint16_t* x, const uint16_t* residual, const float* w, uint16_t* sum, uint16_t* y, void* q8_out, uint32_t n_rows,
                             uint32_t hidden, float eps, int halves) {
     MX_REQUIRE_PTR(x); MX_REQUIRE_PTR(residual); MX_REQUIRE_PTR(w); MX_REQUIRE_PTR(sum); MX_REQUIRE_PTR(q8_out);
-    MX_REQUIRE_SHAPE(n_rows > 0 && n_rows < (1u << 25) && hidden > 0 && hidden % 32 == 0);
+    MX_REQUIRE_SHAPE(n_rows > 0 && hidden > 0 && hidden % 32 == 0);
+    const uint32_t passes = (hidden + kSumThreads * 8 - 1) / (kSumThreads * 8), at_once = passes < kSumPasses ? passes : kSumPasses;
+    MX_REQUIRE_SHAPE((uint64_t)n_rows * at_once < (1u << 25));       // a launch holds fewer than 2^32 threads
     MX_REQUIRE_ALIGN(x, 16); MX_REQUIRE_ALIGN(residual, 16); MX_REQUIRE_ALIGN(w, 16); MX_REQUIRE_ALIGN(sum, 16); MX_REQUIRE_ALIGN(y, 16);
     MX_REQUIRE_ALIGN(q8_out, halves ? 16 : 8);
-    auto launch = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(n_rows), dim3(kSumThreads), 0, as_stream(s), reinterpret_cast<const half_t*>(x), reinterpret_cast<const half_t*>(residual), w,
-                           reinterpret_cast<half_t*>(sum), reinterpret_cast<half_t*>(y), static_cast<uint8_t*>(q8_out), hidden, eps);
+    const SumArgs a = {reinterpret_cast<const half_t*>(x), reinterpret_cast<const half_t*>(residual), w, reinterpret_cast<half_t*>(sum), reinterpret_cast<half_t*>(y), static_cast<uint8_t*>(q8_out),
+                       n_rows, hidden, eps};
+    auto launch = [&](auto kernel, uint32_t workgroups, uint32_t threads, uint32_t lds) {
+        hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(threads), lds, as_stream(s), a);
         return launch_status();
     };
-    const uint32_t passes = (hidden + kSumThreads * 8 - 1) / (kSumThreads * 8);
-#define MX_SUM(P) (halves ? launch(add_norm_q8_kernel<P, true>) : launch(add_norm_q8_kernel<P, false>))
-    switch (passes) {
-        case 1: return MX_SUM(1);
-        case 2: return MX_SUM(2);
-        case 3: return MX_SUM(3);
-        case 4: return MX_SUM(4);
-        case 5: return MX_SUM(5);
-        case 6: return MX_SUM(6);
-        case 7: case 8: return MX_SUM(8);
-        default: return MX_SUM(0);
-    }
-#undef MX_SUM
+    auto form = [&](auto h) {
+        constexpr bool H = decltype(h)::value;
+        if (hidden <= 128) return launch(add_norm_short_kernel<16, H>, (n_rows + 15) / 16, 256, 0);
+        if (hidden <= 256) return launch(add_norm_short_kernel<32, H>, (n_rows + 7) / 8, 256, 0);
+        if (hidden <= 512) return launch(add_norm_short_kernel<64, H>, (n_rows + 3) / 4, 256, 0);
+        const uint32_t threads = kSumThreads * at_once;
+        return hidden <= kSumLds ? launch(add_norm_kernel<H, false>, n_rows, threads, passes * kSumThreads * 16) : launch(add_norm_kernel<H, true>, n_rows, threads, 0);
+    };
+    return halves ? form(Bool<true>()) : form(Bool<false>());
 }
 
 int mx_swiglu_q8(mx_stream_t s, const uint16_t* gate, const uint16_t* up, uint16_t* y, void* q8_out, uint64_t n) {

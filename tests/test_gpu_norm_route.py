@@ -13,7 +13,7 @@ def f16(rng, *shape, scale=1.0):
     return O.round_fp16((rng.standard_normal(shape) * scale).astype(np.float32)).astype(np.float16)
 
 
-@pytest.mark.parametrize("T,H", [(1, 32), (3, 64), (5, 992), (2, 1024), (7, 1056), (1, 4096), (333, 2880), (4, 5120), (2, 6144), (9, 7200), (3, 8192), (2, 8224), (1, 16384), (2050, 128)])
+@pytest.mark.parametrize("T,H", [(1, 32), (3, 64), (5, 992), (2, 1024), (7, 1056), (1, 4096), (333, 2880), (4, 5120), (2, 6144), (9, 7200), (3, 8192), (2, 8224), (1, 16384), (2050, 128), (77, 160), (9, 512), (5, 544), (2, 32768), (3, 32800), (1100, 1024)])
 @pytest.mark.parametrize("halves", [False, True])
 def test_add_rms_norm(mx, T, H, halves):
     """The sum is one fp32 addition rounded to fp16; the norm has the bits of rms_norm_f32w_q8 of that sum, the stream those of the quantizers on it."""

@@ -264,8 +264,9 @@ def test_rows_and_cache(tmp_path):
 
 
 NORM = r"""
-template <int P, bool HALVES> static void norm(uint32_t T, uint32_t hidden, bool in_place, bool want_y) {
-    snprintf(what, sizeof what, "norm of %u rows of %u, %d passes, %s, %s, %s\n", T, hidden, P, HALVES ? "halves" : "blocks", in_place ? "in place" : "apart", want_y ? "rows" : "no rows");
+enum { ROWS, FAR, SHORT };
+template <int KIND, int P, bool HALVES> static void norm(uint32_t T, uint32_t hidden, bool in_place, bool want_y) {
+    snprintf(what, sizeof what, "norm of %u rows of %u, form %d %d, %s, %s, %s\n", T, hidden, KIND, P, HALVES ? "halves" : "blocks", in_place ? "in place" : "apart", want_y ? "rows" : "no rows");
     const size_t n = (size_t)T * hidden, size = HALVES ? 48 : 40;
     Held x(2 * n), res(2 * n), w(4 * hidden), total(2 * n), y(2 * n), q8(n / 32 * size);
     fill(x.as<half_t>(), n); fill(res.as<half_t>(), n);
@@ -273,7 +274,11 @@ template <int P, bool HALVES> static void norm(uint32_t T, uint32_t hidden, bool
     std::vector<half_t> sum(n);
     for (size_t i = 0; i < n; ++i) sum[i] = (half_t)((float)x.as<half_t>()[i] + (float)res.as<half_t>()[i]);
     half_t* const to = in_place ? res.as<half_t>() : total.as<half_t>();
-    run(kSumThreads, T, 1, 0, [&] { add_norm_q8_kernel<P, HALVES>(x.as<half_t>(), res.as<half_t>(), w.as<float>(), to, want_y ? y.as<half_t>() : nullptr, q8.p, hidden, 1e-5f); });
+    const SumArgs a = {x.as<half_t>(), res.as<half_t>(), w.as<float>(), to, want_y ? y.as<half_t>() : nullptr, q8.p, T, hidden, 1e-5f};
+    const uint32_t passes = (hidden + kSumThreads * 8 - 1) / (kSumThreads * 8);
+    if constexpr (KIND == ROWS) run(kSumThreads * std::min(passes, (uint32_t)P), T, 1, passes * kSumThreads * 16, [&] { add_norm_kernel<HALVES, false>(a); });
+    if constexpr (KIND == FAR) run(kSumThreads * std::min(passes, (uint32_t)P), T, 1, 0, [&] { add_norm_kernel<HALVES, true>(a); });
+    if constexpr (KIND == SHORT) run(256, (T + 256 / P - 1) / (256 / P), 1, 0, [&] { add_norm_short_kernel<P, HALVES>(a); });
     for (uint32_t t = 0; t < T; ++t) {
         double sq = 0;
         for (uint32_t i = 0; i < hidden; ++i) sq += (double)(float)sum[t * hidden + i] * (double)(float)sum[t * hidden + i];
@@ -292,8 +297,11 @@ template <int P, bool HALVES> static void norm(uint32_t T, uint32_t hidden, bool
 int main() {
     signal(SIGSEGV, on_fault);
     signal(SIGBUS, on_fault);
-    norm<1, false>(3, 32, false, true); norm<1, true>(2, 992, true, true); norm<1, false>(1, 1024, false, false); norm<2, true>(2, 1056, false, true); norm<3, false>(2, 2880, true, false);
-    norm<4, true>(1, 4096, false, true); norm<8, false>(2, 7200, true, true); norm<0, true>(1, 8224, true, true); norm<0, false>(2, 9216, false, false);
+    // four passes at a time here, where a GPU has eight
+    norm<ROWS, 4, true>(2, 992, true, true); norm<ROWS, 4, false>(1, 1024, false, false); norm<ROWS, 4, false>(2, 1056, true, true); norm<ROWS, 4, true>(1, 2880, false, false);
+    norm<ROWS, 4, false>(2, 4096, false, true); norm<ROWS, 4, true>(1, 8224, true, true); norm<FAR, 4, false>(2, 4128, false, true); norm<FAR, 4, true>(1, 33024, true, false);
+    norm<SHORT, 16, false>(35, 32, false, true); norm<SHORT, 16, true>(16, 96, true, true); norm<SHORT, 16, false>(1, 128, false, false); norm<SHORT, 32, true>(9, 160, true, true);
+    norm<SHORT, 32, false>(3, 256, false, true); norm<SHORT, 64, true>(5, 288, false, true); norm<SHORT, 64, false>(4, 512, true, false);
     return 0;
 }
 """
@@ -311,7 +319,8 @@ def with_header(text):
 
 
 def test_norm(tmp_path):
-    kernel = between("producers.hip", "constexpr int kSumThreads", "// y = half(silu(gate) * up) (swiglu,").replace('asm("" : "+v"(bits));', "")
+    kernel = between("producers.hip", "typedef _Float16 half8", "// y = half(silu(gate) * up) (swiglu,").replace('asm("" : "+v"(bits));', "").replace(
+        "extern __shared__ char sums[];", "char* const sums = shim_lds;")
     B.build_and_run(tmp_path, B.SHIM + MORE + "static float rsqrtf(float x) { return 1.f / sqrtf(x); }\n" + with_header(kernel) + B.CHECK + NORM)
 
 

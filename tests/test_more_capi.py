@@ -56,7 +56,7 @@ def test_norm_refusals(lib):  # noqa: F811
     c = Call(lib, "mx_add_rms_norm_f32w_q8", n_rows=4, hidden=128, eps=1e-5, halves=0)
     for p in ("x", "residual", "w", "sum", "q8_out"):
         assert c.with_(**{p: None}) == NULL, p
-    for bad in (dict(n_rows=0), dict(n_rows=1 << 25), dict(hidden=0), dict(hidden=48), dict(hidden=100)):
+    for bad in (dict(n_rows=0), dict(n_rows=1 << 25), dict(n_rows=1 << 24, hidden=2048), dict(n_rows=1 << 22, hidden=8192), dict(n_rows=1 << 22, hidden=1 << 20), dict(hidden=0), dict(hidden=48), dict(hidden=100)):
         assert c.with_(**bad) == SHAPE, bad
     for bad in (dict(x=P8), dict(residual=P8), dict(w=P8), dict(sum=P2), dict(y=P8), dict(q8_out=0x1004), dict(q8_out=P8, halves=1)):
         assert c.with_(**bad) == ALIGN, bad
