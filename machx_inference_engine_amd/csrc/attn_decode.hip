@@ -601,23 +601,29 @@ __global__ __launch_bounds__(512) void attn_join_kernel(AttnArgs a, uint32_t gro
 struct Plan {
     uint32_t shares;         // 0: a workgroup for each sequence and group of heads
     uint64_t ws_bytes;
+    bool wide;               // workgroups of kWide waves
 };
 // Q4_0: as many as are resident, four workgroups a CU for heads of up to 64, three up to 128, two beyond, rounded down.  us by workgroups (256, 512, 768, 1024): 64 x 8192 tokens of 8 heads of 64 115, 73, 66, 59, of
 // 128 104, 105, 98, 118; 16 x 8192 of 8 heads of 256 67, 53, 75, 58; 16 x 8192 of 3 heads of 128 21.8, 18.4 (513 of them), 15.8, 20.1.
+// Where a workgroup for each sequence and group of heads leaves CUs free, it has eight waves for more than two tiles a wave of four, and for heads of up to 128 takes up to 1024 tokens: us, four waves (and their
+// parts' join) against eight, sequences of 8 heads of 128: one of 512 tokens 8.8, 8.2, of 256 6.7, 6.6; 32 of 512 9.6, 9.4, of 256 7.1, 7.4; of 1024 tokens one 6.1 + 3.4, 10.7, four 7.5 + 4.0, 11.0, 16 10.4 + 4.0, 11.6,
+// 32 16.9 + 4.0, 12.4; of 8 heads of 256 one of 512 11.9, 10.8, of 1024 7.7 + 3.8, 15.0.  More workgroups than CUs wait: 48 of 512 11.4, 15.7.
 enum { kF16 = 0, kQ8 = 1, kQ4 = 2 };   // what a cache holds
 constexpr uint32_t kDirectTiles = 4 * kWaves;
+constexpr int kWide = 8;
 static Plan plan_of(int fmt, uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, uint32_t max_len, uint32_t window) {
     const uint32_t span = window && window < max_len ? window : max_len;
     const uint64_t tiles = window && window < max_len ? span / kTile + 2 : (span + (uint64_t)kTile - 1) / kTile, all = B * tiles;   // a window may begin within a tile
     const uint64_t groups = (uint64_t)Hkv * ((Hq / Hkv + 15) / 16);
-    if (tiles <= kDirectTiles) return {0, 0};
+    const bool wide = fmt == kQ4 && B * groups <= 256 && tiles > 2 * kWaves && tiles <= (D > 128 ? kDirectTiles : 4 * kWide);
+    if (wide || tiles <= kDirectTiles) return {0, 0, wide};
     auto up = [](uint64_t x, uint64_t y) { return (x + y - 1) / y; };
     uint64_t most = up(all, kLeastShare);
     if (most * groups > 128) most = up(all, 2 * kLeastShare) > up(128, groups) ? up(all, 2 * kLeastShare) : up(128, groups);
     uint64_t shares = fmt == kQ4 ? (D > 128 ? 512 : D > 64 ? 768 : 1024) / groups : up(D > 128 ? 256 : D > 64 ? 512 : 768, groups);
     if (shares == 0) shares = 1;
     if (shares > most) shares = most;
-    return {(uint32_t)shares, (shares + B) * Hq * (D + 2) * 4 + (uint64_t)B * 8};
+    return {(uint32_t)shares, (shares + B) * Hq * (D + 2) * 4 + (uint64_t)B * 8, false};
 }
 
 // ---------------------------------------------------------------- Q4_0
@@ -650,8 +656,8 @@ struct Int {
     static constexpr int value = N;
 };
 
-template <int NB, int C>
-__global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void attn_decode_q4_kernel(AttnArgs a) {
+template <int NB, int C, int W = kWaves>
+__global__ __launch_bounds__(W * 64, W > (int)kWaves ? 2 : NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void attn_decode_q4_kernel(AttnArgs a) {
     constexpr uint32_t D = 32 * NB, GP = 16 / C;
     // LDS of a token's codes: an odd number of 16-byte pieces, so that 16 rows meet all banks; the second half of a tile lies four rows further, for the keys' rows 0 .. 3, 8 .. 11, 16 .. 19, 24 .. 27
     constexpr uint32_t ROW = 16 * (NB | 1), HALF = 20 * ROW;
@@ -789,7 +795,7 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
     uint32_t tile = first + wave;
     Ref cur = locate(tile), next = cur;
     load(cur);
-    if (tile + kWaves < last) next = locate(tile + kWaves);
+    if (tile + W < last) next = locate(tile + W);
     half8 qf[NB];
     float off[S];
     float unit;              // of the scores
@@ -831,8 +837,8 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
     float room = 15.f;                         // log2 of the largest weight
     uint32_t most = 15u << 10;                  // scales below this, as bits, leave it as it is
 #pragma unroll 1
-    for (; tile < last; tile += kWaves) {
-        const bool more = tile + kWaves < last;
+    for (; tile < last; tile += W) {
+        const bool more = tile + W < last;
         const bool ok0 = cur.page[0] < a.n_pages, ok1 = cur.page[1] < a.n_pages, full = cur.token >= sp.start && cur.token + kTile <= sp.end && ok0 && ok1;
         auto live = [&](uint32_t t) { return cur.token + t >= sp.start && cur.token + t < sp.end && (t >> 4 ? ok1 : ok0); };
         if (!full) {         // masked tokens' values have no scale, since what lies there may be no number
@@ -973,7 +979,7 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
         }
         if (more) {
             cur = next;
-            if (tile + 2 * kWaves < last) next = locate(tile + 2 * kWaves);
+            if (tile + 2 * W < last) next = locate(tile + 2 * W);
         }
     }
     }
@@ -981,7 +987,7 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
     // ---- the waves' sums: lane (r, g) holds elements 32 n + 16 h + 4 g + 0 .. 3 of its head in o[2 n + h], of the blocks of its column; sum p d of block n is in row n of z, the sum of weights in row NB
     __syncthreads();                         // the tiles' place is taken
     float* ml = lds;                         // [waves][16] (maximum, sum)
-    float* os = lds + kWaves * 32;            // [waves][heads][OS]
+    float* os = lds + W * 32;            // [waves][heads][OS]
     const float l = __shfl(z[NB % 4], NB / 4 * 16 + r);
     if (g == 0 && group == 0) {
         ml[(wave * 16 + r) * 2] = m;
@@ -1003,16 +1009,16 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
         }
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x * 4; i < (heads * D + kWaves * 256 - 1) / (kWaves * 256) * (kWaves * 256); i += kWaves * 256) {
+    for (uint32_t i = threadIdx.x * 4; i < (heads * D + W * 256 - 1) / (W * 256) * (W * 256); i += W * 256) {
         const bool live = i < heads * D;
         const uint32_t h = live ? i / D : 0, d = live ? i - h * D : 0;
         const uint32_t hq = hk * G + head0 + h;
         const float sink = whole && a.sinks ? a.sinks[hq] * kLog2e : -INFINITY;
         float top = sink, total = 0.f;
-        for (uint32_t w = 0; w < kWaves; ++w) top = fmaxf(top, ml[(w * 16 + h) * 2]);
+        for (uint32_t w = 0; w < (uint32_t)W; ++w) top = fmaxf(top, ml[(w * 16 + h) * 2]);
         const float ref = top == -INFINITY ? 0.f : top;
         floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-        for (uint32_t w = 0; w < kWaves; ++w) {
+        for (uint32_t w = 0; w < (uint32_t)W; ++w) {
             const float f = __builtin_amdgcn_exp2f(ml[(w * 16 + h) * 2] - ref);
             total += f * ml[(w * 16 + h) * 2 + 1];
             sum += f * *reinterpret_cast<const floatx4*>(os + (w * heads + h) * OS + d);
@@ -1034,23 +1040,27 @@ __global__ __launch_bounds__(kWaves * 64, NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void at
 }
 
 // ---------------------------------------------------------------- launches
-template <int NB, int C>
-static int launch_q4(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads) {
+template <int NB, int C, int W>
+static int launch_q4_waves(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads) {
     static LdsLimit limit;
-    constexpr uint32_t tiles = kWaves * (2 * 36 * 16 * (NB | 1) + kTile * (2 * NB + 1) * 2), most = kWaves * (32 + 16 / C * (32 * NB + 4)) * 4;
-    const uint32_t sums = kWaves * (32 + heads * (32 * NB + 4)) * 4, lds = tiles > sums ? tiles : sums;
+    constexpr uint32_t tiles = W * (2 * 36 * 16 * (NB | 1) + kTile * (2 * NB + 1) * 2), most = W * (32 + 16 / C * (32 * NB + 4)) * 4;
+    const uint32_t sums = W * (32 + heads * (32 * NB + 4)) * 4, lds = tiles > sums ? tiles : sums;
     if (lds > kLdsDefaultLimit)
-        if (int rc = raise_lds_limit(reinterpret_cast<const void*>(attn_decode_q4_kernel<NB, C>), limit, tiles > most ? tiles : most)) return rc;
-    hipLaunchKernelGGL((attn_decode_q4_kernel<NB, C>), grid, dim3(kWaves * 64), lds, as_stream(s), a);
+        if (int rc = raise_lds_limit(reinterpret_cast<const void*>(attn_decode_q4_kernel<NB, C, W>), limit, tiles > most ? tiles : most)) return rc;
+    hipLaunchKernelGGL((attn_decode_q4_kernel<NB, C, W>), grid, dim3(W * 64), lds, as_stream(s), a);
     return launch_status();
+}
+template <int NB, int C>
+static int launch_q4(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads, bool wide) {
+    return wide ? launch_q4_waves<NB, C, kWide>(s, a, grid, heads) : launch_q4_waves<NB, C, kWaves>(s, a, grid, heads);
 }
 // As many column groups as the heads leave room for and the blocks can use.
 template <int NB>
-static int launch_q4_columns(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads) {
-    if (NB > 4 && heads <= 2) return launch_q4<NB, (NB > 4 ? 8 : 1)>(s, a, grid, heads);
-    if (NB > 2 && heads <= 4) return launch_q4<NB, (NB > 2 ? 4 : 1)>(s, a, grid, heads);
-    if (NB > 1 && heads <= 8) return launch_q4<NB, (NB > 1 ? 2 : 1)>(s, a, grid, heads);
-    return launch_q4<NB, 1>(s, a, grid, heads);
+static int launch_q4_columns(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads, bool wide) {
+    if (NB > 4 && heads <= 2) return launch_q4<NB, (NB > 4 ? 8 : 1)>(s, a, grid, heads, wide);
+    if (NB > 2 && heads <= 4) return launch_q4<NB, (NB > 2 ? 4 : 1)>(s, a, grid, heads, wide);
+    if (NB > 1 && heads <= 8) return launch_q4<NB, (NB > 1 ? 2 : 1)>(s, a, grid, heads, wide);
+    return launch_q4<NB, 1>(s, a, grid, heads, wide);
 }
 template <bool Q8, int DP, int NBLK, bool FULL>
 static int launch_form(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads) {
@@ -1063,16 +1073,16 @@ static int launch_form(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t hea
     hipLaunchKernelGGL((attn_decode_kernel<Q8, DP, NBLK, FULL>), grid, dim3(kWaves * 64), lds, as_stream(s), a);
     return launch_status();
 }
-static int launch_attn(mx_stream_t s, const AttnArgs& a, int fmt, dim3 grid, uint32_t heads) {
+static int launch_attn(mx_stream_t s, const AttnArgs& a, int fmt, dim3 grid, uint32_t heads, bool wide) {
     if (fmt == kQ4) switch (a.D / 32) {
-        case 1: return launch_q4_columns<1>(s, a, grid, heads);
-        case 2: return launch_q4_columns<2>(s, a, grid, heads);
-        case 3: return launch_q4_columns<3>(s, a, grid, heads);
-        case 4: return launch_q4_columns<4>(s, a, grid, heads);
-        case 5: return launch_q4_columns<5>(s, a, grid, heads);
-        case 6: return launch_q4_columns<6>(s, a, grid, heads);
-        case 7: return launch_q4_columns<7>(s, a, grid, heads);
-        default: return launch_q4_columns<8>(s, a, grid, heads);
+        case 1: return launch_q4_columns<1>(s, a, grid, heads, wide);
+        case 2: return launch_q4_columns<2>(s, a, grid, heads, wide);
+        case 3: return launch_q4_columns<3>(s, a, grid, heads, wide);
+        case 4: return launch_q4_columns<4>(s, a, grid, heads, wide);
+        case 5: return launch_q4_columns<5>(s, a, grid, heads, wide);
+        case 6: return launch_q4_columns<6>(s, a, grid, heads, wide);
+        case 7: return launch_q4_columns<7>(s, a, grid, heads, wide);
+        default: return launch_q4_columns<8>(s, a, grid, heads, wide);
     }
     if (fmt == kQ8) switch (a.D / 32) {
         case 1: return launch_form<true, 64, 1, false>(s, a, grid, heads);
@@ -1137,7 +1147,7 @@ static int attn_decode(mx_stream_t s, int fmt, const uint16_t* q, uint64_t q_str
     if (join_groups > 512 / (D / 4)) join_groups = 512 / (D / 4);
     const uint32_t join_threads = (join_groups * (D / 4) + 63) / 64 * 64;
     MX_REQUIRE_SHAPE(!p.shares || (uint64_t)B * Hq * join_threads < (1ull << 32));
-    if (int rc = launch_attn(s, a, fmt, dim3(p.shares ? p.shares : B, (uint32_t)groups), heads)) return rc;
+    if (int rc = launch_attn(s, a, fmt, dim3(p.shares ? p.shares : B, (uint32_t)groups), heads, p.wide)) return rc;
     if (p.shares) {
         hipLaunchKernelGGL(attn_join_kernel, dim3(B * Hq), dim3(join_threads), join_groups * D * 4, as_stream(s), a, join_groups);
         if (int rc = launch_status()) return rc;

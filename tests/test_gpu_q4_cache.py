@@ -164,6 +164,22 @@ def test_every_width_of_head(mx, D, G):
     near(host(attend(mx, q, cache, table, lens)), *Q.attention(q, cache, table, lens, 16, D ** -0.5), "D=%d G=%d" % (D, G))
 
 
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("G,Hkv", [(1, 40), (7, 3), (17, 8), (4, 64)])
+def test_few_sequences_up_to_a_thousand_tokens(mx, D, G, Hkv):
+    """Fewer workgroups than CUs, of more than two tiles a wave: no parts for heads of up to 128, whatever the lengths are in the end."""
+    lens, most = ([1024, 0, 300, 97] if D <= 128 else [512, 0, 300, 97])[:256 // (Hkv * (1 + G // 17))], 1024 if D <= 128 else 512
+    rng, table, cache, q = case(lens, Hkv, G, D, 16, 3 * D + G)
+    assert mx.ops.attn_decode_ws_bytes(len(lens), Hkv * G, Hkv, D, most, fmt="q4_0") == 0
+    assert mx.ops.attn_decode_ws_bytes(len(lens), Hkv * G, Hkv, D, most + 1, fmt="q4_0") > 0
+    sinks = rng.standard_normal(Hkv * G).astype(np.float32)
+    for window in (0, 260):
+        stream = torch.empty(q.size // 32 * 40, dtype=torch.uint8, device="cuda")
+        y = attend(mx, q, cache, table, lens, window=window, sinks=dev(sinks), max_len=most, out_q8=stream)
+        near(host(y), *Q.attention(q, cache, table, lens, 16, D ** -0.5, window, sinks), "D=%d G=%d window %d" % (D, G, window))
+        assert torch.equal(stream, mx.ops.quantize_q8_1(y)) and (host(y)[np.array(lens) == 0] == 0).all()
+
+
 @pytest.mark.parametrize("window", [1, 5, 16, 33, 128, 1000])
 @pytest.mark.parametrize("with_sinks", [False, True])
 def test_window_and_sinks(mx, window, with_sinks):

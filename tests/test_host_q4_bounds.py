@@ -34,7 +34,7 @@ static int shim_dpp_or_rotation(int old, int v, int ctrl, int row_mask, int bank
 """
 
 ATTENTION = r"""
-template <int NB, int C> static void one(uint32_t Hkv, uint32_t G, uint32_t ps, uint32_t window, uint32_t shares, std::vector<int32_t> lens, float scale = 0.3f, float q_size = 1.f, int plant = 0) {
+template <int NB, int C, int W = kWaves> static void one(uint32_t Hkv, uint32_t G, uint32_t ps, uint32_t window, uint32_t shares, std::vector<int32_t> lens, float scale = 0.3f, float q_size = 1.f, int plant = 0) {
     const uint32_t D = 32 * NB, B = (uint32_t)lens.size(), Hq = Hkv * G;
     uint32_t most = 1, pages = 0;
     for (int32_t n : lens) { const uint32_t need = n > 0 ? (n + ps - 1) / ps : 0; most = std::max(most, need); pages += need; }
@@ -76,8 +76,8 @@ template <int NB, int C> static void one(uint32_t Hkv, uint32_t G, uint32_t ps, 
     a.page_shift = (ps & (ps - 1)) == 0 ? (uint32_t)__builtin_ctz(ps) : 32u;
     a.scale = scale * kLog2e;
     const uint32_t heads = std::min(G, 16u);
-    const size_t tiles = kWaves * (2 * 36 * 16 * (NB | 1) + kTile * (2 * NB + 1) * 2), sums = kWaves * (32 + heads * (D + 4)) * 4;   // as the launch asks for
-    run(kWaves * 64, shares ? shares : B, Hkv * ((G + 15) / 16), std::max(tiles, sums), [&] { attn_decode_q4_kernel<NB, C>(a); });
+    const size_t tiles = W * (2 * 36 * 16 * (NB | 1) + kTile * (2 * NB + 1) * 2), sums = W * (32 + heads * (D + 4)) * 4;   // as the launch asks for
+    run(W * 64, shares ? shares : B, Hkv * ((G + 15) / 16), std::max(tiles, sums), [&] { attn_decode_q4_kernel<NB, C, W>(a); });
     if (shares) {
         uint32_t groups = std::min((shares / B + 4) / 4, 512 / (D / 4));
         run((groups * (D / 4) + 63) / 64 * 64, B * Hq, 1, groups * D * 4, [&] { attn_join_kernel(a, groups); });
@@ -136,6 +136,7 @@ ATTENTION_CASES = {
                one<5, 1>(1, 12, 16, 0, 0, {20}); one<7, 2>(1, 5, 16, 0, 0, {20});""",
     "scales": """one<2, 2>(1, 3, 16, 0, 0, {333, 5}, 0.3f, 1.f, 1); one<4, 4>(1, 2, 32, 0, 3, {400, 31}, 0.3f, 1.f, 1); one<2, 2>(2, 1, 48, 0, 0, {17, 100, 1}, 0.3f, 1.f, 2);
                  one<3, 4>(1, 1, 16, 20, 2, {333, 18}, 0.3f, 1.f, 2);""",
+    "eight_waves": "one<4, 4, 8>(1, 3, 16, 0, 0, {300, 0, 5}); one<2, 2, 8>(2, 8, 48, 0, 0, {513}, 0.3f, 1.f, 2); one<8, 1, 8>(1, 17, 16, 290, 0, {333}); one<1, 1, 8>(1, 1, 32, 0, 0, {700}); one<8, 8, 8>(1, 1, 16, 0, 0, {270});",
     "no_numbers": "one<2, 2>(1, 3, 16, 0, 0, {133, 5}, 0.3f, 1.f, 3); one<4, 4>(1, 2, 32, 0, 3, {300, 31}, 0.3f, 1.f, 3); one<4, 2>(1, 5, 32, 0, 0, {100}, 0.3f, 1.f, 3);",
 }
 
