@@ -656,7 +656,7 @@ int mx_moe_topk_from_logits(mx_stream_t s, const uint16_t* logits, int32_t* topk
  *     n_groups > 1: the experts lie in n_groups groups of n_experts / n_groups; a group's worth is its largest c, or the sum of its two largest with MX_ROUTE_TOP2; the topk_groups of
  *     largest worth are kept.  Of the kept experts those of the k largest c are chosen; of equal ones the lowest id (or group) is.
  *     topk_w = half(scale * s / (sum of the chosen s + 1e-20)) with MX_ROUTE_RENORM, half(scale * s) without; the bias is no part of it.
- *     Scores, worths and comparisons are 64 bits, so that what is chosen is that of the exact scores, next to ties too; weights are rounded once.
+ *     Scores, worths and comparisons are 64 bits, and what agrees in these is equal (two logits beyond 37 by their sigmoids); weights are rounded once.
  *     An expert of logit -infinity has score 0 (a softmax over nothing else: all scores 0).  A c that is NaN lies below every number, and is then taken by id; so does a group with one for its worth.
  *     n_experts <= 1024, k <= 64, n_experts % n_groups == 0, n_groups <= 64, 1 <= topk_groups <= n_groups, k <= topk_groups * n_experts / n_groups, n_tokens < 2^26.
  *     MX_ROUTE_TOP2 over groups of one expert: its c.  A token's result is the same bits in every call.  */

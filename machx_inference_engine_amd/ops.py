@@ -908,8 +908,8 @@ def kv_cache(fmt, n_pages, n_kv_heads, page_size, head_dim, device="cuda"):
     if fmt == "f16":
         return tuple(torch.zeros(shape, dtype=_F16, device=device) for _ in range(2))
     _want(fmt in ("q8_0", "q4_0") and head_dim % 32 == 0, "a cache is f16, or q8_0 or q4_0 with heads of whole blocks of 32")
-    codes = torch.zeros(shape, dtype=_I8, device=device) if fmt == "q8_0" else torch.zeros(shape[:3] + (head_dim // 2,), dtype=_U8, device=device)
-    plane = lambda: (codes.clone(), torch.zeros(shape[:3] + (head_dim // 32,), dtype=_F16, device=device))  # noqa: E731
+    codes, dtype = (shape, _I8) if fmt == "q8_0" else (shape[:3] + (head_dim // 2,), _U8)
+    plane = lambda: (torch.zeros(codes, dtype=dtype, device=device), torch.zeros(shape[:3] + (head_dim // 32,), dtype=_F16, device=device))  # noqa: E731
     return plane() + plane()
 
 
@@ -998,6 +998,7 @@ def kv_read(cache, page_table, rows, total_rows, out=None):
 @functools.lru_cache(maxsize=1024)
 def attn_decode_ws_bytes(B, Hq, Hkv, D, max_len, window=0, fmt="f16"):
     """fmt: the cache's format, as kv_cache has it."""
+    _want(fmt in _ATTN_DECODE, "fmt is f16, q8_0 or q4_0")
     n = ctypes.c_uint64()
     query = lib.mx_attn_decode_q4_0_ws_bytes if fmt == "q4_0" else lib.mx_attn_decode_ws_bytes
     rc = query(B, Hq, Hkv, D, max_len, window, ctypes.addressof(n))

@@ -7,7 +7,7 @@ import kv_util as U
 import oracle as O
 import q4_util as Q
 from gpu_util import check, dev, host
-from test_gpu_moe import make_experts
+from test_gpu_moe import check_rows, make_experts
 from test_gpu_norm_route import route
 
 pytestmark = pytest.mark.gpu
@@ -116,6 +116,28 @@ def test_layer_step(mx, B, lens):
         got = layer.step(x, residual, dev(pos), slots_of(layer, pos), dev(pos + 1), cache)
         check_step(layer, got, host(x), host(residual), pos, cache)
         x, residual, pos = got["out"], got["total2"], pos + 1
+
+
+@pytest.mark.parametrize("T", [1, 3, 70])
+def test_prompt_through_the_experts(mx, T):
+    """Routed, packed on the device, through the grouped products: the rows of the token by token form."""
+    layer, ops = Layer(mx, 1, 60), mx.ops
+    rng = np.random.default_rng(T)
+    x, residual = (dev(rng.standard_normal((T, H)).astype(np.float16)) for _ in range(2))
+    _, y, yq = ops.add_rms_norm_f32w_q8(x, residual, layer.norms[1], 1e-5)
+    ids, w = ops.moe_route(ops.moe_router_logits(y, layer.gate), K, bias=layer.bias, n_groups=4, topk_groups=2)
+    off, si, wp, t2p = ops.moe_build_packing_device(ids, w, E)
+    for a, b in zip((off, si, wp, t2p), O.build_moe_packing(host(ids), host(w).astype(np.float32), E)):
+        assert np.array_equal(host(a).astype(np.float64), np.asarray(b, np.float64))
+    (gq, gd), (uq, ud), (dq, dd) = layer.banks
+    rows = ops.quantize_q8_1(ops.moe_gather_rows(y, si, T * K, H))
+    packed = ops.moe_prefill_gate_up_silu_q8(rows, gq, gd, uq, ud, H * EF, H * EF // 32, off, T * K, E, H, EF)
+    h = torch.cat([ops.moe_gate_up_silu_q8(yq.view(T, -1)[t].contiguous(), gq, gd, uq, ud, H * EF, H * EF // 32, ids[t].contiguous(), 1, K, H, EF, n_experts=E) for t in range(T)])
+    check_rows(host(packed)[host(t2p)], host(h), "grouped gate and up")
+    out = ops.moe_prefill_down_q8(ops.quantize_q8_1(packed), dq, dd, H * EF, H * EF // 32, off, wp, T * K, E, H, EF)
+    hq = ops.quantize_q8_1(packed[t2p.long()])
+    down = torch.cat([ops.moe_down_q8(hq.view(T, -1)[t].contiguous(), dq, dd, H * EF, H * EF // 32, ids[t].contiguous(), w[t].contiguous(), 1, K, EF, H, n_experts=E) for t in range(T)])
+    check_rows(host(out)[host(t2p)], host(down), "grouped down")
 
 
 def test_captured_step(mx):

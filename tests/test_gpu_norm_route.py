@@ -46,6 +46,14 @@ def test_in_place_and_without_rows(mx, H):
         assert torch.equal((b, a)[target], (res, x)[target])
 
 
+@pytest.mark.parametrize("H", [128, 1024, 33024])
+def test_one_tensor_for_both(mx, H):
+    x, w = dev(f16(np.random.default_rng(H), 3, H)), dev(np.ones(H, np.float32))
+    h, y, q8 = mx.ops.add_rms_norm_f32w_q8(x, x.clone(), w, 1e-6)
+    for got in (mx.ops.add_rms_norm_f32w_q8(x, x, w, 1e-6), mx.ops.add_rms_norm_f32w_q8(x, x, w, 1e-6, out=(x, torch.empty_like(x), torch.empty_like(q8)))):
+        assert all(torch.equal(a, b) for a, b in zip(got, (h, y, q8)))
+
+
 def test_rows_without_numbers_leave_others_alone(mx):
     rng = np.random.default_rng(1)
     x, res, w = f16(rng, 6, 256), f16(rng, 6, 256), np.ones(256, np.float32)

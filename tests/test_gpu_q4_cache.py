@@ -454,3 +454,28 @@ def test_refusals(mx):
                lambda: ops.kv_read(cache, tab, dev(np.zeros(3, np.int32)), 5)):
         with pytest.raises(ValueError):
             fn()
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q8_0", "q4_0"])
+def test_a_new_cache_takes_its_own_bytes(mx, fmt):
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    cache = mx.ops.kv_cache(fmt, 512, 8, 64, 128)
+    size = sum(t.numel() * t.element_size() for t in cache)
+    assert torch.cuda.max_memory_allocated() - before == size and len({t.data_ptr() for t in cache}) == len(cache) and all((t == 0).all() for t in cache)
+    with pytest.raises(ValueError):
+        mx.ops.attn_decode_ws_bytes(1, 8, 8, 128, 4096, fmt="q4")
+
+
+def test_queries_that_are_no_numbers(mx):
+    """Such a head is NaN, its neighbours in the same products have the bits that they have beside a number; without tokens it is zeros."""
+    lens = [0, 40, 700, 1]
+    rng, table, cache, q = case(lens, 2, 8, 128, 16, 5)
+    want = host(attend(mx, q, cache, table, lens))
+    heads = {1: np.inf, 6: np.nan, 11: -np.inf}
+    for h, x in heads.items():
+        q[:, h, 3 * h % 128] = x
+    y = host(attend(mx, q, cache, table, lens))
+    others = [h for h in range(16) if h not in heads]
+    assert np.isnan(y[1:, list(heads)]).all() and (y[0] == 0).all() and np.array_equal(y[:, others].view(np.uint16), want[:, others].view(np.uint16))
