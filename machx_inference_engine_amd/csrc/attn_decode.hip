@@ -96,6 +96,56 @@ __device__ __forceinline__ Share share_of(const AttnArgs& a, uint32_t share, uin
     return s;
 }
 
+// The same, where each sequence but one costs as much as `extra` tiles more (its queries, first loads and sums): these stand in front of its tiles, so that a share that holds many ends of sequences has fewer
+// tiles.  Not where every share would lie within one sequence without them.  us without them and with 4, 8 (half a share of tiles at most), 12 and 16 (a share at most), ragged sequences of 8 heads of 128: 17 of up to 4000 tokens
+// 16.1, 15.4, 14.6, 14.0, 14.5; 43 of 4000 27.4, 26.0, 24.2, 23.3, 24.1; 100 of 1000 24.9, 21.8, 21.5, 20.8, 21.0; 200 of 3000 70.6, 65.4, 64.6, 64.2, 65.8; equal ones, 64 of 8192 99.0, 97.7, 96.8, 95.9, 97.0, 32 of 2048
+// 20.7, 20.4, 18.0, 19.8; 48 of 1024, which lie within one sequence, 15.7, 17.0, 17.4, 18.6; 16 of 8192 of 8 heads of 256 51.7, 52.6, 54.0, 53.6.
+struct Weighed {
+    uint32_t per, left, b, from, extra;   // per, left and from with the extra tiles
+    int32_t len;
+};
+__device__ __forceinline__ Weighed weighed_share(const AttnArgs& a, uint32_t share, uint32_t lane) {
+    uint32_t total = 0, upto = 0, own = 0, n = 0;
+    int32_t len = 0;
+    for (uint32_t i0 = 0; i0 < a.B; i0 += 64) {
+        len = i0 + lane < a.B ? a.lens[i0 + lane] : 0;
+        own = span_of(a, len).tiles;
+        if (own == 0 && i0 + lane < a.B && share == 0 && blockIdx.y == 0)
+            *reinterpret_cast<uint2*>(a.parts + 2 * (i0 + lane)) = make_uint2(0, 0);   // no part: zeros, whatever the sinks
+        upto = lanes_upto(own);
+        total += lane_value(upto, 63);
+        n += (uint32_t)__builtin_popcountll(__ballot(own != 0));
+    }
+    Weighed s;
+    const uint32_t bare = max(kLeastShare, (total + a.shares - 1) / a.shares);
+    s.extra = n > 1 && (a.B > 64 || __any(upto % bare != 0 && own != 0)) ? min(12u, bare) : 0u;
+    total += n * s.extra;
+    s.per = max(kLeastShare, (total + a.shares - 1) / a.shares);
+    const uint64_t at = (uint64_t)share * s.per;
+    s.left = at < total ? min(s.per, total - (uint32_t)at) : 0u;
+    s.b = s.from = 0;
+    s.len = 0;
+    uint32_t before = 0;
+    for (uint32_t i0 = 0; s.left && i0 < a.B; i0 += 64) {
+        if (a.B > 64) {      // up to 64 sequences: as they were
+            len = i0 + lane < a.B ? a.lens[i0 + lane] : 0;
+            own = span_of(a, len).tiles;
+        }
+        own = own ? own + s.extra : 0u;
+        upto = lanes_upto(own);
+        const uint64_t hit = __ballot(before + upto > (uint32_t)at);
+        if (hit) {
+            const int first = __ffsll((unsigned long long)hit) - 1;
+            s.b = i0 + first;
+            s.from = (uint32_t)at - before - lane_value(upto - own, first);
+            s.len = (int32_t)lane_value((uint32_t)len, first);
+            break;
+        }
+        before += lane_value(upto, 63);
+    }
+    return s;
+}
+
 // Final rows: four consecutive elements of a thread's, all of 8 threads in one block of 32 (D % 32 == 0 where a stream is wanted).
 __device__ __forceinline__ void store_rows(const AttnArgs& a, size_t at, const float (&o)[4], bool live) {
     half_t h[4];
@@ -688,23 +738,30 @@ __global__ __launch_bounds__(W * 64, W > (int)kWaves ? 2 : NB <= 2 ? 4 : NB <= 4
     // bytes 0 1 2 3 of a word of the transposing read are tokens 0 2 1 3 of four places, so that an `and` leaves two consecutive ones; lane r of 16 brings 8 bytes of row r / 2
 #pragma unroll
     for (int k = 0; k < R; ++k) value_at[k] = (8 * g + 2 * (((r >> 2 & 2u) + (r >> 1 & 1u) + k * PS) & 3u) + (r >> 2 & 1u)) * ROW + (g >> 1) * (HALF - 16 * ROW) + (r & 1u) * 8;
-    Share sh = {1, 1, blockIdx.x, 0, 0};
-    if (shared) sh = share_of(a, share, lane);
+    Weighed sh = {1, 1, blockIdx.x, 0, 0, 0};
+    if (shared) sh = weighed_share(a, share, lane);
     else sh.len = a.lens[sh.b];
-    uint32_t b = sh.b, first = sh.from, left = sh.left;
+    uint32_t b = sh.b, at = sh.from, left = sh.left;
     int32_t len = __builtin_amdgcn_readfirstlane(sh.len);
     for (; left; len = __builtin_amdgcn_readfirstlane(left ? a.lens[b + 1] : 0), ++b) {
     const Span sp = span_of(a, len);
-    const uint32_t last = shared ? min(sp.tiles, first + left) : sp.tiles;
-    const bool whole = first == 0 && last == sp.tiles;     // the result itself, not a part of it
-    const size_t out0 = ((size_t)b * a.Hq + hk * G + head0) * D;
+    uint32_t first = 0, last = sp.tiles;
+    const uint32_t done = sh.per - left;
     if (shared) {
         if (sp.tiles == 0) continue;
-        if (first == 0 && blockIdx.y == 0 && threadIdx.x == 0) *reinterpret_cast<uint2*>(a.parts + 2 * b) = make_uint2(share + b, (sh.per - left + sp.tiles - 1) / sh.per + 1);
-        left -= last - first;
+        const uint32_t to = min(sp.tiles + sh.extra, at + left);
+        left -= to - at;
+        first = max(at, sh.extra) - sh.extra;
+        last = max(to, sh.extra) - sh.extra;
+        const uint32_t in_front = done + sh.extra - at;
+        at = 0;
+        if (first == last) continue;
+        if (first == 0 && blockIdx.y == 0 && threadIdx.x == 0) *reinterpret_cast<uint2*>(a.parts + 2 * b) = make_uint2(share + b, (in_front + sp.tiles - 1) / sh.per + 1);
     } else {
         left = 0;
     }
+    const bool whole = first == 0 && last == sp.tiles;     // the result itself, not a part of it
+    const size_t out0 = ((size_t)b * a.Hq + hk * G + head0) * D;
 
     typedef const __attribute__((address_space(4))) int32_t* table_t;
     const table_t table = (table_t)(uintptr_t)(a.table + (size_t)b * a.max_pages);
@@ -1034,7 +1091,6 @@ __global__ __launch_bounds__(W * 64, W > (int)kWaves ? 2 : NB <= 2 ? 4 : NB <= 4
             if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(top, total);
         }
     }
-    first = 0;
     if (left) __syncthreads();               // the sums have been read
     }
 }

@@ -137,6 +137,8 @@ ATTENTION_CASES = {
     "scales": """one<2, 2>(1, 3, 16, 0, 0, {333, 5}, 0.3f, 1.f, 1); one<4, 4>(1, 2, 32, 0, 3, {400, 31}, 0.3f, 1.f, 1); one<2, 2>(2, 1, 48, 0, 0, {17, 100, 1}, 0.3f, 1.f, 2);
                  one<3, 4>(1, 1, 16, 20, 2, {333, 18}, 0.3f, 1.f, 2);""",
     "eight_waves": "one<4, 4, 8>(1, 3, 16, 0, 0, {300, 0, 5}); one<2, 2, 8>(2, 8, 48, 0, 0, {513}, 0.3f, 1.f, 2); one<8, 1, 8>(1, 17, 16, 290, 0, {333}); one<1, 1, 8>(1, 1, 32, 0, 0, {700}); one<8, 8, 8>(1, 1, 16, 0, 0, {270});",
+    "shares": """one<1, 1>(1, 1, 16, 0, 5, {1, 70, 0, 33, 300, 2, 0, 0, 31, 32, 64, 200, 16}); one<1, 1>(1, 2, 16, 0, 3, {128, 128, 128}); one<1, 1>(1, 1, 16, 40, 4, {500, 20, 41, 70, 90, 300}); one<1, 1>(1, 1, 16, 0, 40, {1, 2, 3});
+                 { std::vector<int32_t> many; for (int i = 0; i < 70; ++i) many.push_back(i % 9 == 4 ? 0 : 1 + i * 37 % 130); one<1, 1>(1, 1, 16, 0, 11, many); }""",
     "no_numbers": "one<2, 2>(1, 3, 16, 0, 0, {133, 5}, 0.3f, 1.f, 3); one<4, 4>(1, 2, 32, 0, 3, {300, 31}, 0.3f, 1.f, 3); one<4, 2>(1, 5, 32, 0, 0, {100}, 0.3f, 1.f, 3);",
 }
 
