@@ -772,8 +772,7 @@ def moe_route(logits, k, score="softmax", bias=None, n_groups=1, topk_groups=1, 
     if bias is not None:
         _want(bias.numel() == E, "bias: one for each expert")
         bias_ptr = _dev(bias, _F32, dev, "bias")
-    idx = torch.empty((T, k), dtype=_I32, device=logits.device)
-    w = torch.empty((T, k), dtype=_F16, device=logits.device)
+    idx, w = logits.new_empty((T, k), dtype=_I32), logits.new_empty((T, k), dtype=_F16)
     rc = lib.mx_moe_route(_stream_of(dev), logits_ptr, bias_ptr, idx.data_ptr(), w.data_ptr(), T, E, k, n_groups, topk_groups, flags, scale)
     if rc != 0:
         raise MxError("mx_moe_route", rc)
@@ -816,7 +815,7 @@ def add_rms_norm_f32w_q8(x, residual, w, eps, halves=False, want_y=True, out=Non
         total, y, q8 = out
     else:
         total, y = torch.empty_like(x), torch.empty_like(x) if want_y else None
-        q8 = torch.empty(size, dtype=torch.uint8, device=x.device)
+        q8 = x.new_empty(size, dtype=torch.uint8)
     if residual.shape != shape or total.shape != shape or w.numel() != hidden or q8.numel() != size or (y is not None and y.shape != shape):
         raise ValueError("x, residual, sum and y are [rows, hidden], w has hidden elements, q8 40 (halves: 48) bytes for each 32")
     rc = lib.mx_add_rms_norm_f32w_q8(_stream_of(dev), _dev(x, _F16, dev, "x"), _dev(residual, _F16, dev, "residual"), _dev(w, _F32, dev, "w"), _dev(total, _F16, dev, "sum"),
@@ -888,13 +887,17 @@ def _cache(cache, dev):
         if v.shape != shape or len(shape) != 4:
             raise ValueError("the planes of a cache are [pages, heads, page size, D], both of one shape")
         return (_dev(k, _F16, dev, "k"), _dev(v, _F16, dev, "v")), shape, "f16"
-    _want(len(cache) == 4 and len(shape) == 4, "a cache is (k, v) or (k_qs, k_d, v_qs, v_d), planes [pages, heads, page size, D], of Q4_0 D / 2 bytes")
-    codes, fmt, whole = (_U8, "q4_0", (*shape[:3], 2 * shape[3])) if cache[0].dtype is _U8 else (_I8, "q8_0", shape)
-    scales = shape[:3] + (whole[3] // 32,)
-    if cache[2].shape != shape or cache[1].shape != scales or cache[3].shape != scales:
+    if len(cache) != 4 or len(shape) != 4:
+        raise ValueError("a cache is (k, v) or (k_qs, k_d, v_qs, v_d), planes [pages, heads, page size, D], of Q4_0 D / 2 bytes")
+    k_qs, k_d, v_qs, v_d = cache
+    pages, heads, page_size, D = shape
+    codes, fmt = _I8, "q8_0"
+    if k_qs.dtype is _U8:
+        codes, fmt, D = _U8, "q4_0", 2 * D
+    scales = (pages, heads, page_size, D // 32)
+    if v_qs.shape != shape or k_d.shape != scales or v_d.shape != scales:
         raise ValueError("the planes of a cache have one shape, its scales one for each 32")
-    return (_dev(cache[0], codes, dev, "k_qs"), _dev(cache[1], _F16, dev, "k_d"), _dev(cache[2], codes, dev, "v_qs"),
-            _dev(cache[3], _F16, dev, "v_d")), whole, fmt
+    return (_dev(k_qs, codes, dev, "k_qs"), _dev(k_d, _F16, dev, "k_d"), _dev(v_qs, codes, dev, "v_qs"), _dev(v_d, _F16, dev, "v_d")), (pages, heads, page_size, D), fmt
 
 
 _ROPE_KV_WRITE, _KV_WRITE, _KV_READ, _ATTN_DECODE = ({fmt: getattr(lib, "mx_%s_%s" % (name, fmt)) for fmt in ("f16", "q8_0", "q4_0")}

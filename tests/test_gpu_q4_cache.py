@@ -463,7 +463,8 @@ def test_a_new_cache_takes_its_own_bytes(mx, fmt):
     torch.cuda.reset_peak_memory_stats()
     cache = mx.ops.kv_cache(fmt, 512, 8, 64, 128)
     size = sum(t.numel() * t.element_size() for t in cache)
-    assert torch.cuda.max_memory_allocated() - before == size and len({t.data_ptr() for t in cache}) == len(cache) and all((t == 0).all() for t in cache)
+    # torch's allocator may hand out a block of up to 1 MiB more for each
+    assert size <= torch.cuda.max_memory_allocated() - before <= size + (len(cache) << 20) and len({t.data_ptr() for t in cache}) == len(cache) and all((t == 0).all() for t in cache)
     with pytest.raises(ValueError):
         mx.ops.attn_decode_ws_bytes(1, 8, 8, 128, 4096, fmt="q4")
 
