@@ -83,7 +83,8 @@ __device__ __forceinline__ const half_t* row_of(const RowsArgs& a, uint32_t t, u
 // A quarter of a Q4_0 block, elements 8 l .. 8 l + 7 of its 32 in lane l = lane % 4; the four lanes call together.  d = m / -8 with m the value of largest magnitude, the first
 // of equal ones, code = min(15, floor(8 x / -m + 8.5)).  Gives the lane's dword of the block, the one at Q4Part::at, and d.
 // m is found as the largest of keys magnitude | 31 - element | sign.  A multiply-add with the reciprocal is off by less than 2^-20; 8 x / m + 8.5 is a whole number or at least 2^-13 from one (next
-// to one, 16 x is a multiple of half of m's last place, as is (2 k - 17) m), so that 2^-14 added makes every code that of the exact quotient.
+// to one, 16 x is a multiple of half of m's last place, as is (2 k - 17) m), so that 2^-14 added makes every code that of the exact quotient.  Bound by what rows and prompts are bound by in other formats: the rotated
+// rows of 2047 tokens of 32 + 4 + 4 heads of 128 10.2 us (Q8_0 10.3), one token's 2.6.
 struct Q4Part {
     uint32_t word, at;
     half_t d;
@@ -249,7 +250,7 @@ static int launch_rows(mx_stream_t s, RowsArgs a, uint32_t T, int interleaved) {
 
 // Reading back: a workgroup takes 16 tokens of one sequence (they lie in one page) and 1024 pieces of 8 elements of their keys and values, a thread four, which it
 // requests before it writes the first (4 ragged sequences of 300 tokens with 8 heads of 128, with their write: 11.8 us one after the other, 6.3; long ones run at a
-// copy's rate: 10 k tokens of them in 15.9 us, 5.1 TB/s).
+// copy's rate: 10 k tokens of them in 15.9 us, 5.1 TB/s; of Q4_0 32048 tokens of 4 heads of 128 16.2 us, 5.2 TB/s of mostly writes).
 // Tile numbers are dealt by floor(rows[b] / 16) + b, which leaves room for every sequence's ceil(length / 16).
 constexpr int kReadPieces = 4;
 template <int FMT, bool STREAM>
