@@ -655,9 +655,10 @@ struct Plan {
 };
 // Q4_0: as many as are resident, four workgroups a CU for heads of up to 64, three up to 128, two beyond, rounded down.  us by workgroups (256, 512, 768, 1024): 64 x 8192 tokens of 8 heads of 64 115, 73, 66, 59, of
 // 128 104, 105, 98, 118; 16 x 8192 of 8 heads of 256 67, 53, 75, 58; 16 x 8192 of 3 heads of 128 21.8, 18.4 (513 of them), 15.8, 20.1.
-// Where a workgroup for each sequence and group of heads leaves CUs free, it has eight waves for more than two tiles a wave of four, and for heads of up to 128 takes up to 1024 tokens: us, four waves (and their
-// parts' join) against eight, sequences of 8 heads of 128: one of 512 tokens 8.8, 8.2, of 256 6.7, 6.6; 32 of 512 9.6, 9.4, of 256 7.1, 7.4; of 1024 tokens one 6.1 + 3.4, 10.7, four 7.5 + 4.0, 11.0, 16 10.4 + 4.0, 11.6,
-// 32 16.9 + 4.0, 12.4; of 8 heads of 256 one of 512 11.9, 10.8, of 1024 7.7 + 3.8, 15.0.  More workgroups than CUs wait: 48 of 512 11.4, 15.7.
+// A workgroup for each sequence and group of heads takes up to 1024 tokens, or 512 where wide heads' workgroups would leave CUs free: us, in parts with their join against it, ragged sequences of up to 1000 tokens of 8 heads of
+// 128, 64 of them 16.6 + 4.1, 16.2; 400 56.3 + 4.8, 53.6; of 1024 tokens 64 20.6 + 4.2, 16.9; 200 45.8 + 4.2, 49.3; one of 8 heads of 256 7.6 + 4.0, 15.0; ragged ones of up to 2000 tokens 40 16.0 + 4.0, 23.1; 200 46.1 + 4.2, 51.6.
+// Where it leaves CUs free it has eight waves for more than two tiles a wave of four: us, four (in parts, for more than 512 tokens) against eight, sequences of 8 heads of 128: one of 512 tokens 8.2, 7.6; 32 of 512 9.0, 8.2,
+// of 256 6.7, 7.4; of 1024 tokens one 6.2 + 4.0, 10.0, four 7.8 + 4.0, 10.2, 16 9.9 + 4.0, 10.8, 32 15.0 + 4.0, 11.2; one of 512 of 8 heads of 256 11.4, 10.1.  More workgroups than CUs wait: 48 of 512 10.7, 15.7.
 enum { kF16 = 0, kQ8 = 1, kQ4 = 2 };   // what a cache holds
 constexpr uint32_t kDirectTiles = 4 * kWaves;
 constexpr int kWide = 8;
@@ -665,8 +666,8 @@ static Plan plan_of(int fmt, uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, 
     const uint32_t span = window && window < max_len ? window : max_len;
     const uint64_t tiles = window && window < max_len ? span / kTile + 2 : (span + (uint64_t)kTile - 1) / kTile, all = B * tiles;   // a window may begin within a tile
     const uint64_t groups = (uint64_t)Hkv * ((Hq / Hkv + 15) / 16);
-    const bool wide = fmt == kQ4 && B * groups <= 256 && tiles > 2 * kWaves && tiles <= (D > 128 ? kDirectTiles : 4 * kWide);
-    if (wide || tiles <= kDirectTiles) return {0, 0, wide};
+    const bool few = B * groups <= 256, direct = fmt == kQ4 && (D <= 128 || !few) ? tiles <= 2 * kDirectTiles : tiles <= kDirectTiles;
+    if (direct) return {0, 0, fmt == kQ4 && few && tiles > 2 * kWaves};
     auto up = [](uint64_t x, uint64_t y) { return (x + y - 1) / y; };
     uint64_t most = up(all, kLeastShare);
     if (most * groups > 128) most = up(all, 2 * kLeastShare) > up(128, groups) ? up(all, 2 * kLeastShare) : up(128, groups);
@@ -708,7 +709,7 @@ struct Int {
     static constexpr int value = N;
 };
 
-template <int NB, int C, int W = kWaves>
+template <int NB, int C, int W, bool SHARED>
 __global__ __launch_bounds__(W * 64, W > (int)kWaves ? 2 : NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void attn_decode_q4_kernel(AttnArgs a) {
     constexpr uint32_t D = 32 * NB, GP = 16 / C;
     // LDS of a token's codes: an odd number of 16-byte pieces, so that 16 rows meet all banks; the second half of a tile lies four rows further, for the keys' rows 0 .. 3, 8 .. 11, 16 .. 19, 24 .. 27
@@ -722,7 +723,6 @@ __global__ __launch_bounds__(W * 64, W > (int)kWaves ? 2 : NB <= 2 ? 4 : NB <= 4
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15u, g = lane >> 4;
     const uint32_t G = a.Hq / a.Hkv, tiles_of_heads = (G + 15) / 16;
     const uint32_t hk = blockIdx.y / tiles_of_heads, head0 = (blockIdx.y - hk * tiles_of_heads) * 16, heads = min(16u, G - head0);
-    const bool shared = a.shares != 0;
     const uint32_t share = blockIdx.x;
     char* const keys = reinterpret_cast<char*>(lds) + wave * WAVE;
     char* const values = keys + CODES;
@@ -740,16 +740,38 @@ __global__ __launch_bounds__(W * 64, W > (int)kWaves ? 2 : NB <= 2 ? 4 : NB <= 4
     // bytes 0 1 2 3 of a word of the transposing read are tokens 0 2 1 3 of four places, so that an `and` leaves two consecutive ones; lane r of 16 brings 8 bytes of row r / 2
 #pragma unroll
     for (int k = 0; k < R; ++k) value_at[k] = (8 * g + 2 * (((r >> 2 & 2u) + (r >> 1 & 1u) + k * PS) & 3u) + (r >> 2 & 1u)) * ROW + (g >> 1) * (HALF - 16 * ROW) + (r & 1u) * 8;
+    typedef const __attribute__((address_space(4))) int32_t* table_t;
+    struct Ref {             // a tile's first token and, for its two halves, page and place in the page
+        uint32_t token, page[2], off[2];
+    };
+    auto page_of = [&](uint32_t t) { return a.page_shift < 32 ? t >> a.page_shift : t / a.page_size; };
+    auto locate = [&](uint32_t b, uint32_t tile) {
+        const table_t table = (table_t)(uintptr_t)(a.table + (size_t)b * a.max_pages);
+        Ref f;
+        f.token = tile * kTile;
+        const uint32_t c0 = page_of(f.token), o0 = f.token - c0 * a.page_size;
+        const bool next = o0 + 16 >= a.page_size;
+        f.off[0] = o0;
+        f.off[1] = next ? 0 : o0 + 16;
+        f.page[0] = (uint32_t)table[min(c0, a.max_pages - 1)];
+        f.page[1] = (uint32_t)table[min(next ? c0 + 1 : c0, a.max_pages - 1)];
+        return f;
+    };
     Weighed sh = {1, 1, blockIdx.x, 0, 0, 0};
-    if (shared) sh = weighed_share(a, share, lane);
-    else sh.len = a.lens[sh.b];
+    Ref early = {};          // without a window the first tile's page is asked for together with the length: 128 tokens 5.6 -> 5.2 us
+    if (SHARED) {
+        sh = weighed_share(a, share, lane);
+    } else {
+        sh.len = a.lens[sh.b];
+        early = locate(sh.b, wave);
+    }
     uint32_t b = sh.b, at = sh.from, left = sh.left;
     int32_t len = __builtin_amdgcn_readfirstlane(sh.len);
     for (; left; len = __builtin_amdgcn_readfirstlane(left ? a.lens[b + 1] : 0), ++b) {
     const Span sp = span_of(a, len);
     uint32_t first = 0, last = sp.tiles;
     const uint32_t done = sh.per - left;
-    if (shared) {
+    if (SHARED) {
         if (sp.tiles == 0) continue;
         const uint32_t to = min(sp.tiles + sh.extra, at + left);
         left -= to - at;
@@ -765,23 +787,6 @@ __global__ __launch_bounds__(W * 64, W > (int)kWaves ? 2 : NB <= 2 ? 4 : NB <= 4
     const bool whole = first == 0 && last == sp.tiles;     // the result itself, not a part of it
     const size_t out0 = ((size_t)b * a.Hq + hk * G + head0) * D;
 
-    typedef const __attribute__((address_space(4))) int32_t* table_t;
-    const table_t table = (table_t)(uintptr_t)(a.table + (size_t)b * a.max_pages);
-    struct Ref {             // a tile's first token and, for its two halves, page and place in the page
-        uint32_t token, page[2], off[2];
-    };
-    auto page_of = [&](uint32_t t) { return a.page_shift < 32 ? t >> a.page_shift : t / a.page_size; };
-    auto locate = [&](uint32_t tile) {
-        Ref f;
-        f.token = (sp.tile0 + tile) * kTile;
-        const uint32_t c0 = page_of(f.token), o0 = f.token - c0 * a.page_size;
-        const bool next = o0 + 16 >= a.page_size;
-        f.off[0] = o0;
-        f.off[1] = next ? 0 : o0 + 16;
-        f.page[0] = (uint32_t)table[c0];                          // c0 < max_pages: the tile's first token is in front of the sequence's end
-        f.page[1] = (uint32_t)table[min(next ? c0 + 1 : c0, a.max_pages - 1)];
-        return f;
-    };
     auto row_of = [&](const Ref& f, int h) { return ((size_t)(f.page[h] < a.n_pages ? f.page[h] : 0u) * a.Hkv + hk) * a.page_size + f.off[h]; };
 
     uint4 kr[LP], vr[LP];
@@ -852,9 +857,11 @@ __global__ __launch_bounds__(W * 64, W > (int)kWaves ? 2 : NB <= 2 ? 4 : NB <= 4
         }
     }
     uint32_t tile = first + wave;
-    Ref cur = locate(tile), next = cur;
+    Ref cur = early, next;
+    if (SHARED || a.window) cur = locate(b, sp.tile0 + tile);
+    next = cur;
     load(cur);
-    if (tile + W < last) next = locate(tile + W);
+    if (tile + W < last) next = locate(b, sp.tile0 + tile + W);
     half8 qf[NB];
     float off[S];
     float unit;              // of the scores
@@ -1038,7 +1045,7 @@ __global__ __launch_bounds__(W * 64, W > (int)kWaves ? 2 : NB <= 2 ? 4 : NB <= 4
         }
         if (more) {
             cur = next;
-            if (tile + 2 * W < last) next = locate(tile + 2 * W);
+            if (tile + 2 * W < last) next = locate(b, sp.tile0 + tile + 2 * W);
         }
     }
     }
@@ -1098,19 +1105,20 @@ __global__ __launch_bounds__(W * 64, W > (int)kWaves ? 2 : NB <= 2 ? 4 : NB <= 4
 }
 
 // ---------------------------------------------------------------- launches
-template <int NB, int C, int W>
-static int launch_q4_waves(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads) {
+template <int NB, int C, int W, bool SHARED>
+static int launch_q4_form(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads) {
     static LdsLimit limit;
     constexpr uint32_t tiles = W * (2 * 36 * 16 * (NB | 1) + kTile * (2 * NB + 1) * 2), most = W * (32 + 16 / C * (32 * NB + 4)) * 4;
     const uint32_t sums = W * (32 + heads * (32 * NB + 4)) * 4, lds = tiles > sums ? tiles : sums;
     if (lds > kLdsDefaultLimit)
-        if (int rc = raise_lds_limit(reinterpret_cast<const void*>(attn_decode_q4_kernel<NB, C, W>), limit, tiles > most ? tiles : most)) return rc;
-    hipLaunchKernelGGL((attn_decode_q4_kernel<NB, C, W>), grid, dim3(W * 64), lds, as_stream(s), a);
+        if (int rc = raise_lds_limit(reinterpret_cast<const void*>(attn_decode_q4_kernel<NB, C, W, SHARED>), limit, tiles > most ? tiles : most)) return rc;
+    hipLaunchKernelGGL((attn_decode_q4_kernel<NB, C, W, SHARED>), grid, dim3(W * 64), lds, as_stream(s), a);
     return launch_status();
 }
 template <int NB, int C>
 static int launch_q4(mx_stream_t s, const AttnArgs& a, dim3 grid, uint32_t heads, bool wide) {
-    return wide ? launch_q4_waves<NB, C, kWide>(s, a, grid, heads) : launch_q4_waves<NB, C, kWaves>(s, a, grid, heads);
+    if (a.shares) return launch_q4_form<NB, C, kWaves, true>(s, a, grid, heads);
+    return wide ? launch_q4_form<NB, C, kWide, false>(s, a, grid, heads) : launch_q4_form<NB, C, kWaves, false>(s, a, grid, heads);
 }
 // As many column groups as the heads leave room for and the blocks can use.
 template <int NB>

@@ -151,9 +151,11 @@ LENS = {"one": [1], "edges": [0, 1, 15, 16, 17, 31, 32, 33, 47, 48, 63, 64, 65, 
 def test_attn_decode(mx, lens, Hkv, G, D, ps):
     lens = LENS[lens]
     rng, table, cache, q = case(lens, Hkv, G, D, ps, 100 + D + len(lens))
-    y = attend(mx, q, cache, table, lens)
-    near(host(y), *Q.attention(q, cache, table, lens, ps, D ** -0.5), "attention")
-    assert (host(y)[np.array(lens) == 0] == 0).all()
+    want, tol = Q.attention(q, cache, table, lens, ps, D ** -0.5)
+    for max_len in (None, 1 << 20):          # the longest of them, and a length that asks for parts
+        y = attend(mx, q, cache, table, lens, max_len=max_len)
+        near(host(y), want, tol, "max_len %s" % max_len)
+        assert (host(y)[np.array(lens) == 0] == 0).all()
 
 
 @pytest.mark.parametrize("D", [32, 64, 96, 128, 160, 192, 224, 256])
@@ -161,7 +163,9 @@ def test_attn_decode(mx, lens, Hkv, G, D, ps):
 def test_every_width_of_head(mx, D, G):
     lens = [130, 0, 19, 1, 800]
     rng, table, cache, q = case(lens, 2, G, D, 16, D + G)
-    near(host(attend(mx, q, cache, table, lens)), *Q.attention(q, cache, table, lens, 16, D ** -0.5), "D=%d G=%d" % (D, G))
+    want, tol = Q.attention(q, cache, table, lens, 16, D ** -0.5)
+    for max_len in (None, 1 << 20):          # whole, in parts
+        near(host(attend(mx, q, cache, table, lens, max_len=max_len)), want, tol, "D=%d G=%d max_len %s" % (D, G, max_len))
 
 
 @pytest.mark.parametrize("D", [32, 64, 96, 128, 160, 192, 224, 256])

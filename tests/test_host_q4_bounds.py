@@ -77,7 +77,7 @@ template <int NB, int C, int W = kWaves> static void one(uint32_t Hkv, uint32_t 
     a.scale = scale * kLog2e;
     const uint32_t heads = std::min(G, 16u);
     const size_t tiles = W * (2 * 36 * 16 * (NB | 1) + kTile * (2 * NB + 1) * 2), sums = W * (32 + heads * (D + 4)) * 4;   // as the launch asks for
-    run(W * 64, shares ? shares : B, Hkv * ((G + 15) / 16), std::max(tiles, sums), [&] { attn_decode_q4_kernel<NB, C, W>(a); });
+    run(W * 64, shares ? shares : B, Hkv * ((G + 15) / 16), std::max(tiles, sums), [&] { if (shares) attn_decode_q4_kernel<NB, C, W, true>(a); else attn_decode_q4_kernel<NB, C, W, false>(a); });
     if (shares) {
         uint32_t groups = std::min((shares / B + 4) / 4, 512 / (D / 4));
         run((groups * (D / 4) + 63) / 64 * 64, B * Hq, 1, groups * D * 4, [&] { attn_join_kernel(a, groups); });
