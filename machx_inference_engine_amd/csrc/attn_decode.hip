@@ -696,7 +696,7 @@ static Plan plan_of(int fmt, uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, 
 //   * p d must stay in fp16's range: the largest weight is 2^(15 - k), 2^k above every scale that this wave has met (k > 0 only for values beyond 8).
 // Precision as above: p d is held to 2^-22, or 2^-39 + k of the largest weight's; what the offsets cancel in the fp32 sums is at most 15 / 8 of the values' own size.
 // Large caches are bound by memory, with the vector pipe busy half and the matrix pipe a quarter of the time: 64 x 8192 tokens of 8 heads of 128, 605 MB, 96 to 99 us, 6.1 to 6.3 TB/s; one sequence of 131071, 151 MB, 29.2. Small ones by what
-// is waited for in turn: launch, length, page, tile and the waves' sums are 5.6 us, each further tile of a wave 1.1 (2.2 where three workgroups share a CU).  Requests two and four tiles ahead gain nothing.
+// is waited for in turn: launch, length and page, tile and the waves' sums are 5.2 us, each further tile of a wave 1.0 (2.2 where three workgroups share a CU).  Requests two and four tiles ahead gain nothing.
 
 // Eight codes' operand: the low or high codes (mask 0x000f000f, 0x00f000f0) of the bytes of two words, even bytes of a word in front of its odd ones.
 __device__ __forceinline__ half8 codes_f16(uint32_t a, uint32_t b, uint32_t mask) {
