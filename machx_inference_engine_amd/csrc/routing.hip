@@ -431,14 +431,14 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             taken[j] |= hit[j];
-            high[j] = hit[j] >> lane & 1ull ? 0u : high[j];
+            high[j] = __builtin_amdgcn_inverse_ballot_w64(hit[j]) ? 0u : high[j];
         }
     }
     double factor = (double)a.scale;
     if (a.flags & MX_ROUTE_RENORM) {
         double sum = 0.0;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) sum += taken[j] >> lane & 1ull ? score[j] : 0.0;
+        for (int j = 0; j < NJ; ++j) sum += __builtin_amdgcn_inverse_ballot_w64(taken[j]) ? score[j] : 0.0;
         factor /= wave_sum_f64(sum) + 1e-20;
     }
     uint32_t at = 0;         // chosen experts of lower lanes
@@ -446,7 +446,7 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
     for (int j = 0; j < NJ; ++j) at = (uint32_t)__builtin_amdgcn_mbcnt_hi((uint32_t)(taken[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)taken[j], at));
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
-        if (taken[j] >> lane & 1ull) {
+        if (__builtin_amdgcn_inverse_ballot_w64(taken[j])) {
             a.topk_idx[(size_t)t * a.K + at] = (int32_t)(e0 + j);
             a.topk_w[(size_t)t * a.K + at] = (half_t)(score[j] * factor);
             ++at;

@@ -10,6 +10,7 @@ template <class T> static T __shfl(T v, int l) { return from_lane(v, 9, 64, l & 
 template <class T> static T __shfl_xor(T v, int m) { return from_lane(v, 9, 64, lane_id() ^ m); }
 #define __builtin_amdgcn_mbcnt_lo(m, c) ((uint32_t)__builtin_popcount((m) & (lane_id() < 32 ? (1u << lane_id()) - 1u : 0xFFFFFFFFu)) + (c))
 #define __builtin_amdgcn_mbcnt_hi(m, c) ((uint32_t)__builtin_popcount((m) & (lane_id() < 32 ? 0u : (1u << (lane_id() - 32)) - 1u)) + (c))
+#define __builtin_amdgcn_inverse_ballot_w64(m) (((uint64_t)(m) >> lane_id() & 1ull) != 0)
 static uint32_t __umulhi(uint32_t a, uint32_t b) { return (uint32_t)((uint64_t)a * b >> 32); }
 // sixteen lanes bring the halves of eight rows of 16 bytes; lane r gets byte r of each
 template <class V> static V shim_tr8(V* p) {
