@@ -1,4 +1,6 @@
 """GPU: the Q4_0 key-value cache, written with and without rotation and read back, and the attention of one token over it, against plain forms in 64 bits."""
+import gc
+
 import numpy as np
 import pytest
 import torch
@@ -462,6 +464,7 @@ def test_refusals(mx):
 
 @pytest.mark.parametrize("fmt", ["f16", "q8_0", "q4_0"])
 def test_a_new_cache_takes_its_own_bytes(mx, fmt):
+    gc.collect()
     torch.cuda.synchronize()
     before = torch.cuda.memory_allocated()
     torch.cuda.reset_peak_memory_stats()
