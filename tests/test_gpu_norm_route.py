@@ -65,6 +65,18 @@ def test_rows_without_numbers_leave_others_alone(mx):
     assert np.isinf(h[3, 200]) and np.isinf(h[4, 0]) and np.isnan(y[3, 200]) and (np.delete(y[3], 200) == 0).all()
 
 
+def test_norm_offsets_beyond_32_bits(mx):
+    H, T = 8192, (1 << 32) // 8192 + 3
+    x, res, w = torch.zeros(T, H, dtype=torch.float16, device="cuda"), torch.ones(T, H, dtype=torch.float16, device="cuda"), torch.ones(H, device="cuda")
+    rng = np.random.default_rng(3)
+    at = torch.tensor([0, 1, T - 4, T - 1], device="cuda")
+    x[at], res[at] = dev(f16(rng, 4, H)), dev(f16(rng, 4, H))
+    want = mx.ops.add_rms_norm_f32w_q8(x[at], res[at], w, 1e-5, want_y=False)
+    q8 = torch.empty(T * (H // 32) * 40, dtype=torch.uint8, device="cuda")
+    mx.ops.add_rms_norm_f32w_q8(x, res, w, 1e-5, out=(res, None, q8))
+    assert torch.equal(res[at], want[0]) and torch.equal(q8.view(T, -1)[at], want[2].view(4, -1)) and (res[T - 2] == 1).all()
+
+
 def test_norm_refusals(mx):
     x, w = torch.zeros(4, 64, dtype=torch.float16, device="cuda"), torch.ones(64, device="cuda")
     fn = mx.ops.add_rms_norm_f32w_q8
@@ -214,6 +226,16 @@ def test_route_captured(mx):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(i, idx) and torch.equal(v, w)
+
+
+def test_route_offsets_beyond_32_bits(mx):
+    T, E = (1 << 32) // 1024 + 5, 1024
+    logits = torch.zeros(T, E, dtype=torch.float16, device="cuda")
+    at = torch.tensor([0, 7, T - 5, T - 2, T - 1], device="cuda")
+    logits[at] = dev(np.random.default_rng(4).standard_normal((5, E)).astype(np.float16))
+    idx, w = mx.ops.moe_route(logits, 8, n_groups=8, topk_groups=2)
+    want = mx.ops.moe_route(logits[at], 8, n_groups=8, topk_groups=2)
+    assert torch.equal(idx[at], want[0]) and torch.equal(w[at], want[1]) and torch.equal(idx[T - 3], torch.arange(8, dtype=torch.int32, device="cuda"))
 
 
 def test_route_refusals(mx):
