@@ -48,18 +48,23 @@ __global__ __launch_bounds__(kNormThreads) void norm_q8_kernel(const XT* x, cons
         const bool live = i < hidden;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
         if (live) {
+            float o[4];
             half_t h4[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float o;
                 if (GATED) {
                     const float xn = load_act(xr + i + j) * r;
                     const float gz = (float)z[(size_t)row * hidden + i + j];
-                    o = ((float)w[i + j] * xn) * (gz / (1.f + __expf(-gz)));
+                    o[j] = ((float)w[i + j] * xn) * (gz / (1.f + __expf(-gz)));
                 } else {
-                    o = (load_act(xr + i + j) * r) * (float)w[i + j];
+                    o[j] = (load_act(xr + i + j) * r) * (float)w[i + j];
                 }
-                h4[j] = (half_t)o;
+            }
+            // the stream goes by what is stored: without this the compiler rounds a product to fp32 and then to fp16 for the row, at once to fp16 for the stream
+            asm("" : "+v"(o[0]), "+v"(o[1]), "+v"(o[2]), "+v"(o[3]));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                h4[j] = (half_t)o[j];
                 v[j] = (float)h4[j];
             }
             *reinterpret_cast<uint2*>(yr + i) = *reinterpret_cast<const uint2*>(h4);
