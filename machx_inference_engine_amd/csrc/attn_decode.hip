@@ -831,8 +831,10 @@ __global__ __launch_bounds__(W * 64, W > (int)kWaves ? 2 : NB <= 2 ? 4 : NB <= 4
                     return n * kTile + (t & 24u) + (((t >> 1) - turn_of(n)) & 3u) * 2 + (t & 1u);
                 };
                 const uint32_t p0 = place(2 * w), p1 = place(2 * w + 1);
-                reinterpret_cast<uint16_t*>(k_scales)[p0] = (uint16_t)ks[i];
-                reinterpret_cast<uint16_t*>(k_scales)[p1] = (uint16_t)(ks[i] >> 16);
+                // an infinity becomes a NaN: a score of -infinity would leave its token out
+                const uint32_t kd = ks[i] | (((ks[i] & 0x7C007C00u) + 0x04000400u) & 0x80008000u) >> 6;
+                reinterpret_cast<uint16_t*>(k_scales)[p0] = (uint16_t)kd;
+                reinterpret_cast<uint16_t*>(k_scales)[p1] = (uint16_t)(kd >> 16);
                 reinterpret_cast<uint16_t*>(v_scales)[p0] = (uint16_t)vs[i];
                 reinterpret_cast<uint16_t*>(v_scales)[p1] = (uint16_t)(vs[i] >> 16);
             }
