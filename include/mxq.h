@@ -712,7 +712,7 @@ int mx_swiglu_oai_q8(mx_stream_t s, const uint16_t* gate, const uint16_t* up, ui
  * 65504, fp16's largest number, is stored as 127 * 516: it reads back as an infinity, and attention weighs it as 65532.  Scales written elsewhere may be as large as that, 516.  n_pages * page_size < 2^31; offsets into a plane take 64 bits.
  * Or of Q4_0 planes (D % 32 == 0), [Hkv][page_size][D / 2] bytes and scales as Q8_0's: of a block of 32 the weight format's 16 bytes, elements j and j + 16 in the low and high half of byte j, value = d * (code - 8),
  * d = fp16(m / -8) with m the value of largest magnitude, the first of equal ones, code = min(15, floor(8 x / -m + 8.5)) of the exact quotient.  A block of a NaN or an infinity reads back as NaN.  Any scale
- * may stand in a plane that was written elsewhere; one that is no number makes its block NaN.
+ * may stand in a plane that was written elsewhere; one that is no number, an infinity too, makes its block NaN (in attention a block of keys: the heads that read it).
  *
  * All row pointers and planes 16-byte aligned, strides multiples of 8.  What one launch cannot hold (2^32 threads) is refused: never T < 2^22 with
  * T * D * (all heads, key and value heads too) < 2^34, nor total_rows / 16 + B < 2^24.

@@ -317,10 +317,12 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const void* k_cache, const
         if (!live[u]) continue;
         half8 y = __builtin_bit_cast(half8, got[u]);
         if (FMT != kF16) {
+            // a scale that is no number makes its block NaN, an infinite one too
+            const float scale = FMT == kQ4 && !(fabsf((float)d[u]) <= 65504.f) ? NAN : (float)d[u];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const uint32_t code = (j < 4 ? got[u].x : got[u].y) >> (8 * (j & 3));
-                y[j] = f32_to_f16_rne((FMT == kQ8 ? (float)(int8_t)code : (float)(int)(code & 15u) - 8.f) * (float)d[u]);
+                y[j] = f32_to_f16_rne((FMT == kQ8 ? (float)(int8_t)code : (float)(int)(code & 15u) - 8.f) * scale);
             }
         }
         half8* const out = reinterpret_cast<half8*>((is_v[u] ? v_out : k_out) + (size_t)(row0 + t0) * Hkv * D) + at[u];

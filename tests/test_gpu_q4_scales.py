@@ -30,3 +30,27 @@ def test_infinite_scales_of_keys(mx, D, G, sign):
         # outside the window it is not read
         win = host(attend(mx, q, c, table, lens, max_len=most, window=30))
         assert np.isfinite(win[[0, 2]]).all() and np.isnan(win[[1, 3]]).all()
+
+
+@pytest.mark.parametrize("T", [70, 20000])
+def test_reading_back(mx, T):
+    """A block whose scale is infinite or NaN reads back as NaN whole, its neighbours as they are; the largest number that a scale may be gives infinities, and zeros where codes are 8."""
+    rng = np.random.default_rng(T)
+    n_pages, Hkv, D = -(-T // 16), 4, 128
+    cache = Q.random_cache(rng, n_pages, Hkv, 16, D)
+    table, ends = dev(rng.permutation(n_pages).astype(np.int32)[None]), dev(np.array([0, T], np.int32))
+    want = mx.ops.kv_read(cache, table, ends, T)
+    odd = [float("inf"), -float("inf"), float("nan"), 65504.0]
+    at = torch.from_numpy(rng.integers(0, 40, tuple(cache[1].shape))).cuda()
+    for d in (cache[1], cache[3]):
+        for i, x in enumerate(odd):
+            d[at == i] = x
+    got = mx.ops.kv_read(cache, table, ends, T)
+    t = torch.arange(T, device="cuda")
+    page = table[0].long()[t // 16]
+    of = at[page, :, t % 16].repeat_interleave(32, -1)                 # [T, Hkv, D]: what stands in an element's scale
+    for w, g, codes in zip(want, got, cache[::2]):
+        assert torch.equal(g[of > 3], w[of > 3]) and g[of < 3].isnan().all()
+        c = codes[page, :, t % 16].unflatten(-1, (-1, 16))
+        c = torch.cat((c & 15, c >> 4), -1).flatten(-2).float() - 8
+        assert torch.equal(g[of == 3], (c * 65504.0).half()[of == 3])

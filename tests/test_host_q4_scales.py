@@ -23,3 +23,15 @@ KEY_CASES = """one<2, 2>(1, 3, 16, 0, 0, {33, 5, 1, 0, 16}, 0.3f, 1.f, 4); one<4
 
 def test_keys(tmp_path):
     B.build_and_run(tmp_path, B.SHIM + Q.MORE + Q.attention_source() + B.CHECK + KEYS.replace("CASES", KEY_CASES))
+
+
+READ = replaced(replaced(replaced(Q.CACHE, "    memset(ko.p, 0xFF, ko.n);", """    for (size_t i = 0; i < values / 32; i += 1 + rnd(5)) (rnd(2) ? kd : vd).as<half_t>()[i] = (half_t)(rnd(3) ? rnd(2) ? INFINITY : -INFINITY : rnd(2) ? NAN : 65504.f);
+    memset(ko.p, 0xFF, ko.n);"""), "                    if ((float)want !=", """                    const float d = (float)(side ? vd : kd).as<half_t>()[r * (D / 32) + e / 32], got = (float)(side ? vo : ko).as<half_t>()[dst];
+                    if (std::isnan(d) || std::isinf(d)) { if (!std::isnan(got)) wrong("a number of a block that has none: "); continue; }
+                    if ((float)want !="""), "static void cache(uint32_t T", "[[maybe_unused]] static void cache(uint32_t T")
+
+
+def test_reading_back(tmp_path):
+    source = B.source("kv_cache.hip", "// ---------------------------------------------------------------- argument checks")
+    source = source.replace("constexpr uint32_t kPromptTokens", "#if 0\nconstexpr uint32_t kPromptTokens").replace("// Reading back: a workgroup", "#endif\n// Reading back: a workgroup")
+    B.build_and_run(tmp_path, B.SHIM + Q.MORE + source + B.CHECK + READ.replace("READ_LAUNCH", Q.READ_LAUNCH))
