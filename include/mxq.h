@@ -658,7 +658,7 @@ int mx_moe_topk_from_logits(mx_stream_t s, const uint16_t* logits, int32_t* topk
  *     topk_w = half(scale * s / (sum of the chosen s + 1e-20)) with MX_ROUTE_RENORM, half(scale * s) without; the bias is no part of it.
  *     Scores, worths and comparisons are 64 bits, and what agrees in these is equal (two logits beyond 37 by their sigmoids); weights are rounded once.
  *     An expert of logit -infinity has score 0 (a softmax over nothing else: all scores 0).  A c that is NaN lies below every number, and is then taken by id; so does a group with one for its worth.
- *     n_experts <= 1024, k <= 64, n_experts % n_groups == 0, n_groups <= 64, 1 <= topk_groups <= n_groups, k <= topk_groups * n_experts / n_groups, n_tokens < 2^26.
+ *     n_experts <= 1024, k <= 64, n_experts % n_groups == 0, n_groups <= 64, 1 <= topk_groups <= n_groups, k <= topk_groups * n_experts / n_groups, n_tokens <= 2^26 - 4.
  *     MX_ROUTE_TOP2 over groups of one expert: its c.  A token's result is the same bits in every call.  */
 enum { MX_ROUTE_SIGMOID = 1, MX_ROUTE_RENORM = 2, MX_ROUTE_TOP2 = 4, MX_ROUTE_F32 = 8 };
 int mx_moe_router_logits(mx_stream_t s, const uint16_t* x, const float* W_gate, float* logits, uint32_t n_tokens, uint32_t hidden, uint32_t n_experts);

@@ -626,7 +626,8 @@ int mx_moe_router_logits(mx_stream_t s, const uint16_t* x, const float* W_gate, 
 int mx_moe_route(mx_stream_t s, const void* logits, const float* bias, int32_t* topk_idx, uint16_t* topk_w, uint32_t n_tokens, uint32_t n_experts, uint32_t k,
                  uint32_t n_groups, uint32_t topk_groups, uint32_t flags, float scale) {
     MX_REQUIRE_PTR(logits); MX_REQUIRE_PTR(topk_idx); MX_REQUIRE_PTR(topk_w);
-    MX_REQUIRE_SHAPE(n_tokens > 0 && n_tokens < (1u << 26) && n_experts > 0 && n_experts <= 1024 && n_groups > 0 && n_groups <= 64 && n_experts % n_groups == 0);
+    // four tokens a workgroup of 256 threads, and a launch holds fewer than 2^32
+    MX_REQUIRE_SHAPE(n_tokens > 0 && n_tokens <= (1u << 26) - 4 && n_experts > 0 && n_experts <= 1024 && n_groups > 0 && n_groups <= 64 && n_experts % n_groups == 0);
     const uint32_t size = n_experts / n_groups;
     MX_REQUIRE_SHAPE(topk_groups > 0 && topk_groups <= n_groups && k > 0 && k <= (uint32_t)kMaxTopK && k <= topk_groups * size && flags < 16u);
     MX_REQUIRE_ALIGN(logits, flags & MX_ROUTE_F32 ? 4 : 2); MX_REQUIRE_ALIGN(bias, 4); MX_REQUIRE_ALIGN(topk_idx, 4); MX_REQUIRE_ALIGN(topk_w, 2);
