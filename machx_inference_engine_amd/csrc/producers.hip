@@ -291,7 +291,12 @@ int mx_add_rms_norm_f32w_q8(mx_stream_t s, const uint16_t* x, const uint16_t* re
         if (hidden <= 256) return launch(add_norm_short_kernel<32, H>, (n_rows + 7) / 8, 256, 0);
         if (hidden <= 512) return launch(add_norm_short_kernel<64, H>, (n_rows + 3) / 4, 256, 0);
         const uint32_t threads = kSumThreads * at_once;
-        return hidden <= kSumLds ? launch(add_norm_kernel<H, false>, n_rows, threads, passes * kSumThreads * 16) : launch(add_norm_kernel<H, true>, n_rows, threads, 0);
+        if (hidden > kSumLds) return launch(add_norm_kernel<H, true>, n_rows, threads, 0);
+        static LdsLimit limit;
+        const uint32_t lds = passes * kSumThreads * 16;
+        if (lds + kSumThreads / 32 * sizeof(float) > kLdsDefaultLimit)       // with the kernel's own
+            if (int rc = raise_lds_limit(reinterpret_cast<const void*>(add_norm_kernel<H, false>), limit, lds)) return rc;
+        return launch(add_norm_kernel<H, false>, n_rows, threads, lds);
     };
     return halves ? form(Bool<true>()) : form(Bool<false>());
 }
