@@ -747,11 +747,15 @@ def moe_topk_from_logits(logits, k):
 
 def moe_router_logits(x, W_gate):
     """x fp16 [T, H], W_gate fp32 [E, H] -> fp32 [T, E], the logits that moe_router goes by."""
+    dev = _current_device()
     T, H = x.shape
     E = W_gate.shape[0]
-    _want(W_gate.dtype is _F32 and W_gate.shape == (E, H), "W_gate is fp32 [experts, H]")
-    logits = torch.empty((T, E), dtype=_F32, device=x.device)
-    _call("mx_moe_router_logits", _f16(x), _ptr(W_gate), _ptr(logits), T, H, E)
+    _want(W_gate.shape == (E, H), "W_gate is fp32 [experts, H]")
+    x_ptr, gate_ptr = _dev(x, _F16, dev, "x"), _dev(W_gate, _F32, dev, "W_gate")
+    logits = x.new_empty((T, E), dtype=_F32)
+    rc = lib.mx_moe_router_logits(_stream_of(dev), x_ptr, gate_ptr, logits.data_ptr(), T, H, E)
+    if rc != 0:
+        raise MxError("mx_moe_router_logits", rc)
     return logits
 
 
