@@ -96,10 +96,16 @@ __device__ __forceinline__ Share share_of(const AttnArgs& a, uint32_t share, uin
     return s;
 }
 
-// The same, where each sequence but one costs as much as `extra` tiles more (its queries, first loads and sums): these stand in front of its tiles, so that a share that holds many ends of sequences has fewer
-// tiles.  Not where every share would lie within one sequence without them.  us without them and with 4, 8 (half a share of tiles at most), 12 and 16 (a share at most), ragged sequences of 8 heads of 128: 17 of up to 4000 tokens
-// 16.1, 15.4, 14.6, 14.0, 14.5; 43 of 4000 27.4, 26.0, 24.2, 23.3, 24.1; 100 of 1000 24.9, 21.8, 21.5, 20.8, 21.0; 200 of 3000 70.6, 65.4, 64.6, 64.2, 65.8; equal ones, 64 of 8192 99.0, 97.7, 96.8, 95.9, 97.0, 32 of 2048
-// 20.7, 20.4, 18.0, 19.8; 48 of 1024, which lie within one sequence, 15.7, 17.0, 17.4, 18.6; 16 of 8192 of 8 heads of 256 51.7, 52.6, 54.0, 53.6.
+// The same, where each sequence but one costs as much as `extra` tiles more (its queries, first loads and sums): these stand in front of its tiles, so that a share that holds many ends of sequences
+// has fewer tiles.  12, and no more than a share has; none where every share would lie within one sequence without them.
+// us by extra tiles, 8 heads of 128 unless said:       0     4     8    12    16
+//   ragged,  17 of up to 4000 tokens                16.1  15.4  14.6  14.0  14.5
+//            43 of 4000                             27.4  26.0  24.2  23.3  24.1
+//            100 of 1000                            24.9  21.8  21.5  20.8  21.0
+//            200 of 3000                            70.6  65.4  64.6  64.2  65.8
+//   equal,   64 of 8192                             99.0  97.7  96.8  95.9  97.0
+// (of 8: half a share's tiles at most).  Four of the numbers, from none upward: 32 of 2048 20.7, 20.4, 18.0, 19.8; 48 of 1024, which lie within one sequence, 15.7, 17.0, 17.4, 18.6; 16 of 8192 of
+// 8 heads of 256 51.7, 52.6, 54.0, 53.6.
 struct Weighed {
     uint32_t per, left, b, from, extra;   // per, left and from with the extra tiles
     int32_t len;
@@ -653,12 +659,19 @@ struct Plan {
     uint64_t ws_bytes;
     bool wide;               // workgroups of kWide waves
 };
-// Q4_0: as many as are resident, four workgroups a CU for heads of up to 64, three up to 128, two beyond, rounded down.  us by workgroups (256, 512, 768, 1024): 64 x 8192 tokens of 8 heads of 64 115, 73, 66, 59, of
-// 128 104, 105, 98, 118; 16 x 8192 of 8 heads of 256 67, 53, 75, 58; 16 x 8192 of 3 heads of 128 21.8, 18.4 (513 of them), 15.8, 20.1.
-// A workgroup for each sequence and group of heads takes up to 1024 tokens, or 512 where wide heads' workgroups would leave CUs free: us, in parts with their join against it, ragged sequences of up to 1000 tokens of 8 heads of
-// 128, 64 of them 16.6 + 4.1, 16.2; 400 56.3 + 4.8, 53.6; of 1024 tokens 64 20.6 + 4.2, 16.9; 200 45.8 + 4.2, 49.3; one of 8 heads of 256 7.6 + 4.0, 15.0; ragged ones of up to 2000 tokens 40 16.0 + 4.0, 23.1; 200 46.1 + 4.2, 51.6.
-// Where it leaves CUs free it has eight waves for more than two tiles a wave of four: us, four (in parts, for more than 512 tokens) against eight, sequences of 8 heads of 128: one of 512 tokens 8.2, 7.6; 32 of 512 9.0, 8.2,
-// of 256 6.7, 7.4; of 1024 tokens one 6.2 + 4.0, 10.0, four 7.8 + 4.0, 10.2, 16 9.9 + 4.0, 10.8, 32 15.0 + 4.0, 11.2; one of 512 of 8 heads of 256 11.4, 10.1.  More workgroups than CUs wait: 48 of 512 10.7, 15.7.
+// Q4_0.  In parts: as many workgroups as are resident, four a CU for heads of up to 64, three up to 128, two beyond, rounded down.  us by workgroups:
+//                                          256   512   768  1024
+//   64 x 8192 tokens of 8 heads of  64     115    73    66    59
+//                                  128     104   105    98   118
+//   16 x 8192 tokens of 8 heads of 256      67    53    75    58
+//                       3 heads of 128    21.8  18.4  15.8  20.1    (513 for 512)
+// Whole: a workgroup for each sequence and group of heads takes up to 1024 tokens, or 512 where wide heads' workgroups would leave CUs free.  us in parts + join, whole (8 heads of 128 unless said):
+//   ragged, up to 1000 tokens: 64 sequences 16.6 + 4.1, 16.2; 400 56.3 + 4.8, 53.6; up to 2000: 40 16.0 + 4.0, 23.1; 200 46.1 + 4.2, 51.6
+//   of 1024 tokens: 64 sequences 20.6 + 4.2, 16.9; 200 45.8 + 4.2, 49.3; one of 8 heads of 256 7.6 + 4.0, 15.0
+// Of eight waves where whole sequences leave CUs free and are longer than two tiles a wave of four (more workgroups than CUs would wait: 48 of 512 10.7, 15.7).  us of four waves (in parts, for more than
+// 512 tokens), of eight:
+//   of  512 tokens: one 8.2, 7.6; 32 9.0, 8.2; one of 8 heads of 256 11.4, 10.1; of 256: 32 6.7, 7.4
+//   of 1024 tokens: one 6.2 + 4.0, 10.0; four 7.8 + 4.0, 10.2; 16 9.9 + 4.0, 10.8; 32 15.0 + 4.0, 11.2
 enum { kF16 = 0, kQ8 = 1, kQ4 = 2 };   // what a cache holds
 constexpr uint32_t kDirectTiles = 4 * kWaves;
 constexpr int kWide = 8;
@@ -695,7 +708,7 @@ static Plan plan_of(int fmt, uint32_t B, uint32_t Hq, uint32_t Hkv, uint32_t D, 
 //     sum of weights too.  Every product's 16 rows are the low or the high codes of one block: the bytes of a block's column of 8 tokens come from LDS by the transposing read.
 //   * p d must stay in fp16's range: the largest weight is 2^(15 - k), 2^k above every scale that this wave has met (k > 0 only for values beyond 8).
 // Precision as above: p d is held to 2^-22, or 2^-39 + k of the largest weight's; what the offsets cancel in the fp32 sums is at most 15 / 8 of the values' own size.
-// Large caches are bound by memory, with the vector pipe busy half and the matrix pipe a quarter of the time: 64 x 8192 tokens of 8 heads of 128, 605 MB, 96 to 99 us, 6.1 to 6.3 TB/s; one sequence of 131071, 151 MB, 29.2. Small ones by what
+// Large caches are bound by memory, with the vector pipe busy half and the matrix pipe a quarter of the time: 64 x 8192 tokens of 8 heads of 128, 605 MB, 95 to 99 us, 6.1 to 6.3 TB/s; one sequence of 131071, 151 MB, 29.0. Small ones by what
 // is waited for in turn: launch, length and page, tile and the waves' sums are 5.2 us, each further tile of a wave 1.0 (2.2 where three workgroups share a CU).  Requests two and four tiles ahead gain nothing.
 
 // Eight codes' operand: the low or high codes (mask 0x000f000f, 0x00f000f0) of the bytes of two words, even bytes of a word in front of its odd ones.
@@ -712,7 +725,7 @@ struct Int {
 template <int NB, int C, int W, bool SHARED>
 __global__ __launch_bounds__(W * 64, W > (int)kWaves ? 2 : NB <= 2 ? 4 : NB <= 4 ? 3 : 2) void attn_decode_q4_kernel(AttnArgs a) {
     constexpr uint32_t D = 32 * NB, GP = 16 / C;
-    // LDS of a token's codes: an odd number of 16-byte pieces, so that 16 rows meet all banks; the second half of a tile lies four rows further, for the keys' rows 0 .. 3, 8 .. 11, 16 .. 19, 24 .. 27
+    // LDS of a token's codes: an odd number of 16-byte pieces, so that 16 rows meet all banks (conflicts of all accesses together: 3.0 cycles an LDS instruction for heads of 128, 1.5 of 64); the second half of a tile lies four rows further, for the keys' rows 0 .. 3, 8 .. 11, 16 .. 19, 24 .. 27
     constexpr uint32_t ROW = 16 * (NB | 1), HALF = 20 * ROW;
     constexpr uint32_t CODES = HALF + 16 * ROW, KS = kTile * NB * 2, VS = kTile * (NB + 1) * 2, WAVE = 2 * CODES + KS + VS;
     constexpr int S = (NB + C - 1) / C;

@@ -126,8 +126,8 @@ __device__ __forceinline__ void normed(const SumArgs& a, size_t at, const half8&
 
 // A workgroup takes a row, 128 threads each 1024 elements of it (a pass), up to eight passes at once; they meet in LDS (FAR, for rows beyond it: in the sum that they wrote), where 128 threads sum
 // the squares in the order above, lane by lane of half as many as block_sum has.
-// Bound by memory, 8 bytes and the stream's 1.25 or 1.5 an element: 8192 x 4096 51.6 us, 6.0 TB/s; one row of 4096 2.5 us.  With 128 threads for the whole row, which keep it in registers: 61.9 and
-// 3.6; 2048 x 16384 68 for 56, 333 x 2880 5.6 for 4.8.
+// Bound by memory, 8 bytes and the stream's 1.25 or 1.5 an element: 8192 x 4096 53 us, 5.8 TB/s; one row of 4096 2.7 us.  With 128 threads for the whole row, which keep it in registers, the least of
+// 21 launches: 61.9 for 51.6 and 3.6 for 2.5; 2048 x 16384 68 for 56, 333 x 2880 5.6 for 4.8.
 constexpr uint32_t kSumThreads = 128, kSumPasses = 8, kSumLds = 32768;      // elements that LDS holds
 template <bool HALVES, bool FAR>
 __global__ __launch_bounds__(kSumThreads * kSumPasses) void add_norm_kernel(SumArgs a) {

@@ -290,7 +290,7 @@ __device__ __forceinline__ void merge_two(uint64_t& first, uint64_t& second, uin
 
 // One wave a token, lane l holds experts NJ l .. NJ l + NJ - 1: scores in 64 bits and, as integers of the same order, what they are chosen by.  K rounds of a maximum over the wave: the upper halves of the
 // keys decide, and where several have the largest the lower halves and then the lowest id; who is taken is kept in scalar masks, which are the conditions of what follows.  The chosen meet in LDS and lane i
-// writes the i-th.  4096 tokens to 8 of 256 experts in groups 8.8 us (rounds over whole keys 11.5, shifted masks 10.5, every lane writing its own 10.2, bias by bias 9.4), one token of 128 experts 2.8 (3.5, 3.2, 3.0).
+// writes the i-th.  4096 tokens to 8 of 256 experts in groups 8.8 us (rounds over whole keys 11.5, shifted masks 10.5, every lane writing its own 10.2, bias by bias 9.4), one token of 128 experts 2.9 (3.5, 3.2, 3.0).
 // Bound by the vector instructions and, for few tokens, by their latency one after the other.
 template <int NJ>
 __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
