@@ -3,7 +3,6 @@ import numpy as np
 import pytest
 import torch
 
-import kv_util as U
 import q4_util as Q
 from gpu_util import dev, host
 from test_gpu_q4_cache import attend, case
